@@ -56,6 +56,10 @@ enum {
 
 /* 16-bit storage formats (src/shaders.rs:27-40, `Half`). */
 enum { QA_F16 = 0, QA_BF16 = 1 };
+/* An 8-bit storage format of a paged cache alone (qa_paged_kv.dtype): sign, 4
+ * exponent bits with bias 7, 3 mantissa bits; largest value 448, no infinity
+ * (OCP E4M3).  No counterpart in the reference. */
+enum { QA_E4M3 = 2 };
 
 /* qa_linear_desc.flags */
 enum {
@@ -279,6 +283,144 @@ typedef struct qa_attention_desc {
   int64_t ldo;
 } qa_attention_desc;
 int qa_attention_prefill(qa_ctx* ctx, const qa_attention_desc* desc);
+
+/* ---- several sequences at once: the paged cache ----
+ *
+ * No counterpart in the reference, whose decoder runs one clip's prompt over one
+ * dense cache (src/decoder.rs:1305-1657).  These calls run the same layer over
+ * several sequences of different length, whole prompts, parts of prompts and
+ * single tokens mixed in one batch, with caches that grow page by page:
+ * qa_mrope_rows once per step, then per layer qa_kv_append and
+ * qa_attention_paged in the places of qa_qk_norm_rope and
+ * qa_attention_prefill. */
+
+/* cos / sin rows for tokens whose positions have several axes: 1 (text), 2
+ * (height, width) or 3 (time, height, width, src/mrope.rs:55-89).  Frequency j <
+ * hd / 2 turns by pos[a(j)][t] * theta^(-2j / hd); a(j) is 0 for the first sec0
+ * frequencies, 1 for the next sec1, 2 for the last sec2, or, with
+ * QA_MROPE_INTERLEAVED, j mod axes where j < axes * sec of that axis and 0
+ * elsewhere.  Angle, cosine and sine are f64, rounded to f32 and then to the
+ * 16-bit format `dtype`, stored widened, the second half of a row repeating the
+ * first: with all axes equal, the rows of qa_rope_tables.
+ *   pos      int32 [axes][ldpos], any values, ldpos >= tokens
+ *   cos, sin f32 [tokens][hd], 16-byte aligned
+ * hd a multiple of 8 up to 256; sec0 + sec1 + sec2 = hd / 2 with none negative, those
+ * past `axes` zero. */
+enum { QA_MROPE_INTERLEAVED = 1u << 0 };
+typedef struct qa_mrope_desc {
+  uint32_t dtype;
+  uint32_t flags; /* 0 or QA_MROPE_INTERLEAVED */
+  int64_t tokens;
+  int32_t hd, axes, sec0, sec1, sec2;
+  double theta;
+  const int32_t* pos;
+  int64_t ldpos;
+  float* cos;
+  float* sin;
+} qa_mrope_desc;
+int qa_mrope_rows(qa_ctx* ctx, const qa_mrope_desc* desc);
+
+/* One layer's paged cache and the batch that uses it.
+ *   k        [num_pages][nkvh][page][hd]
+ *   v        [num_pages][nkvh][hd][page]  (transposed within a page)
+ *            in the 16-bit format of the call or in QA_E4M3; page 16, 32 or 64
+ *            tokens, hd 64 or 128; both 16-byte aligned
+ *   k_scale, v_scale  f32 [num_pages][nkvh], QA_E4M3 alone: an element stands
+ *            for its e4m3 value times its page's and head's scale
+ *   table    int32 [seqs][ldtable]: entry i of a sequence is the page of its
+ *            positions i * page ..  An entry outside [0, num_pages) is no page.
+ *   row_start int32 [seqs + 1], rising: rows row_start[s] .. row_start[s + 1] - 1
+ *            of the batch are sequence s's new ones; it may have none
+ *   kv_len   int32 [seqs]: its keys with the new rows, whose positions are
+ *            kv_len - rows .. kv_len - 1
+ *   max_rows, max_len  bounds of one sequence's rows and keys, max_len <= ldtable *
+ *            page: they set the launch, so that a captured call can be replayed
+ *            on other lengths
+ * table, row_start and kv_len are device memory, read by the kernels, and whatever
+ * they hold no call reads or writes outside its buffers: rows past the batch or
+ * past max_rows, positions below zero or past max_len and entries that are no
+ * page are left out.  Rows that no sequence has are left as they are.  Two new
+ * rows must not share a slot; a page may be in several tables while it is only
+ * read. */
+typedef struct qa_paged_kv {
+  uint32_t dtype; /* the call's 16-bit format, or QA_E4M3 */
+  int32_t page;
+  int32_t nkvh, hd;
+  int64_t num_pages;
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  const int32_t* table;
+  int64_t ldtable;
+  int64_t seqs;
+  const int32_t* row_start;
+  const int32_t* kv_len;
+  int64_t max_rows, max_len;
+} qa_paged_kv;
+
+/* qa_qk_norm_rope for a packed batch: per-head q / k RMSNorm and rotate-half RoPE
+ * of the fused qkv rows, q to q_out, K and V (verbatim) to their pages.
+ *   qkv     [tokens][(nqh + 2 nkvh) hd], row stride ldqkv: q heads, k, v
+ *   cos,sin f32 [tokens][hd], a row for each row of the batch (qa_mrope_rows)
+ *   q_out   [tokens][nqh hd], row stride ldq
+ * In a QA_E4M3 cache a page's scale is the least power of two p with amax <= 448 p
+ * over what the page holds of that head (2^-110 <= p <= 2^120), rounded to
+ * nearest even: rows that go into a page's first slot set it anew, later rows
+ * can only raise it, and the whole page is then rounded again (exactly, but for
+ * what falls below 2^-6 p).  An infinity is stored as the largest value, NaN as
+ * NaN; neither counts for the scale.  Strides multiples of 8; every buffer
+ * 16-byte aligned. */
+typedef struct qa_kv_append_desc {
+  uint32_t dtype;
+  uint32_t flags; /* reserved, must be 0 */
+  int64_t tokens;
+  int32_t nqh;
+  float eps;
+  const void* qkv;
+  int64_t ldqkv;
+  const float* qn_w; /* [hd] */
+  const float* kn_w; /* [hd] */
+  const float* cos;
+  const float* sin;
+  void* q_out;
+  int64_t ldq;
+  const qa_paged_kv* kv;
+} qa_kv_append_desc;
+int qa_kv_append(qa_ctx* ctx, const qa_kv_append_desc* desc);
+
+/* Causal GQA attention of a packed batch over the paged cache (after
+ * qa_kv_append): the row at position p attends to its sequence's keys 0 .. p, q
+ * head h to kv head h / (nqh / nkvh), softmax of q.k / sqrt(hd) in f32,
+ * out[t][h hd + j] = round(sum_t p_t v_t[j]).  Keys on an entry that is no page do
+ * not count; a row without keys gives zeros.  What the pages hold behind a
+ * sequence's last key is not looked at.  Scales may be any positive numbers.
+ *   q    [tokens][nqh hd], row stride ldq, as qa_kv_append writes it
+ *   out  [tokens][nqh hd], row stride ldo, the o projection's input
+ *   workspace  16-byte aligned device memory for partial results, of the bytes
+ *        that qa_attention_paged_workspace gives for these sizes (NULL where
+ *        that is 0); its contents need not be kept or cleared, and calls that may
+ *        run at the same time (two graphs, two contexts) need one each
+ * Strides multiples of 8; q and out 16-byte aligned.  The probabilities enter
+ * the P.V product as two 16-bit terms, as in qa_attention_prefill's default. */
+typedef struct qa_paged_attention_desc {
+  uint32_t dtype;
+  uint32_t flags; /* reserved, must be 0 */
+  int64_t tokens;
+  int32_t nqh;
+  const void* q;
+  int64_t ldq;
+  const qa_paged_kv* kv;
+  void* out;
+  int64_t ldo;
+  void* workspace;
+  size_t workspace_bytes;
+} qa_paged_attention_desc;
+int qa_attention_paged(qa_ctx* ctx, const qa_paged_attention_desc* desc);
+/* The workspace of that call in bytes, from its sizes alone (dtype, nqh, tokens and
+ * the kv's dtype, page, nkvh, hd, seqs, max_rows, max_len): pointers are not looked
+ * at.  Host function, no device needed. */
+int qa_attention_paged_workspace(const qa_paged_attention_desc* desc, size_t* bytes);
 
 /* ---- audio tower ops around the projections ---- */
 

@@ -31,9 +31,11 @@ INCLUDE_DIR = os.path.join(os.path.dirname(_HERE), "include")
 # include/qa.h constants
 QA_OK, QA_EINVAL, QA_ENOMEM, QA_EDEVICE, QA_EUNSUPPORTED = 0, -1, -2, -3, -4
 F16, BF16 = 0, 1
+E4M3 = 2  # qa_paged_kv.dtype alone
 ACCUMULATE, EPI_GELU, EPI_SILU_MUL, TRANSB, BIAS_ROWS = 1, 2, 4, 8, 16
 QA_ATTN_P16 = 1  # qa_attention_desc.flags
 QA_CONV_GELU, QA_CONV_TOKEN_MAJOR = 1, 2  # qa_conv_desc.flags
+MROPE_INTERLEAVED = 1  # qa_mrope_desc.flags
 
 _STATUS = {
     QA_EINVAL: "QA_EINVAL",
@@ -152,6 +154,88 @@ class AttentionDesc(ctypes.Structure):
         ("q0", ctypes.c_int64),
         ("out", ctypes.c_void_p),
         ("ldo", ctypes.c_int64),
+    ]
+
+
+class MropeDesc(ctypes.Structure):
+    """qa_mrope_desc (include/qa.h)."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_uint32),
+        ("flags", ctypes.c_uint32),
+        ("tokens", ctypes.c_int64),
+        ("hd", ctypes.c_int32),
+        ("axes", ctypes.c_int32),
+        ("sec0", ctypes.c_int32),
+        ("sec1", ctypes.c_int32),
+        ("sec2", ctypes.c_int32),
+        ("theta", ctypes.c_double),
+        ("pos", ctypes.c_void_p),
+        ("ldpos", ctypes.c_int64),
+        ("cos", ctypes.c_void_p),
+        ("sin", ctypes.c_void_p),
+    ]
+
+
+class PagedKV(ctypes.Structure):
+    """qa_paged_kv (include/qa.h)."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_uint32),
+        ("page", ctypes.c_int32),
+        ("nkvh", ctypes.c_int32),
+        ("hd", ctypes.c_int32),
+        ("num_pages", ctypes.c_int64),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("table", ctypes.c_void_p),
+        ("ldtable", ctypes.c_int64),
+        ("seqs", ctypes.c_int64),
+        ("row_start", ctypes.c_void_p),
+        ("kv_len", ctypes.c_void_p),
+        ("max_rows", ctypes.c_int64),
+        ("max_len", ctypes.c_int64),
+    ]
+
+
+class KvAppendDesc(ctypes.Structure):
+    """qa_kv_append_desc (include/qa.h)."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_uint32),
+        ("flags", ctypes.c_uint32),
+        ("tokens", ctypes.c_int64),
+        ("nqh", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("qkv", ctypes.c_void_p),
+        ("ldqkv", ctypes.c_int64),
+        ("qn_w", ctypes.c_void_p),
+        ("kn_w", ctypes.c_void_p),
+        ("cos", ctypes.c_void_p),
+        ("sin", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p),
+        ("ldq", ctypes.c_int64),
+        ("kv", ctypes.POINTER(PagedKV)),
+    ]
+
+
+class PagedAttentionDesc(ctypes.Structure):
+    """qa_paged_attention_desc (include/qa.h)."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_uint32),
+        ("flags", ctypes.c_uint32),
+        ("tokens", ctypes.c_int64),
+        ("nqh", ctypes.c_int32),
+        ("q", ctypes.c_void_p),
+        ("ldq", ctypes.c_int64),
+        ("kv", ctypes.POINTER(PagedKV)),
+        ("out", ctypes.c_void_p),
+        ("ldo", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
     ]
 
 
@@ -283,6 +367,7 @@ EXPORTS = (
     "qa_linear_noalloc", "qa_linear_noalloc_scratch_floats", "qa_prefetch_hint",
     "qa_time_next_launch",
     "qa_mlp_fused", "qa_rms_norm", "qa_qk_norm_rope", "qa_attention_prefill",
+    "qa_mrope_rows", "qa_kv_append", "qa_attention_paged", "qa_attention_paged_workspace",
     "qa_layer_norm", "qa_window_attention", "qa_add_position_table", "qa_conv2d_3x3s2",
     "qa_mel_filterbank", "qa_log_mel", "qa_rope_tables", "qa_embed_scatter", "qa_timestamp_head",
     "qa_last_error", "qa_version",
@@ -320,6 +405,10 @@ def lib() -> ctypes.CDLL:
         L.qa_rms_norm.argtypes = [vp, ctypes.POINTER(RmsNormDesc)]
         L.qa_qk_norm_rope.argtypes = [vp, ctypes.POINTER(QkRopeDesc)]
         L.qa_attention_prefill.argtypes = [vp, ctypes.POINTER(AttentionDesc)]
+        L.qa_mrope_rows.argtypes = [vp, ctypes.POINTER(MropeDesc)]
+        L.qa_kv_append.argtypes = [vp, ctypes.POINTER(KvAppendDesc)]
+        L.qa_attention_paged.argtypes = [vp, ctypes.POINTER(PagedAttentionDesc)]
+        L.qa_attention_paged_workspace.argtypes = [ctypes.POINTER(PagedAttentionDesc), ctypes.POINTER(sz)]
         L.qa_layer_norm.argtypes = [vp, ctypes.POINTER(LayerNormDesc)]
         L.qa_window_attention.argtypes = [vp, ctypes.POINTER(WindowAttentionDesc)]
         L.qa_add_position_table.argtypes = [vp, ctypes.POINTER(PositionAddDesc)]
@@ -452,6 +541,15 @@ class Context:
     def attention_prefill(self, desc: AttentionDesc) -> None:
         check(lib().qa_attention_prefill(self.handle, ctypes.byref(desc)))
 
+    def mrope_rows(self, desc: MropeDesc) -> None:
+        check(lib().qa_mrope_rows(self.handle, ctypes.byref(desc)))
+
+    def kv_append(self, desc: KvAppendDesc) -> None:
+        check(lib().qa_kv_append(self.handle, ctypes.byref(desc)))
+
+    def attention_paged(self, desc: PagedAttentionDesc) -> None:
+        check(lib().qa_attention_paged(self.handle, ctypes.byref(desc)))
+
     def layer_norm(self, desc: LayerNormDesc) -> None:
         check(lib().qa_layer_norm(self.handle, ctypes.byref(desc)))
 
@@ -472,6 +570,13 @@ class Context:
 
     def timestamp_head(self, desc: HeadDesc) -> None:
         check(lib().qa_timestamp_head(self.handle, ctypes.byref(desc)))
+
+
+def attention_paged_workspace(desc: PagedAttentionDesc) -> int:
+    """qa_attention_paged_workspace (host): bytes of workspace for a call of desc's sizes."""
+    size = ctypes.c_size_t()
+    check(lib().qa_attention_paged_workspace(ctypes.byref(desc), ctypes.byref(size)))
+    return size.value
 
 
 def mel_filterbank(n_mels: int = 128, n_fft: int = 400, sample_rate: int = 16000) -> np.ndarray:

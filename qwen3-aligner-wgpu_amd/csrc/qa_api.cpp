@@ -472,6 +472,60 @@ NextLaunch take_next_launch(qa_ctx* ctx) {
   return n;
 }
 
+// The sizes of a paged cache and its batch (of no buffer yet): 0 or the failure.
+int check_paged_sizes(const char* fn, const qa_paged_kv* kv, uint32_t dtype, int64_t tokens, int64_t nqh) {
+  if (dtype != QA_F16 && dtype != QA_BF16)
+    return fail(QA_EINVAL, "%s: dtype %u is neither QA_F16 nor QA_BF16", fn, dtype);
+  if (!kv) return fail(QA_EINVAL, "%s: null kv", fn);
+  if (kv->dtype != dtype && kv->dtype != QA_E4M3)
+    return fail(QA_EINVAL, "%s: the cache's dtype %u is neither the call's nor QA_E4M3", fn, kv->dtype);
+  if (kv->page != 16 && kv->page != 32 && kv->page != 64)
+    return fail(QA_EUNSUPPORTED, "%s: page=%d (16, 32 or 64)", fn, kv->page);
+  if (kv->hd != 64 && kv->hd != 128) return fail(QA_EUNSUPPORTED, "%s: hd=%d (64 or 128)", fn, kv->hd);
+  if (kv->nkvh <= 0 || nqh <= 0 || nqh % kv->nkvh || nqh > 65536)
+    return fail(QA_EINVAL, "%s: need nqh (<= 65536) a multiple of nkvh > 0", fn);
+  if (tokens < 0 || tokens > kI32 || kv->seqs < 0 || kv->seqs > kI32 || kv->max_rows < 0 || kv->max_rows > kI32)
+    return fail(QA_EINVAL, "%s: tokens, seqs and max_rows must be in [0, 2^31)", fn);
+  if (kv->max_len < 0 || kv->max_len > kI32 - 128)
+    return fail(QA_EINVAL, "%s: max_len must be in [0, 2^31 - 128)", fn);
+  return ok();
+}
+// ... and its buffers.
+int check_paged(const char* fn, const qa_paged_kv* kv, uint32_t dtype, int64_t tokens, int64_t nqh) {
+  if (int rc = check_paged_sizes(fn, kv, dtype, tokens, nqh)) return rc;
+  if (kv->num_pages <= 0 || kv->num_pages > kI32)
+    return fail(QA_EINVAL, "%s: num_pages must be in (0, 2^31)", fn);
+  if (kv->ldtable < 0 || kv->ldtable > kI32 || kv->max_len > kv->ldtable * kv->page)
+    return fail(QA_EINVAL, "%s: max_len=%lld is more than a table row's %lld pages of %d hold", fn, (long long)kv->max_len,
+                (long long)kv->ldtable, kv->page);
+  if (!kv->k || !kv->v || !kv->table || !kv->row_start || !kv->kv_len ||
+      (kv->dtype == QA_E4M3 && (!kv->k_scale || !kv->v_scale)))
+    return fail(QA_EINVAL, "%s: null cache pointer", fn);
+  if (!aligned(kv->k, 16) || !aligned(kv->v, 16) || !aligned(kv->table, 4) || !aligned(kv->row_start, 4) ||
+      !aligned(kv->kv_len, 4) || !aligned(kv->k_scale, 4) || !aligned(kv->v_scale, 4))
+    return fail(QA_EINVAL, "%s: misaligned cache pointer (k and v 16-byte aligned)", fn);
+  return ok();
+}
+qa::PagedParams paged_params(const qa_paged_kv& kv, int64_t tokens) {
+  qa::PagedParams p{};
+  p.k = kv.k;
+  p.v = kv.v;
+  p.k_scale = kv.k_scale;
+  p.v_scale = kv.v_scale;
+  p.table = kv.table;
+  p.row_start = kv.row_start;
+  p.kv_len = kv.kv_len;
+  p.num_pages = kv.num_pages;
+  p.ldtable = kv.ldtable;
+  p.tokens = tokens;
+  p.seqs = (int)kv.seqs;
+  p.max_rows = (int)std::min(kv.max_rows, tokens);
+  p.max_len = (int)kv.max_len;
+  p.nkvh = kv.nkvh;
+  p.lp = kv.page == 16 ? 4 : kv.page == 32 ? 5 : 6;
+  return p;
+}
+
 // Launch a validated, planned projection with split-K partials in `ws`.
 int launch_linear(qa_ctx* ctx, const qa_linear_desc* d, const qa::Plan& plan, float* ws,
                   const NextLaunch& nl) {
@@ -853,6 +907,130 @@ int qa_attention_prefill(qa_ctx* ctx, const qa_attention_desc* d) {
   p.scale = 1.0f / sqrtf((float)d->hd);
   const hipError_t e = qa::launch_attention((int)d->dtype, p, (d->flags & QA_ATTN_P16) != 0, ctx->stream);
   return e == hipSuccess ? ok() : hip_fail(e, "qa_attention_prefill launch");
+}
+
+int qa_mrope_rows(qa_ctx* ctx, const qa_mrope_desc* d) {
+  if (!d) return fail(QA_EINVAL, "qa_mrope_rows: null argument");
+  if (d->dtype != QA_F16 && d->dtype != QA_BF16)
+    return fail(QA_EINVAL, "qa_mrope_rows: dtype %u is neither QA_F16 nor QA_BF16", d->dtype);
+  if (d->flags & ~(uint32_t)QA_MROPE_INTERLEAVED)
+    return fail(QA_EINVAL, "qa_mrope_rows: unknown flags 0x%x", d->flags & ~(uint32_t)QA_MROPE_INTERLEAVED);
+  if (d->hd <= 0 || d->hd % 8 || d->hd > 2 * qa::kMropeHalf)
+    return fail(QA_EINVAL, "qa_mrope_rows: hd=%d must be a multiple of 8 up to %d", d->hd, 2 * qa::kMropeHalf);
+  if (d->axes < 1 || d->axes > 3) return fail(QA_EINVAL, "qa_mrope_rows: axes=%d (1, 2 or 3)", d->axes);
+  const int64_t sec[3] = {d->sec0, d->sec1, d->sec2};
+  if (sec[0] < 0 || sec[1] < 0 || sec[2] < 0 || sec[0] + sec[1] + sec[2] != d->hd / 2 || (d->axes < 3 && sec[2]) ||
+      (d->axes < 2 && sec[1]))
+    return fail(QA_EINVAL, "qa_mrope_rows: the axes' sections must be >= 0 and add up to hd / 2");
+  if (d->tokens < 0 || d->tokens > kI32 || d->ldpos < d->tokens || d->ldpos > kI32)
+    return fail(QA_EINVAL, "qa_mrope_rows: need 0 <= tokens <= ldpos < 2^31");
+  if (!(d->theta > 0.0) || !std::isfinite(d->theta)) return fail(QA_EINVAL, "qa_mrope_rows: theta must be a positive number");
+  if (!d->pos || !d->cos || !d->sin) return fail(QA_EINVAL, "qa_mrope_rows: null pointer");
+  if (!aligned(d->pos, 4) || !aligned(d->cos, 16) || !aligned(d->sin, 16))
+    return fail(QA_EINVAL, "qa_mrope_rows: cos and sin must be 16-byte aligned");
+  if (!ctx) return fail(QA_EINVAL, "qa_mrope_rows: null context");
+  if (d->tokens == 0) return ok();
+  if (int rc = set_device(ctx)) return rc;
+  qa::MropeParams p{};
+  p.pos = d->pos;
+  p.cos = d->cos;
+  p.sin = d->sin;
+  p.tokens = d->tokens;
+  p.ldpos = d->ldpos;
+  p.hd = d->hd;
+  for (int j = 0; j < d->hd / 2; ++j) {
+    const int a = j % d->axes;
+    p.inv[j] = 1.0 / std::pow(d->theta, 2.0 * j / d->hd);  // as qa_rope_tables forms it
+    p.axis[j] = (uint8_t)((d->flags & QA_MROPE_INTERLEAVED) ? (j < d->axes * sec[a] ? a : 0)
+                                                            : j < sec[0] ? 0 : j < sec[0] + sec[1] ? 1 : 2);
+  }
+  const hipError_t e = qa::launch_mrope_rows((int)d->dtype, p, ctx->stream);
+  return e == hipSuccess ? ok() : hip_fail(e, "qa_mrope_rows launch");
+}
+
+int qa_kv_append(qa_ctx* ctx, const qa_kv_append_desc* d) {
+  if (!d) return fail(QA_EINVAL, "qa_kv_append: null argument");
+  if (d->flags) return fail(QA_EINVAL, "qa_kv_append: flags must be 0");
+  if (int rc = check_paged("qa_kv_append", d->kv, d->dtype, d->tokens, d->nqh)) return rc;
+  const qa_paged_kv& kv = *d->kv;
+  if (d->ldqkv < ((int64_t)d->nqh + 2 * (int64_t)kv.nkvh) * kv.hd || d->ldqkv % 8)
+    return fail(QA_EINVAL, "qa_kv_append: ldqkv must be >= the fused q|k|v width and a multiple of 8");
+  if (d->ldq < (int64_t)d->nqh * kv.hd || d->ldq % 8)
+    return fail(QA_EINVAL, "qa_kv_append: ldq must be >= nqh*hd and a multiple of 8");
+  if (!d->qkv || !d->qn_w || !d->kn_w || !d->cos || !d->sin || !d->q_out)
+    return fail(QA_EINVAL, "qa_kv_append: null pointer");
+  if (!aligned(d->qkv, 16) || !aligned(d->qn_w, 16) || !aligned(d->kn_w, 16) || !aligned(d->cos, 16) ||
+      !aligned(d->sin, 16) || !aligned(d->q_out, 16))
+    return fail(QA_EINVAL, "qa_kv_append: buffers must be 16-byte aligned");
+  if (!(d->eps >= 0.0f)) return fail(QA_EINVAL, "qa_kv_append: eps must be >= 0");
+  qa::AppendParams p{};
+  p.kv = paged_params(kv, d->tokens);
+  // blocks: four (row, group of heads) each, and one for each page a sequence may touch
+  const int64_t most = qa::pages_touched(p.kv.max_rows, p.kv.lp);
+  if ((d->tokens * ((d->nqh + 1024 / kv.hd - 1) / (1024 / kv.hd)) + 3) / 4 > kI32 / 2 ||
+      (double)most * (double)kv.seqs * kv.nkvh > kI32 / 2)
+    return fail(QA_EINVAL, "qa_kv_append: the batch is too large for one launch");
+  if (!ctx) return fail(QA_EINVAL, "qa_kv_append: null context");
+  if (d->tokens == 0 || kv.seqs == 0) return ok();
+  if (int rc = set_device(ctx)) return rc;
+  p.qkv = (const uint16_t*)d->qkv;
+  p.qn = d->qn_w;
+  p.kn = d->kn_w;
+  p.cos = d->cos;
+  p.sin = d->sin;
+  p.q_out = (uint16_t*)d->q_out;
+  p.ldqkv = d->ldqkv;
+  p.ldq = d->ldq;
+  p.nqh = d->nqh;
+  p.eps = d->eps;
+  const hipError_t e = qa::launch_kv_append((int)d->dtype, kv.dtype == QA_E4M3, kv.hd, p, ctx->stream);
+  return e == hipSuccess ? ok() : hip_fail(e, "qa_kv_append launch");
+}
+
+int qa_attention_paged_workspace(const qa_paged_attention_desc* d, size_t* bytes) {
+  if (!d || !bytes) return fail(QA_EINVAL, "qa_attention_paged_workspace: null argument");
+  *bytes = 0;
+  if (int rc = check_paged_sizes("qa_attention_paged_workspace", d->kv, d->dtype, d->tokens, d->nqh)) return rc;
+  qa::PagedAttnParams p{};
+  p.kv = paged_params(*d->kv, d->tokens);
+  p.nqh = d->nqh;
+  p.rep = d->nqh / d->kv->nkvh;
+  *bytes = qa::paged_attention_workspace(d->kv->hd, p);
+  return ok();
+}
+
+int qa_attention_paged(qa_ctx* ctx, const qa_paged_attention_desc* d) {
+  if (!d) return fail(QA_EINVAL, "qa_attention_paged: null argument");
+  if (d->flags) return fail(QA_EINVAL, "qa_attention_paged: flags must be 0");
+  if (int rc = check_paged("qa_attention_paged", d->kv, d->dtype, d->tokens, d->nqh)) return rc;
+  const qa_paged_kv& kv = *d->kv;
+  const int64_t width = (int64_t)d->nqh * kv.hd;
+  if (d->ldq < width || d->ldq % 8 || d->ldo < width || d->ldo % 8)
+    return fail(QA_EINVAL, "qa_attention_paged: ldq and ldo must be >= nqh*hd and multiples of 8");
+  if (!d->q || !d->out) return fail(QA_EINVAL, "qa_attention_paged: null pointer");
+  if (!aligned(d->q, 16) || !aligned(d->out, 16) || !aligned(d->workspace, 16))
+    return fail(QA_EINVAL, "qa_attention_paged: buffers must be 16-byte aligned");
+  qa::PagedAttnParams p{};
+  p.kv = paged_params(kv, d->tokens);
+  p.nqh = d->nqh;
+  p.rep = d->nqh / kv.nkvh;
+  const size_t need = qa::paged_attention_workspace(kv.hd, p);
+  if (need && (!d->workspace || d->workspace_bytes < need))
+    return fail(QA_EINVAL, "qa_attention_paged: a workspace of %zu bytes is needed, %zu given", need,
+                d->workspace ? d->workspace_bytes : (size_t)0);
+  if ((double)kv.seqs * (double)p.kv.max_rows * d->nqh > kI32 / 2)
+    return fail(QA_EINVAL, "qa_attention_paged: the batch is too large for one launch");
+  if (!ctx) return fail(QA_EINVAL, "qa_attention_paged: null context");
+  if (d->tokens == 0 || kv.seqs == 0 || kv.max_rows == 0) return ok();
+  if (int rc = set_device(ctx)) return rc;
+  p.q = (const uint16_t*)d->q;
+  p.out = (uint16_t*)d->out;
+  p.ws = (float*)d->workspace;
+  p.ldq = d->ldq;
+  p.ldo = d->ldo;
+  p.scale = 1.0f / sqrtf((float)kv.hd);
+  const hipError_t e = qa::launch_attention_paged((int)d->dtype, kv.dtype == QA_E4M3, kv.hd, p, ctx->stream);
+  return e == hipSuccess ? ok() : hip_fail(e, "qa_attention_paged launch");
 }
 
 int qa_conv2d_3x3s2(qa_ctx* ctx, const qa_conv_desc* d) {

@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include "qa.h"
+#include "qa_paged.h"
 
 namespace qa {
 
@@ -347,6 +348,44 @@ struct HeadParams {
   float eps;
 };
 hipError_t launch_timestamp_head(int dtype, const HeadParams& p, hipStream_t stream);
+
+// qa_mrope_rows (qa_rope_rows.hip).
+constexpr int kMropeHalf = 128;  // frequencies at most
+struct MropeParams {
+  const int32_t* pos;  // [axes][ldpos]
+  float *cos, *sin;    // [tokens][hd]
+  int64_t tokens, ldpos;
+  int hd;
+  double inv[kMropeHalf];    // theta^(-2j / hd)
+  uint8_t axis[kMropeHalf];  // the axis of frequency j
+};
+hipError_t launch_mrope_rows(int dtype, const MropeParams& p, hipStream_t s);
+
+// qa_kv_append (qa_paged_append.hip).
+struct AppendParams {
+  const uint16_t* qkv;
+  const float *qn, *kn, *cos, *sin;
+  uint16_t* q_out;
+  int64_t ldqkv, ldq;
+  int nqh;
+  float eps;
+  PagedParams kv;
+};
+hipError_t launch_kv_append(int dtype, bool e4m3, int hd, const AppendParams& p, hipStream_t s);
+
+// qa_attention_paged (qa_paged_attention.hip).
+struct PagedAttnParams {
+  const uint16_t* q;
+  uint16_t* out;
+  float* ws;
+  int64_t ldq, ldo;
+  int nqh, rep;  // rep = nqh / nkvh
+  float scale;
+  PagedParams kv;
+};
+// Bytes of workspace that a call of these sizes takes.
+size_t paged_attention_workspace(int hd, const PagedAttnParams& p);
+hipError_t launch_attention_paged(int dtype, bool e4m3, int hd, const PagedAttnParams& p, hipStream_t s);
 
 // p16: probabilities rounded once to the 16-bit format (else two 16-bit terms).
 hipError_t launch_attention(int dtype, const AttnParams& p, bool p16, hipStream_t stream);
