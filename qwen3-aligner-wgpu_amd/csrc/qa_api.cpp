@@ -486,8 +486,8 @@ int check_paged_sizes(const char* fn, const qa_paged_kv* kv, uint32_t dtype, int
     return fail(QA_EINVAL, "%s: need nqh (<= 65536) a multiple of nkvh > 0", fn);
   if (tokens < 0 || tokens > kI32 || kv->seqs < 0 || kv->seqs > kI32 || kv->max_rows < 0 || kv->max_rows > kI32)
     return fail(QA_EINVAL, "%s: tokens, seqs and max_rows must be in [0, 2^31)", fn);
-  if (kv->max_len < 0 || kv->max_len > kI32 - 128)
-    return fail(QA_EINVAL, "%s: max_len must be in [0, 2^31 - 128)", fn);
+  if (kv->max_len < 0 || kv->max_len > 1 << 30)
+    return fail(QA_EINVAL, "%s: max_len must be in [0, 2^30]", fn);
   return ok();
 }
 // ... and its buffers.
@@ -1018,7 +1018,7 @@ int qa_attention_paged(qa_ctx* ctx, const qa_paged_attention_desc* d) {
   if (need && (!d->workspace || d->workspace_bytes < need))
     return fail(QA_EINVAL, "qa_attention_paged: a workspace of %zu bytes is needed, %zu given", need,
                 d->workspace ? d->workspace_bytes : (size_t)0);
-  if ((double)kv.seqs * (double)p.kv.max_rows * d->nqh > kI32 / 2)
+  if (qa::paged_attention_blocks(p) > kI32 / 2)
     return fail(QA_EINVAL, "qa_attention_paged: the batch is too large for one launch");
   if (!ctx) return fail(QA_EINVAL, "qa_attention_paged: null context");
   if (d->tokens == 0 || kv.seqs == 0 || kv.max_rows == 0) return ok();

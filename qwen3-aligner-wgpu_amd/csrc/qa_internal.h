@@ -383,7 +383,8 @@ struct PagedAttnParams {
   float scale;
   PagedParams kv;
 };
-// Bytes of workspace that a call of these sizes takes.
+// Blocks of the larger of a call's launches, and the bytes of its workspace.
+int64_t paged_attention_blocks(const PagedAttnParams& p);
 size_t paged_attention_workspace(int hd, const PagedAttnParams& p);
 hipError_t launch_attention_paged(int dtype, bool e4m3, int hd, const PagedAttnParams& p, hipStream_t s);
 
