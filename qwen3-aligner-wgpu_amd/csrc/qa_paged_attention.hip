@@ -24,6 +24,9 @@
 // Keys are split: a block's waves take turns at its 64-key blocks (WK) and join
 // through LDS; beyond `chunk` keys further blocks take the next chunk, write
 // (O, max, sum) to the workspace, and paged_join_kernel joins them.
+#include <stdlib.h>
+#include <type_traits>
+
 #include "qa_internal.h"
 
 namespace qa {
@@ -55,10 +58,21 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   else
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
 }
+// (a, b) minus their 16-bit roundings h = pack2(a, b), as two 16-bit values.  The
+// differences are exact in f32.  f16: v_fma_mix_f32 reads its half of h as it
+// lies, -h * 1 + a; a and b come from ordinary VALU instructions or v_exp_f32, and h,
+// a compiler instruction's result that reads both, lies between them and the
+// statements, so that no wait state is missing.
 template <int DT>
-__device__ __forceinline__ f32x2 unpack2(uint32_t h) {
-  if constexpr (DT == QA_F16) return __builtin_convertvector(__builtin_bit_cast(f16x2, h), f32x2);
-  else return (f32x2){__uint_as_float(h << 16), __uint_as_float(h & 0xffff0000u)};
+__device__ __forceinline__ uint32_t residue2(uint32_t h, float a, float b) {
+  if constexpr (DT == QA_F16) {
+    float x, y;
+    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(x) : "v"(h), "v"(a));
+    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(y) : "v"(h), "v"(b));
+    return pack2<DT>(x, y);
+  } else {
+    return pack2<DT>(a - __uint_as_float(h << 16), b - __uint_as_float(h & 0xffff0000u));
+  }
 }
 // Eight e4m3 values (two words) as a 16-bit fragment; exact in both formats.
 template <int DT>
@@ -75,6 +89,27 @@ __device__ __forceinline__ u32x4 widen_e4m3(uint32_t a, uint32_t b) {
                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true))};
 }
 
+#define QA_LDS __attribute__((address_space(3)))
+
+template <int N>
+__device__ __forceinline__ void wait_vmcnt() {
+  static_assert(N >= 0 && N < 64, "vmcnt is 6 bits");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt((N & 0xF) | ((N >> 4) << 14) | (0x7 << 4) | (0xF << 8));
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+// Every LDS read so far has its data: what it read may be overwritten.
+__device__ __forceinline__ void wait_lds() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(0xF | (0x3 << 14) | (0x7 << 4) | (0x0 << 8));
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// A value that all of a wave's lanes have, as a scalar.
+__device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 // Maximum and sum over the four lanes that share a column (lane ^ 16, lane ^ 32).
 __device__ __forceinline__ float column_max(float v) {
   auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -89,38 +124,60 @@ __device__ __forceinline__ float column_sum(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// How a sequence's rows and keys are divided among blocks of 256 threads: tiles
-// of WQ x RT x 16 rows (few rows: one column group, all waves on the keys), chunks
-// of keys.  Both kernels and the host go by it.
-constexpr int kFewRows = 16;
-struct Split {
-  int few_chunk, few_chunks;    // sequences of at most kFewRows (row, head) pairs
-  int many_chunk, many_chunks;  // the others
-  int tiles;                    // tiles of the longest of those, 0: there are none
-  int units;                    // blocks per sequence and kv head
-  int parts;                    // partial results per row, 1: no workspace
+// Sizes that a call's formats give.
+template <int DT, bool F8, int HD>
+struct Cfg {
+  static constexpr int PV = F8 ? (int)QA_BF16 : DT;              // format of the P.V product
+  static constexpr float kBias = PV == QA_F16 ? 7.f : 0.f;       // f16 p scaled by 2^7: normal down to 2^-21
+  static constexpr int ES = F8 ? 1 : 2;                          // bytes of a cache element
+  static constexpr int CR = HD * ES / 16;                        // 16-byte chunks of a K row
+  static constexpr int LCR = CR == 16 ? 4 : CR == 8 ? 3 : 2;
+  static constexpr int KS = CR / 4;                              // 64-byte slices of a K row
+  static constexpr int QS = HD / 32;                             // products over d
+  static constexpr int ND = HD / 16;                             // d tiles
+  static constexpr int VS = F8 ? 1 : 2;                          // chunks of a V row's 16 keys
+  static constexpr int LI = CR;                                  // DMA instructions of a tile, K's and V's alike
+  static constexpr int TILE = 64 * HD * ES;                      // bytes of a K or V tile
 };
-constexpr int kManyRT = 2, kManyWQ = 4;
+
+// How a call's rows and keys are divided among blocks.
+//  * few: a sequence of at most kFewRows (row, head) pairs is one column group; a
+//    block's four waves take turns at a chunk of its keys, each with tiles of its
+//    own.
+//  * many: tiles of kManyRows pairs.
+constexpr int kFewRows = 16, kFewWaves = 4;
+constexpr int kManyRows = 64, kManyWaves = 8;
+struct Split {
+  int few, many;                // which of the two kernels run
+  int few_chunk, few_chunks;    // keys of a part, parts of the longest sequence
+  int many_chunk, many_chunks;
+  int tiles;                    // tiles of the longest sequence of `many`
+  int parts;                    // partial results per row; 1: no workspace
+};
 
 Split split_of(const PagedAttnParams& p) {
   Split s{};
   const int64_t rows = (int64_t)p.kv.max_rows * p.rep, len = p.kv.max_len > 1 ? p.kv.max_len : 1;
-  const bool many = rows > kFewRows;
   const int64_t heads = (int64_t)p.kv.seqs * p.kv.nkvh;
   auto divide = [&](int64_t blocks, int64_t want, int64_t least, int* chunk, int* chunks) {
-    int64_t parts = blocks > 0 ? (want + blocks - 1) / blocks : 1;
+    const int64_t parts = blocks > 0 ? (want + blocks - 1) / blocks : 1;
     int64_t c = (len + parts - 1) / parts;
-    c = (c < least ? least : c) + 255 & ~(int64_t)255;
+    c = ((c < least ? least : c) + 255) & ~(int64_t)255;
     *chunk = (int)c;
     *chunks = (int)((len + c - 1) / c);
   };
-  divide(heads, 1024, 512, &s.few_chunk, &s.few_chunks);
-  if (many) {
-    constexpr int tr = 16 * kManyRT * kManyWQ;
-    s.tiles = (int)((rows + tr - 1) / tr);
-    divide(heads * s.tiles, 512, 512, &s.many_chunk, &s.many_chunks);
+  s.many = rows > kFewRows;
+  // where every sequence has to have the most rows for the batch to be as long as
+  // it is, none is a short one
+  s.few = !s.many || (int64_t)p.kv.seqs * p.kv.max_rows > p.kv.tokens;
+  static const int W=getenv("QA_PW")?atoi(getenv("QA_PW")):256, Lc=getenv("QA_PL")?atoi(getenv("QA_PL")):512;
+  static const int MW=getenv("QA_MW")?atoi(getenv("QA_MW")):256, ML=getenv("QA_ML")?atoi(getenv("QA_ML")):512;
+  s.few_chunks = s.many_chunks = 1;
+  if (s.few) divide(heads, W, Lc, &s.few_chunk, &s.few_chunks);
+  if (s.many) {
+    s.tiles = (int)((rows + kManyRows - 1) / kManyRows);
+    divide(heads * s.tiles, MW, ML, &s.many_chunk, &s.many_chunks);
   }
-  s.units = s.tiles * s.many_chunks > s.few_chunks ? s.tiles * s.many_chunks : s.few_chunks;
   s.parts = s.many_chunks > s.few_chunks ? s.many_chunks : s.few_chunks;
   return s;
 }
@@ -133,344 +190,653 @@ __device__ __forceinline__ float* part_stats(const PagedAttnParams& p, const Spl
   return p.ws + p.kv.tokens * p.nqh * sp.parts * hd;
 }
 
-// One tile over the keys of one chunk.
-template <int DT, bool F8, int HD, int RT, int WQ, int WK>
-__device__ __forceinline__ void tile_body(const PagedAttnParams& p, const Split& sp, const SeqSpan& sq, int s, int h, int tile,
-                                          int part, int chunk, unsigned char* smem) {
-  constexpr int PV = F8 ? (int)QA_BF16 : DT;  // format of the P.V product
-  constexpr float kBias = PV == QA_F16 ? 7.f : 0.f;  // f16 p scaled by 2^7: normal down to 2^-21
-  constexpr int ES = F8 ? 1 : 2, E16 = 16 / ES;  // element size, elements of 16 bytes
-  constexpr int KS = HD * ES / 64;               // 64-byte slices of a K row
-  constexpr int QS = HD / 32;                    // products over d
-  constexpr int ND = HD / 16;                    // d tiles
-  constexpr int VS = F8 ? 1 : 2;                 // 16-byte loads of a V row's 16 keys
-  const PagedParams& kv = p.kv;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int c = lane & 15, g = lane >> 4;
-  const int wq = wave / WK, wk = wave % WK;
-  const int R0 = (tile * WQ + wq) * RT * 16, NR = sq.n * p.rep;
-
-  // rows of this lane's columns; columns past the last repeat it and store nothing
+// The (row, head) pairs of a wave's columns; columns past the last repeat it and
+// store nothing.
+template <int RT>
+struct Columns {
   int pos[RT], head[RT];
   int64_t tok[RT];
-  u32x4 q[RT][QS];
+  bool on[RT];
+  __device__ __forceinline__ void set(const PagedAttnParams& p, const SeqSpan& sq, int h, int R0, int c) {
+    const int NR = sq.n * p.rep;
+    asm volatile("" : "+v"(c));  // formed again for the result, not held across the loop
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      on[r] = R0 + r * 16 + c < NR;
+      const int R = min(R0 + r * 16 + c, NR - 1), i = R / p.rep;
+      head[r] = h * p.rep + R % p.rep;
+      tok[r] = sq.row0 + i;
+      pos[r] = sq.pos0 + i;
+    }
+  }
+};
+
+template <int DT, bool F8, int HD, int RT>
+__device__ __forceinline__ void load_q(const PagedAttnParams& p, const Columns<RT>& col, int g, u32x4 (&q)[RT][HD / 32]) {
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
-    const int R = min(R0 + r * 16 + c, NR - 1);
-    const int i = R / p.rep;
-    head[r] = h * p.rep + R % p.rep;
-    tok[r] = sq.row0 + i;
-    pos[r] = sq.pos0 + i;
-    const uint16_t* src = p.q + tok[r] * p.ldq + (int64_t)head[r] * HD;
+    const uint16_t* src = p.q + col.tok[r] * p.ldq + (int64_t)col.head[r] * HD;
 #pragma unroll
-    for (int e = 0; e < QS; ++e)
+    for (int e = 0; e < HD / 32; ++e)  // in the order in which a K row's chunks come
       q[r][e] = *reinterpret_cast<const u32x4*>(src + (F8 ? (e >> 1) * 64 + g * 16 + (e & 1) * 8 : e * 32 + g * 8));
   }
-  const int top = sq.pos0 + (min(R0 + RT * 16, NR) - 1) / p.rep + 1;  // keys that the wave's last row sees
-  const int k0 = part * chunk, k1 = min(k0 + chunk, top);
-  const int nb = R0 < NR && k1 > k0 ? (k1 - k0 + 63) / 64 : 0;
-  const int steps = (nb - wk + WK - 1) / WK;
+}
 
-  f32x4 o[RT][ND] = {};
+// A 64-key block's K and V tiles in LDS.  K: 64 rows of CR chunks; V: the block's
+// pages one after the other, each HD rows of CP chunks.  Both are copies of the
+// pages but for the order of chunks within a row: chunk ^ f(row), with f such that
+// the 16 lanes whose 16-byte reads the LDS serves at once (of lanes 0-31: 0-3,
+// 12-15, 20-27 and the others) find 16 different bank groups.  In a fragment read
+// lane (c, g) wants row c and a chunk that g adds to; so f depends on c, and for
+// V on the page size.
+__device__ __forceinline__ int swap3(int v) { return (0x1320 >> (4 * v)) & 3; }  // 0, 2, 3, 1
+template <int CR>
+__device__ __forceinline__ int k_swizzle(int c) {
+  return CR == 16 ? c : CR == 8 ? c >> 1 : swap3(c >> 2);
+}
+template <bool F8>
+__device__ __forceinline__ int v_swizzle(int c, int lcp) {
+  if (F8) return lcp == 2 ? swap3(c >> 2) : 0;
+  return lcp == 3 ? (c >> 1) & 5 : c >> 3;
+}
+// A DMA instruction copies 1 KB; those of a tile are dealt out to OF waves, of which
+// this is `mine`.  A page's are a run of PER, and what they add to the page's and the
+// tile's address is the same, so it goes into the instruction.  Pages that are
+// none come as zeros (a resource of no bytes).  ids: lane 4 j + a holds the page of
+// keys 16 a .. of block j.
+template <int OF, int PER, class Off>
+__device__ __forceinline__ void copy_page(const unsigned char* src, int bytes, unsigned char* to, int mine, Off off) {
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(src), (short)0, bytes, 0x00020000);
+#pragma unroll
+  for (int b = 0; b < (PER + 3) / 4; ++b) {  // 4 KB: the reach of the instruction's offset
+    QA_LDS void* dst = (QA_LDS void*)(to + b * 4096 + mine * 1024);
+    const int at = b * 4096 + mine * 1024;
+    auto one = [&](auto i) {
+      constexpr int I = decltype(i)::value;
+      if constexpr (I * OF < 4)
+        if (b * 4 + I * OF < PER) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, dst, 16, off(b * 4 + I * OF), at, I * OF * 1024, 0);
+    };
+    one(std::integral_constant<int, 0>{});
+    one(std::integral_constant<int, 1>{});
+    one(std::integral_constant<int, 2>{});
+    one(std::integral_constant<int, 3>{});
+  }
+}
+template <int DT, bool F8, int HD, int OF, int LP, bool K>
+__device__ __forceinline__ void load_pages(const PagedParams& kv, int h, int ids, int j, int mine, unsigned char* to) {
+  using C = Cfg<DT, F8, HD>;
+  constexpr int PER = C::LI >> (6 - LP), PB = HD * C::ES << LP;  // instructions and bytes of a page
+  constexpr int CW = K ? C::CR : (1 << LP) * C::ES / 16;          // chunks of a row
+  int ln = threadIdx.x & 63;
+  asm volatile("" : "+v"(ln));  // lane offsets are formed anew, not kept across the loop
+  // the part of f(row) that the lane gives; instruction n of the page adds its own
+  int f;
+  if constexpr (K) f = CW == 16 ? ln >> 4 & 3 : CW == 8 ? ln >> 4 & 1 : 0;
+  else if constexpr (F8) f = CW == 4 ? swap3(ln >> 4 & 3) : 0;
+  else f = CW == 4 ? ln >> 5 : ln >> 4 & 1;
+  const uint32_t lane_off = (uint32_t)((ln & ~(CW - 1)) | ((ln & (CW - 1)) ^ f)) * 16;
+  auto off_k = [&](int n, int pg) {  // n / KS: the 16 keys
+    const int g = (pg << (LP - 4)) + n / C::KS;
+    return lane_off ^ (uint32_t)((CW == 16 ? g << 2 : CW == 8 ? g << 1 : swap3(g)) << 4);
+  };
+  auto off_v = [&](int n) { return lane_off ^ (uint32_t)(!F8 && CW == 8 ? (n & 1) << 6 : 0); };
+  auto page_src = [&](int pg, int* bytes) {
+    const int id = __builtin_amdgcn_readlane(ids, j * 4 + (pg << (LP - 4)));
+    *bytes = id < 0 ? 0 : PB;
+    const uint64_t at = ((uint64_t)(uint32_t)max(id, 0) * (uint32_t)kv.nkvh + (uint32_t)h) * PB;
+    return (const unsigned char*)(K ? kv.k : kv.v) + at;
+  };
+  if constexpr (PER >= OF) {
+#pragma unroll
+    for (int pg = 0; pg < 64 >> LP; ++pg) {
+      int bytes;
+      const unsigned char* src = page_src(pg, &bytes);
+      copy_page<OF, PER>(src, bytes, to + pg * PER * 1024, mine, [&](int n) {
+        if constexpr (K) return off_k(C::KS >= OF ? n : n + mine, pg);  // (of OF instructions side by side: one 16 keys, or not)
+        else return OF == 1 ? off_v(n) : off_v(mine);
+      });
+    }
+  } else {  // fewer instructions to a page than waves: pages side by side
+    constexpr int PP = OF / PER;
+#pragma unroll
+    for (int p0 = 0; p0 < 64 >> LP; p0 += PP) {
+      const int pg = p0 + mine / PER, n = mine % PER;
+      int bytes;
+      const unsigned char* src = page_src(pg, &bytes);
+      copy_page<1, 1>(src + n * 1024, bytes - n * 1024 > 0 ? bytes - n * 1024 : 0, to + pg * PER * 1024 + n * 1024, 0, [&](int) {
+        if constexpr (K) return off_k(n, pg);
+        else return off_v(n);
+      });
+    }
+  }
+}
+template <int DT, bool F8, int HD, int OF, bool K>
+__device__ __forceinline__ void load_tile(const PagedParams& kv, int h, int ids, int j, int mine, unsigned char* to) {
+  if (kv.lp == 6) load_pages<DT, F8, HD, OF, 6, K>(kv, h, ids, j, mine, to);
+  else if (kv.lp == 5) load_pages<DT, F8, HD, OF, 5, K>(kv, h, ids, j, mine, to);
+  else load_pages<DT, F8, HD, OF, 4, K>(kv, h, ids, j, mine, to);
+}
+// Fragment addresses in the tiles.  K: product t reads row 16 (c / 4) + 4 t + c % 4,
+// slice e the chunk 4 e + g.  V: row d, the chunks of keys 16 g ..
+template <int DT, bool F8, int HD>
+__device__ __forceinline__ int k_frag(int c, int g) {
+  using C = Cfg<DT, F8, HD>;
+  return ((16 * (c >> 2) + (c & 3)) * C::CR + (g ^ k_swizzle<C::CR>(c))) * 16;
+}
+template <int DT, bool F8, int HD>
+__device__ __forceinline__ int v_frag(int c, int g, int e, int lcp) {
+  const int x = g * Cfg<DT, F8, HD>::VS + e;  // the block's chunk x of this row
+  return ((((x >> lcp) * HD + c) << lcp) + ((x & ((1 << lcp) - 1)) ^ v_swizzle<F8>(c, lcp))) * 16;
+}
+
+// S = K.Q^T of a block.  (The empty statements here and in weigh() keep the
+// fragments' addresses from being formed outside the loop and held there.)
+template <int DT, bool F8, int HD, int RT>
+__device__ __forceinline__ void scores(const unsigned char* kt, int ka, const u32x4 (&q)[RT][HD / 32], f32x4 (&sc)[RT][4]) {
+  using C = Cfg<DT, F8, HD>;
+  asm volatile("" : "+v"(ka));
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) sc[r][t] = f32x4{0, 0, 0, 0};
+  // product t + 1's fragments are read while product t multiplies
+  u32x4 x[2][C::KS];
+  auto read = [&](int t) {
+#pragma unroll
+    for (int e = 0; e < C::KS; ++e) x[t & 1][e] = *reinterpret_cast<const u32x4*>(kt + (ka ^ (e << 6)) + 4 * t * C::CR * 16);
+  };
+  read(0);
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    if (t < 3) read(t + 1);
+#pragma unroll
+    for (int e = 0; e < C::KS; ++e) {
+      if constexpr (F8) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const u32x4 a = widen_e4m3<DT>(x[t & 1][e][2 * j], x[t & 1][e][2 * j + 1]);
+#pragma unroll
+          for (int r = 0; r < RT; ++r) sc[r][t] = mfma<DT>(a, q[r][2 * e + j], sc[r][t]);
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < RT; ++r) sc[r][t] = mfma<DT>(x[t & 1][e], q[r][e], sc[r][t]);
+      }
+    }
+    if constexpr (RT > 1) __builtin_amdgcn_sched_barrier(0);  // no more fragments at once: the registers are full
+  }
+}
+
+// Mask, online softmax and the two 16-bit terms of P.  `have`: how many of the
+// lane's 16 keys from kg on the sequence has (on a page); `f`: the scores'
+// factor, log2 e / sqrt(hd) and the K scale; `vs`: the V scale.
+template <int DT, bool F8, int HD, int RT>
+__device__ __forceinline__ void softmax(f32x4 (&sc)[RT][4], const int (&pos)[RT], int kg, int have, float f, float vs, float (&m)[RT],
+                                        float (&l)[RT], f32x4 (&o)[RT][HD / 16], u32x4 (&ph)[RT][2], u32x4 (&pl)[RT][2]) {
+  using C = Cfg<DT, F8, HD>;
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const int see = min(have, pos[r] + 1 - kg);
+    if (__builtin_amdgcn_ballot_w64(see < 16)) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (4 * t + e >= see) sc[r][t][e] = -INFINITY;
+    }
+    float x[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) x[t] = fmaxf(fmaxf(sc[r][t][0], sc[r][t][1]), fmaxf(sc[r][t][2], sc[r][t][3]));
+    const float bm = column_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * f);
+    if (__builtin_amdgcn_ballot_w64(bm > m[r] + kLazy)) {
+      const float mn = fmaxf(m[r], bm);
+      const float al = __builtin_amdgcn_exp2f(m[r] - (mn == -INFINITY ? 0.f : mn));
+      l[r] *= al;
+#pragma unroll
+      for (int d = 0; d < C::ND; ++d) o[r][d] *= al;
+      m[r] = mn;
+    }
+    const float mb = (m[r] == -INFINITY ? 0.f : m[r]) - C::kBias;
+    float sum[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      float w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r][t][e], f, -mb));
+      sum[t] = (w[0] + w[1]) + (w[2] + w[3]);
+      if constexpr (F8) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] *= vs;
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t hi = pack2<C::PV>(w[2 * e], w[2 * e + 1]);
+        ph[r][t >> 1][2 * (t & 1) + e] = hi;
+        pl[r][t >> 1][2 * (t & 1) + e] = residue2<C::PV>(hi, w[2 * e], w[2 * e + 1]);
+      }
+    }
+    l[r] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  }
+}
+
+// What a V tile holds behind the sequence's keys, or for no page, may be anything, NaN
+// too, and 0 * NaN is not 0: a lane clears those elements of the chunks that it
+// will read itself.
+template <int DT, bool F8, int HD>
+__device__ __forceinline__ void clear_tail(unsigned char* vt, const int (&va)[Cfg<DT, F8, HD>::VS], int lcp, int have) {
+  using C = Cfg<DT, F8, HD>;
+  uint32_t keep[C::VS * 4];
+#pragma unroll
+  for (int w = 0; w < C::VS * 4; ++w) {
+    const int n = have - w * (4 / C::ES);  // elements of word w that are keys
+    keep[w] = n >= 4 / C::ES ? ~0u : n <= 0 ? 0u : (1u << (8 * C::ES * n)) - 1;
+  }
+#pragma unroll 1
+  for (int d = 0; d < C::ND; ++d)
+#pragma unroll
+    for (int e = 0; e < C::VS; ++e) {
+      u32x4* x = reinterpret_cast<u32x4*>(vt + va[e] + (d * 256 << lcp));
+      *x &= u32x4{keep[4 * e], keep[4 * e + 1], keep[4 * e + 2], keep[4 * e + 3]};
+    }
+}
+
+// O^T += V^T.P^T of a block.
+template <int DT, bool F8, int HD, int RT>
+__device__ __forceinline__ void weigh(const unsigned char* vt, const int (&va)[Cfg<DT, F8, HD>::VS], int lcp, const u32x4 (&ph)[RT][2],
+                                      const u32x4 (&pl)[RT][2], f32x4 (&o)[RT][HD / 16]) {
+  using C = Cfg<DT, F8, HD>;
+  int at[C::VS];
+#pragma unroll
+  for (int e = 0; e < C::VS; ++e) {
+    at[e] = va[e];
+    asm volatile("" : "+v"(at[e]));
+  }
+  u32x4 x[2][C::VS];
+  auto read = [&](int d) {
+#pragma unroll
+    for (int e = 0; e < C::VS; ++e) x[d & 1][e] = *reinterpret_cast<const u32x4*>(vt + at[e] + (d * 256 << lcp));
+  };
+  read(0);
+#pragma unroll
+  for (int d = 0; d < C::ND; ++d) {
+    if (d + 1 < C::ND) read(d + 1);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      u32x4 a;
+      if constexpr (F8) a = widen_e4m3<QA_BF16>(x[d & 1][0][2 * j], x[d & 1][0][2 * j + 1]);
+      else a = x[d & 1][j];
+#pragma unroll
+      for (int r = 0; r < RT; ++r) o[r][d] = mfma<C::PV>(a, ph[r][j], o[r][d]);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) o[r][d] = mfma<C::PV>(a, pl[r][j], o[r][d]);
+    }
+    if constexpr (RT > 1) __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// The waves that worked on the same columns joined through LDS (in order), each with
+// ND / NS of the d tiles, and the result or its part written.  Group a = wave / GW
+// took a part of the keys, wave % GW the columns.
+template <int DT, bool F8, int HD, int RT, int GW, int NS>
+__device__ __forceinline__ void finish(const PagedAttnParams& p, const Split& sp, const SeqSpan& sq, int h, int R0, int part, bool whole,
+                                       float (&m)[RT], float (&l)[RT], const f32x4 (&o)[RT][HD / 16], unsigned char* smem) {
+  constexpr int ND = HD / 16, NM = ND / NS;
+  const int lane = threadIdx.x & 63, wave = scalar((int)(threadIdx.x >> 6)), g = lane >> 4, ns = wave / GW, wg = wave % GW;
+  Columns<RT> col;
+  col.set(p, sq, h, R0, lane & 15);
+  f32x4* xo = reinterpret_cast<f32x4*>(smem);                                        // [wave][RT][ND][64]
+  float* xs = reinterpret_cast<float*>(smem + (size_t)GW * NS * RT * ND * 64 * 16);  // [wave][RT][2][64]
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+#pragma unroll
+    for (int d = 0; d < ND; ++d) xo[((wave * RT + r) * ND + d) * 64 + lane] = o[r][d];
+    xs[(wave * RT + r) * 128 + lane] = m[r];
+    xs[(wave * RT + r) * 128 + 64 + lane] = column_sum(l[r]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    float mm = -INFINITY, al[NS], ll = 0.f;
+#pragma unroll
+    for (int a = 0; a < NS; ++a) {
+      al[a] = xs[((a * GW + wg) * RT + r) * 128 + lane];
+      mm = fmaxf(mm, al[a]);
+    }
+    const float mu = mm == -INFINITY ? 0.f : mm;
+    f32x4 w[NM] = {};
+#pragma unroll
+    for (int a = 0; a < NS; ++a) {
+      const int at = (a * GW + wg) * RT + r;
+      al[a] = __builtin_amdgcn_exp2f(al[a] - mu);
+      ll += xs[at * 128 + 64 + lane] * al[a];
+#pragma unroll
+      for (int d = 0; d < NM; ++d) w[d] += xo[(at * ND + ns * NM + d) * 64 + lane] * al[a];
+    }
+    if (!col.on[r]) continue;
+    if (whole) {
+      const float inv = ll == 0.f ? 0.f : 1.0f / ll;  // no key: zeros
+      uint16_t* dst = p.out + col.tok[r] * p.ldo + (int64_t)col.head[r] * HD + 4 * g;
+#pragma unroll
+      for (int d = 0; d < NM; ++d) {
+        const f32x4 y = w[d] * inv;
+        *reinterpret_cast<u32x2*>(dst + (ns * NM + d) * 16) = u32x2{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
+      }
+    } else {
+      const int64_t at = part_index(p, sp, col.tok[r], col.head[r], part);
+      float* dst = p.ws + at * HD + 4 * g;
+#pragma unroll
+      for (int d = 0; d < NM; ++d) *reinterpret_cast<f32x4*>(dst + (ns * NM + d) * 16) = w[d];
+      if (ns == 0 && g == 0) *reinterpret_cast<f32x2*>(part_stats(p, sp, HD) + at * 2) = (f32x2){mm, ll};
+    }
+  }
+}
+
+// Page ids, and e4m3 scales, of 16 blocks: lane 4 j + a those of the 16 keys from
+// key(j) + 16 a on.
+template <bool F8, class Key>
+__device__ __forceinline__ void fetch_ids(const PagedParams& kv, const SeqSpan& sq, int s, int h, int left, Key key, int* ids, float* ks,
+                                          float* vs) {
+  const int lane = threadIdx.x & 63, pos = key(lane >> 2) + 16 * (lane & 3);
+  *ids = (lane >> 2) < left && pos < sq.len ? page_at(kv, s, pos) : -1;
+  if constexpr (F8) {
+    const int64_t at = (int64_t)max(*ids, 0) * kv.nkvh + h;
+    const float x = kv.k_scale[at], y = kv.v_scale[at];
+    *ks = *ids < 0 ? 1.f : x;
+    *vs = *ids < 0 ? 0.f : y;
+  }
+}
+
+// Sequences of few rows: every wave has its own tiles, and waits for its own loads
+// alone.  K of the next block is under way while this one's softmax and P.V run, V
+// from P.V to P.V.  Block: kv head fastest, then part, then sequence.
+template <int DT, bool F8, int HD>
+constexpr int few_lds() {
+  constexpr int tiles = kFewWaves * 2 * Cfg<DT, F8, HD>::TILE, join = kFewWaves * 64 * (HD + 8);
+  return tiles > join ? tiles : join;
+}
+template <int DT, bool F8, int HD>
+__global__ void __launch_bounds__(64 * kFewWaves) paged_few_kernel(const PagedAttnParams p, const Split sp) {
+  using C = Cfg<DT, F8, HD>;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[few_lds<DT, F8, HD>()];
+  const PagedParams& kv = p.kv;
+  const int h = (int)(blockIdx.x % kv.nkvh);
+  const int part = (int)(blockIdx.x / kv.nkvh % sp.few_chunks), s = (int)(blockIdx.x / kv.nkvh / sp.few_chunks);
+  const SeqSpan sq = seq_span(kv, s);
+  if (sq.n == 0 || sq.n * p.rep > kFewRows) return;
+  const int end = sq.pos0 + sq.n;  // keys that the last row sees
+  const int k0 = part * sp.few_chunk, k1 = min(k0 + sp.few_chunk, end);
+  if (part > 0 && k0 >= end) return;
+  const int lane = threadIdx.x & 63, wave = scalar((int)(threadIdx.x >> 6)), c = lane & 15, g = lane >> 4;
+  const int nb = k1 > k0 ? (k1 - k0 + 63) >> 6 : 0, steps = (nb - wave + kFewWaves - 1) / kFewWaves;
+  auto key_of = [&](int it) { return k0 + (wave + it * kFewWaves) * 64; };
+  unsigned char *kt = smem + wave * 2 * C::TILE, *vt = kt + C::TILE;
+  const int lcp = kv.lp - (F8 ? 4 : 3);
+  int ids = -1;
+  float ksc = 1.f, vsc = 0.f;
+  auto fetch = [&](int it) {
+    fetch_ids<F8>(kv, sq, s, h, steps - it, [&](int j) { return key_of(it + j); }, &ids, &ksc, &vsc);
+  };
+  Columns<1> col;
+  col.set(p, sq, h, 0, c);
+  u32x4 q[1][C::QS];
+  load_q<DT, F8, HD, 1>(p, col, g, q);
+  if (steps > 0) {
+    fetch(0);
+    load_tile<DT, F8, HD, 1, true>(kv, h, ids, 0, 0, kt);
+    load_tile<DT, F8, HD, 1, false>(kv, h, ids, 0, 0, vt);
+  }
+  f32x4 o[1][C::ND] = {};
+  float m[1] = {-INFINITY}, l[1] = {0.f};
+  const int ka = k_frag<DT, F8, HD>(c, g);
+  int va[C::VS];
+#pragma unroll
+  for (int e = 0; e < C::VS; ++e) va[e] = v_frag<DT, F8, HD>(c, g, e, lcp);
+  for (int it = 0; it < steps; ++it) {
+    const bool more = it + 1 < steps;
+    const int kg = key_of(it) + 16 * g, src = (it & 15) * 4 + g;
+    const int have = __shfl(ids, src, 64) < 0 ? 0 : sq.len - kg;
+    float ks = 1.f, vs = 0.f;
+    if constexpr (F8) {
+      ks = __shfl(ksc, src, 64);
+      vs = __shfl(vsc, src, 64);
+    }
+    wait_vmcnt<C::LI>();  // K is there; V's loads came after it
+    f32x4 sc[1][4];
+    scores<DT, F8, HD, 1>(kt, ka, q, sc);
+    wait_lds();
+    if (more) {
+      if ((it & 15) == 15) fetch(it + 1);
+      load_tile<DT, F8, HD, 1, true>(kv, h, ids, (it + 1) & 15, 0, kt);
+    }
+    u32x4 ph[1][2], pl[1][2];
+    softmax<DT, F8, HD, 1>(sc, col.pos, kg, have, p.scale * kLog2e * ks, vs, m, l, o, ph, pl);
+    if (more) wait_vmcnt<C::LI>();  // V is there; the next K's loads came after it
+    else wait_vmcnt<0>();
+    if (__builtin_amdgcn_ballot_w64(have < 16)) clear_tail<DT, F8, HD>(vt, va, lcp, have);
+    weigh<DT, F8, HD, 1>(vt, va, lcp, ph, pl, o);
+    wait_lds();
+    if (more) load_tile<DT, F8, HD, 1, false>(kv, h, ids, (it + 1) & 15, 0, vt);
+  }
+  __syncthreads();  // the tiles' LDS is the join's
+  finish<DT, F8, HD, 1, 1, kFewWaves>(p, sp, sq, h, 0, part, end <= sp.few_chunk, m, l, o, smem);
+}
+
+// Tiles of 64 (row, head) pairs: NS key splits of GW waves with 32 columns each.  A
+// split's waves share its tiles.  A step is an MFMA phase (P.V of the block before,
+// S of this one) and a VALU phase (softmax, the next loads); every phase ends in
+// a block barrier, and the upper half of the splits runs one phase behind the
+// lower, so that of the two waves on a SIMD one multiplies while the other is at
+// its softmax.
+__device__ __forceinline__ void phase_barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+template <int DT, bool F8, int HD, int GW>
+constexpr int many_buffers() {  // buffers of each tile: two where 128 KB hold them
+  return kManyWaves / GW * 2 * Cfg<DT, F8, HD>::TILE * 2 <= 131072 ? 2 : 1;
+}
+template <int DT, bool F8, int HD, int GW>
+constexpr int many_lds() {
+  constexpr int tiles = kManyWaves / GW * 2 * Cfg<DT, F8, HD>::TILE * many_buffers<DT, F8, HD, GW>();
+  constexpr int join = kManyWaves * 2 * 64 * (HD + 8);
+  return tiles > join ? tiles : join;
+}
+template <int DT, bool F8, int HD, int GW>
+__global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const PagedAttnParams p, const Split sp) {
+  using C = Cfg<DT, F8, HD>;
+  constexpr int RT = 2, NS = kManyWaves / GW, NB = many_buffers<DT, F8, HD, GW>(), WL = C::LI / GW;  // WL: a wave's loads of a tile
+  constexpr int TR = GW * RT * 16;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[many_lds<DT, F8, HD, GW>()];
+  const PagedParams& kv = p.kv;
+  const int h = (int)(blockIdx.x % kv.nkvh);
+  const int64_t b = blockIdx.x / kv.nkvh;
+  const int per = sp.tiles * sp.many_chunks, u = (int)(b % per), s = (int)(b / per);
+  const SeqSpan sq = seq_span(kv, s);
+  const int NR = sq.n * p.rep;
+  if (NR == 0 || (sp.few && NR <= kFewRows)) return;
+  // the last tiles, which see the most keys, first
+  const int tile = (NR + TR - 1) / TR - 1 - u % sp.tiles, part = u / sp.tiles;
+  if (tile < 0) return;
+  const int end = sq.pos0 + (min((tile + 1) * TR, NR) - 1) / p.rep + 1;
+  const int k0 = part * sp.many_chunk, k1 = min(k0 + sp.many_chunk, end);
+  if (part > 0 && k0 >= end) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+  const int ns = wave / GW, wg = wave % GW, off = ns / (NS / 2);
+  const int nb = k1 > k0 ? (k1 - k0 + 63) >> 6 : 0, steps = (nb - ns + NS - 1) / NS;
+  auto key_of = [&](int it) { return k0 + (ns + it * NS) * 64; };
+  // (the wave's number is left to the compiler as a lane's value: with scalar
+  // control flow it spills; what a DMA instruction takes is made scalar below)
+  unsigned char* base = smem + ns * 2 * NB * C::TILE;
+  auto kt = [&](int it) { return base + (it & (NB - 1)) * C::TILE; };
+  auto vt = [&](int it) { return base + (NB + (it & (NB - 1))) * C::TILE; };
+  const int lcp = kv.lp - (F8 ? 4 : 3);
+  // two windows of 16 blocks' ids: loads run up to two blocks ahead of the softmax
+  int ids0 = -1, ids1 = -1;
+  float ks0 = 1.f, ks1 = 1.f, vs0 = 0.f, vs1 = 0.f;
+  auto fetch = [&](int w) {
+    int id = -1;
+    float x = 1.f, y = 0.f;
+    fetch_ids<F8>(kv, sq, s, h, steps - 16 * w, [&](int j) { return key_of(16 * w + j); }, &id, &x, &y);
+    ids0 = w & 1 ? ids0 : id;
+    ks0 = w & 1 ? ks0 : x;
+    vs0 = w & 1 ? vs0 : y;
+    ids1 = w & 1 ? id : ids1;
+    ks1 = w & 1 ? x : ks1;
+    vs1 = w & 1 ? y : vs1;
+  };
+  auto ids_of = [&](int it) { return it >> 4 & 1 ? ids1 : ids0; };
+  auto issue_k = [&](int it) { load_tile<DT, F8, HD, GW, true>(kv, h, ids_of(it), scalar(it & 15), scalar(wg), smem + scalar((int)(kt(it) - smem))); };
+  auto issue_v = [&](int it) { load_tile<DT, F8, HD, GW, false>(kv, h, ids_of(it), scalar(it & 15), scalar(wg), smem + scalar((int)(vt(it) - smem))); };
+  // refill(j), in step j's VALU phase: K of block j + NB (S of j has read its slot),
+  // V of block j + NB - 1 (P.V of j - 1 has).  Step i's MFMA phase needs K(i) and
+  // V(i - 1), of refill(i - NB): with two buffers refill(i - 1) may be under way.
+  auto ahead = [&](int j) { return NB == 1 ? 0 : (j + 2 < steps) + (j + 1 < steps); };
+  auto wait_ahead = [&](int j) {
+    const int n = ahead(j);
+    if (n == 2) wait_vmcnt<2 * WL>();
+    else if (n == 1) wait_vmcnt<WL>();
+    else wait_vmcnt<0>();
+  };
+  Columns<RT> col;
+  col.set(p, sq, h, (tile * GW + wg) * RT * 16, c);
+  u32x4 q[RT][C::QS];
+  load_q<DT, F8, HD, RT>(p, col, g, q);
+  if (steps > 0) {
+    fetch(0);
+    if (steps > 16) fetch(1);
+    issue_k(0);
+    if (NB == 2 && steps > 1) issue_k(1);
+    if (NB == 2) issue_v(0);
+  }
+  f32x4 o[RT][C::ND] = {};
   float m[RT], l[RT];
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     m[r] = -INFINITY;
     l[r] = 0.f;
   }
-  const int pmask = (1 << kv.lp) - 1;
-  const int gk = c >> 2;  // the 16-key group that this lane's K rows are in
-  auto key_of = [&](int it) { return k0 + (wk + it * WK) * 64; };
-  auto id_of = [&](int pos) { return pos < sq.len ? page_at(kv, s, pos) : -1; };
-  u32x4 kr[4][KS], vr[ND][VS];
-  float ks = 1.f, vs = 0.f;
-  auto load_k = [&](int it, int id) {
-    const int64_t at = page_base(kv, max(id, 0), h, HD) + (int64_t)(((key_of(it) + 16 * gk) & pmask) + (c & 3)) * HD + g * E16;
-    const unsigned char* src = (const unsigned char*)kv.k + at * ES;
+  f32x4 sc[RT][4];
+  u32x4 ph[RT][2], pl[RT][2];
+  const int ka = k_frag<DT, F8, HD>(c, g);
+  int va[C::VS];
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int e = 0; e < KS; ++e) kr[t][e] = *reinterpret_cast<const u32x4*>(src + 4 * t * HD * ES + e * 64);
-  };
-  auto load_v = [&](int it, int id) {
-    const int64_t at = page_base(kv, max(id, 0), h, HD) + ((int64_t)c << kv.lp) + ((key_of(it) + 16 * g) & pmask);
-    const unsigned char* src = (const unsigned char*)kv.v + at * ES;
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-      for (int e = 0; e < VS; ++e) vr[d][e] = *reinterpret_cast<const u32x4*>(src + (((int64_t)d * 16 << kv.lp) * ES + e * 16));
-  };
-  auto load_scales = [&](int id, float* a, float* b) {
-    if constexpr (F8) {
-      const int64_t at = (int64_t)max(id, 0) * kv.nkvh + h;
-      const float x = kv.k_scale[at], y = kv.v_scale[at];
-      *a = id < 0 ? 1.f : x;
-      *b = id < 0 ? 0.f : y;
-    }
-  };
-
-  int idk = -1, idv = -1, idk1 = -1, idv1 = -1;
-  float ks1 = 1.f, vs1 = 0.f;
-  if (steps > 0) {
-    idk = id_of(key_of(0) + 16 * gk);
-    idv = id_of(key_of(0) + 16 * g);
-    if (steps > 1) {
-      idk1 = id_of(key_of(1) + 16 * gk);
-      idv1 = id_of(key_of(1) + 16 * g);
-    }
-    load_k(0, idk);
-    load_v(0, idv);
-    load_scales(idv, &ks, &vs);
-  }
-  for (int it = 0; it < steps; ++it) {
-    const int kg = key_of(it) + 16 * g;  // the lane's first key
-    // S = K.Q^T
-    f32x4 sc[RT][4] = {};
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int e = 0; e < QS; ++e) {
-        u32x4 a;
-        if constexpr (F8) a = widen_e4m3<DT>(kr[t][e >> 1][2 * (e & 1)], kr[t][e >> 1][2 * (e & 1) + 1]);
-        else a = kr[t][e];
-#pragma unroll
-        for (int r = 0; r < RT; ++r) sc[r][t] = mfma<DT>(a, q[r][e], sc[r][t]);
-      }
-    // the next block's K, and the page ids of the one after
-    const int idv_now = idv;
-    if (it + 1 < steps) {
-      load_k(it + 1, idk1);
-      load_scales(idv1, &ks1, &vs1);
-      idk = idk1;
-      idv = idv1;
-      if (it + 2 < steps) {
-        idk1 = id_of(key_of(it + 2) + 16 * gk);
-        idv1 = id_of(key_of(it + 2) + 16 * g);
-      }
-    }
-    // keys of the lane that the sequence has; what lies behind them, or on no
-    // page, may hold anything, NaN too, and 0 * NaN is not 0
-    const int have = idv_now < 0 ? 0 : sq.len - kg;
-    const float f = p.scale * kLog2e * ks;
-    u32x4 ph[RT][2], pl[RT][2];
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      const int see = min(have, pos[r] + 1 - kg);
-      if (__builtin_amdgcn_ballot_w64(see < 16)) {
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (4 * t + e >= see) sc[r][t][e] = -INFINITY;
-      }
-      float x[4];
-#pragma unroll
-      for (int t = 0; t < 4; ++t) x[t] = fmaxf(fmaxf(sc[r][t][0], sc[r][t][1]), fmaxf(sc[r][t][2], sc[r][t][3]));
-      const float bm = column_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * f);
-      if (__builtin_amdgcn_ballot_w64(bm > m[r] + kLazy)) {
-        const float mn = fmaxf(m[r], bm);
-        const float al = __builtin_amdgcn_exp2f(m[r] - (mn == -INFINITY ? 0.f : mn));
-        l[r] *= al;
-#pragma unroll
-        for (int d = 0; d < ND; ++d) o[r][d] *= al;
-        m[r] = mn;
-      }
-      const float mb = (m[r] == -INFINITY ? 0.f : m[r]) - kBias;
-      float sum[4];
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        float w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r][t][e], f, -mb));
-        sum[t] = (w[0] + w[1]) + (w[2] + w[3]);
+  for (int e = 0; e < C::VS; ++e) va[e] = v_frag<DT, F8, HD>(c, g, e, lcp);
+  int have = 16;  // the lane's keys in the block of the last softmax
+  const int n0 = (nb + NS - 1) / NS, n1 = (nb + NS / 2 - 1) / NS;  // most steps of either half
+  const int phases = max(2 * n0 + 1, 2 * n1 + 2);
+  if (off == 0) wait_vmcnt<0>();
+  phase_barrier();
+  for (int ph_no = 0; ph_no < phases; ++ph_no) {
+    const int my = ph_no - off, it = my >> 1;
+    if (my >= 0 && my <= 2 * steps) {
+      if ((my & 1) == 0) {
+        if (it > 0) {
+          if (__builtin_amdgcn_ballot_w64(have < 16)) clear_tail<DT, F8, HD>(vt(it - 1), va, lcp, have);
+          weigh<DT, F8, HD, RT>(vt(it - 1), va, lcp, ph, pl, o);
+        }
+        if (it < steps) scores<DT, F8, HD, RT>(kt(it), ka, q, sc);
+      } else {
+        const int kg = key_of(it) + 16 * g, src = (it & 15) * 4 + g;
+        have = __shfl(ids_of(it), src, 64) < 0 ? 0 : sq.len - kg;
+        float ks = 1.f, vs = 0.f;
         if constexpr (F8) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] *= vs;
+          ks = __shfl(it >> 4 & 1 ? ks1 : ks0, src, 64);
+          vs = __shfl(it >> 4 & 1 ? vs1 : vs0, src, 64);
         }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint32_t hi = pack2<PV>(w[2 * e], w[2 * e + 1]);
-          const f32x2 b = unpack2<PV>(hi);
-          ph[r][t >> 1][2 * (t & 1) + e] = hi;
-          pl[r][t >> 1][2 * (t & 1) + e] = pack2<PV>(w[2 * e] - b[0], w[2 * e + 1] - b[1]);
-        }
-      }
-      l[r] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    }
-    if (__builtin_amdgcn_ballot_w64(have < 16)) {
-#pragma unroll
-      for (int w = 0; w < VS * 4; ++w) {
-        const int n = have - w * (4 / ES);  // elements of word w that are keys
-        const uint32_t mask = n >= 4 / ES ? ~0u : n <= 0 ? 0u : (1u << (8 * ES * n)) - 1;
-#pragma unroll
-        for (int d = 0; d < ND; ++d) vr[d][w >> 2][w & 3] &= mask;
+        if (it > 0 && (it & 15) == 0 && 16 * (it >> 4) + 16 < steps) fetch((it >> 4) + 1);
+        if (it + NB < steps) issue_k(it + NB);
+        if (it + NB - 1 < steps) issue_v(it + NB - 1);
+        softmax<DT, F8, HD, RT>(sc, col.pos, kg, have, p.scale * kLog2e * ks, vs, m, l, o, ph, pl);
       }
     }
-    // O^T += V^T.P^T
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        u32x4 a;
-        if constexpr (F8) a = widen_e4m3<QA_BF16>(vr[d][0][2 * j], vr[d][0][2 * j + 1]);
-        else a = vr[d][j];
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          o[r][d] = mfma<PV>(a, ph[r][j], o[r][d]);
-          o[r][d] = mfma<PV>(a, pl[r][j], o[r][d]);
-        }
-      }
-    if (it + 1 < steps) load_v(it + 1, idv);
-    ks = ks1;
-    vs = vs1;
+    const int next = ph_no + 1 - off;
+    if (next >= 0 && (next & 1) == 0 && (next >> 1) <= steps) wait_ahead((next >> 1) - 1);
+    wait_lds();
+    phase_barrier();
   }
-
-#pragma unroll
-  for (int r = 0; r < RT; ++r) l[r] = column_sum(l[r]);
-  // this wave's d tiles of the block's result, joined over the WK waves in order
-  constexpr int NM = ND / WK;
-  f32x4 w[RT][NM];
-  if constexpr (WK > 1) {
-    f32x4* xo = reinterpret_cast<f32x4*>(smem);                                         // [wave][RT][ND][64]
-    float* xs = reinterpret_cast<float*>(smem + (size_t)WQ * WK * RT * ND * 64 * 16);   // [wave][RT][2][64]
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-#pragma unroll
-      for (int d = 0; d < ND; ++d) xo[((wave * RT + r) * ND + d) * 64 + lane] = o[r][d];
-      xs[((wave * RT + r) * 2) * 64 + lane] = m[r];
-      xs[((wave * RT + r) * 2 + 1) * 64 + lane] = l[r];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      float mm = -INFINITY;
-      for (int a = 0; a < WK; ++a) mm = fmaxf(mm, xs[(((wq * WK + a) * RT + r) * 2) * 64 + lane]);
-      const float mu = mm == -INFINITY ? 0.f : mm;
-      float ll = 0.f;
-#pragma unroll
-      for (int d = 0; d < NM; ++d) w[r][d] = f32x4{0, 0, 0, 0};
-      for (int a = 0; a < WK; ++a) {
-        const int at = (wq * WK + a) * RT + r;
-        const float al = __builtin_amdgcn_exp2f(xs[at * 2 * 64 + lane] - mu);
-        ll += xs[(at * 2 + 1) * 64 + lane] * al;
-#pragma unroll
-        for (int d = 0; d < NM; ++d) w[r][d] += xo[(at * ND + wk * NM + d) * 64 + lane] * al;
-      }
-      m[r] = mm;
-      l[r] = ll;
-    }
-  } else {
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-#pragma unroll
-      for (int d = 0; d < NM; ++d) w[r][d] = o[r][d];
-  }
-  // the tile's keys are one chunk: the result; else its part of it
-  const int last = min((tile + 1) * WQ * RT * 16, NR) - 1;
-  const bool whole = sq.pos0 + last / p.rep + 1 <= chunk;
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    if (R0 + r * 16 + c >= NR) continue;
-    if (whole) {
-      const float inv = l[r] == 0.f ? 0.f : 1.0f / l[r];  // no key: zeros
-      uint16_t* dst = p.out + tok[r] * p.ldo + (int64_t)head[r] * HD + 4 * g;
-#pragma unroll
-      for (int d = 0; d < NM; ++d) {
-        const f32x4 y = w[r][d] * inv;
-        *reinterpret_cast<u32x2*>(dst + (wk * NM + d) * 16) = u32x2{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
-      }
-    } else {
-      const int64_t at = part_index(p, sp, tok[r], head[r], part);
-      float* dst = p.ws + at * HD + 4 * g;
-#pragma unroll
-      for (int d = 0; d < NM; ++d) *reinterpret_cast<f32x4*>(dst + (wk * NM + d) * 16) = w[r][d];
-      if (wk == 0 && g == 0) {
-        float* st = part_stats(p, sp, HD) + at * 2;
-        st[0] = m[r];
-        st[1] = l[r];
-      }
-    }
-  }
+  finish<DT, F8, HD, RT, GW, NS>(p, sp, sq, h, (tile * GW + wg) * RT * 16, part, end <= sp.many_chunk, m, l, o, smem);
 }
 
-template <int HD, int RT, int WQ, int WK>
-constexpr int body_lds() {
-  return WK > 1 ? WQ * WK * RT * 64 * (HD / 16 * 16 + 8) : 16;
-}
-
-// Block -> kv head fastest (with 8 of them a head's blocks share an XCD's L2), then
-// unit, then sequence.  A sequence's units are its chunks, or its tiles times
-// their chunks, the last tiles (the longest) first.
-template <int DT, bool F8, int HD, bool MANY>
-__global__ void __launch_bounds__(256, MANY ? 1 : 2) paged_attention_kernel(const PagedAttnParams p, const Split sp) {
-  __shared__ __attribute__((aligned(16))) unsigned char smem[body_lds<HD, 1, 1, 4>()];
-  const int h = (int)(blockIdx.x % p.kv.nkvh);
-  const int u = (int)(blockIdx.x / p.kv.nkvh % sp.units), s = (int)(blockIdx.x / p.kv.nkvh / sp.units);
-  const SeqSpan sq = seq_span(p.kv, s);
-  if (sq.n == 0) return;
-  const int NR = sq.n * p.rep;
-  if (!MANY || NR <= kFewRows) {
-    if (u >= sp.few_chunks || (u > 0 && u * sp.few_chunk >= sq.pos0 + sq.n)) return;
-    tile_body<DT, F8, HD, 1, 1, 4>(p, sp, sq, s, h, 0, u, sp.few_chunk, smem);
-  } else {
-    constexpr int tr = 16 * kManyRT * kManyWQ;
-    const int tiles = (NR + tr - 1) / tr;
-    const int tile = tiles - 1 - u % sp.tiles, part = u / sp.tiles;
-    if (tile < 0 || part >= sp.many_chunks) return;
-    const int last = min((tile + 1) * tr, NR) - 1;
-    if (part > 0 && part * sp.many_chunk >= sq.pos0 + last / p.rep + 1) return;
-    tile_body<DT, F8, HD, kManyRT, kManyWQ, 1>(p, sp, sq, s, h, tile, part, sp.many_chunk, smem);
-  }
-}
-
-// The parts of a row and head joined: one wave each, HD / 64 elements a lane.
+// The parts of a (row, head) pair joined (the first `pairs` of each sequence and kv head): a block each, HD / 4 threads to a part, so
+// that 8 (hd 128) or 16 (hd 64) parts load at once and each thread has four of
+// those rounds in flight; the partial sums then meet in LDS.
 template <int DT, int HD>
-__global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p, const Split sp) {
-  const int lane = threadIdx.x & 63;
-  const int64_t b = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int head = (int)(b % p.nqh);
-  const int64_t si = b / p.nqh;
-  const int s = (int)(si / p.kv.max_rows), i = (int)(si % p.kv.max_rows);
-  if (s >= p.kv.seqs) return;
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p, const Split sp, int pairs) {
+  constexpr int TP = HD / 4, NP = 256 / TP;  // threads to a part, parts at once
+  __shared__ f32x4 xo[NP][TP];
+  __shared__ float xs[NP];
+  const int h = (int)(blockIdx.x % p.kv.nkvh);
+  const int64_t b = blockIdx.x / p.kv.nkvh;
+  const int s = (int)(b / pairs), R = (int)(b % pairs);
   const SeqSpan sq = seq_span(p.kv, s);
-  if (i >= sq.n) return;
-  const int NR = sq.n * p.rep, R = i * p.rep + head % p.rep;
-  const bool few = NR <= kFewRows;
-  constexpr int tr = 16 * kManyRT * kManyWQ;
-  const int last = few ? NR - 1 : min((R / tr + 1) * tr, NR) - 1;
+  const int NR = sq.n * p.rep;
+  if (R >= NR) return;
+  const int i = R / p.rep, head = h * p.rep + R % p.rep;
+  const bool few = sp.few && NR <= kFewRows;
+  const int last = few ? NR - 1 : min((R / kManyRows + 1) * kManyRows, NR) - 1;
   const int chunk = few ? sp.few_chunk : sp.many_chunk, keys = sq.pos0 + last / p.rep + 1;
   if (keys <= chunk) return;  // its tile has written the result
   const int parts = (keys + chunk - 1) / chunk;
   const int64_t t = sq.row0 + i, at = part_index(p, sp, t, head, 0);
   const float* st = part_stats(p, sp, HD) + at * 2;
+  const int lane = threadIdx.x & 63, pt = threadIdx.x / TP, d = threadIdx.x % TP;
   float mm = -INFINITY;
   for (int a = lane; a < parts; a += 64) mm = fmaxf(mm, st[2 * a]);
 #pragma unroll
   for (int e = 32; e > 0; e >>= 1) mm = fmaxf(mm, __shfl_xor(mm, e, 64));
   const float mu = mm == -INFINITY ? 0.f : mm;
-  float ll = 0.f, y[HD / 64] = {};
-  const float* src = p.ws + at * HD + lane * (HD / 64);
-  for (int a = 0; a < parts; ++a) {
-    const float al = __builtin_amdgcn_exp2f(st[2 * a] - mu);
-    ll += st[2 * a + 1] * al;
+  float ll = 0.f;
+  f32x4 y = {0, 0, 0, 0};
+  const float* src = p.ws + at * HD + d * 4;
+  for (int a0 = pt; a0 < parts; a0 += 4 * NP) {
+    f32x4 v[4];
+    f32x2 ml[4];
 #pragma unroll
-    for (int e = 0; e < HD / 64; ++e) y[e] += src[(int64_t)a * HD + e] * al;
+    for (int e = 0; e < 4; ++e) {
+      const int a = min(a0 + e * NP, parts - 1);
+      v[e] = *reinterpret_cast<const f32x4*>(src + (int64_t)a * HD);
+      ml[e] = *reinterpret_cast<const f32x2*>(st + 2 * a);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float al = a0 + e * NP < parts ? __builtin_amdgcn_exp2f(ml[e][0] - mu) : 0.f;
+      ll += ml[e][1] * al;
+      y += v[e] * al;
+    }
   }
-  const float inv = ll == 0.f ? 0.f : 1.0f / ll;
-  uint16_t* dst = p.out + t * p.ldo + (int64_t)head * HD + lane * (HD / 64);
-  if constexpr (HD == 128) *reinterpret_cast<uint32_t*>(dst) = pack2<DT>(y[0] * inv, y[1] * inv);
-  else *dst = (uint16_t)pack2<DT>(y[0] * inv, 0.f);
+  xo[pt][d] = y;
+  if (d == 0) xs[pt] = ll;
+  __syncthreads();
+  if (pt > 0) return;
+  for (int e = 1; e < NP; ++e) {
+    y += xo[e][d];
+    ll += xs[e];
+  }
+  y *= ll == 0.f ? 0.f : 1.0f / ll;
+  *reinterpret_cast<u32x2*>(p.out + t * p.ldo + (int64_t)head * HD + d * 4) = u32x2{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
+}
+
+// Pairs of a sequence and kv head that may come in parts.
+int64_t join_pairs(const PagedAttnParams& p, const Split& sp) {
+  const int64_t rows = (int64_t)p.kv.max_rows * p.rep;
+  return sp.many_chunks > 1 || rows < kFewRows ? rows : kFewRows;
 }
 
 template <int DT, bool F8, int HD>
 hipError_t launch_one(const PagedAttnParams& p, hipStream_t s) {
   const Split sp = split_of(p);
-  const dim3 grid((unsigned)((int64_t)p.kv.seqs * p.kv.nkvh * sp.units));
-  if (sp.tiles) hipLaunchKernelGGL((paged_attention_kernel<DT, F8, HD, true>), grid, dim3(256), 0, s, p, sp);
-  else hipLaunchKernelGGL((paged_attention_kernel<DT, F8, HD, false>), grid, dim3(256), 0, s, p, sp);
+  const int64_t heads = (int64_t)p.kv.seqs * p.kv.nkvh;
+  if (sp.many)
+    hipLaunchKernelGGL((paged_many_kernel<DT, F8, HD, 2>), dim3((unsigned)(heads * sp.tiles * sp.many_chunks)), dim3(64 * kManyWaves), 0,
+                       s, p, sp);
+  if (sp.few)
+    hipLaunchKernelGGL((paged_few_kernel<DT, F8, HD>), dim3((unsigned)(heads * sp.few_chunks)), dim3(64 * kFewWaves), 0, s, p, sp);
   if (sp.parts > 1) {
-    const int64_t rows = (int64_t)p.kv.seqs * p.kv.max_rows * p.nqh;
-    hipLaunchKernelGGL((paged_join_kernel<DT, HD>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, p, sp);
+    const int64_t pairs = join_pairs(p, sp);
+    hipLaunchKernelGGL((paged_join_kernel<DT, HD>), dim3((unsigned)(heads * pairs)), dim3(256), 0, s, p, sp, (int)pairs);
   }
   return hipGetLastError();
 }
@@ -485,9 +851,9 @@ hipError_t launch_dt(bool e4m3, int hd, const PagedAttnParams& p, hipStream_t s)
 
 int64_t paged_attention_blocks(const PagedAttnParams& p) {
   const Split sp = split_of(p);
-  const int64_t rows = (int64_t)p.kv.seqs * p.kv.max_rows, blocks = (int64_t)p.kv.seqs * p.kv.nkvh;
-  // saturating: the caller compares with a bound far below
-  const double most = (double)rows * p.nqh > (double)blocks * sp.units ? (double)rows * p.nqh : (double)blocks * sp.units;
+  // in doubles, as no product of these sizes need fit 64 bits; the caller compares with a bound far below
+  const double heads = (double)p.kv.seqs * p.kv.nkvh, rows = (double)p.kv.max_rows * p.rep;
+  const double most = heads * fmax(fmax((double)sp.tiles * sp.many_chunks, sp.few_chunks), rows);
   return most > 9e18 ? INT64_MAX : (int64_t)most;
 }
 
