@@ -146,11 +146,12 @@ struct Cfg {
 //    own.
 //  * many: tiles of kManyRows pairs.
 constexpr int kFewRows = 16, kFewWaves = 4;
-constexpr int kManyRows = 64, kManyWaves = 8;
+constexpr int kManyWaves = 8;
 struct Split {
   int few, many;                // which of the two kernels run
   int few_chunk, few_chunks;    // keys of a part, parts of the longest sequence
   int many_chunk, many_chunks;
+  int many_rows;                // pairs of a tile
   int tiles;                    // tiles of the longest sequence of `many`
   int parts;                    // partial results per row; 1: no workspace
 };
@@ -175,7 +176,9 @@ Split split_of(const PagedAttnParams& p) {
   s.few_chunks = s.many_chunks = 1;
   if (s.few) divide(heads, W, Lc, &s.few_chunk, &s.few_chunks);
   if (s.many) {
-    s.tiles = (int)((rows + kManyRows - 1) / kManyRows);
+    static const int GWE=getenv("QA_GW")?atoi(getenv("QA_GW")):2;
+    s.many_rows = 32 * GWE;
+    s.tiles = (int)((rows + s.many_rows - 1) / s.many_rows);
     divide(heads * s.tiles, MW, ML, &s.many_chunk, &s.many_chunks);
   }
   s.parts = s.many_chunks > s.few_chunks ? s.many_chunks : s.few_chunks;
@@ -222,6 +225,16 @@ __device__ __forceinline__ void load_q(const PagedAttnParams& p, const Columns<R
   }
 }
 
+// The compiler waits here for q's loads, not at their use in the loop, where the
+// tiles' loads would be waited for with them.
+template <int RT, int QS>
+__device__ __forceinline__ void keep(u32x4 (&q)[RT][QS]) {
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int e = 0; e < QS; ++e) asm volatile("" : "+v"(q[r][e]));
+}
+
 // A 64-key block's K and V tiles in LDS.  K: 64 rows of CR chunks; V: the block's
 // pages one after the other, each HD rows of CP chunks.  Both are copies of the
 // pages but for the order of chunks within a row: chunk ^ f(row), with f such that
@@ -242,8 +255,12 @@ __device__ __forceinline__ int v_swizzle(int c, int lcp) {
 // A DMA instruction copies 1 KB; those of a tile are dealt out to OF waves, of which
 // this is `mine`.  A page's are a run of PER, and what they add to the page's and the
 // tile's address is the same, so it goes into the instruction.  Pages that are
-// none come as zeros (a resource of no bytes).  ids: lane 4 j + a holds the page of
-// keys 16 a .. of block j.
+// none come as zeros (a resource of no bytes).  Pages: lane 4 j + a holds where the
+// page of keys 16 a .. of block j begins, in bytes from either pool's start, or a
+// negative number.
+struct Pages {
+  int lo, hi;
+};
 template <int OF, int PER, class Off>
 __device__ __forceinline__ void copy_page(const unsigned char* src, int bytes, unsigned char* to, int mine, Off off) {
   const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(src), (short)0, bytes, 0x00020000);
@@ -263,7 +280,7 @@ __device__ __forceinline__ void copy_page(const unsigned char* src, int bytes, u
   }
 }
 template <int DT, bool F8, int HD, int OF, int LP, bool K>
-__device__ __forceinline__ void load_pages(const PagedParams& kv, int h, int ids, int j, int mine, unsigned char* to) {
+__device__ __forceinline__ void load_pages(const PagedParams& kv, const Pages& pages, int j, int mine, unsigned char* to) {
   using C = Cfg<DT, F8, HD>;
   constexpr int PER = C::LI >> (6 - LP), PB = HD * C::ES << LP;  // instructions and bytes of a page
   constexpr int CW = K ? C::CR : (1 << LP) * C::ES / 16;          // chunks of a row
@@ -281,10 +298,10 @@ __device__ __forceinline__ void load_pages(const PagedParams& kv, int h, int ids
   };
   auto off_v = [&](int n) { return lane_off ^ (uint32_t)(!F8 && CW == 8 ? (n & 1) << 6 : 0); };
   auto page_src = [&](int pg, int* bytes) {
-    const int id = __builtin_amdgcn_readlane(ids, j * 4 + (pg << (LP - 4)));
-    *bytes = id < 0 ? 0 : PB;
-    const uint64_t at = ((uint64_t)(uint32_t)max(id, 0) * (uint32_t)kv.nkvh + (uint32_t)h) * PB;
-    return (const unsigned char*)(K ? kv.k : kv.v) + at;
+    const int lo = __builtin_amdgcn_readlane(pages.lo, j * 4 + (pg << (LP - 4)));
+    const int hi = __builtin_amdgcn_readlane(pages.hi, j * 4 + (pg << (LP - 4)));
+    *bytes = hi < 0 ? 0 : PB;
+    return (const unsigned char*)(K ? kv.k : kv.v) + ((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
   };
   if constexpr (PER >= OF) {
 #pragma unroll
@@ -311,10 +328,10 @@ __device__ __forceinline__ void load_pages(const PagedParams& kv, int h, int ids
   }
 }
 template <int DT, bool F8, int HD, int OF, bool K>
-__device__ __forceinline__ void load_tile(const PagedParams& kv, int h, int ids, int j, int mine, unsigned char* to) {
-  if (kv.lp == 6) load_pages<DT, F8, HD, OF, 6, K>(kv, h, ids, j, mine, to);
-  else if (kv.lp == 5) load_pages<DT, F8, HD, OF, 5, K>(kv, h, ids, j, mine, to);
-  else load_pages<DT, F8, HD, OF, 4, K>(kv, h, ids, j, mine, to);
+__device__ __forceinline__ void load_tile(const PagedParams& kv, const Pages& pages, int j, int mine, unsigned char* to) {
+  if (kv.lp == 6) load_pages<DT, F8, HD, OF, 6, K>(kv, pages, j, mine, to);
+  else if (kv.lp == 5) load_pages<DT, F8, HD, OF, 5, K>(kv, pages, j, mine, to);
+  else load_pages<DT, F8, HD, OF, 4, K>(kv, pages, j, mine, to);
 }
 // Fragment addresses in the tiles.  K: product t reads row 16 (c / 4) + 4 t + c % 4,
 // slice e the chunk 4 e + g.  V: row d, the chunks of keys 16 g ..
@@ -327,44 +344,6 @@ template <int DT, bool F8, int HD>
 __device__ __forceinline__ int v_frag(int c, int g, int e, int lcp) {
   const int x = g * Cfg<DT, F8, HD>::VS + e;  // the block's chunk x of this row
   return ((((x >> lcp) * HD + c) << lcp) + ((x & ((1 << lcp) - 1)) ^ v_swizzle<F8>(c, lcp))) * 16;
-}
-
-// S = K.Q^T of a block.  (The empty statements here and in weigh() keep the
-// fragments' addresses from being formed outside the loop and held there.)
-template <int DT, bool F8, int HD, int RT>
-__device__ __forceinline__ void scores(const unsigned char* kt, int ka, const u32x4 (&q)[RT][HD / 32], f32x4 (&sc)[RT][4]) {
-  using C = Cfg<DT, F8, HD>;
-  asm volatile("" : "+v"(ka));
-#pragma unroll
-  for (int r = 0; r < RT; ++r)
-#pragma unroll
-    for (int t = 0; t < 4; ++t) sc[r][t] = f32x4{0, 0, 0, 0};
-  // product t + 1's fragments are read while product t multiplies
-  u32x4 x[2][C::KS];
-  auto read = [&](int t) {
-#pragma unroll
-    for (int e = 0; e < C::KS; ++e) x[t & 1][e] = *reinterpret_cast<const u32x4*>(kt + (ka ^ (e << 6)) + 4 * t * C::CR * 16);
-  };
-  read(0);
-#pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    if (t < 3) read(t + 1);
-#pragma unroll
-    for (int e = 0; e < C::KS; ++e) {
-      if constexpr (F8) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const u32x4 a = widen_e4m3<DT>(x[t & 1][e][2 * j], x[t & 1][e][2 * j + 1]);
-#pragma unroll
-          for (int r = 0; r < RT; ++r) sc[r][t] = mfma<DT>(a, q[r][2 * e + j], sc[r][t]);
-        }
-      } else {
-#pragma unroll
-        for (int r = 0; r < RT; ++r) sc[r][t] = mfma<DT>(x[t & 1][e], q[r][e], sc[r][t]);
-      }
-    }
-    if constexpr (RT > 1) __builtin_amdgcn_sched_barrier(0);  // no more fragments at once: the registers are full
-  }
 }
 
 // Mask, online softmax and the two 16-bit terms of P.  `have`: how many of the
@@ -440,37 +419,71 @@ __device__ __forceinline__ void clear_tail(unsigned char* vt, const int (&va)[Cf
     }
 }
 
-// O^T += V^T.P^T of a block.
-template <int DT, bool F8, int HD, int RT>
-__device__ __forceinline__ void weigh(const unsigned char* vt, const int (&va)[Cfg<DT, F8, HD>::VS], int lcp, const u32x4 (&ph)[RT][2],
-                                      const u32x4 (&pl)[RT][2], f32x4 (&o)[RT][HD / 16]) {
+// The products of a block: O^T += V^T.P^T (PVT) over the V tile at vt, and S = K.Q^T
+// (SQT) over the K tile at kt; the two may be of different blocks.  They run in
+// slices, a d tile of V or the 16 keys of a K product, AHEAD of which the
+// fragments are read.  (The empty statements keep the fragments' addresses from
+// being formed outside the loop and held there.)
+template <int DT, bool F8, int HD, int RT, bool PVT, bool SQT>
+__device__ __forceinline__ void multiply(const unsigned char* vt, const int (&va)[Cfg<DT, F8, HD>::VS], int lcp, const u32x4 (&ph)[RT][2],
+                                         const u32x4 (&pl)[RT][2], f32x4 (&o)[RT][HD / 16], const unsigned char* kt, int ka,
+                                         const u32x4 (&q)[RT][HD / 32], f32x4 (&sc)[RT][4]) {
   using C = Cfg<DT, F8, HD>;
-  int at[C::VS];
+  constexpr int NV = PVT ? C::ND : 0, NK = SQT ? 4 : 0, N = NV + NK;
+  constexpr int AHEAD = 2, B = AHEAD + 1;
+  int at[C::VS], ak = ka;
+  asm volatile("" : "+v"(ak));
 #pragma unroll
   for (int e = 0; e < C::VS; ++e) {
     at[e] = va[e];
     asm volatile("" : "+v"(at[e]));
   }
-  u32x4 x[2][C::VS];
-  auto read = [&](int d) {
+  u32x4 x[B][C::KS > C::VS ? C::KS : C::VS];
+  constexpr int P = C::ND / 4 + 1;  // both: the four K products come between the d tiles
+  auto is_k = [](int n) { return PVT && SQT ? n % P == P - 1 : SQT; };
+  auto index = [&](int n) { return PVT && SQT ? (is_k(n) ? n / P : n - n / P) : n; };
+  auto read = [&](int n) {
+    if (is_k(n)) {
 #pragma unroll
-    for (int e = 0; e < C::VS; ++e) x[d & 1][e] = *reinterpret_cast<const u32x4*>(vt + at[e] + (d * 256 << lcp));
-  };
-  read(0);
+      for (int e = 0; e < C::KS; ++e) x[n % B][e] = *reinterpret_cast<const u32x4*>(kt + (ak ^ (e << 6)) + 4 * index(n) * C::CR * 16);
+    } else {
 #pragma unroll
-  for (int d = 0; d < C::ND; ++d) {
-    if (d + 1 < C::ND) read(d + 1);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      u32x4 a;
-      if constexpr (F8) a = widen_e4m3<QA_BF16>(x[d & 1][0][2 * j], x[d & 1][0][2 * j + 1]);
-      else a = x[d & 1][j];
-#pragma unroll
-      for (int r = 0; r < RT; ++r) o[r][d] = mfma<C::PV>(a, ph[r][j], o[r][d]);
-#pragma unroll
-      for (int r = 0; r < RT; ++r) o[r][d] = mfma<C::PV>(a, pl[r][j], o[r][d]);
+      for (int e = 0; e < C::VS; ++e) x[n % B][e] = *reinterpret_cast<const u32x4*>(vt + at[e] + (index(n) * 256 << lcp));
     }
-    if constexpr (RT > 1) __builtin_amdgcn_sched_barrier(0);
+  };
+#pragma unroll
+  for (int n = 0; n < AHEAD && n < N; ++n) read(n);
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    if (n + AHEAD < N) read(n + AHEAD);
+    if (is_k(n)) {
+      const int t = index(n);
+#pragma unroll
+      for (int e = 0; e < C::QS; ++e) {
+        u32x4 a;
+        if constexpr (F8) a = widen_e4m3<DT>(x[n % B][e >> 1][2 * (e & 1)], x[n % B][e >> 1][2 * (e & 1) + 1]);
+        else a = x[n % B][e];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) sc[r][t] = mfma<DT>(a, q[r][e], e ? sc[r][t] : f32x4{0, 0, 0, 0});
+      }
+    } else {
+      const int d = index(n);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        u32x4 a;
+        if constexpr (F8) a = widen_e4m3<QA_BF16>(x[n % B][0][2 * j], x[n % B][0][2 * j + 1]);
+        else a = x[n % B][j];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) o[r][d] = mfma<C::PV>(a, ph[r][j], o[r][d]);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) o[r][d] = mfma<C::PV>(a, pl[r][j], o[r][d]);
+      }
+    }
+    if constexpr (RT > 1) {  // in this order: more fragments at once than these do not fit the registers
+      if (n + AHEAD < N && is_k(n + AHEAD)) __builtin_amdgcn_sched_group_barrier(0x100, C::KS, 0);
+      else if (n + AHEAD < N) __builtin_amdgcn_sched_group_barrier(0x100, C::VS, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
 }
 
@@ -531,19 +544,33 @@ __device__ __forceinline__ void finish(const PagedAttnParams& p, const Split& sp
   }
 }
 
-// Page ids, and e4m3 scales, of 16 blocks: lane 4 j + a those of the 16 keys from
-// key(j) + 16 a on.
-template <bool F8, class Key>
-__device__ __forceinline__ void fetch_ids(const PagedParams& kv, const SeqSpan& sq, int s, int h, int left, Key key, int* ids, float* ks,
-                                          float* vs) {
+// Pages, and e4m3 scales, of 16 blocks: lane 4 j + a those of the 16 keys from
+// key(j) + 16 a on.  holes: some page of the sequence's keys is none.
+template <bool F8, int HD, class Key>
+__device__ __forceinline__ void fetch_pages(const PagedParams& kv, const SeqSpan& sq, int s, int h, int left, Key key, Pages* pages,
+                                            float* ks, float* vs, bool* holes) {
   const int lane = threadIdx.x & 63, pos = key(lane >> 2) + 16 * (lane & 3);
-  *ids = (lane >> 2) < left && pos < sq.len ? page_at(kv, s, pos) : -1;
+  const bool in = (lane >> 2) < left && pos < sq.len;
+  const int id = in ? page_at(kv, s, pos) : -1;
+  *holes |= __builtin_amdgcn_ballot_w64(in && id < 0) != 0;
+  const int64_t at = id < 0 ? -1 : page_base(kv, id, h, HD) * (F8 ? 1 : 2);
+  *pages = {(int)at, (int)(at >> 32)};
   if constexpr (F8) {
-    const int64_t at = (int64_t)max(*ids, 0) * kv.nkvh + h;
-    const float x = kv.k_scale[at], y = kv.v_scale[at];
-    *ks = *ids < 0 ? 1.f : x;
-    *vs = *ids < 0 ? 0.f : y;
+    const int64_t sc = (int64_t)max(id, 0) * kv.nkvh + h;
+    const float x = kv.k_scale[sc], y = kv.v_scale[sc];
+    *ks = id < 0 ? 1.f : x;
+    *vs = id < 0 ? 0.f : y;
   }
+}
+
+// What lane 4 j + g holds, for each lane's g, without a trip to the LDS.
+__device__ __forceinline__ int of_keys(int v, int j, int g) {
+  const int a = __builtin_amdgcn_readlane(v, 4 * j), b = __builtin_amdgcn_readlane(v, 4 * j + 1);
+  const int c = __builtin_amdgcn_readlane(v, 4 * j + 2), d = __builtin_amdgcn_readlane(v, 4 * j + 3);
+  return g & 2 ? (g & 1 ? d : c) : (g & 1 ? b : a);
+}
+__device__ __forceinline__ float of_keys(float v, int j, int g) {
+  return __uint_as_float((uint32_t)of_keys((int)__float_as_uint(v), j, g));
 }
 
 // Sequences of few rows: every wave has its own tiles, and waits for its own loads
@@ -571,10 +598,11 @@ __global__ void __launch_bounds__(64 * kFewWaves) paged_few_kernel(const PagedAt
   auto key_of = [&](int it) { return k0 + (wave + it * kFewWaves) * 64; };
   unsigned char *kt = smem + wave * 2 * C::TILE, *vt = kt + C::TILE;
   const int lcp = kv.lp - (F8 ? 4 : 3);
-  int ids = -1;
+  Pages pages = {-1, -1};
   float ksc = 1.f, vsc = 0.f;
+  bool holes = false;
   auto fetch = [&](int it) {
-    fetch_ids<F8>(kv, sq, s, h, steps - it, [&](int j) { return key_of(it + j); }, &ids, &ksc, &vsc);
+    fetch_pages<F8, HD>(kv, sq, s, h, steps - it, [&](int j) { return key_of(it + j); }, &pages, &ksc, &vsc, &holes);
   };
   Columns<1> col;
   col.set(p, sq, h, 0, c);
@@ -582,9 +610,10 @@ __global__ void __launch_bounds__(64 * kFewWaves) paged_few_kernel(const PagedAt
   load_q<DT, F8, HD, 1>(p, col, g, q);
   if (steps > 0) {
     fetch(0);
-    load_tile<DT, F8, HD, 1, true>(kv, h, ids, 0, 0, kt);
-    load_tile<DT, F8, HD, 1, false>(kv, h, ids, 0, 0, vt);
+    load_tile<DT, F8, HD, 1, true>(kv, pages, 0, 0, kt);
+    load_tile<DT, F8, HD, 1, false>(kv, pages, 0, 0, vt);
   }
+  keep(q);
   f32x4 o[1][C::ND] = {};
   float m[1] = {-INFINITY}, l[1] = {0.f};
   const int ka = k_frag<DT, F8, HD>(c, g);
@@ -593,29 +622,30 @@ __global__ void __launch_bounds__(64 * kFewWaves) paged_few_kernel(const PagedAt
   for (int e = 0; e < C::VS; ++e) va[e] = v_frag<DT, F8, HD>(c, g, e, lcp);
   for (int it = 0; it < steps; ++it) {
     const bool more = it + 1 < steps;
-    const int kg = key_of(it) + 16 * g, src = (it & 15) * 4 + g;
-    const int have = __shfl(ids, src, 64) < 0 ? 0 : sq.len - kg;
+    const int kg = key_of(it) + 16 * g;
+    int have = sq.len - kg;
+    if (holes && of_keys(pages.hi, it & 15, g) < 0) have = 0;
     float ks = 1.f, vs = 0.f;
     if constexpr (F8) {
-      ks = __shfl(ksc, src, 64);
-      vs = __shfl(vsc, src, 64);
+      ks = of_keys(ksc, it & 15, g);
+      vs = of_keys(vsc, it & 15, g);
     }
     wait_vmcnt<C::LI>();  // K is there; V's loads came after it
     f32x4 sc[1][4];
-    scores<DT, F8, HD, 1>(kt, ka, q, sc);
+    u32x4 ph[1][2], pl[1][2];
+    multiply<DT, F8, HD, 1, false, true>(vt, va, lcp, ph, pl, o, kt, ka, q, sc);
     wait_lds();
     if (more) {
       if ((it & 15) == 15) fetch(it + 1);
-      load_tile<DT, F8, HD, 1, true>(kv, h, ids, (it + 1) & 15, 0, kt);
+      load_tile<DT, F8, HD, 1, true>(kv, pages, (it + 1) & 15, 0, kt);
     }
-    u32x4 ph[1][2], pl[1][2];
     softmax<DT, F8, HD, 1>(sc, col.pos, kg, have, p.scale * kLog2e * ks, vs, m, l, o, ph, pl);
     if (more) wait_vmcnt<C::LI>();  // V is there; the next K's loads came after it
     else wait_vmcnt<0>();
     if (__builtin_amdgcn_ballot_w64(have < 16)) clear_tail<DT, F8, HD>(vt, va, lcp, have);
-    weigh<DT, F8, HD, 1>(vt, va, lcp, ph, pl, o);
+    multiply<DT, F8, HD, 1, true, false>(vt, va, lcp, ph, pl, o, kt, ka, q, sc);
     wait_lds();
-    if (more) load_tile<DT, F8, HD, 1, false>(kv, h, ids, (it + 1) & 15, 0, vt);
+    if (more) load_tile<DT, F8, HD, 1, false>(kv, pages, (it + 1) & 15, 0, vt);
   }
   __syncthreads();  // the tiles' LDS is the join's
   finish<DT, F8, HD, 1, 1, kFewWaves>(p, sp, sq, h, 0, part, end <= sp.few_chunk, m, l, o, smem);
@@ -673,23 +703,26 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
   auto kt = [&](int it) { return base + (it & (NB - 1)) * C::TILE; };
   auto vt = [&](int it) { return base + (NB + (it & (NB - 1))) * C::TILE; };
   const int lcp = kv.lp - (F8 ? 4 : 3);
-  // two windows of 16 blocks' ids: loads run up to two blocks ahead of the softmax
-  int ids0 = -1, ids1 = -1;
+  // two windows of 16 blocks' pages: loads run up to two blocks ahead of the softmax
+  bool holes = false;
+  Pages pages0 = {-1, -1}, pages1 = {-1, -1};
   float ks0 = 1.f, ks1 = 1.f, vs0 = 0.f, vs1 = 0.f;
   auto fetch = [&](int w) {
-    int id = -1;
+    Pages pg = {-1, -1};
     float x = 1.f, y = 0.f;
-    fetch_ids<F8>(kv, sq, s, h, steps - 16 * w, [&](int j) { return key_of(16 * w + j); }, &id, &x, &y);
-    ids0 = w & 1 ? ids0 : id;
+    fetch_pages<F8, HD>(kv, sq, s, h, steps - 16 * w, [&](int j) { return key_of(16 * w + j); }, &pg, &x, &y, &holes);
+    pages0.lo = w & 1 ? pages0.lo : pg.lo;
+    pages0.hi = w & 1 ? pages0.hi : pg.hi;
     ks0 = w & 1 ? ks0 : x;
     vs0 = w & 1 ? vs0 : y;
-    ids1 = w & 1 ? id : ids1;
+    pages1.lo = w & 1 ? pg.lo : pages1.lo;
+    pages1.hi = w & 1 ? pg.hi : pages1.hi;
     ks1 = w & 1 ? x : ks1;
     vs1 = w & 1 ? y : vs1;
   };
-  auto ids_of = [&](int it) { return it >> 4 & 1 ? ids1 : ids0; };
-  auto issue_k = [&](int it) { load_tile<DT, F8, HD, GW, true>(kv, h, ids_of(it), scalar(it & 15), scalar(wg), smem + scalar((int)(kt(it) - smem))); };
-  auto issue_v = [&](int it) { load_tile<DT, F8, HD, GW, false>(kv, h, ids_of(it), scalar(it & 15), scalar(wg), smem + scalar((int)(vt(it) - smem))); };
+  auto pages_of = [&](int it) { return it >> 4 & 1 ? pages1 : pages0; };
+  auto issue_k = [&](int it) { load_tile<DT, F8, HD, GW, true>(kv, pages_of(it), scalar(it & 15), scalar(wg), smem + scalar((int)(kt(it) - smem))); };
+  auto issue_v = [&](int it) { load_tile<DT, F8, HD, GW, false>(kv, pages_of(it), scalar(it & 15), scalar(wg), smem + scalar((int)(vt(it) - smem))); };
   // refill(j), in step j's VALU phase: K of block j + NB (S of j has read its slot),
   // V of block j + NB - 1 (P.V of j - 1 has).  Step i's MFMA phase needs K(i) and
   // V(i - 1), of refill(i - NB): with two buffers refill(i - 1) may be under way.
@@ -711,6 +744,7 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
     if (NB == 2 && steps > 1) issue_k(1);
     if (NB == 2) issue_v(0);
   }
+  keep(q);
   f32x4 o[RT][C::ND] = {};
   float m[RT], l[RT];
 #pragma unroll
@@ -733,18 +767,18 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
     const int my = ph_no - off, it = my >> 1;
     if (my >= 0 && my <= 2 * steps) {
       if ((my & 1) == 0) {
-        if (it > 0) {
-          if (__builtin_amdgcn_ballot_w64(have < 16)) clear_tail<DT, F8, HD>(vt(it - 1), va, lcp, have);
-          weigh<DT, F8, HD, RT>(vt(it - 1), va, lcp, ph, pl, o);
-        }
-        if (it < steps) scores<DT, F8, HD, RT>(kt(it), ka, q, sc);
+        if (it > 0 && __builtin_amdgcn_ballot_w64(have < 16)) clear_tail<DT, F8, HD>(vt(it - 1), va, lcp, have);
+        if (it > 0 && it < steps) multiply<DT, F8, HD, RT, true, true>(vt(it - 1), va, lcp, ph, pl, o, kt(it), ka, q, sc);
+        else if (it > 0) multiply<DT, F8, HD, RT, true, false>(vt(it - 1), va, lcp, ph, pl, o, kt(it), ka, q, sc);
+        else if (steps > 0) multiply<DT, F8, HD, RT, false, true>(vt(it), va, lcp, ph, pl, o, kt(it), ka, q, sc);
       } else {
-        const int kg = key_of(it) + 16 * g, src = (it & 15) * 4 + g;
-        have = __shfl(ids_of(it), src, 64) < 0 ? 0 : sq.len - kg;
+        const int kg = key_of(it) + 16 * g, j = scalar(it & 15);
+        have = sq.len - kg;
+        if (holes && of_keys(pages_of(it).hi, j, g) < 0) have = 0;
         float ks = 1.f, vs = 0.f;
         if constexpr (F8) {
-          ks = __shfl(it >> 4 & 1 ? ks1 : ks0, src, 64);
-          vs = __shfl(it >> 4 & 1 ? vs1 : vs0, src, 64);
+          ks = of_keys(it >> 4 & 1 ? ks1 : ks0, j, g);
+          vs = of_keys(it >> 4 & 1 ? vs1 : vs0, j, g);
         }
         if (it > 0 && (it & 15) == 0 && 16 * (it >> 4) + 16 < steps) fetch((it >> 4) + 1);
         if (it + NB < steps) issue_k(it + NB);
@@ -776,7 +810,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p
   if (R >= NR) return;
   const int i = R / p.rep, head = h * p.rep + R % p.rep;
   const bool few = sp.few && NR <= kFewRows;
-  const int last = few ? NR - 1 : min((R / kManyRows + 1) * kManyRows, NR) - 1;
+  const int last = few ? NR - 1 : min((R / sp.many_rows + 1) * sp.many_rows, NR) - 1;
   const int chunk = few ? sp.few_chunk : sp.many_chunk, keys = sq.pos0 + last / p.rep + 1;
   if (keys <= chunk) return;  // its tile has written the result
   const int parts = (keys + chunk - 1) / chunk;
@@ -829,9 +863,11 @@ template <int DT, bool F8, int HD>
 hipError_t launch_one(const PagedAttnParams& p, hipStream_t s) {
   const Split sp = split_of(p);
   const int64_t heads = (int64_t)p.kv.seqs * p.kv.nkvh;
-  if (sp.many)
-    hipLaunchKernelGGL((paged_many_kernel<DT, F8, HD, 2>), dim3((unsigned)(heads * sp.tiles * sp.many_chunks)), dim3(64 * kManyWaves), 0,
-                       s, p, sp);
+  if (sp.many) {
+    const dim3 grid((unsigned)(heads * sp.tiles * sp.many_chunks)), block(64 * kManyWaves);
+    if (sp.many_rows == 64) hipLaunchKernelGGL((paged_many_kernel<DT, F8, HD, 2>), grid, block, 0, s, p, sp);
+    else hipLaunchKernelGGL((paged_many_kernel<DT, F8, HD, 4>), grid, block, 0, s, p, sp);
+  }
   if (sp.few)
     hipLaunchKernelGGL((paged_few_kernel<DT, F8, HD>), dim3((unsigned)(heads * sp.few_chunks)), dim3(64 * kFewWaves), 0, s, p, sp);
   if (sp.parts > 1) {
