@@ -279,24 +279,26 @@ __device__ __forceinline__ void copy_page(const unsigned char* src, int bytes, u
     one(std::integral_constant<int, 3>{});
   }
 }
-template <int DT, bool F8, int HD, int OF, int LP, bool K>
+template <int DT, bool F8, int HD, bool W32, int OF, int LP, bool K>
 __device__ __forceinline__ void load_pages(const PagedParams& kv, const Pages& pages, int j, int mine, unsigned char* to) {
   using C = Cfg<DT, F8, HD>;
   constexpr int PER = C::LI >> (6 - LP), PB = HD * C::ES << LP;  // instructions and bytes of a page
   constexpr int CW = K ? C::CR : (1 << LP) * C::ES / 16;          // chunks of a row
   int ln = threadIdx.x & 63;
   asm volatile("" : "+v"(ln));  // lane offsets are formed anew, not kept across the loop
-  // the part of f(row) that the lane gives; instruction n of the page adds its own
+  // the part of f(row) that the lane gives, and the one of instruction n of page pg
   int f;
-  if constexpr (K) f = CW == 16 ? ln >> 4 & 3 : CW == 8 ? ln >> 4 & 1 : 0;
+  if constexpr (W32) f = (ln >> 4) & 3 & (CW - 1);  // chunk M of a page: f = (M / 16) % CW
+  else if constexpr (K) f = CW == 16 ? ln >> 4 & 3 : CW == 8 ? ln >> 4 & 1 : 0;
   else if constexpr (F8) f = CW == 4 ? swap3(ln >> 4 & 3) : 0;
   else f = CW == 4 ? ln >> 5 : ln >> 4 & 1;
   const uint32_t lane_off = (uint32_t)((ln & ~(CW - 1)) | ((ln & (CW - 1)) ^ f)) * 16;
-  auto off_k = [&](int n, int pg) {  // n / KS: the 16 keys
-    const int g = (pg << (LP - 4)) + n / C::KS;
-    return lane_off ^ (uint32_t)((CW == 16 ? g << 2 : CW == 8 ? g << 1 : swap3(g)) << 4);
+  auto off = [&](int n, int pg) {
+    if constexpr (W32) return lane_off ^ (uint32_t)((4 * n & (CW - 1)) << 4);
+    const int g = (pg << (LP - 4)) + n / C::KS;  // K: the 16 keys
+    if constexpr (K) return lane_off ^ (uint32_t)((CW == 16 ? g << 2 : CW == 8 ? g << 1 : swap3(g)) << 4);
+    return lane_off ^ (uint32_t)(!F8 && CW == 8 ? (n & 1) << 6 : 0);
   };
-  auto off_v = [&](int n) { return lane_off ^ (uint32_t)(!F8 && CW == 8 ? (n & 1) << 6 : 0); };
   auto page_src = [&](int pg, int* bytes) {
     const int lo = __builtin_amdgcn_readlane(pages.lo, j * 4 + (pg << (LP - 4)));
     const int hi = __builtin_amdgcn_readlane(pages.hi, j * 4 + (pg << (LP - 4)));
@@ -308,10 +310,7 @@ __device__ __forceinline__ void load_pages(const PagedParams& kv, const Pages& p
     for (int pg = 0; pg < 64 >> LP; ++pg) {
       int bytes;
       const unsigned char* src = page_src(pg, &bytes);
-      copy_page<OF, PER>(src, bytes, to + pg * PER * 1024, mine, [&](int n) {
-        if constexpr (K) return off_k(C::KS >= OF ? n : n + mine, pg);  // (of OF instructions side by side: one 16 keys, or not)
-        else return OF == 1 ? off_v(n) : off_v(mine);
-      });
+      copy_page<OF, PER>(src, bytes, to + pg * PER * 1024, mine, [&](int n) { return off(n + mine, pg); });
     }
   } else {  // fewer instructions to a page than waves: pages side by side
     constexpr int PP = OF / PER;
@@ -320,18 +319,16 @@ __device__ __forceinline__ void load_pages(const PagedParams& kv, const Pages& p
       const int pg = p0 + mine / PER, n = mine % PER;
       int bytes;
       const unsigned char* src = page_src(pg, &bytes);
-      copy_page<1, 1>(src + n * 1024, bytes - n * 1024 > 0 ? bytes - n * 1024 : 0, to + pg * PER * 1024 + n * 1024, 0, [&](int) {
-        if constexpr (K) return off_k(n, pg);
-        else return off_v(n);
-      });
+      copy_page<1, 1>(src + n * 1024, bytes - n * 1024 > 0 ? bytes - n * 1024 : 0, to + (pg * PER + n) * 1024, 0,
+                      [&](int) { return off(n, pg); });
     }
   }
 }
-template <int DT, bool F8, int HD, int OF, bool K>
+template <int DT, bool F8, int HD, bool W32, int OF, bool K>
 __device__ __forceinline__ void load_tile(const PagedParams& kv, const Pages& pages, int j, int mine, unsigned char* to) {
-  if (kv.lp == 6) load_pages<DT, F8, HD, OF, 6, K>(kv, pages, j, mine, to);
-  else if (kv.lp == 5) load_pages<DT, F8, HD, OF, 5, K>(kv, pages, j, mine, to);
-  else load_pages<DT, F8, HD, OF, 4, K>(kv, pages, j, mine, to);
+  if (kv.lp == 6) load_pages<DT, F8, HD, W32, OF, 6, K>(kv, pages, j, mine, to);
+  else if (kv.lp == 5) load_pages<DT, F8, HD, W32, OF, 5, K>(kv, pages, j, mine, to);
+  else load_pages<DT, F8, HD, W32, OF, 4, K>(kv, pages, j, mine, to);
 }
 // Fragment addresses in the tiles.  K: product t reads row 16 (c / 4) + 4 t + c % 4,
 // slice e the chunk 4 e + g.  V: row d, the chunks of keys 16 g ..
@@ -398,6 +395,12 @@ __device__ __forceinline__ void softmax(f32x4 (&sc)[RT][4], const int (&pos)[RT]
   }
 }
 
+// Mask of word w of a run of elements of which `left` are keys.
+template <int ES>
+__device__ __forceinline__ uint32_t tail_mask(int left, int w) {
+  const int n = left - w * (4 / ES);
+  return n >= 4 / ES ? ~0u : n <= 0 ? 0u : (1u << (8 * ES * n)) - 1;
+}
 // What a V tile holds behind the sequence's keys, or for no page, may be anything, NaN
 // too, and 0 * NaN is not 0: a lane clears those elements of the chunks that it
 // will read itself.
@@ -406,10 +409,7 @@ __device__ __forceinline__ void clear_tail(unsigned char* vt, const int (&va)[Cf
   using C = Cfg<DT, F8, HD>;
   uint32_t keep[C::VS * 4];
 #pragma unroll
-  for (int w = 0; w < C::VS * 4; ++w) {
-    const int n = have - w * (4 / C::ES);  // elements of word w that are keys
-    keep[w] = n >= 4 / C::ES ? ~0u : n <= 0 ? 0u : (1u << (8 * C::ES * n)) - 1;
-  }
+  for (int w = 0; w < C::VS * 4; ++w) keep[w] = tail_mask<C::ES>(have, w);
 #pragma unroll 1
   for (int d = 0; d < C::ND; ++d)
 #pragma unroll
@@ -573,6 +573,12 @@ __device__ __forceinline__ float of_keys(float v, int j, int g) {
   return __uint_as_float((uint32_t)of_keys((int)__float_as_uint(v), j, g));
 }
 
+// Lane l's value for the lanes' lower half, lane l + 1's for the upper.
+__device__ __forceinline__ int of_half(int v, int l, int h) {
+  const int a = __builtin_amdgcn_readlane(v, l), b = __builtin_amdgcn_readlane(v, l + 1);
+  return h ? b : a;
+}
+
 // Sequences of few rows: every wave has its own tiles, and waits for its own loads
 // alone.  K of the next block is under way while this one's softmax and P.V run, V
 // from P.V to P.V.  Block: kv head fastest, then part, then sequence.
@@ -610,8 +616,8 @@ __global__ void __launch_bounds__(64 * kFewWaves) paged_few_kernel(const PagedAt
   load_q<DT, F8, HD, 1>(p, col, g, q);
   if (steps > 0) {
     fetch(0);
-    load_tile<DT, F8, HD, 1, true>(kv, pages, 0, 0, kt);
-    load_tile<DT, F8, HD, 1, false>(kv, pages, 0, 0, vt);
+    load_tile<DT, F8, HD, false, 1, true>(kv, pages, 0, 0, kt);
+    load_tile<DT, F8, HD, false, 1, false>(kv, pages, 0, 0, vt);
   }
   keep(q);
   f32x4 o[1][C::ND] = {};
@@ -637,7 +643,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) paged_few_kernel(const PagedAt
     wait_lds();
     if (more) {
       if ((it & 15) == 15) fetch(it + 1);
-      load_tile<DT, F8, HD, 1, true>(kv, pages, (it + 1) & 15, 0, kt);
+      load_tile<DT, F8, HD, false, 1, true>(kv, pages, (it + 1) & 15, 0, kt);
     }
     softmax<DT, F8, HD, 1>(sc, col.pos, kg, have, p.scale * kLog2e * ks, vs, m, l, o, ph, pl);
     if (more) wait_vmcnt<C::LI>();  // V is there; the next K's loads came after it
@@ -645,18 +651,165 @@ __global__ void __launch_bounds__(64 * kFewWaves) paged_few_kernel(const PagedAt
     if (__builtin_amdgcn_ballot_w64(have < 16)) clear_tail<DT, F8, HD>(vt, va, lcp, have);
     multiply<DT, F8, HD, 1, true, false>(vt, va, lcp, ph, pl, o, kt, ka, q, sc);
     wait_lds();
-    if (more) load_tile<DT, F8, HD, 1, false>(kv, pages, (it + 1) & 15, 0, vt);
+    if (more) load_tile<DT, F8, HD, false, 1, false>(kv, pages, (it + 1) & 15, 0, vt);
   }
   __syncthreads();  // the tiles' LDS is the join's
   finish<DT, F8, HD, 1, 1, kFewWaves>(p, sp, sq, h, 0, part, end <= sp.few_chunk, m, l, o, smem);
 }
 
-// Tiles of 64 (row, head) pairs: NS key splits of GW waves with 32 columns each.  A
-// split's waves share its tiles.  A step is an MFMA phase (P.V of the block before,
-// S of this one) and a VALU phase (softmax, the next loads); every phase ends in
-// a block barrier, and the upper half of the splits runs one phase behind the
-// lower, so that of the two waves on a SIMD one multiplies while the other is at
-// its softmax.
+// ---- tiles of 64 or 128 (row, head) pairs ----
+//
+// NS key splits of GW waves with 32 columns each, on v_mfma_f32_32x32x16: lane
+// (c = lane & 31, h = lane >> 5) gets rows 8 a + 4 h + b of each 32-key product (a, b
+// < 4), which are given keys 16 h + 4 a + b, so that it has 16 keys of its column in a
+// row, twice.  A split's waves share its tiles.  A step is an MFMA phase (P.V of
+// the block before, S of this one) and a VALU phase (softmax, the next loads); every
+// phase ends in a block barrier, and the upper half of the splits runs one phase
+// behind the lower, so that of the two waves on a SIMD one multiplies while the
+// other is at its softmax.
+// Rows' parts of the chunk order here: f = (16-byte chunk number in the page / 16)
+// modulo the row's chunks, for K and V alike; with the keys above the lanes that the
+// LDS serves at once find 16 bank groups, whatever the page size.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+template <int DT>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (DT == QA_F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ float pair_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float pair_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// P.V of one block (PVT) and S of another (SQT).  HD / 16 slices: two 32-row d tiles of
+// V against 16 keys of P, and 16 of d of both 32-key products; the fragments are
+// read AHEAD slices before.  (The empty statements keep their addresses from being
+// formed outside the loop and held there.)
+template <int DT, bool F8, int HD, bool PVT, bool SQT>
+__device__ __forceinline__ void multiply32(const unsigned char* vt, const int (&va)[F8 ? 2 : 4], int lcp, const u32x4 (&ph)[2][2],
+                                           const u32x4 (&pl)[2][2], f32x16 (&o)[HD / 32], const unsigned char* kt, int ka,
+                                           const u32x4 (&q)[HD / 16], f32x16 (&sc)[2]) {
+  using C = Cfg<DT, F8, HD>;
+  constexpr int N = HD / 16, DP = HD / 64;  // slices, pairs of d tiles
+  constexpr int EACH = F8 ? 2 : 1;          // slices that one read serves
+  constexpr int AHEAD = 1, B = AHEAD + 1;
+  int at[F8 ? 2 : 4], ak = ka;
+  asm volatile("" : "+v"(ak));
+#pragma unroll
+  for (int e = 0; e < (F8 ? 2 : 4); ++e) {
+    at[e] = va[e];
+    asm volatile("" : "+v"(at[e]));
+  }
+  u32x4 x[B][2], y[B][2];
+  // slice n: keys' half kt = n / (2 DP), d tiles 2 ((n / 2) % DP) and the next, 16 keys' half j = n % 2
+  auto read = [&](int i) {  // reads number i, for slices EACH i ..
+    const int n = i * EACH;
+    if constexpr (PVT) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        x[i % B][u] = *reinterpret_cast<const u32x4*>(vt + at[F8 ? n / (2 * DP) : n / (2 * DP) * 2 + n % 2] +
+                                                      ((2 * (n / 2 % DP) + u) * 512 << lcp));
+    }
+    if constexpr (SQT) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) y[i % B][u] = *reinterpret_cast<const u32x4*>(kt + (ak ^ (i << 5)) + u * 32 * C::CR * 16);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < AHEAD && i < N / EACH; ++i) read(i);
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const int i = n / EACH, half = n / (2 * DP), d = 2 * (n / 2 % DP), j = n % 2;
+    const bool reads = n % EACH == 0 && i + AHEAD < N / EACH;
+    if (reads) read(i + AHEAD);
+    u32x4 v[2];
+    if constexpr (PVT) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if constexpr (F8) v[u] = widen_e4m3<QA_BF16>(x[i % B][u][2 * j], x[i % B][u][2 * j + 1]);
+        else v[u] = x[i % B][u];
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) o[d + u] = mfma32<C::PV>(v[u], ph[half][j], o[d + u]);
+    }
+    if constexpr (SQT) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        u32x4 a;
+        if constexpr (F8) a = widen_e4m3<DT>(y[i % B][u][2 * j], y[i % B][u][2 * j + 1]);
+        else a = y[i % B][u];
+        sc[u] = mfma32<DT>(a, q[n], n ? sc[u] : f32x16{0});
+      }
+    }
+    if constexpr (PVT) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) o[d + u] = mfma32<C::PV>(v[u], pl[half][j], o[d + u]);
+    }
+    constexpr int R = (PVT ? 2 : 0) + (SQT ? 2 : 0);
+    if (reads) __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+    __builtin_amdgcn_sched_barrier(0);  // no more fragments at once than the registers hold
+  }
+}
+
+// softmax() for a lane with one column and keys kg + 16 h .., kg + 32 + 16 h .. (two
+// runs of 16, a page each).
+template <int DT, bool F8, int HD>
+__device__ __forceinline__ void softmax32(f32x16 (&sc)[2], int pos, int kg, const int (&have)[2], const float (&f)[2],
+                                          const float (&vs)[2], float& m, float& l, f32x16 (&o)[HD / 32], u32x4 (&ph)[2][2],
+                                          u32x4 (&pl)[2][2]) {
+  using C = Cfg<DT, F8, HD>;
+  float top[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int see = min(have[u], pos + 1 - kg - 32 * u);
+    if (__builtin_amdgcn_ballot_w64(see < 16)) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (e >= see) sc[u][e] = -INFINITY;
+    }
+    float x[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) x[t] = fmaxf(fmaxf(sc[u][4 * t], sc[u][4 * t + 1]), fmaxf(sc[u][4 * t + 2], sc[u][4 * t + 3]));
+    top[u] = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+  }
+  const float bm = pair_max(F8 ? fmaxf(top[0] * f[0], top[1] * f[1]) : fmaxf(top[0], top[1]) * f[0]);
+  if (__builtin_amdgcn_ballot_w64(bm > m + kLazy)) {
+    const float mn = fmaxf(m, bm);
+    const float al = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+    l *= al;
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d) o[d] *= al;
+    m = mn;
+  }
+  const float mb = (m == -INFINITY ? 0.f : m) - C::kBias;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      float w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][4 * t + e], f[u], -mb));
+        sum[e] += w[e];
+        if constexpr (F8) w[e] *= vs[u];
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t hi = pack2<C::PV>(w[2 * e], w[2 * e + 1]);
+        ph[u][t >> 1][2 * (t & 1) + e] = hi;
+        pl[u][t >> 1][2 * (t & 1) + e] = residue2<C::PV>(hi, w[2 * e], w[2 * e + 1]);
+      }
+    }
+  l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+
 __device__ __forceinline__ void phase_barrier() {
   __builtin_amdgcn_sched_barrier(0);
   asm volatile("" ::: "memory");
@@ -671,38 +824,38 @@ constexpr int many_buffers() {  // buffers of each tile: two where 128 KB hold t
 template <int DT, bool F8, int HD, int GW>
 constexpr int many_lds() {
   constexpr int tiles = kManyWaves / GW * 2 * Cfg<DT, F8, HD>::TILE * many_buffers<DT, F8, HD, GW>();
-  constexpr int join = kManyWaves * 2 * 64 * (HD + 8);
+  constexpr int join = kManyWaves * 64 * 4 * (HD / 2 + 2);
   return tiles > join ? tiles : join;
 }
 template <int DT, bool F8, int HD, int GW>
 __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const PagedAttnParams p, const Split sp) {
   using C = Cfg<DT, F8, HD>;
-  constexpr int RT = 2, NS = kManyWaves / GW, NB = many_buffers<DT, F8, HD, GW>(), WL = C::LI / GW;  // WL: a wave's loads of a tile
-  constexpr int TR = GW * RT * 16;
+  constexpr int NS = kManyWaves / GW, NB = many_buffers<DT, F8, HD, GW>(), WL = C::LI / GW;  // WL: a wave's loads of a tile
+  constexpr int TR = GW * 32, VX = F8 ? 2 : 4;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[many_lds<DT, F8, HD, GW>()];
   const PagedParams& kv = p.kv;
-  const int h = (int)(blockIdx.x % kv.nkvh);
+  const int kvh = (int)(blockIdx.x % kv.nkvh);
   const int64_t b = blockIdx.x / kv.nkvh;
-  const int per = sp.tiles * sp.many_chunks, u = (int)(b % per), s = (int)(b / per);
+  const int per = sp.tiles * sp.many_chunks, un = (int)(b % per), s = (int)(b / per);
   const SeqSpan sq = seq_span(kv, s);
   const int NR = sq.n * p.rep;
   if (NR == 0 || (sp.few && NR <= kFewRows)) return;
   // the last tiles, which see the most keys, first
-  const int tile = (NR + TR - 1) / TR - 1 - u % sp.tiles, part = u / sp.tiles;
+  const int tile = (NR + TR - 1) / TR - 1 - un % sp.tiles, part = un / sp.tiles;
   if (tile < 0) return;
   const int end = sq.pos0 + (min((tile + 1) * TR, NR) - 1) / p.rep + 1;
   const int k0 = part * sp.many_chunk, k1 = min(k0 + sp.many_chunk, end);
   if (part > 0 && k0 >= end) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+  // (the wave's number is left to the compiler as a lane's value: with scalar
+  // control flow it spills; what a DMA instruction takes is made scalar below)
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 31, h = lane >> 5;
   const int ns = wave / GW, wg = wave % GW, off = ns / (NS / 2);
   const int nb = k1 > k0 ? (k1 - k0 + 63) >> 6 : 0, steps = (nb - ns + NS - 1) / NS;
   auto key_of = [&](int it) { return k0 + (ns + it * NS) * 64; };
-  // (the wave's number is left to the compiler as a lane's value: with scalar
-  // control flow it spills; what a DMA instruction takes is made scalar below)
   unsigned char* base = smem + ns * 2 * NB * C::TILE;
   auto kt = [&](int it) { return base + (it & (NB - 1)) * C::TILE; };
   auto vt = [&](int it) { return base + (NB + (it & (NB - 1))) * C::TILE; };
-  const int lcp = kv.lp - (F8 ? 4 : 3);
+  const int lcp = kv.lp - (F8 ? 4 : 3), cp = 1 << lcp;
   // two windows of 16 blocks' pages: loads run up to two blocks ahead of the softmax
   bool holes = false;
   Pages pages0 = {-1, -1}, pages1 = {-1, -1};
@@ -710,7 +863,7 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
   auto fetch = [&](int w) {
     Pages pg = {-1, -1};
     float x = 1.f, y = 0.f;
-    fetch_pages<F8, HD>(kv, sq, s, h, steps - 16 * w, [&](int j) { return key_of(16 * w + j); }, &pg, &x, &y, &holes);
+    fetch_pages<F8, HD>(kv, sq, s, kvh, steps - 16 * w, [&](int j) { return key_of(16 * w + j); }, &pg, &x, &y, &holes);
     pages0.lo = w & 1 ? pages0.lo : pg.lo;
     pages0.hi = w & 1 ? pages0.hi : pg.hi;
     ks0 = w & 1 ? ks0 : x;
@@ -721,8 +874,12 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
     vs1 = w & 1 ? y : vs1;
   };
   auto pages_of = [&](int it) { return it >> 4 & 1 ? pages1 : pages0; };
-  auto issue_k = [&](int it) { load_tile<DT, F8, HD, GW, true>(kv, pages_of(it), scalar(it & 15), scalar(wg), smem + scalar((int)(kt(it) - smem))); };
-  auto issue_v = [&](int it) { load_tile<DT, F8, HD, GW, false>(kv, pages_of(it), scalar(it & 15), scalar(wg), smem + scalar((int)(vt(it) - smem))); };
+  auto issue_k = [&](int it) {
+    load_tile<DT, F8, HD, true, GW, true>(kv, pages_of(it), scalar(it & 15), scalar(wg), smem + scalar((int)(kt(it) - smem)));
+  };
+  auto issue_v = [&](int it) {
+    load_tile<DT, F8, HD, true, GW, false>(kv, pages_of(it), scalar(it & 15), scalar(wg), smem + scalar((int)(vt(it) - smem)));
+  };
   // refill(j), in step j's VALU phase: K of block j + NB (S of j has read its slot),
   // V of block j + NB - 1 (P.V of j - 1 has).  Step i's MFMA phase needs K(i) and
   // V(i - 1), of refill(i - NB): with two buffers refill(i - 1) may be under way.
@@ -733,10 +890,29 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
     else if (n == 1) wait_vmcnt<WL>();
     else wait_vmcnt<0>();
   };
-  Columns<RT> col;
-  col.set(p, sq, h, (tile * GW + wg) * RT * 16, c);
-  u32x4 q[RT][C::QS];
-  load_q<DT, F8, HD, RT>(p, col, g, q);
+  // the lane's (row, head) pair; lanes past the last repeat it and store nothing
+  auto pair_of = [&](int64_t* tok, int* head) {
+    int R = (tile * GW + wg) * 32 + c;
+    asm volatile("" : "+v"(R));  // formed again for the result, not held across the loop
+    const bool on = R < NR;
+    R = min(R, NR - 1);
+    const int i = R / p.rep;
+    *tok = sq.row0 + i;
+    *head = kvh * p.rep + R - i * p.rep;
+    return on;
+  };
+  u32x4 q[1][HD / 16];
+  int pos;
+  {
+    int64_t tok;
+    int head;
+    pair_of(&tok, &head);
+    pos = (int)(tok - sq.row0) + sq.pos0;
+    const uint16_t* src = p.q + tok * p.ldq + (int64_t)head * HD;
+#pragma unroll
+    for (int e = 0; e < HD / 16; ++e)  // in the order in which a K row's chunks come
+      q[0][e] = *reinterpret_cast<const u32x4*>(src + (F8 ? e / 2 * 32 + h * 16 + e % 2 * 8 : e * 16 + h * 8));
+  }
   if (steps > 0) {
     fetch(0);
     if (steps > 16) fetch(1);
@@ -745,20 +921,21 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
     if (NB == 2) issue_v(0);
   }
   keep(q);
-  f32x4 o[RT][C::ND] = {};
-  float m[RT], l[RT];
+  f32x16 o[HD / 32] = {};
+  float m = -INFINITY, l = 0.f;
+  f32x16 sc[2];
+  u32x4 ph[2][2], pl[2][2];
+  // fragment addresses: K row of the lane's key in a 32-key product, slice e at ^ (e << 5);
+  // V row c, the chunks of the lane's keys
+  const int key = 16 * (c >> 2 & 1) + 4 * (c >> 3) + (c & 3);
+  const int ka = (key * C::CR + (h ^ (key >> (4 - C::LCR) & (C::CR - 1)))) * 16;
+  int va[VX];
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    m[r] = -INFINITY;
-    l[r] = 0.f;
+  for (int e = 0; e < VX; ++e) {
+    const int x = F8 ? 2 * e + h : 4 * (e >> 1) + 2 * h + (e & 1);  // the block's chunk of the row
+    va[e] = ((((x >> lcp) * HD + c) << lcp) + ((x & (cp - 1)) ^ (c >> (4 - lcp) & (cp - 1)))) * 16;
   }
-  f32x4 sc[RT][4];
-  u32x4 ph[RT][2], pl[RT][2];
-  const int ka = k_frag<DT, F8, HD>(c, g);
-  int va[C::VS];
-#pragma unroll
-  for (int e = 0; e < C::VS; ++e) va[e] = v_frag<DT, F8, HD>(c, g, e, lcp);
-  int have = 16;  // the lane's keys in the block of the last softmax
+  int have[2] = {16, 16};  // the lane's keys in the block of the last softmax
   const int n0 = (nb + NS - 1) / NS, n1 = (nb + NS / 2 - 1) / NS;  // most steps of either half
   const int phases = max(2 * n0 + 1, 2 * n1 + 2);
   if (off == 0) wait_vmcnt<0>();
@@ -767,23 +944,38 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
     const int my = ph_no - off, it = my >> 1;
     if (my >= 0 && my <= 2 * steps) {
       if ((my & 1) == 0) {
-        if (it > 0 && __builtin_amdgcn_ballot_w64(have < 16)) clear_tail<DT, F8, HD>(vt(it - 1), va, lcp, have);
-        if (it > 0 && it < steps) multiply<DT, F8, HD, RT, true, true>(vt(it - 1), va, lcp, ph, pl, o, kt(it), ka, q, sc);
-        else if (it > 0) multiply<DT, F8, HD, RT, true, false>(vt(it - 1), va, lcp, ph, pl, o, kt(it), ka, q, sc);
-        else if (steps > 0) multiply<DT, F8, HD, RT, false, true>(vt(it), va, lcp, ph, pl, o, kt(it), ka, q, sc);
+        if (it > 0 && __builtin_amdgcn_ballot_w64(min(have[0], have[1]) < 16)) {
+          // V behind the sequence's keys, or for no page, may be anything, NaN too: a
+          // lane clears those elements of the chunks that it will read itself
+#pragma unroll
+          for (int e = 0; e < VX; ++e)
+#pragma unroll 1
+            for (int d = 0; d < HD / 32; ++d) {
+              u32x4* x = reinterpret_cast<u32x4*>(vt(it - 1) + va[e] + (d * 512 << lcp));
+              const int left = F8 ? have[e] : have[e >> 1] - 8 * (e & 1);
+              *x &= u32x4{tail_mask<C::ES>(left, 0), tail_mask<C::ES>(left, 1), tail_mask<C::ES>(left, 2), tail_mask<C::ES>(left, 3)};
+            }
+        }
+        if (it > 0 && it < steps) multiply32<DT, F8, HD, true, true>(vt(it - 1), va, lcp, ph, pl, o, kt(it), ka, q[0], sc);
+        else if (it > 0) multiply32<DT, F8, HD, true, false>(vt(it - 1), va, lcp, ph, pl, o, kt(it), ka, q[0], sc);
+        else if (steps > 0) multiply32<DT, F8, HD, false, true>(vt(it), va, lcp, ph, pl, o, kt(it), ka, q[0], sc);
       } else {
-        const int kg = key_of(it) + 16 * g, j = scalar(it & 15);
-        have = sq.len - kg;
-        if (holes && of_keys(pages_of(it).hi, j, g) < 0) have = 0;
-        float ks = 1.f, vs = 0.f;
-        if constexpr (F8) {
-          ks = of_keys(it >> 4 & 1 ? ks1 : ks0, j, g);
-          vs = of_keys(it >> 4 & 1 ? vs1 : vs0, j, g);
+        const int kg = key_of(it) + 16 * h, j = scalar(it & 15);
+        float f[2], vs[2] = {0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          have[u] = sq.len - kg - 32 * u;
+          if (holes && of_half(pages_of(it).hi, 4 * j + 2 * u, h) < 0) have[u] = 0;
+          f[u] = p.scale * kLog2e;
+          if constexpr (F8) {
+            f[u] *= __int_as_float(of_half(__float_as_int(it >> 4 & 1 ? ks1 : ks0), 4 * j + 2 * u, h));
+            vs[u] = __int_as_float(of_half(__float_as_int(it >> 4 & 1 ? vs1 : vs0), 4 * j + 2 * u, h));
+          }
         }
         if (it > 0 && (it & 15) == 0 && 16 * (it >> 4) + 16 < steps) fetch((it >> 4) + 1);
         if (it + NB < steps) issue_k(it + NB);
         if (it + NB - 1 < steps) issue_v(it + NB - 1);
-        softmax<DT, F8, HD, RT>(sc, col.pos, kg, have, p.scale * kLog2e * ks, vs, m, l, o, ph, pl);
+        softmax32<DT, F8, HD>(sc, pos, kg, have, f, vs, m, l, o, ph, pl);
       }
     }
     const int next = ph_no + 1 - off;
@@ -791,7 +983,54 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
     wait_lds();
     phase_barrier();
   }
-  finish<DT, F8, HD, RT, GW, NS>(p, sp, sq, h, (tile * GW + wg) * RT * 16, part, end <= sp.many_chunk, m, l, o, smem);
+
+  // the splits joined through LDS (in order), each with 1 / NS of the four-element
+  // pieces, and the result or its part written
+  constexpr int PC = HD / 8, NM = PC / NS;  // pieces of a lane: d = 32 (i / 4) + 8 (i % 4) + 4 h ..
+  f32x4* xo = reinterpret_cast<f32x4*>(smem);                                     // [wave][PC][64]
+  float* xs = reinterpret_cast<float*>(smem + (size_t)kManyWaves * PC * 64 * 16);  // [wave][2][64]
+#pragma unroll
+  for (int i = 0; i < PC; ++i) {
+    const f32x16& a = o[i / 4];
+    const int e = 4 * (i % 4);
+    xo[(wave * PC + i) * 64 + lane] = f32x4{a[e], a[e + 1], a[e + 2], a[e + 3]};
+  }
+  xs[wave * 128 + lane] = m;
+  xs[wave * 128 + 64 + lane] = pair_sum(l);
+  __syncthreads();
+  float mm = -INFINITY, al[NS], ll = 0.f;
+#pragma unroll
+  for (int a = 0; a < NS; ++a) {
+    al[a] = xs[(a * GW + wg) * 128 + lane];
+    mm = fmaxf(mm, al[a]);
+  }
+  const float mu = mm == -INFINITY ? 0.f : mm;
+  f32x4 w[NM] = {};
+#pragma unroll
+  for (int a = 0; a < NS; ++a) {
+    al[a] = __builtin_amdgcn_exp2f(al[a] - mu);
+    ll += xs[(a * GW + wg) * 128 + 64 + lane] * al[a];
+#pragma unroll
+    for (int i = 0; i < NM; ++i) w[i] += xo[((a * GW + wg) * PC + ns * NM + i) * 64 + lane] * al[a];
+  }
+  int64_t tok;
+  int head;
+  if (!pair_of(&tok, &head)) return;
+  auto d_of = [&](int i) { return 32 * ((ns * NM + i) >> 2) + 8 * ((ns * NM + i) & 3) + 4 * h; };
+  if (end <= sp.many_chunk) {
+    const float inv = ll == 0.f ? 0.f : 1.0f / ll;  // no key: zeros
+    uint16_t* dst = p.out + tok * p.ldo + (int64_t)head * HD;
+#pragma unroll
+    for (int i = 0; i < NM; ++i) {
+      const f32x4 y = w[i] * inv;
+      *reinterpret_cast<u32x2*>(dst + d_of(i)) = u32x2{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
+    }
+  } else {
+    const int64_t at = part_index(p, sp, tok, head, part);
+#pragma unroll
+    for (int i = 0; i < NM; ++i) *reinterpret_cast<f32x4*>(p.ws + at * HD + d_of(i)) = w[i];
+    if (ns == 0 && h == 0) *reinterpret_cast<f32x2*>(part_stats(p, sp, HD) + at * 2) = (f32x2){mm, ll};
+  }
 }
 
 // The parts of a (row, head) pair joined (the first `pairs` of each sequence and kv head): a block each, HD / 4 threads to a part, so
