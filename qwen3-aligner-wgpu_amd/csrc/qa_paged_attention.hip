@@ -179,7 +179,9 @@ Split split_of(const PagedAttnParams& p) {
     static const int GWE=getenv("QA_GW")?atoi(getenv("QA_GW")):2;
     s.many_rows = 32 * GWE;
     s.tiles = (int)((rows + s.many_rows - 1) / s.many_rows);
-    divide(heads * s.tiles, MW, ML, &s.many_chunk, &s.many_chunks);
+    // the tiles that a batch of this many rows can have, besides the short ends
+    const int64_t tiles = (p.kv.tokens * p.rep + s.many_rows - 1) / s.many_rows;
+    divide(tiles * p.kv.nkvh, MW, ML, &s.many_chunk, &s.many_chunks);
   }
   s.parts = s.many_chunks > s.few_chunks ? s.many_chunks : s.few_chunks;
   return s;
@@ -588,12 +590,11 @@ constexpr int few_lds() {
   return tiles > join ? tiles : join;
 }
 template <int DT, bool F8, int HD>
-__global__ void __launch_bounds__(64 * kFewWaves) paged_few_kernel(const PagedAttnParams p, const Split sp) {
+__device__ __forceinline__ void few_block(const PagedAttnParams& p, const Split& sp, int block, unsigned char* smem) {
   using C = Cfg<DT, F8, HD>;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[few_lds<DT, F8, HD>()];
   const PagedParams& kv = p.kv;
-  const int h = (int)(blockIdx.x % kv.nkvh);
-  const int part = (int)(blockIdx.x / kv.nkvh % sp.few_chunks), s = (int)(blockIdx.x / kv.nkvh / sp.few_chunks);
+  const int h = block % kv.nkvh;
+  const int part = block / kv.nkvh % sp.few_chunks, s = block / kv.nkvh / sp.few_chunks;
   const SeqSpan sq = seq_span(kv, s);
   if (sq.n == 0 || sq.n * p.rep > kFewRows) return;
   const int end = sq.pos0 + sq.n;  // keys that the last row sees
@@ -655,6 +656,12 @@ __global__ void __launch_bounds__(64 * kFewWaves) paged_few_kernel(const PagedAt
   }
   __syncthreads();  // the tiles' LDS is the join's
   finish<DT, F8, HD, 1, 1, kFewWaves>(p, sp, sq, h, 0, part, end <= sp.few_chunk, m, l, o, smem);
+}
+
+template <int DT, bool F8, int HD>
+__global__ void __launch_bounds__(64 * kFewWaves) paged_few_kernel(const PagedAttnParams p, const Split sp) {
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[few_lds<DT, F8, HD>()];
+  few_block<DT, F8, HD>(p, sp, (int)blockIdx.x, smem);
 }
 
 // ---- tiles of 64 or 128 (row, head) pairs ----
@@ -824,8 +831,8 @@ constexpr int many_buffers() {  // buffers of each tile: two where 128 KB hold t
 template <int DT, bool F8, int HD, int GW>
 constexpr int many_lds() {
   constexpr int tiles = kManyWaves / GW * 2 * Cfg<DT, F8, HD>::TILE * many_buffers<DT, F8, HD, GW>();
-  constexpr int join = kManyWaves * 64 * 4 * (HD / 2 + 2);
-  return tiles > join ? tiles : join;
+  constexpr int join = kManyWaves * 64 * 4 * (HD / 2 + 2), few = few_lds<DT, F8, HD>();
+  return tiles > join ? (tiles > few ? tiles : few) : (join > few ? join : few);
 }
 template <int DT, bool F8, int HD, int GW>
 __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const PagedAttnParams p, const Split sp) {
@@ -834,9 +841,14 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
   constexpr int TR = GW * 32, VX = F8 ? 2 : 4;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[many_lds<DT, F8, HD, GW>()];
   const PagedParams& kv = p.kv;
+  const int per = sp.tiles * sp.many_chunks, mine = (int)blockIdx.x - per * kv.nkvh * kv.seqs;
+  if (mine >= 0) {  // behind them, the blocks of the sequences of few rows, four waves each
+    if (threadIdx.x < 64 * kFewWaves) few_block<DT, F8, HD>(p, sp, mine, smem);
+    return;
+  }
   const int kvh = (int)(blockIdx.x % kv.nkvh);
-  const int64_t b = blockIdx.x / kv.nkvh;
-  const int per = sp.tiles * sp.many_chunks, un = (int)(b % per), s = (int)(b / per);
+  const int b = blockIdx.x / kv.nkvh;
+  const int un = b % per, s = b / per;
   const SeqSpan sq = seq_span(kv, s);
   const int NR = sq.n * p.rep;
   if (NR == 0 || (sp.few && NR <= kFewRows)) return;
@@ -1033,69 +1045,79 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
   }
 }
 
-// The parts of a (row, head) pair joined (the first `pairs` of each sequence and kv head): a block each, HD / 4 threads to a part, so
-// that 8 (hd 128) or 16 (hd 64) parts load at once and each thread has four of
-// those rounds in flight; the partial sums then meet in LDS.
+// The parts of (row, head) pairs joined, HD / 4 threads to a part, four parts in
+// flight for each thread.  A short sequence's pair may have many parts: a block
+// takes one, 8 (hd 128) or 16 (hd 64) parts at once, whose sums meet in LDS.  A long
+// sequence's have few: a block takes 8 or 16 pairs, one part after the other.
 template <int DT, int HD>
-__global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p, const Split sp, int pairs) {
-  constexpr int TP = HD / 4, NP = 256 / TP;  // threads to a part, parts at once
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p, const Split sp, int groups) {
+  constexpr int TP = HD / 4, NP = 256 / TP;
   __shared__ f32x4 xo[NP][TP];
   __shared__ float xs[NP];
-  const int h = (int)(blockIdx.x % p.kv.nkvh);
-  const int64_t b = blockIdx.x / p.kv.nkvh;
-  const int s = (int)(b / pairs), R = (int)(b % pairs);
+  const int h = (int)(blockIdx.x % p.kv.nkvh), b = (int)(blockIdx.x / p.kv.nkvh);
+  const int s = b / groups;
   const SeqSpan sq = seq_span(p.kv, s);
   const int NR = sq.n * p.rep;
-  if (R >= NR) return;
-  const int i = R / p.rep, head = h * p.rep + R % p.rep;
   const bool few = sp.few && NR <= kFewRows;
+  const int lane = threadIdx.x & 63, pt = threadIdx.x / TP, d = threadIdx.x % TP;
+  const int R = few ? b % groups : b % groups * NP + pt;
+  if (R >= NR) return;  // (few: the block as one)
+  const int chunk = few ? sp.few_chunk : sp.many_chunk;
   const int last = few ? NR - 1 : min((R / sp.many_rows + 1) * sp.many_rows, NR) - 1;
-  const int chunk = few ? sp.few_chunk : sp.many_chunk, keys = sq.pos0 + last / p.rep + 1;
+  const int keys = sq.pos0 + last / p.rep + 1;
   if (keys <= chunk) return;  // its tile has written the result
   const int parts = (keys + chunk - 1) / chunk;
+  const int i = R / p.rep, head = h * p.rep + R % p.rep;
   const int64_t t = sq.row0 + i, at = part_index(p, sp, t, head, 0);
   const float* st = part_stats(p, sp, HD) + at * 2;
-  const int lane = threadIdx.x & 63, pt = threadIdx.x / TP, d = threadIdx.x % TP;
+  const float* src = p.ws + at * HD + d * 4;
   float mm = -INFINITY;
-  for (int a = lane; a < parts; a += 64) mm = fmaxf(mm, st[2 * a]);
+  if (few) {
+    for (int a = lane; a < parts; a += 64) mm = fmaxf(mm, st[2 * a]);
 #pragma unroll
-  for (int e = 32; e > 0; e >>= 1) mm = fmaxf(mm, __shfl_xor(mm, e, 64));
+    for (int e = 32; e > 0; e >>= 1) mm = fmaxf(mm, __shfl_xor(mm, e, 64));
+  } else {
+    for (int a = 0; a < parts; ++a) mm = fmaxf(mm, st[2 * a]);
+  }
   const float mu = mm == -INFINITY ? 0.f : mm;
+  const int first = few ? pt : 0, step = few ? NP : 1;
   float ll = 0.f;
   f32x4 y = {0, 0, 0, 0};
-  const float* src = p.ws + at * HD + d * 4;
-  for (int a0 = pt; a0 < parts; a0 += 4 * NP) {
+  for (int a0 = first; a0 < parts; a0 += 4 * step) {
     f32x4 v[4];
     f32x2 ml[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int a = min(a0 + e * NP, parts - 1);
+      const int a = min(a0 + e * step, parts - 1);
       v[e] = *reinterpret_cast<const f32x4*>(src + (int64_t)a * HD);
       ml[e] = *reinterpret_cast<const f32x2*>(st + 2 * a);
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float al = a0 + e * NP < parts ? __builtin_amdgcn_exp2f(ml[e][0] - mu) : 0.f;
+      const float al = a0 + e * step < parts ? __builtin_amdgcn_exp2f(ml[e][0] - mu) : 0.f;
       ll += ml[e][1] * al;
       y += v[e] * al;
     }
   }
-  xo[pt][d] = y;
-  if (d == 0) xs[pt] = ll;
-  __syncthreads();
-  if (pt > 0) return;
-  for (int e = 1; e < NP; ++e) {
-    y += xo[e][d];
-    ll += xs[e];
+  if (few) {
+    xo[pt][d] = y;
+    if (d == 0) xs[pt] = ll;
+    __syncthreads();
+    if (pt > 0) return;
+    for (int e = 1; e < NP; ++e) {
+      y += xo[e][d];
+      ll += xs[e];
+    }
   }
   y *= ll == 0.f ? 0.f : 1.0f / ll;
   *reinterpret_cast<u32x2*>(p.out + t * p.ldo + (int64_t)head * HD + d * 4) = u32x2{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
 }
 
-// Pairs of a sequence and kv head that may come in parts.
-int64_t join_pairs(const PagedAttnParams& p, const Split& sp) {
-  const int64_t rows = (int64_t)p.kv.max_rows * p.rep;
-  return sp.many_chunks > 1 || rows < kFewRows ? rows : kFewRows;
+// Blocks of the join for a sequence and kv head.
+int64_t join_groups(const PagedAttnParams& p, const Split& sp, int hd) {
+  const int64_t rows = (int64_t)p.kv.max_rows * p.rep, few = rows < kFewRows ? rows : kFewRows;
+  const int64_t many = (rows + 1024 / hd - 1) / (1024 / hd);
+  return sp.many_chunks > 1 && many > few ? many : few;
 }
 
 template <int DT, bool F8, int HD>
@@ -1103,15 +1125,15 @@ hipError_t launch_one(const PagedAttnParams& p, hipStream_t s) {
   const Split sp = split_of(p);
   const int64_t heads = (int64_t)p.kv.seqs * p.kv.nkvh;
   if (sp.many) {
-    const dim3 grid((unsigned)(heads * sp.tiles * sp.many_chunks)), block(64 * kManyWaves);
+    const dim3 grid((unsigned)(heads * (sp.tiles * sp.many_chunks + (sp.few ? sp.few_chunks : 0)))), block(64 * kManyWaves);
     if (sp.many_rows == 64) hipLaunchKernelGGL((paged_many_kernel<DT, F8, HD, 2>), grid, block, 0, s, p, sp);
     else hipLaunchKernelGGL((paged_many_kernel<DT, F8, HD, 4>), grid, block, 0, s, p, sp);
-  }
-  if (sp.few)
+  } else {
     hipLaunchKernelGGL((paged_few_kernel<DT, F8, HD>), dim3((unsigned)(heads * sp.few_chunks)), dim3(64 * kFewWaves), 0, s, p, sp);
+  }
   if (sp.parts > 1) {
-    const int64_t pairs = join_pairs(p, sp);
-    hipLaunchKernelGGL((paged_join_kernel<DT, HD>), dim3((unsigned)(heads * pairs)), dim3(256), 0, s, p, sp, (int)pairs);
+    const int64_t groups = join_groups(p, sp, HD);
+    hipLaunchKernelGGL((paged_join_kernel<DT, HD>), dim3((unsigned)(heads * groups)), dim3(256), 0, s, p, sp, (int)groups);
   }
   return hipGetLastError();
 }
