@@ -995,7 +995,7 @@ int qa_attention_paged_workspace(const qa_paged_attention_desc* d, size_t* bytes
   p.kv = paged_params(*d->kv, d->tokens);
   p.nqh = d->nqh;
   p.rep = d->nqh / d->kv->nkvh;
-  *bytes = qa::paged_attention_workspace(d->kv->hd, p);
+  *bytes = qa::paged_attention_workspace(d->kv->dtype == QA_E4M3, d->kv->hd, p);
   return ok();
 }
 
@@ -1014,11 +1014,11 @@ int qa_attention_paged(qa_ctx* ctx, const qa_paged_attention_desc* d) {
   p.kv = paged_params(kv, d->tokens);
   p.nqh = d->nqh;
   p.rep = d->nqh / kv.nkvh;
-  const size_t need = qa::paged_attention_workspace(kv.hd, p);
+  const size_t need = qa::paged_attention_workspace(kv.dtype == QA_E4M3, kv.hd, p);
   if (need && (!d->workspace || d->workspace_bytes < need))
     return fail(QA_EINVAL, "qa_attention_paged: a workspace of %zu bytes is needed, %zu given", need,
                 d->workspace ? d->workspace_bytes : (size_t)0);
-  if (qa::paged_attention_blocks(p) > kI32 / 2)
+  if (qa::paged_attention_blocks(kv.dtype == QA_E4M3, kv.hd, p) > kI32 / 2)
     return fail(QA_EINVAL, "qa_attention_paged: the batch is too large for one launch");
   if (!ctx) return fail(QA_EINVAL, "qa_attention_paged: null context");
   if (d->tokens == 0 || kv.seqs == 0 || kv.max_rows == 0) return ok();

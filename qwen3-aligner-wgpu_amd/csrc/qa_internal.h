@@ -384,8 +384,8 @@ struct PagedAttnParams {
   PagedParams kv;
 };
 // Blocks of the larger of a call's launches, and the bytes of its workspace.
-int64_t paged_attention_blocks(const PagedAttnParams& p);
-size_t paged_attention_workspace(int hd, const PagedAttnParams& p);
+int64_t paged_attention_blocks(bool e4m3, int hd, const PagedAttnParams& p);
+size_t paged_attention_workspace(bool e4m3, int hd, const PagedAttnParams& p);
 hipError_t launch_attention_paged(int dtype, bool e4m3, int hd, const PagedAttnParams& p, hipStream_t s);
 
 // p16: probabilities rounded once to the 16-bit format (else two 16-bit terms).

@@ -24,7 +24,6 @@
 // Keys are split: a block's waves take turns at its 64-key blocks (WK) and join
 // through LDS; beyond `chunk` keys further blocks take the next chunk, write
 // (O, max, sum) to the workspace, and paged_join_kernel joins them.
-#include <stdlib.h>
 #include <type_traits>
 
 #include "qa_internal.h"
@@ -140,28 +139,40 @@ struct Cfg {
   static constexpr int TILE = 64 * HD * ES;                      // bytes of a K or V tile
 };
 
-// How a call's rows and keys are divided among blocks.
+// How a call's rows and keys are divided among blocks, from its sizes alone (lengths
+// are on the device), so that the workspace is known without one.
 //  * few: a sequence of at most kFewRows (row, head) pairs is one column group; a
 //    block's four waves take turns at a chunk of its keys, each with tiles of its
-//    own.
-//  * many: tiles of kManyRows pairs.
+//    own.  Bound by the cache's bytes: enough blocks for the LDS of every CU, cut into
+//    chunks of 256 keys (a block of keys for each wave) or more and at most 32, as
+//    the join reads them all.  Unsplit up to 512 keys: one step behind 322 keys 9.2
+//    us in one part, 10.7 in two; behind 1500 13.1 in three of 512, 11.1 in six of 256.
+//    Blocks wanted, us: 64 heads behind 8000 (f16) 256 43.4, 512 45.9, 1024 52.6;
+//    256 behind 4352 (f16) 70.1, 73.8, 81; 192 behind 8192 (e4m3, whose blocks fit
+//    two to a CU) 62.8, 52.5, 53.4; 8 behind 32770 (e4m3) 19.2, in 64 parts 21.3.
+//  * many: tiles of 64 or 128 pairs.  Of 64 up to 700 tiles: 128-row blocks load each
+//    tile for twice the rows, but are half as many, each with twice the steps (8 kv
+//    heads, no past, 64 -> 128, us: 1500 rows 29.8 -> 41.9, 2500 67 -> 65, 3500 108 ->
+//    92, 4334 155 -> 144).  Their keys are split while the CUs take the parts at once:
+//    64 rows behind 16000 keys 178 us whole, 28.8 in 32 parts; but 771 behind 1536
+//    (200 blocks) 35 whole, 45 in two, as half the CUs' parts have to wait.
 constexpr int kFewRows = 16, kFewWaves = 4;
 constexpr int kManyWaves = 8;
+constexpr int kCus = 256;
 struct Split {
-  int few, many;                // which of the two kernels run
+  int few, many;                // which of the two kinds the batch may hold
   int few_chunk, few_chunks;    // keys of a part, parts of the longest sequence
   int many_chunk, many_chunks;
   int many_rows;                // pairs of a tile
-  int tiles;                    // tiles of the longest sequence of `many`
+  int tiles;                    // tiles that all sequences of `many` can have together
   int parts;                    // partial results per row; 1: no workspace
 };
 
-Split split_of(const PagedAttnParams& p) {
+Split split_of(const PagedAttnParams& p, bool e4m3, int hd) {
   Split s{};
   const int64_t rows = (int64_t)p.kv.max_rows * p.rep, len = p.kv.max_len > 1 ? p.kv.max_len : 1;
   const int64_t heads = (int64_t)p.kv.seqs * p.kv.nkvh;
-  auto divide = [&](int64_t blocks, int64_t want, int64_t least, int* chunk, int* chunks) {
-    const int64_t parts = blocks > 0 ? (want + blocks - 1) / blocks : 1;
+  auto divide = [&](int64_t parts, int64_t least, int* chunk, int* chunks) {
     int64_t c = (len + parts - 1) / parts;
     c = ((c < least ? least : c) + 255) & ~(int64_t)255;
     *chunk = (int)c;
@@ -171,17 +182,22 @@ Split split_of(const PagedAttnParams& p) {
   // where every sequence has to have the most rows for the batch to be as long as
   // it is, none is a short one
   s.few = !s.many || (int64_t)p.kv.seqs * p.kv.max_rows > p.kv.tokens;
-  static const int W=getenv("QA_PW")?atoi(getenv("QA_PW")):256, Lc=getenv("QA_PL")?atoi(getenv("QA_PL")):512;
-  static const int MW=getenv("QA_MW")?atoi(getenv("QA_MW")):256, ML=getenv("QA_ML")?atoi(getenv("QA_ML")):512;
   s.few_chunks = s.many_chunks = 1;
-  if (s.few) divide(heads, W, Lc, &s.few_chunk, &s.few_chunks);
+  if (s.few) {
+    const int64_t want = !e4m3 && hd == 128 ? kCus : 2 * kCus, parts = heads ? (want + heads - 1) / heads : 1;
+    divide(len <= 512 ? 1 : parts < 32 ? parts : 32, 256, &s.few_chunk, &s.few_chunks);
+  }
   if (s.many) {
-    static const int GWE=getenv("QA_GW")?atoi(getenv("QA_GW")):2;
-    s.many_rows = 32 * GWE;
-    s.tiles = (int)((rows + s.many_rows - 1) / s.many_rows);
-    // the tiles that a batch of this many rows can have, besides the short ends
-    const int64_t tiles = (p.kv.tokens * p.rep + s.many_rows - 1) / s.many_rows;
-    divide(tiles * p.kv.nkvh, MW, ML, &s.many_chunk, &s.many_chunks);
+    // full tiles of a batch of this many rows, and a sequence's short last one; a
+    // sequence has to have rows for that, more than few where `few` takes the others
+    const int64_t pairs = p.kv.tokens * p.rep, least = s.few ? kFewRows + 1 : p.rep;
+    const int64_t ends = pairs / least < p.kv.seqs ? pairs / least : p.kv.seqs;
+    auto about = [&](int64_t r) { return p.kv.nkvh * ((pairs + r - 1) / r > ends ? (pairs + r - 1) / r : ends); };
+    s.many_rows = about(64) > 700 ? 128 : 64;
+    const int64_t most = (int64_t)p.kv.seqs * ((rows + s.many_rows - 1) / s.many_rows);
+    s.tiles = (int)(pairs / s.many_rows + ends < most ? pairs / s.many_rows + ends : most);
+    const int64_t blocks = about(s.many_rows);
+    divide(blocks > 0 && blocks < kCus ? kCus / blocks : 1, 512, &s.many_chunk, &s.many_chunks);
   }
   s.parts = s.many_chunks > s.few_chunks ? s.many_chunks : s.few_chunks;
   return s;
@@ -834,6 +850,36 @@ constexpr int many_lds() {
   constexpr int join = kManyWaves * 64 * 4 * (HD / 2 + 2), few = few_lds<DT, F8, HD>();
   return tiles > join ? (tiles > few ? tiles : few) : (join > few ? join : few);
 }
+// Tile number u of all the sequences' tiles of TR pairs, one sequence after the
+// other, in each the last first (it sees the most keys): every wave adds up the
+// sequences' tiles, 64 sequences at a time.
+template <int TR>
+__device__ __forceinline__ bool find_tile(const PagedAttnParams& p, const Split& sp, int u, int* seq, int* tile) {
+  const PagedParams& kv = p.kv;
+  const int lane = threadIdx.x & 63;
+  for (int s0 = 0; s0 < kv.seqs; s0 += 64) {
+    int mine = 0;
+    if (s0 + lane < kv.seqs) {
+      const int NR = seq_span(kv, s0 + lane).n * p.rep;
+      mine = sp.few && NR <= kFewRows ? 0 : (NR + TR - 1) / TR;
+    }
+    int upto = mine;
+#pragma unroll
+    for (int e = 1; e < 64; e <<= 1) {
+      const int x = __shfl_up(upto, e, 64);
+      upto += lane >= e ? x : 0;
+    }
+    const uint64_t after = __builtin_amdgcn_ballot_w64(upto > u);
+    if (after) {
+      const int at = __builtin_ctzll(after);
+      *seq = scalar(s0 + at);
+      *tile = __builtin_amdgcn_readlane(upto, at) - 1 - u;
+      return true;
+    }
+    u -= __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
+}
 template <int DT, bool F8, int HD, int GW>
 __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const PagedAttnParams p, const Split sp) {
   using C = Cfg<DT, F8, HD>;
@@ -841,20 +887,17 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
   constexpr int TR = GW * 32, VX = F8 ? 2 : 4;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[many_lds<DT, F8, HD, GW>()];
   const PagedParams& kv = p.kv;
-  const int per = sp.tiles * sp.many_chunks, mine = (int)blockIdx.x - per * kv.nkvh * kv.seqs;
+  const int mine = (int)blockIdx.x - sp.tiles * sp.many_chunks * kv.nkvh;
   if (mine >= 0) {  // behind them, the blocks of the sequences of few rows, four waves each
     if (threadIdx.x < 64 * kFewWaves) few_block<DT, F8, HD>(p, sp, mine, smem);
     return;
   }
   const int kvh = (int)(blockIdx.x % kv.nkvh);
-  const int b = blockIdx.x / kv.nkvh;
-  const int un = b % per, s = b / per;
+  const int part = blockIdx.x / kv.nkvh / sp.tiles;
+  int tile, s;
+  if (!find_tile<TR>(p, sp, blockIdx.x / kv.nkvh % sp.tiles, &s, &tile)) return;
   const SeqSpan sq = seq_span(kv, s);
   const int NR = sq.n * p.rep;
-  if (NR == 0 || (sp.few && NR <= kFewRows)) return;
-  // the last tiles, which see the most keys, first
-  const int tile = (NR + TR - 1) / TR - 1 - un % sp.tiles, part = un / sp.tiles;
-  if (tile < 0) return;
   const int end = sq.pos0 + (min((tile + 1) * TR, NR) - 1) / p.rep + 1;
   const int k0 = part * sp.many_chunk, k1 = min(k0 + sp.many_chunk, end);
   if (part > 0 && k0 >= end) return;
@@ -1122,10 +1165,11 @@ int64_t join_groups(const PagedAttnParams& p, const Split& sp, int hd) {
 
 template <int DT, bool F8, int HD>
 hipError_t launch_one(const PagedAttnParams& p, hipStream_t s) {
-  const Split sp = split_of(p);
+  const Split sp = split_of(p, F8, HD);
   const int64_t heads = (int64_t)p.kv.seqs * p.kv.nkvh;
   if (sp.many) {
-    const dim3 grid((unsigned)(heads * (sp.tiles * sp.many_chunks + (sp.few ? sp.few_chunks : 0)))), block(64 * kManyWaves);
+    const dim3 grid((unsigned)((int64_t)p.kv.nkvh * sp.tiles * sp.many_chunks + (sp.few ? heads * sp.few_chunks : 0)));
+    const dim3 block(64 * kManyWaves);
     if (sp.many_rows == 64) hipLaunchKernelGGL((paged_many_kernel<DT, F8, HD, 2>), grid, block, 0, s, p, sp);
     else hipLaunchKernelGGL((paged_many_kernel<DT, F8, HD, 4>), grid, block, 0, s, p, sp);
   } else {
@@ -1146,16 +1190,16 @@ hipError_t launch_dt(bool e4m3, int hd, const PagedAttnParams& p, hipStream_t s)
 
 }  // namespace
 
-int64_t paged_attention_blocks(const PagedAttnParams& p) {
-  const Split sp = split_of(p);
+int64_t paged_attention_blocks(bool e4m3, int hd, const PagedAttnParams& p) {
+  const Split sp = split_of(p, e4m3, hd);
   // in doubles, as no product of these sizes need fit 64 bits; the caller compares with a bound far below
   const double heads = (double)p.kv.seqs * p.kv.nkvh, rows = (double)p.kv.max_rows * p.rep;
-  const double most = heads * fmax(fmax((double)sp.tiles * sp.many_chunks, sp.few_chunks), rows);
+  const double most = fmax(heads * fmax(sp.few_chunks, rows), heads * sp.few_chunks + (double)p.kv.nkvh * sp.tiles * sp.many_chunks);
   return most > 9e18 ? INT64_MAX : (int64_t)most;
 }
 
-size_t paged_attention_workspace(int hd, const PagedAttnParams& p) {
-  const Split sp = split_of(p);
+size_t paged_attention_workspace(bool e4m3, int hd, const PagedAttnParams& p) {
+  const Split sp = split_of(p, e4m3, hd);
   return sp.parts > 1 ? (size_t)p.kv.tokens * p.nqh * sp.parts * (hd + 2) * sizeof(float) : 0;
 }
 
