@@ -362,7 +362,8 @@ typedef struct qa_paged_kv {
 /* qa_qk_norm_rope for a packed batch: per-head q / k RMSNorm and rotate-half RoPE
  * of the fused qkv rows, q to q_out, K and V (verbatim) to their pages.
  *   qkv     [tokens][(nqh + 2 nkvh) hd], row stride ldqkv: q heads, k, v
- *   cos,sin f32 [tokens][hd], a row for each row of the batch (qa_mrope_rows)
+ *   cos,sin f32 [tokens][hd], a row for each row of the batch, its second half
+ *           repeating the first (qa_mrope_rows), which alone is read
  *   q_out   [tokens][nqh hd], row stride ldq
  * In a QA_E4M3 cache a page's scale is the least power of two p with amax <= 448 p
  * over what the page holds of that head (2^-110 <= p <= 2^120), rounded to

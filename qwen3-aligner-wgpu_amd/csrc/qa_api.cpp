@@ -965,10 +965,8 @@ int qa_kv_append(qa_ctx* ctx, const qa_kv_append_desc* d) {
   if (!(d->eps >= 0.0f)) return fail(QA_EINVAL, "qa_kv_append: eps must be >= 0");
   qa::AppendParams p{};
   p.kv = paged_params(kv, d->tokens);
-  // blocks: four (row, group of heads) each, and one for each page a sequence may touch
-  const int64_t most = qa::pages_touched(p.kv.max_rows, p.kv.lp);
-  if ((d->tokens * ((d->nqh + 1024 / kv.hd - 1) / (1024 / kv.hd)) + 3) / 4 > kI32 / 2 ||
-      (double)most * (double)kv.seqs * kv.nkvh > kI32 / 2)
+  // blocks: four rows each, and one for each page a sequence may touch
+  if ((double)qa::pages_touched(p.kv.max_rows, p.kv.lp) * (double)kv.seqs * kv.nkvh > kI32 / 2)
     return fail(QA_EINVAL, "qa_kv_append: the batch is too large for one launch");
   if (!ctx) return fail(QA_EINVAL, "qa_kv_append: null context");
   if (d->tokens == 0 || kv.seqs == 0) return ok();

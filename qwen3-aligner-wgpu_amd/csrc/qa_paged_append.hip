@@ -2,8 +2,10 @@
 // RMSNorm and rotation as in qk_norm_rope_kernel, q to its rows, K and V to the
 // slots of their sequences' pages, in the 16-bit format or in e4m3.
 //
-// One grid.  The first blocks take the q heads, HD / 16 lanes to a head, each
-// lane with the 8-element chunk c and its rotation partners, chunk c + HD / 16.
+// One grid.  The first blocks take the q heads, a wave to a row, HD / 16 lanes to a
+// head, each lane with the 8-element chunk c and its rotation partners, chunk c +
+// HD / 16; the row's cosines and sines and the norm's weights stay in registers
+// from head to head.
 // Each other block takes one (sequence, page, kv head): the rows of this call
 // that fall into that page, K and V.  A page is one block's because an e4m3 page
 // has one scale: its block finds the largest new value, raises the scale if it
@@ -55,27 +57,32 @@ __device__ __forceinline__ float finite_abs(float x) {
   return a < INFINITY ? a : 0.f;  // NaN too
 }
 
-// The normed and rotated chunks c and c + HD / 16 of a q or k head, for the
-// HD / 16 lanes that share it (all of them call, `on` or not).
-template <int DT, int HD>
-__device__ __forceinline__ void norm_rope(const uint16_t* raw, const float* nw, const float* cs, const float* sn,
-                                          int c, float eps, bool on, float* xa, float* xb) {
-  constexpr int L = HD / 16, half = HD / 2;
-  u32x4 va = {0, 0, 0, 0}, vb = {0, 0, 0, 0};
-  f32x4 t[12] = {};
-  if (on) {
-    va = *reinterpret_cast<const u32x4*>(raw + 8 * c);
-    vb = *reinterpret_cast<const u32x4*>(raw + half + 8 * c);
+// What a lane needs for its chunk c of every head: the norm's weights of both chunks,
+// and the row's cosines and sines (whose second half repeats the first).
+struct Turn {
+  float wa[8], wb[8], co[8], si[8];
+};
+__device__ __forceinline__ void load8(float* to, const float* from) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      t[h] = *reinterpret_cast<const f32x4*>(nw + 8 * c + 4 * h);
-      t[2 + h] = *reinterpret_cast<const f32x4*>(nw + half + 8 * c + 4 * h);
-      t[4 + h] = *reinterpret_cast<const f32x4*>(cs + 8 * c + 4 * h);
-      t[6 + h] = *reinterpret_cast<const f32x4*>(cs + half + 8 * c + 4 * h);
-      t[8 + h] = *reinterpret_cast<const f32x4*>(sn + 8 * c + 4 * h);
-      t[10 + h] = *reinterpret_cast<const f32x4*>(sn + half + 8 * c + 4 * h);
-    }
+  for (int h = 0; h < 2; ++h) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(from + 4 * h);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) to[4 * h + e] = v[e];
   }
+}
+template <int HD>
+__device__ __forceinline__ Turn load_turn(const float* nw, const float* cs, const float* sn, int c) {
+  Turn t;
+  load8(t.wa, nw + 8 * c);
+  load8(t.wb, nw + HD / 2 + 8 * c);
+  load8(t.co, cs + 8 * c);
+  load8(t.si, sn + 8 * c);
+  return t;
+}
+// The normed and rotated chunks of a q or k head from its raw ones, for the HD / 16
+// lanes that share it (all of them call).
+template <int DT, int HD>
+__device__ __forceinline__ void norm_rope(u32x4 va, u32x4 vb, const Turn& t, float eps, float* xa, float* xb) {
   float s = 0.f;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
@@ -91,14 +98,13 @@ __device__ __forceinline__ void norm_rope(const uint16_t* raw, const float* nw, 
     s += xb[e] * xb[e];
   }
 #pragma unroll
-  for (int o = 1; o < L; o <<= 1) s += __shfl_xor(s, o, 64);
+  for (int o = 1; o < HD / 16; o <<= 1) s += __shfl_xor(s, o, 64);
   const float inv = 1.0f / sqrtf(s / (float)HD + eps);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const int h = e >> 2, i = e & 3;
-    const float a = xa[e] * inv * t[h][i], b = xb[e] * inv * t[2 + h][i];
-    xa[e] = a * t[4 + h][i] - b * t[8 + h][i];
-    xb[e] = b * t[6 + h][i] + a * t[10 + h][i];
+    const float a = xa[e] * inv * t.wa[e], b = xb[e] * inv * t.wb[e];
+    xa[e] = a * t.co[e] - b * t.si[e];
+    xb[e] = b * t.co[e] + a * t.si[e];
   }
 }
 
@@ -109,23 +115,33 @@ __device__ __forceinline__ u32x4 pack8(const float* x) {
 
 template <int DT, int HD>
 __device__ __forceinline__ void q_part(const AppendParams& p, int64_t bx) {
-  constexpr int L = HD / 16, hpw = 64 / L;
-  const int lane = threadIdx.x & 63;
-  const int groups = (p.nqh + hpw - 1) / hpw;
-  const int64_t item = bx * 4 + (threadIdx.x >> 6);
-  const int64_t t = item / groups;
+  constexpr int L = HD / 16, hpw = 64 / L;  // lanes to a head, heads at once
+  const int lane = threadIdx.x & 63, c = lane % L, sub = lane / L;
+  const int64_t t = bx * 4 + (threadIdx.x >> 6);
   // rows of no sequence keep what they hold
   const int64_t t0 = p.kv.row_start[0], t1 = p.kv.row_start[p.kv.seqs];
   if (t >= p.kv.tokens || t < t0 || t >= t1) return;
-  const int head = (int)(item % groups) * hpw + lane / L, c = lane % L;
-  const bool on = head < p.nqh;
-  float xa[8], xb[8];
-  norm_rope<DT, HD>(p.qkv + t * p.ldqkv + (int64_t)(on ? head : 0) * HD, p.qn, p.cos + t * HD, p.sin + t * HD, c, p.eps, on,
-                    xa, xb);
-  if (!on) return;
-  uint16_t* dst = p.q_out + t * p.ldq + (int64_t)head * HD + 8 * c;
-  *reinterpret_cast<u32x4*>(dst) = pack8<DT>(xa);
-  *reinterpret_cast<u32x4*>(dst + HD / 2) = pack8<DT>(xb);
+  const Turn turn = load_turn<HD>(p.qn, p.cos + t * HD, p.sin + t * HD, c);
+  const uint16_t* src = p.qkv + t * p.ldqkv + 8 * c;
+  uint16_t* dst = p.q_out + t * p.ldq + 8 * c;
+  auto load = [&](int head, u32x4* a, u32x4* b) {  // past the last head: the last again
+    const uint16_t* raw = src + (int64_t)min(head, p.nqh - 1) * HD;
+    *a = *reinterpret_cast<const u32x4*>(raw);
+    *b = *reinterpret_cast<const u32x4*>(raw + HD / 2);
+  };
+  u32x4 va, vb, na, nb;
+  load(sub, &va, &vb);
+  for (int h0 = 0; h0 < p.nqh; h0 += hpw) {
+    load(h0 + hpw + sub, &na, &nb);  // the next heads, while these are at work
+    float xa[8], xb[8];
+    norm_rope<DT, HD>(va, vb, turn, p.eps, xa, xb);
+    if (h0 + sub < p.nqh) {
+      *reinterpret_cast<u32x4*>(dst + (int64_t)(h0 + sub) * HD) = pack8<DT>(xa);
+      *reinterpret_cast<u32x4*>(dst + (int64_t)(h0 + sub) * HD + HD / 2) = pack8<DT>(xb);
+    }
+    va = na;
+    vb = nb;
+  }
 }
 
 // A page's 8-bit values rounded again to a scale 1 / ratio times the old one.
@@ -141,12 +157,11 @@ __device__ __forceinline__ void rescale(uint8_t* page, int bytes, float ratio) {
   }
 }
 
-template <int DT, bool F8, int HD>
+template <int DT, bool F8, int HD, int NP>
 __device__ __forceinline__ void kv_part(const AppendParams& p, int64_t b, int slots) {
-  constexpr int L = HD / 16;          // lanes to a row
-  constexpr int RP = 256 / L;         // rows in a pass
-  constexpr int NP = (64 + RP - 1) / RP;  // passes over the largest page
-  __shared__ uint16_t tile[64][HD + 2];
+  constexpr int L = HD / 16;   // lanes to a row
+  constexpr int RP = 256 / L;  // rows in a pass; NP: passes over a page
+  __shared__ uint16_t tile[NP * RP][HD + 2];
   __shared__ float top[2][4];
   const PagedParams& kv = p.kv;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -175,29 +190,26 @@ __device__ __forceinline__ void kv_part(const AppendParams& p, int64_t b, int sl
   for (int i = 0; i < NP; ++i) {
     const int r = i * RP + tid / L, c = tid % L;
     const bool on = r < nr;
-    const uint16_t* row = src + (int64_t)(on ? r : 0) * p.ldqkv;
-    const float* cs = p.cos + (t0 + (on ? r : 0)) * HD;
-    const float* sn = p.sin + (t0 + (on ? r : 0)) * HD;
-    if (on) {
+    const int at = on ? r : nr - 1;  // lanes past the last row do it again, and store nothing
+    const uint16_t* row = src + (int64_t)at * p.ldqkv;
+    const u32x4 wk[2] = {*reinterpret_cast<const u32x4*>(row + 8 * c), *reinterpret_cast<const u32x4*>(row + HD / 2 + 8 * c)};
+    const Turn turn = load_turn<HD>(p.kn, p.cos + (t0 + at) * HD, p.sin + (t0 + at) * HD, c);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(row + (int64_t)kv.nkvh * HD + 16 * c + 8 * u);
+    for (int u = 0; u < 2; ++u) {
+      const u32x4 w = *reinterpret_cast<const u32x4*>(row + (int64_t)kv.nkvh * HD + 16 * c + 8 * u);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          *reinterpret_cast<uint32_t*>(&tile[r][16 * c + 8 * u + 2 * e]) = w[e];
-          if constexpr (F8) {
-            const f32x2 f = widen2<DT>(w[e]);
-            va = fmaxf(va, fmaxf(finite_abs(f[0]), finite_abs(f[1])));
-          }
+      for (int e = 0; e < 4; ++e) {
+        if (on) *reinterpret_cast<uint32_t*>(&tile[r][16 * c + 8 * u + 2 * e]) = w[e];
+        if constexpr (F8) {
+          const f32x2 f = widen2<DT>(w[e]);
+          va = fmaxf(va, fmaxf(finite_abs(f[0]), finite_abs(f[1])));
         }
       }
     }
-    norm_rope<DT, HD>(row, p.kn, cs, sn, c, p.eps, on, xa[i], xb[i]);
+    norm_rope<DT, HD>(wk[0], wk[1], turn, p.eps, xa[i], xb[i]);
     if constexpr (F8) {
-      if (on) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ka = fmaxf(ka, fmaxf(finite_abs(xa[i][e]), finite_abs(xb[i][e])));
-      }
+      for (int e = 0; e < 8; ++e) ka = fmaxf(ka, fmaxf(finite_abs(xa[i][e]), finite_abs(xb[i][e])));
     }
   }
   float kinv = 1.f, vinv = 1.f;
@@ -289,18 +301,18 @@ __device__ __forceinline__ void kv_part(const AppendParams& p, int64_t b, int sl
   }
 }
 
-template <int DT, bool F8, int HD>
+template <int DT, bool F8, int HD, int NP>
 __global__ void __launch_bounds__(256) kv_append_kernel(const AppendParams p, int64_t qblocks, int slots) {
   if ((int64_t)blockIdx.x < qblocks) q_part<DT, HD>(p, blockIdx.x);
-  else kv_part<DT, F8, HD>(p, blockIdx.x - qblocks, slots);
+  else kv_part<DT, F8, HD, NP>(p, blockIdx.x - qblocks, slots);
 }
 
 template <int DT, bool F8, int HD>
 hipError_t launch_one(const AppendParams& p, hipStream_t s) {
-  const int64_t hpw = 1024 / HD, items = p.kv.tokens * ((p.nqh + hpw - 1) / hpw), qb = (items + 3) / 4;
-  const int64_t slots = pages_touched(p.kv.max_rows, p.kv.lp);
-  hipLaunchKernelGGL((kv_append_kernel<DT, F8, HD>), dim3((unsigned)(qb + slots * p.kv.seqs * p.kv.nkvh)), dim3(256), 0, s, p,
-                     qb, (int)slots);
+  const int64_t qb = (p.kv.tokens + 3) / 4, slots = pages_touched(p.kv.max_rows, p.kv.lp);
+  const dim3 grid((unsigned)(qb + slots * p.kv.seqs * p.kv.nkvh));
+  if (HD == 128 && p.kv.lp == 6) hipLaunchKernelGGL((kv_append_kernel<DT, F8, HD, HD / 64>), grid, dim3(256), 0, s, p, qb, (int)slots);
+  else hipLaunchKernelGGL((kv_append_kernel<DT, F8, HD, 1>), grid, dim3(256), 0, s, p, qb, (int)slots);
   return hipGetLastError();
 }
 
