@@ -564,12 +564,19 @@ __device__ __forceinline__ void finish(const PagedAttnParams& p, const Split& sp
 
 // Pages, and e4m3 scales, of 16 blocks: lane 4 j + a those of the 16 keys from
 // key(j) + 16 a on.  holes: some page of the sequence's keys is none.
+// page_ids() is the part that does not need the sequence's length, so that the first
+// load can go out together with it.
+template <class Key>
+__device__ __forceinline__ int page_ids(const PagedParams& kv, int s, Key key) {
+  const int lane = threadIdx.x & 63;
+  return page_at(kv, s, key(lane >> 2) + 16 * (lane & 3));
+}
 template <bool F8, int HD, class Key>
-__device__ __forceinline__ void fetch_pages(const PagedParams& kv, const SeqSpan& sq, int s, int h, int left, Key key, Pages* pages,
+__device__ __forceinline__ void fetch_pages(const PagedParams& kv, const SeqSpan& sq, int found, int h, int left, Key key, Pages* pages,
                                             float* ks, float* vs, bool* holes) {
   const int lane = threadIdx.x & 63, pos = key(lane >> 2) + 16 * (lane & 3);
   const bool in = (lane >> 2) < left && pos < sq.len;
-  const int id = in ? page_at(kv, s, pos) : -1;
+  const int id = in ? found : -1;
   *holes |= __builtin_amdgcn_ballot_w64(in && id < 0) != 0;
   const int64_t at = id < 0 ? -1 : page_base(kv, id, h, HD) * (F8 ? 1 : 2);
   *pages = {(int)at, (int)(at >> 32)};
@@ -611,28 +618,30 @@ __device__ __forceinline__ void few_block(const PagedAttnParams& p, const Split&
   const PagedParams& kv = p.kv;
   const int h = block % kv.nkvh;
   const int part = block / kv.nkvh % sp.few_chunks, s = block / kv.nkvh / sp.few_chunks;
+  const int wave = scalar((int)(threadIdx.x >> 6)), k0 = part * sp.few_chunk;
+  auto key_of = [&](int it) { return k0 + (wave + it * kFewWaves) * 64; };
+  const int found = page_ids(kv, s, key_of);
   const SeqSpan sq = seq_span(kv, s);
   if (sq.n == 0 || sq.n * p.rep > kFewRows) return;
   const int end = sq.pos0 + sq.n;  // keys that the last row sees
-  const int k0 = part * sp.few_chunk, k1 = min(k0 + sp.few_chunk, end);
+  const int k1 = min(k0 + sp.few_chunk, end);
   if (part > 0 && k0 >= end) return;
-  const int lane = threadIdx.x & 63, wave = scalar((int)(threadIdx.x >> 6)), c = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const int nb = k1 > k0 ? (k1 - k0 + 63) >> 6 : 0, steps = (nb - wave + kFewWaves - 1) / kFewWaves;
-  auto key_of = [&](int it) { return k0 + (wave + it * kFewWaves) * 64; };
   unsigned char *kt = smem + wave * 2 * C::TILE, *vt = kt + C::TILE;
   const int lcp = kv.lp - (F8 ? 4 : 3);
   Pages pages = {-1, -1};
   float ksc = 1.f, vsc = 0.f;
   bool holes = false;
-  auto fetch = [&](int it) {
-    fetch_pages<F8, HD>(kv, sq, s, h, steps - it, [&](int j) { return key_of(it + j); }, &pages, &ksc, &vsc, &holes);
+  auto fetch = [&](int it, int ids) {
+    fetch_pages<F8, HD>(kv, sq, ids, h, steps - it, [&](int j) { return key_of(it + j); }, &pages, &ksc, &vsc, &holes);
   };
   Columns<1> col;
   col.set(p, sq, h, 0, c);
   u32x4 q[1][C::QS];
   load_q<DT, F8, HD, 1>(p, col, g, q);
   if (steps > 0) {
-    fetch(0);
+    fetch(0, found);
     load_tile<DT, F8, HD, false, 1, true>(kv, pages, 0, 0, kt);
     load_tile<DT, F8, HD, false, 1, false>(kv, pages, 0, 0, vt);
   }
@@ -659,7 +668,7 @@ __device__ __forceinline__ void few_block(const PagedAttnParams& p, const Split&
     multiply<DT, F8, HD, 1, false, true>(vt, va, lcp, ph, pl, o, kt, ka, q, sc);
     wait_lds();
     if (more) {
-      if ((it & 15) == 15) fetch(it + 1);
+      if ((it & 15) == 15) fetch(it + 1, page_ids(kv, s, [&](int j) { return key_of(it + 1 + j); }));
       load_tile<DT, F8, HD, false, 1, true>(kv, pages, (it + 1) & 15, 0, kt);
     }
     softmax<DT, F8, HD, 1>(sc, col.pos, kg, have, p.scale * kLog2e * ks, vs, m, l, o, ph, pl);
@@ -854,13 +863,15 @@ constexpr int many_lds() {
 // other, in each the last first (it sees the most keys): every wave adds up the
 // sequences' tiles, 64 sequences at a time.
 template <int TR>
-__device__ __forceinline__ bool find_tile(const PagedAttnParams& p, const Split& sp, int u, int* seq, int* tile) {
+__device__ __forceinline__ bool find_tile(const PagedAttnParams& p, const Split& sp, int u, int* seq, SeqSpan* sq, int* tile) {
   const PagedParams& kv = p.kv;
   const int lane = threadIdx.x & 63;
   for (int s0 = 0; s0 < kv.seqs; s0 += 64) {
     int mine = 0;
+    SeqSpan q = {};
     if (s0 + lane < kv.seqs) {
-      const int NR = seq_span(kv, s0 + lane).n * p.rep;
+      q = seq_span(kv, s0 + lane);
+      const int NR = q.n * p.rep;
       mine = sp.few && NR <= kFewRows ? 0 : (NR + TR - 1) / TR;
     }
     int upto = mine;
@@ -874,6 +885,10 @@ __device__ __forceinline__ bool find_tile(const PagedAttnParams& p, const Split&
       const int at = __builtin_ctzll(after);
       *seq = scalar(s0 + at);
       *tile = __builtin_amdgcn_readlane(upto, at) - 1 - u;
+      sq->row0 = __builtin_amdgcn_readlane((int)q.row0, at);
+      sq->n = __builtin_amdgcn_readlane(q.n, at);
+      sq->pos0 = __builtin_amdgcn_readlane(q.pos0, at);
+      sq->len = __builtin_amdgcn_readlane(q.len, at);
       return true;
     }
     u -= __builtin_amdgcn_readlane(upto, 63);
@@ -895,8 +910,8 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
   const int kvh = (int)(blockIdx.x % kv.nkvh);
   const int part = blockIdx.x / kv.nkvh / sp.tiles;
   int tile, s;
-  if (!find_tile<TR>(p, sp, blockIdx.x / kv.nkvh % sp.tiles, &s, &tile)) return;
-  const SeqSpan sq = seq_span(kv, s);
+  SeqSpan sq;
+  if (!find_tile<TR>(p, sp, blockIdx.x / kv.nkvh % sp.tiles, &s, &sq, &tile)) return;
   const int NR = sq.n * p.rep;
   const int end = sq.pos0 + (min((tile + 1) * TR, NR) - 1) / p.rep + 1;
   const int k0 = part * sp.many_chunk, k1 = min(k0 + sp.many_chunk, end);
@@ -918,7 +933,8 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
   auto fetch = [&](int w) {
     Pages pg = {-1, -1};
     float x = 1.f, y = 0.f;
-    fetch_pages<F8, HD>(kv, sq, s, kvh, steps - 16 * w, [&](int j) { return key_of(16 * w + j); }, &pg, &x, &y, &holes);
+    auto key = [&](int j) { return key_of(16 * w + j); };
+    fetch_pages<F8, HD>(kv, sq, page_ids(kv, s, key), kvh, steps - 16 * w, key, &pg, &x, &y, &holes);
     pages0.lo = w & 1 ? pages0.lo : pg.lo;
     pages0.hi = w & 1 ? pages0.hi : pg.hi;
     ks0 = w & 1 ? ks0 : x;
