@@ -305,7 +305,7 @@ int qa_attention_prefill(qa_ctx* ctx, const qa_attention_desc* desc);
  *   pos      int32 [axes][ldpos], any values, ldpos >= tokens
  *   cos, sin f32 [tokens][hd], 16-byte aligned
  * hd a multiple of 8 up to 256; sec0 + sec1 + sec2 = hd / 2 with none negative, those
- * past `axes` zero. */
+ * past `axes` zero; theta >= 1. */
 enum { QA_MROPE_INTERLEAVED = 1u << 0 };
 typedef struct qa_mrope_desc {
   uint32_t dtype;

@@ -84,6 +84,7 @@ bool aligned(const void* p, size_t a) { return ((uintptr_t)p % a) == 0; }
 constexpr uint32_t kKnownFlags =
     QA_ACCUMULATE | QA_EPI_GELU | QA_EPI_SILU_MUL | QA_TRANSB | QA_BIAS_ROWS;
 constexpr int64_t kI32 = 0x7fffffff;
+constexpr int64_t kBlocks = 0xffffffffLL / 512;  // a grid has less than 2^32 threads: blocks of up to 512
 
 // Byte span [lo, hi) an operand covers over all batches.
 struct Span {
@@ -922,9 +923,10 @@ int qa_mrope_rows(qa_ctx* ctx, const qa_mrope_desc* d) {
   if (sec[0] < 0 || sec[1] < 0 || sec[2] < 0 || sec[0] + sec[1] + sec[2] != d->hd / 2 || (d->axes < 3 && sec[2]) ||
       (d->axes < 2 && sec[1]))
     return fail(QA_EINVAL, "qa_mrope_rows: the axes' sections must be >= 0 and add up to hd / 2");
-  if (d->tokens < 0 || d->tokens > kI32 || d->ldpos < d->tokens || d->ldpos > kI32)
+  if (d->tokens < 0 || d->ldpos < d->tokens || d->ldpos > kI32)
     return fail(QA_EINVAL, "qa_mrope_rows: need 0 <= tokens <= ldpos < 2^31");
-  if (!(d->theta > 0.0) || !std::isfinite(d->theta)) return fail(QA_EINVAL, "qa_mrope_rows: theta must be a positive number");
+  if (d->tokens / (256 / (d->hd / 8)) >= kBlocks) return fail(QA_EINVAL, "qa_mrope_rows: the batch is too large for one launch");
+  if (!(d->theta >= 1.0) || !std::isfinite(d->theta)) return fail(QA_EINVAL, "qa_mrope_rows: theta must be a number >= 1");
   if (!d->pos || !d->cos || !d->sin) return fail(QA_EINVAL, "qa_mrope_rows: null pointer");
   if (!aligned(d->pos, 4) || !aligned(d->cos, 16) || !aligned(d->sin, 16))
     return fail(QA_EINVAL, "qa_mrope_rows: cos and sin must be 16-byte aligned");
@@ -966,7 +968,7 @@ int qa_kv_append(qa_ctx* ctx, const qa_kv_append_desc* d) {
   qa::AppendParams p{};
   p.kv = paged_params(kv, d->tokens);
   // blocks: four rows each, and one for each page a sequence may touch
-  if ((double)qa::pages_touched(p.kv.max_rows, p.kv.lp) * (double)kv.seqs * kv.nkvh > kI32 / 2)
+  if ((double)d->tokens / 4 + (double)qa::pages_touched(p.kv.max_rows, p.kv.lp) * (double)kv.seqs * kv.nkvh >= kBlocks)
     return fail(QA_EINVAL, "qa_kv_append: the batch is too large for one launch");
   if (!ctx) return fail(QA_EINVAL, "qa_kv_append: null context");
   if (d->tokens == 0 || kv.seqs == 0) return ok();
@@ -1016,7 +1018,7 @@ int qa_attention_paged(qa_ctx* ctx, const qa_paged_attention_desc* d) {
   if (need && (!d->workspace || d->workspace_bytes < need))
     return fail(QA_EINVAL, "qa_attention_paged: a workspace of %zu bytes is needed, %zu given", need,
                 d->workspace ? d->workspace_bytes : (size_t)0);
-  if (qa::paged_attention_blocks(kv.dtype == QA_E4M3, kv.hd, p) > kI32 / 2)
+  if (qa::paged_attention_blocks(kv.dtype == QA_E4M3, kv.hd, p) > kBlocks)
     return fail(QA_EINVAL, "qa_attention_paged: the batch is too large for one launch");
   if (!ctx) return fail(QA_EINVAL, "qa_attention_paged: null context");
   if (d->tokens == 0 || kv.seqs == 0 || kv.max_rows == 0) return ok();

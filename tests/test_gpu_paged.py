@@ -59,7 +59,7 @@ def _axes_of(hd, axes, sec, inter):
 @pytest.mark.parametrize("hd,sec,inter,n", [
     (128, (64,), False, 1), (128, (64,), True, 5), (128, (24, 20, 20), True, 300), (128, (16, 24, 24), False, 257), (64, (12, 20), False, 33),
     (64, (12, 20), True, 64), (8, (2, 1, 1), True, 3), (256, (128,), False, 9), (256, (0, 100, 28), False, 19), (128, (64, 0, 0), True, 7),
-    (128, (0, 32, 32), True, 40)])
+    (128, (0, 32, 32), True, 40), (24, (5, 4, 3), True, 200), (200, (100,), False, 31), (88, (20, 24), True, 47)])
 def test_mrope_rows(ctx, pkg, dtype, hd, sec, inter, n):
     rng = np.random.default_rng(hd + n)
     pos = rng.integers(0, 5000, (len(sec), n))

@@ -101,7 +101,7 @@ def test_null_arguments(pkg):
     (dict(dtype=E4M3), "dtype"), (dict(flags=2), "flags"), (dict(hd=124, sec0=22), "multiple of 8"), (dict(hd=264, sec0=92), "up to 256"),
     (dict(hd=0), "multiple of 8"), (dict(axes=0), "axes"), (dict(axes=4), "axes"), (dict(sec0=25), "sections"), (dict(axes=2), "sections"),
     (dict(sec0=65, sec1=-1, sec2=0), "sections"), (dict(axes=1, sec0=44, sec2=0), "sections"), (dict(tokens=5), "ldpos"), (dict(tokens=-1), "tokens"),
-    (dict(theta=0.0), "theta"), (dict(theta=float("nan")), "theta"), (dict(theta=float("inf")), "theta"), (dict(pos=None), "null"),
+    (dict(theta=0.0), "theta"), (dict(theta=0.999), "theta"), (dict(theta=float("nan")), "theta"), (dict(theta=float("inf")), "theta"), (dict(pos=None), "null"),
     (dict(cos=0x200004), "aligned"), (dict(pos=0x100002), "aligned"),
 ])
 def test_mrope_refusals(pkg, kw, needle):
@@ -109,6 +109,12 @@ def test_mrope_refusals(pkg, kw, needle):
 
 
 def test_batches_past_one_launch_are_refused(pkg):
+    wide = _mrope(pkg, tokens=2 ** 28, ldpos=2 ** 28)  # a grid of 2^32 threads
+    _refused(pkg, pkg.lib().qa_mrope_rows, wide, pkg.QA_EINVAL, "too large")
+    many = _kv(pkg, seqs=1, max_rows=4, max_len=128)
+    _refused(pkg, pkg.lib().qa_kv_append, _append(pkg, many, tokens=2 ** 26), pkg.QA_EINVAL, "too large")
+    big = _kv(pkg, seqs=2 ** 23, max_rows=1, max_len=128)
+    _refused(pkg, pkg.lib().qa_attention_paged, _attention(pkg, big, workspace_bytes=2 ** 62), pkg.QA_EINVAL, "too large")
     big = _kv(pkg, seqs=2 ** 30, max_rows=4, max_len=128)
     _refused(pkg, pkg.lib().qa_kv_append, _append(pkg, big), pkg.QA_EINVAL, "too large")
     _refused(pkg, pkg.lib().qa_attention_paged, _attention(pkg, big, workspace_bytes=2 ** 62), pkg.QA_EINVAL, "too large")
