@@ -1107,19 +1107,32 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
 // The parts of (row, head) pairs joined, HD / 4 threads to a part, four parts in
 // flight for each thread.  A short sequence's pair may have many parts: a block
 // takes one, 8 (hd 128) or 16 (hd 64) parts at once, whose sums meet in LDS.  A long
-// sequence's have few: a block takes 8 or 16 pairs, one part after the other.
+// sequence's have few: a block takes 8 or 16 pairs of a tile, one part after the
+// other.  The grid: the tiles' blocks, as in paged_many_kernel, then the short
+// sequences' pairs; of either as many as had to be split.
+template <int HD>
+constexpr int kJoinPairs = 1024 / HD;
 template <int DT, int HD>
-__global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p, const Split sp, int groups) {
-  constexpr int TP = HD / 4, NP = 256 / TP;
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p, const Split sp, int groups, int few_rows) {
+  constexpr int TP = HD / 4, NP = kJoinPairs<HD>;
   __shared__ f32x4 xo[NP][TP];
   __shared__ float xs[NP];
-  const int h = (int)(blockIdx.x % p.kv.nkvh), b = (int)(blockIdx.x / p.kv.nkvh);
-  const int s = b / groups;
-  const SeqSpan sq = seq_span(p.kv, s);
-  const int NR = sq.n * p.rep;
-  const bool few = sp.few && NR <= kFewRows;
+  const int h = (int)(blockIdx.x % p.kv.nkvh), b = (int)(blockIdx.x / p.kv.nkvh), mine = b - groups;
   const int lane = threadIdx.x & 63, pt = threadIdx.x / TP, d = threadIdx.x % TP;
-  const int R = few ? b % groups : b % groups * NP + pt;
+  const bool few = mine >= 0;
+  SeqSpan sq;
+  int R;
+  if (few) {
+    sq = seq_span(p.kv, mine / few_rows);
+    R = mine % few_rows;
+    if (sq.n * p.rep > kFewRows) return;
+  } else {
+    const int per = sp.many_rows / NP;  // blocks of a tile
+    int s, tile;
+    if (!(sp.many_rows == 64 ? find_tile<64>(p, sp, b / per, &s, &sq, &tile) : find_tile<128>(p, sp, b / per, &s, &sq, &tile))) return;
+    R = tile * sp.many_rows + b % per * NP + pt;
+  }
+  const int NR = sq.n * p.rep;
   if (R >= NR) return;  // (few: the block as one)
   const int chunk = few ? sp.few_chunk : sp.many_chunk;
   const int last = few ? NR - 1 : min((R / sp.many_rows + 1) * sp.many_rows, NR) - 1;
@@ -1172,11 +1185,11 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p
   *reinterpret_cast<u32x2*>(p.out + t * p.ldo + (int64_t)head * HD + d * 4) = u32x2{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
 }
 
-// Blocks of the join for a sequence and kv head.
-int64_t join_groups(const PagedAttnParams& p, const Split& sp, int hd) {
-  const int64_t rows = (int64_t)p.kv.max_rows * p.rep, few = rows < kFewRows ? rows : kFewRows;
-  const int64_t many = (rows + 1024 / hd - 1) / (1024 / hd);
-  return sp.many_chunks > 1 && many > few ? many : few;
+// Blocks of the join, for a kv head: the tiles', and those of a short sequence.
+int64_t join_groups(const PagedAttnParams& p, const Split& sp, int hd, int64_t* few_rows) {
+  const int64_t rows = (int64_t)p.kv.max_rows * p.rep;
+  *few_rows = sp.few_chunks == 1 ? 0 : rows < kFewRows ? rows : kFewRows;
+  return sp.many_chunks == 1 ? 0 : (int64_t)sp.tiles * (sp.many_rows * hd / 1024);
 }
 
 template <int DT, bool F8, int HD>
@@ -1192,8 +1205,10 @@ hipError_t launch_one(const PagedAttnParams& p, hipStream_t s) {
     hipLaunchKernelGGL((paged_few_kernel<DT, F8, HD>), dim3((unsigned)(heads * sp.few_chunks)), dim3(64 * kFewWaves), 0, s, p, sp);
   }
   if (sp.parts > 1) {
-    const int64_t groups = join_groups(p, sp, HD);
-    hipLaunchKernelGGL((paged_join_kernel<DT, HD>), dim3((unsigned)(heads * groups)), dim3(256), 0, s, p, sp, (int)groups);
+    int64_t few_rows;
+    const int64_t groups = join_groups(p, sp, HD, &few_rows);
+    hipLaunchKernelGGL((paged_join_kernel<DT, HD>), dim3((unsigned)(p.kv.nkvh * groups + heads * few_rows)), dim3(256), 0, s, p, sp, (int)groups,
+                       (int)few_rows);
   }
   return hipGetLastError();
 }
@@ -1209,8 +1224,8 @@ hipError_t launch_dt(bool e4m3, int hd, const PagedAttnParams& p, hipStream_t s)
 int64_t paged_attention_blocks(bool e4m3, int hd, const PagedAttnParams& p) {
   const Split sp = split_of(p, e4m3, hd);
   // in doubles, as no product of these sizes need fit 64 bits; the caller compares with a bound far below
-  const double heads = (double)p.kv.seqs * p.kv.nkvh, rows = (double)p.kv.max_rows * p.rep;
-  const double most = fmax(heads * fmax(sp.few_chunks, rows), heads * sp.few_chunks + (double)p.kv.nkvh * sp.tiles * sp.many_chunks);
+  const double heads = (double)p.kv.seqs * p.kv.nkvh, tiles = (double)p.kv.nkvh * sp.tiles;
+  const double most = fmax(heads * kFewRows + tiles * 16, heads * sp.few_chunks + tiles * sp.many_chunks);
   return most > 9e18 ? INT64_MAX : (int64_t)most;
 }
 
