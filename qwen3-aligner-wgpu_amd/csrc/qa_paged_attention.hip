@@ -3,27 +3,38 @@
 //
 // Row i of a sequence with n rows and len keys sees keys 0 .. len - n + i:
 // out = sum_t p_t v_t / sum_t p_t, p_t = exp(q.k_t / sqrt(hd) - max).  The q heads of a
-// kv head and the rows of a sequence are one list, R = i * rep + head: a tile takes
-// 16 of them to each of RT column groups, so a step of one token fills the matrix
-// cores' columns with the q heads of its kv head, and a prompt with its rows.
+// kv head and the rows of a sequence are one list, R = i * rep + head, and a tile
+// takes 16, 64 or 128 of its pairs as the columns of the products S = K.Q^T and
+// O^T += V^T.P^T: a step of one token fills columns with the q heads of its kv head, a
+// prompt with its rows, and every key is read once for all of them.
 //
-// A wave takes 64 keys a step, K and V straight from the pages into fragments:
-//  * S = K.Q^T on v_mfma_f32_16x16x32 (A = 16 keys x 32 d, B = the tile's q).  A lane
-//    (c = lane & 15, g = lane >> 4) gets rows 4 g .. 4 g + 3 of each of four products;
-//    row m of product t is given key 16 (m / 4) + 4 t + m % 4, so that the lane ends
-//    up with keys 16 g .. 16 g + 15 of column c, all of them in one page.
-//  * online softmax in the log2 domain; a lane has its column's statistics, joined
-//    over g; the maximum moves only when it grows by more than 2^8.
-//  * O^T += V^T.P^T: lane (d = c, g) reads keys 16 g .. of the page's V row d, 16 or 32
-//    bytes in a run, in the order in which P lies in its registers.
-// Probabilities go into the product as two 16-bit terms (value and rounding
-// residue).  Over an e4m3 cache K is widened to the call's format (exactly), its
-// scale goes into the score's factor, and V's into p in f32; P and V are
-// multiplied as bf16 there, whose range takes any scale.
+// K and V go to LDS in blocks of 64 keys by DMA (buffer_load ... lds), page by page, a
+// page's resource being its own bytes, so that a hole in the table comes as
+// zeros.  (Straight from the pages into fragments, a load instruction touches 16
+// rows, and the address unit bounds the kernel: 90 us where the tiles take 35.)  Chunks of
+// 16 bytes lie within their row in an order that leaves fragment reads without
+// bank conflicts (0.3 % of LDS cycles; 28 % in plain order).  The rows of a product
+// are given those keys that leave a lane with 16 consecutive keys of its column, in the
+// order in which its fragment of V has them: P goes from one product into the
+// other in registers.
 //
-// Keys are split: a block's waves take turns at its 64-key blocks (WK) and join
-// through LDS; beyond `chunk` keys further blocks take the next chunk, write
-// (O, max, sum) to the workspace, and paged_join_kernel joins them.
+// Online softmax in the log2 domain; the maximum moves only when it grows by more
+// than 2^8, so nearly every step leaves O as it is.  Probabilities go into the
+// product as two 16-bit terms (value and rounding residue), which keeps P.V at
+// f32's accuracy for a second product of P's; in f16 they are scaled by 2^7, so that
+// small ones stay normal.  Over an e4m3 cache K is widened to the call's format
+// (exactly), its scale goes into the score's factor, and V's into p in f32; P and V
+// are multiplied as bf16 there, whose range takes any scale.
+//
+// Sequences of up to 16 pairs (single tokens): paged_few_kernel.  Bound by the
+// cache's bytes: 32 sequences of up to 4353 keys, 8 kv heads of 128, 342 MB in f16: 70 us,
+// 4.9 TB/s (a large copy: 5.1); 64 of up to 8193 in e4m3, 598 MB: 133 us, 4.5 TB/s.  The
+// smallest calls by latency: one sequence of 323 keys 8.9 us, of which launching is 4.
+// Longer ones: paged_many_kernel, bound by the two phases of a step, of which the
+// softmax is as long as the products: 771 rows behind 1536 keys, 16 heads of 128:
+// 35 us, 346 TFLOP/s, 519 with the products of the residues; 4334 rows 144 us.
+// Keys of long sequences are split among blocks, which leave (O, max, sum) in the
+// workspace for paged_join_kernel.
 #include <type_traits>
 
 #include "qa_internal.h"
@@ -211,46 +222,37 @@ __device__ __forceinline__ float* part_stats(const PagedAttnParams& p, const Spl
   return p.ws + p.kv.tokens * p.nqh * sp.parts * hd;
 }
 
-// The (row, head) pairs of a wave's columns; columns past the last repeat it and
-// store nothing.
-template <int RT>
-struct Columns {
-  int pos[RT], head[RT];
-  int64_t tok[RT];
-  bool on[RT];
-  __device__ __forceinline__ void set(const PagedAttnParams& p, const SeqSpan& sq, int h, int R0, int c) {
+// The (row, head) pair of a lane's column; columns past the last repeat it and store
+// nothing.
+struct Column {
+  int pos, head;
+  int64_t tok;
+  bool on;
+  __device__ __forceinline__ void set(const PagedAttnParams& p, const SeqSpan& sq, int h, int c) {
     const int NR = sq.n * p.rep;
     asm volatile("" : "+v"(c));  // formed again for the result, not held across the loop
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      on[r] = R0 + r * 16 + c < NR;
-      const int R = min(R0 + r * 16 + c, NR - 1), i = R / p.rep;
-      head[r] = h * p.rep + R % p.rep;
-      tok[r] = sq.row0 + i;
-      pos[r] = sq.pos0 + i;
-    }
+    on = c < NR;
+    const int R = min(c, NR - 1), i = R / p.rep;
+    head = h * p.rep + R % p.rep;
+    tok = sq.row0 + i;
+    pos = sq.pos0 + i;
   }
 };
 
-template <int DT, bool F8, int HD, int RT>
-__device__ __forceinline__ void load_q(const PagedAttnParams& p, const Columns<RT>& col, int g, u32x4 (&q)[RT][HD / 32]) {
+template <bool F8, int HD>
+__device__ __forceinline__ void load_q(const PagedAttnParams& p, const Column& col, int g, u32x4 (&q)[HD / 32]) {
+  const uint16_t* src = p.q + col.tok * p.ldq + (int64_t)col.head * HD;
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const uint16_t* src = p.q + col.tok[r] * p.ldq + (int64_t)col.head[r] * HD;
-#pragma unroll
-    for (int e = 0; e < HD / 32; ++e)  // in the order in which a K row's chunks come
-      q[r][e] = *reinterpret_cast<const u32x4*>(src + (F8 ? (e >> 1) * 64 + g * 16 + (e & 1) * 8 : e * 32 + g * 8));
-  }
+  for (int e = 0; e < HD / 32; ++e)  // in the order in which a K row's chunks come
+    q[e] = *reinterpret_cast<const u32x4*>(src + (F8 ? (e >> 1) * 64 + g * 16 + (e & 1) * 8 : e * 32 + g * 8));
 }
 
 // The compiler waits here for q's loads, not at their use in the loop, where the
 // tiles' loads would be waited for with them.
-template <int RT, int QS>
-__device__ __forceinline__ void keep(u32x4 (&q)[RT][QS]) {
+template <int N>
+__device__ __forceinline__ void keep(u32x4 (&q)[N]) {
 #pragma unroll
-  for (int r = 0; r < RT; ++r)
-#pragma unroll
-    for (int e = 0; e < QS; ++e) asm volatile("" : "+v"(q[r][e]));
+  for (int e = 0; e < N; ++e) asm volatile("" : "+v"(q[e]));
 }
 
 // A 64-key block's K and V tiles in LDS.  K: 64 rows of CR chunks; V: the block's
@@ -364,53 +366,50 @@ __device__ __forceinline__ int v_frag(int c, int g, int e, int lcp) {
 // Mask, online softmax and the two 16-bit terms of P.  `have`: how many of the
 // lane's 16 keys from kg on the sequence has (on a page); `f`: the scores'
 // factor, log2 e / sqrt(hd) and the K scale; `vs`: the V scale.
-template <int DT, bool F8, int HD, int RT>
-__device__ __forceinline__ void softmax(f32x4 (&sc)[RT][4], const int (&pos)[RT], int kg, int have, float f, float vs, float (&m)[RT],
-                                        float (&l)[RT], f32x4 (&o)[RT][HD / 16], u32x4 (&ph)[RT][2], u32x4 (&pl)[RT][2]) {
+template <int DT, bool F8, int HD>
+__device__ __forceinline__ void softmax(f32x4 (&sc)[4], int pos, int kg, int have, float f, float vs, float& m, float& l, f32x4 (&o)[HD / 16],
+                                        u32x4 (&ph)[2], u32x4 (&pl)[2]) {
   using C = Cfg<DT, F8, HD>;
+  const int see = min(have, pos + 1 - kg);
+  if (__builtin_amdgcn_ballot_w64(see < 16)) {
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const int see = min(have, pos[r] + 1 - kg);
-    if (__builtin_amdgcn_ballot_w64(see < 16)) {
+    for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (4 * t + e >= see) sc[r][t][e] = -INFINITY;
-    }
-    float x[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) x[t] = fmaxf(fmaxf(sc[r][t][0], sc[r][t][1]), fmaxf(sc[r][t][2], sc[r][t][3]));
-    const float bm = column_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * f);
-    if (__builtin_amdgcn_ballot_w64(bm > m[r] + kLazy)) {
-      const float mn = fmaxf(m[r], bm);
-      const float al = __builtin_amdgcn_exp2f(m[r] - (mn == -INFINITY ? 0.f : mn));
-      l[r] *= al;
-#pragma unroll
-      for (int d = 0; d < C::ND; ++d) o[r][d] *= al;
-      m[r] = mn;
-    }
-    const float mb = (m[r] == -INFINITY ? 0.f : m[r]) - C::kBias;
-    float sum[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      float w[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r][t][e], f, -mb));
-      sum[t] = (w[0] + w[1]) + (w[2] + w[3]);
-      if constexpr (F8) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] *= vs;
-      }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const uint32_t hi = pack2<C::PV>(w[2 * e], w[2 * e + 1]);
-        ph[r][t >> 1][2 * (t & 1) + e] = hi;
-        pl[r][t >> 1][2 * (t & 1) + e] = residue2<C::PV>(hi, w[2 * e], w[2 * e + 1]);
-      }
-    }
-    l[r] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      for (int e = 0; e < 4; ++e)
+        if (4 * t + e >= see) sc[t][e] = -INFINITY;
   }
+  float x[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) x[t] = fmaxf(fmaxf(sc[t][0], sc[t][1]), fmaxf(sc[t][2], sc[t][3]));
+  const float bm = column_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * f);
+  if (__builtin_amdgcn_ballot_w64(bm > m + kLazy)) {
+    const float mn = fmaxf(m, bm);
+    const float al = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+    l *= al;
+#pragma unroll
+    for (int d = 0; d < C::ND; ++d) o[d] *= al;
+    m = mn;
+  }
+  const float mb = (m == -INFINITY ? 0.f : m) - C::kBias;
+  float sum[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    float w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][e], f, -mb));
+    sum[t] = (w[0] + w[1]) + (w[2] + w[3]);
+    if constexpr (F8) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] *= vs;
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const uint32_t hi = pack2<C::PV>(w[2 * e], w[2 * e + 1]);
+      ph[t >> 1][2 * (t & 1) + e] = hi;
+      pl[t >> 1][2 * (t & 1) + e] = residue2<C::PV>(hi, w[2 * e], w[2 * e + 1]);
+    }
+  }
+  l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
 // Mask of word w of a run of elements of which `left` are keys.
@@ -437,128 +436,113 @@ __device__ __forceinline__ void clear_tail(unsigned char* vt, const int (&va)[Cf
     }
 }
 
-// The products of a block: O^T += V^T.P^T (PVT) over the V tile at vt, and S = K.Q^T
-// (SQT) over the K tile at kt; the two may be of different blocks.  They run in
-// slices, a d tile of V or the 16 keys of a K product, AHEAD of which the
-// fragments are read.  (The empty statements keep the fragments' addresses from
-// being formed outside the loop and held there.)
-template <int DT, bool F8, int HD, int RT, bool PVT, bool SQT>
-__device__ __forceinline__ void multiply(const unsigned char* vt, const int (&va)[Cfg<DT, F8, HD>::VS], int lcp, const u32x4 (&ph)[RT][2],
-                                         const u32x4 (&pl)[RT][2], f32x4 (&o)[RT][HD / 16], const unsigned char* kt, int ka,
-                                         const u32x4 (&q)[RT][HD / 32], f32x4 (&sc)[RT][4]) {
+// The products of a block: S = K.Q^T over the K tile at kt, and O^T += V^T.P^T over
+// the V tile at vt, in slices (the 16 keys of a K product, a d tile of V), the
+// fragments read kAhead slices before.  (The empty statements keep the fragments'
+// addresses from being formed outside the loop and held there.)
+constexpr int kAhead = 2;
+template <int DT, bool F8, int HD>
+__device__ __forceinline__ void multiply_k(const unsigned char* kt, int ka, const u32x4 (&q)[HD / 32], f32x4 (&sc)[4]) {
   using C = Cfg<DT, F8, HD>;
-  constexpr int NV = PVT ? C::ND : 0, NK = SQT ? 4 : 0, N = NV + NK;
-  constexpr int AHEAD = 2, B = AHEAD + 1;
-  int at[C::VS], ak = ka;
-  asm volatile("" : "+v"(ak));
+  constexpr int B = kAhead + 1;
+  asm volatile("" : "+v"(ka));
+  u32x4 x[B][C::KS];
+  auto read = [&](int t) {
+#pragma unroll
+    for (int e = 0; e < C::KS; ++e) x[t % B][e] = *reinterpret_cast<const u32x4*>(kt + (ka ^ (e << 6)) + 4 * t * C::CR * 16);
+  };
+#pragma unroll
+  for (int t = 0; t < kAhead; ++t) read(t);
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    if (t + kAhead < 4) read(t + kAhead);
+#pragma unroll
+    for (int e = 0; e < C::QS; ++e) {
+      u32x4 a;
+      if constexpr (F8) a = widen_e4m3<DT>(x[t % B][e >> 1][2 * (e & 1)], x[t % B][e >> 1][2 * (e & 1) + 1]);
+      else a = x[t % B][e];
+      sc[t] = mfma<DT>(a, q[e], e ? sc[t] : f32x4{0, 0, 0, 0});
+    }
+  }
+}
+template <int DT, bool F8, int HD>
+__device__ __forceinline__ void multiply_v(const unsigned char* vt, const int (&va)[Cfg<DT, F8, HD>::VS], int lcp, const u32x4 (&ph)[2],
+                                           const u32x4 (&pl)[2], f32x4 (&o)[HD / 16]) {
+  using C = Cfg<DT, F8, HD>;
+  constexpr int B = kAhead + 1;
+  int at[C::VS];
 #pragma unroll
   for (int e = 0; e < C::VS; ++e) {
     at[e] = va[e];
     asm volatile("" : "+v"(at[e]));
   }
-  u32x4 x[B][C::KS > C::VS ? C::KS : C::VS];
-  constexpr int P = C::ND / 4 + 1;  // both: the four K products come between the d tiles
-  auto is_k = [](int n) { return PVT && SQT ? n % P == P - 1 : SQT; };
-  auto index = [&](int n) { return PVT && SQT ? (is_k(n) ? n / P : n - n / P) : n; };
-  auto read = [&](int n) {
-    if (is_k(n)) {
+  u32x4 x[B][C::VS];
+  auto read = [&](int d) {
 #pragma unroll
-      for (int e = 0; e < C::KS; ++e) x[n % B][e] = *reinterpret_cast<const u32x4*>(kt + (ak ^ (e << 6)) + 4 * index(n) * C::CR * 16);
-    } else {
-#pragma unroll
-      for (int e = 0; e < C::VS; ++e) x[n % B][e] = *reinterpret_cast<const u32x4*>(vt + at[e] + (index(n) * 256 << lcp));
-    }
+    for (int e = 0; e < C::VS; ++e) x[d % B][e] = *reinterpret_cast<const u32x4*>(vt + at[e] + (d * 256 << lcp));
   };
 #pragma unroll
-  for (int n = 0; n < AHEAD && n < N; ++n) read(n);
+  for (int d = 0; d < kAhead; ++d) read(d);
 #pragma unroll
-  for (int n = 0; n < N; ++n) {
-    if (n + AHEAD < N) read(n + AHEAD);
-    if (is_k(n)) {
-      const int t = index(n);
+  for (int d = 0; d < C::ND; ++d) {
+    if (d + kAhead < C::ND) read(d + kAhead);
 #pragma unroll
-      for (int e = 0; e < C::QS; ++e) {
-        u32x4 a;
-        if constexpr (F8) a = widen_e4m3<DT>(x[n % B][e >> 1][2 * (e & 1)], x[n % B][e >> 1][2 * (e & 1) + 1]);
-        else a = x[n % B][e];
-#pragma unroll
-        for (int r = 0; r < RT; ++r) sc[r][t] = mfma<DT>(a, q[r][e], e ? sc[r][t] : f32x4{0, 0, 0, 0});
-      }
-    } else {
-      const int d = index(n);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        u32x4 a;
-        if constexpr (F8) a = widen_e4m3<QA_BF16>(x[n % B][0][2 * j], x[n % B][0][2 * j + 1]);
-        else a = x[n % B][j];
-#pragma unroll
-        for (int r = 0; r < RT; ++r) o[r][d] = mfma<C::PV>(a, ph[r][j], o[r][d]);
-#pragma unroll
-        for (int r = 0; r < RT; ++r) o[r][d] = mfma<C::PV>(a, pl[r][j], o[r][d]);
-      }
-    }
-    if constexpr (RT > 1) {  // in this order: more fragments at once than these do not fit the registers
-      if (n + AHEAD < N && is_k(n + AHEAD)) __builtin_amdgcn_sched_group_barrier(0x100, C::KS, 0);
-      else if (n + AHEAD < N) __builtin_amdgcn_sched_group_barrier(0x100, C::VS, 0);
-      __builtin_amdgcn_sched_barrier(0);
+    for (int j = 0; j < 2; ++j) {
+      u32x4 a;
+      if constexpr (F8) a = widen_e4m3<QA_BF16>(x[d % B][0][2 * j], x[d % B][0][2 * j + 1]);
+      else a = x[d % B][j];
+      o[d] = mfma<C::PV>(a, ph[j], o[d]);
+      o[d] = mfma<C::PV>(a, pl[j], o[d]);
     }
   }
 }
 
-// The waves that worked on the same columns joined through LDS (in order), each with
-// ND / NS of the d tiles, and the result or its part written.  Group a = wave / GW
-// took a part of the keys, wave % GW the columns.
-template <int DT, bool F8, int HD, int RT, int GW, int NS>
-__device__ __forceinline__ void finish(const PagedAttnParams& p, const Split& sp, const SeqSpan& sq, int h, int R0, int part, bool whole,
-                                       float (&m)[RT], float (&l)[RT], const f32x4 (&o)[RT][HD / 16], unsigned char* smem) {
-  constexpr int ND = HD / 16, NM = ND / NS;
-  const int lane = threadIdx.x & 63, wave = scalar((int)(threadIdx.x >> 6)), g = lane >> 4, ns = wave / GW, wg = wave % GW;
-  Columns<RT> col;
-  col.set(p, sq, h, R0, lane & 15);
-  f32x4* xo = reinterpret_cast<f32x4*>(smem);                                        // [wave][RT][ND][64]
-  float* xs = reinterpret_cast<float*>(smem + (size_t)GW * NS * RT * ND * 64 * 16);  // [wave][RT][2][64]
+// The waves' results joined through LDS (in order), each wave with its share of the d
+// tiles, and the result or its part written.
+template <int DT, int HD>
+__device__ __forceinline__ void finish(const PagedAttnParams& p, const Split& sp, const SeqSpan& sq, int h, int part, bool whole, float m, float l,
+                                       const f32x4 (&o)[HD / 16], unsigned char* smem) {
+  constexpr int ND = HD / 16, NM = ND / kFewWaves;
+  const int lane = threadIdx.x & 63, wave = scalar((int)(threadIdx.x >> 6)), g = lane >> 4;
+  Column col;
+  col.set(p, sq, h, lane & 15);
+  f32x4* xo = reinterpret_cast<f32x4*>(smem);                                    // [wave][ND][64]
+  float* xs = reinterpret_cast<float*>(smem + (size_t)kFewWaves * ND * 64 * 16);  // [wave][2][64]
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-#pragma unroll
-    for (int d = 0; d < ND; ++d) xo[((wave * RT + r) * ND + d) * 64 + lane] = o[r][d];
-    xs[(wave * RT + r) * 128 + lane] = m[r];
-    xs[(wave * RT + r) * 128 + 64 + lane] = column_sum(l[r]);
-  }
+  for (int d = 0; d < ND; ++d) xo[(wave * ND + d) * 64 + lane] = o[d];
+  xs[wave * 128 + lane] = m;
+  xs[wave * 128 + 64 + lane] = column_sum(l);
   __syncthreads();
+  float mm = -INFINITY, al[kFewWaves], ll = 0.f;
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    float mm = -INFINITY, al[NS], ll = 0.f;
+  for (int a = 0; a < kFewWaves; ++a) {
+    al[a] = xs[a * 128 + lane];
+    mm = fmaxf(mm, al[a]);
+  }
+  const float mu = mm == -INFINITY ? 0.f : mm;
+  f32x4 w[NM] = {};
 #pragma unroll
-    for (int a = 0; a < NS; ++a) {
-      al[a] = xs[((a * GW + wg) * RT + r) * 128 + lane];
-      mm = fmaxf(mm, al[a]);
+  for (int a = 0; a < kFewWaves; ++a) {
+    al[a] = __builtin_amdgcn_exp2f(al[a] - mu);
+    ll += xs[a * 128 + 64 + lane] * al[a];
+#pragma unroll
+    for (int d = 0; d < NM; ++d) w[d] += xo[(a * ND + wave * NM + d) * 64 + lane] * al[a];
+  }
+  if (!col.on) return;
+  if (whole) {
+    const float inv = ll == 0.f ? 0.f : 1.0f / ll;  // no key: zeros
+    uint16_t* dst = p.out + col.tok * p.ldo + (int64_t)col.head * HD + 4 * g;
+#pragma unroll
+    for (int d = 0; d < NM; ++d) {
+      const f32x4 y = w[d] * inv;
+      *reinterpret_cast<u32x2*>(dst + (wave * NM + d) * 16) = u32x2{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
     }
-    const float mu = mm == -INFINITY ? 0.f : mm;
-    f32x4 w[NM] = {};
+  } else {
+    const int64_t at = part_index(p, sp, col.tok, col.head, part);
+    float* dst = p.ws + at * HD + 4 * g;
 #pragma unroll
-    for (int a = 0; a < NS; ++a) {
-      const int at = (a * GW + wg) * RT + r;
-      al[a] = __builtin_amdgcn_exp2f(al[a] - mu);
-      ll += xs[at * 128 + 64 + lane] * al[a];
-#pragma unroll
-      for (int d = 0; d < NM; ++d) w[d] += xo[(at * ND + ns * NM + d) * 64 + lane] * al[a];
-    }
-    if (!col.on[r]) continue;
-    if (whole) {
-      const float inv = ll == 0.f ? 0.f : 1.0f / ll;  // no key: zeros
-      uint16_t* dst = p.out + col.tok[r] * p.ldo + (int64_t)col.head[r] * HD + 4 * g;
-#pragma unroll
-      for (int d = 0; d < NM; ++d) {
-        const f32x4 y = w[d] * inv;
-        *reinterpret_cast<u32x2*>(dst + (ns * NM + d) * 16) = u32x2{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
-      }
-    } else {
-      const int64_t at = part_index(p, sp, col.tok[r], col.head[r], part);
-      float* dst = p.ws + at * HD + 4 * g;
-#pragma unroll
-      for (int d = 0; d < NM; ++d) *reinterpret_cast<f32x4*>(dst + (ns * NM + d) * 16) = w[d];
-      if (ns == 0 && g == 0) *reinterpret_cast<f32x2*>(part_stats(p, sp, HD) + at * 2) = (f32x2){mm, ll};
-    }
+    for (int d = 0; d < NM; ++d) *reinterpret_cast<f32x4*>(dst + (wave * NM + d) * 16) = w[d];
+    if (wave == 0 && g == 0) *reinterpret_cast<f32x2*>(part_stats(p, sp, HD) + at * 2) = (f32x2){mm, ll};
   }
 }
 
@@ -636,18 +620,18 @@ __device__ __forceinline__ void few_block(const PagedAttnParams& p, const Split&
   auto fetch = [&](int it, int ids) {
     fetch_pages<F8, HD>(kv, sq, ids, h, steps - it, [&](int j) { return key_of(it + j); }, &pages, &ksc, &vsc, &holes);
   };
-  Columns<1> col;
-  col.set(p, sq, h, 0, c);
-  u32x4 q[1][C::QS];
-  load_q<DT, F8, HD, 1>(p, col, g, q);
+  Column col;
+  col.set(p, sq, h, c);
+  u32x4 q[C::QS];
+  load_q<F8, HD>(p, col, g, q);
   if (steps > 0) {
     fetch(0, found);
     load_tile<DT, F8, HD, false, 1, true>(kv, pages, 0, 0, kt);
     load_tile<DT, F8, HD, false, 1, false>(kv, pages, 0, 0, vt);
   }
   keep(q);
-  f32x4 o[1][C::ND] = {};
-  float m[1] = {-INFINITY}, l[1] = {0.f};
+  f32x4 o[C::ND] = {};
+  float m = -INFINITY, l = 0.f;
   const int ka = k_frag<DT, F8, HD>(c, g);
   int va[C::VS];
 #pragma unroll
@@ -663,24 +647,24 @@ __device__ __forceinline__ void few_block(const PagedAttnParams& p, const Split&
       vs = of_keys(vsc, it & 15, g);
     }
     wait_vmcnt<C::LI>();  // K is there; V's loads came after it
-    f32x4 sc[1][4];
-    u32x4 ph[1][2], pl[1][2];
-    multiply<DT, F8, HD, 1, false, true>(vt, va, lcp, ph, pl, o, kt, ka, q, sc);
+    f32x4 sc[4];
+    u32x4 ph[2], pl[2];
+    multiply_k<DT, F8, HD>(kt, ka, q, sc);
     wait_lds();
     if (more) {
       if ((it & 15) == 15) fetch(it + 1, page_ids(kv, s, [&](int j) { return key_of(it + 1 + j); }));
       load_tile<DT, F8, HD, false, 1, true>(kv, pages, (it + 1) & 15, 0, kt);
     }
-    softmax<DT, F8, HD, 1>(sc, col.pos, kg, have, p.scale * kLog2e * ks, vs, m, l, o, ph, pl);
+    softmax<DT, F8, HD>(sc, col.pos, kg, have, p.scale * kLog2e * ks, vs, m, l, o, ph, pl);
     if (more) wait_vmcnt<C::LI>();  // V is there; the next K's loads came after it
     else wait_vmcnt<0>();
     if (__builtin_amdgcn_ballot_w64(have < 16)) clear_tail<DT, F8, HD>(vt, va, lcp, have);
-    multiply<DT, F8, HD, 1, true, false>(vt, va, lcp, ph, pl, o, kt, ka, q, sc);
+    multiply_v<DT, F8, HD>(vt, va, lcp, ph, pl, o);
     wait_lds();
     if (more) load_tile<DT, F8, HD, false, 1, false>(kv, pages, (it + 1) & 15, 0, vt);
   }
   __syncthreads();  // the tiles' LDS is the join's
-  finish<DT, F8, HD, 1, 1, kFewWaves>(p, sp, sq, h, 0, part, end <= sp.few_chunk, m, l, o, smem);
+  finish<DT, HD>(p, sp, sq, h, part, end <= sp.few_chunk, m, l, o, smem);
 }
 
 template <int DT, bool F8, int HD>
@@ -904,6 +888,7 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
   const PagedParams& kv = p.kv;
   const int mine = (int)blockIdx.x - sp.tiles * sp.many_chunks * kv.nkvh;
   if (mine >= 0) {  // behind them, the blocks of the sequences of few rows, four waves each
+    // (the other waves end here, and a barrier waits for no wave that has ended)
     if (threadIdx.x < 64 * kFewWaves) few_block<DT, F8, HD>(p, sp, mine, smem);
     return;
   }
@@ -972,7 +957,7 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
     *head = kvh * p.rep + R - i * p.rep;
     return on;
   };
-  u32x4 q[1][HD / 16];
+  u32x4 q[HD / 16];
   int pos;
   {
     int64_t tok;
@@ -982,7 +967,7 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
     const uint16_t* src = p.q + tok * p.ldq + (int64_t)head * HD;
 #pragma unroll
     for (int e = 0; e < HD / 16; ++e)  // in the order in which a K row's chunks come
-      q[0][e] = *reinterpret_cast<const u32x4*>(src + (F8 ? e / 2 * 32 + h * 16 + e % 2 * 8 : e * 16 + h * 8));
+      q[e] = *reinterpret_cast<const u32x4*>(src + (F8 ? e / 2 * 32 + h * 16 + e % 2 * 8 : e * 16 + h * 8));
   }
   if (steps > 0) {
     fetch(0);
@@ -1027,9 +1012,9 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
               *x &= u32x4{tail_mask<C::ES>(left, 0), tail_mask<C::ES>(left, 1), tail_mask<C::ES>(left, 2), tail_mask<C::ES>(left, 3)};
             }
         }
-        if (it > 0 && it < steps) multiply32<DT, F8, HD, true, true>(vt(it - 1), va, lcp, ph, pl, o, kt(it), ka, q[0], sc);
-        else if (it > 0) multiply32<DT, F8, HD, true, false>(vt(it - 1), va, lcp, ph, pl, o, kt(it), ka, q[0], sc);
-        else if (steps > 0) multiply32<DT, F8, HD, false, true>(vt(it), va, lcp, ph, pl, o, kt(it), ka, q[0], sc);
+        if (it > 0 && it < steps) multiply32<DT, F8, HD, true, true>(vt(it - 1), va, lcp, ph, pl, o, kt(it), ka, q, sc);
+        else if (it > 0) multiply32<DT, F8, HD, true, false>(vt(it - 1), va, lcp, ph, pl, o, kt(it), ka, q, sc);
+        else if (steps > 0) multiply32<DT, F8, HD, false, true>(vt(it), va, lcp, ph, pl, o, kt(it), ka, q, sc);
       } else {
         const int kg = key_of(it) + 16 * h, j = scalar(it & 15);
         float f[2], vs[2] = {0.f, 0.f};
