@@ -334,14 +334,15 @@ int qa_mrope_rows(qa_ctx* ctx, const qa_mrope_desc* desc);
  *   kv_len   int32 [seqs]: its keys with the new rows, whose positions are
  *            kv_len - rows .. kv_len - 1
  *   max_rows, max_len  bounds of one sequence's rows and keys, max_len <= ldtable *
- *            page: they set the launch, so that a captured call can be replayed
- *            on other lengths
+ *            page and <= 2^30: they set the launch, so that a captured call can
+ *            be replayed on other lengths
+ * The call's q heads are a multiple of nkvh, 65536 at most.
  * table, row_start and kv_len are device memory, read by the kernels, and whatever
  * they hold no call reads or writes outside its buffers: rows past the batch or
- * past max_rows, positions below zero or past max_len and entries that are no
- * page are left out.  Rows that no sequence has are left as they are.  Two new
- * rows must not share a slot; a page may be in several tables while it is only
- * read. */
+ * past max_rows, positions below zero and entries that are no page are left out,
+ * and a kv_len past max_len counts as max_len.  Rows that no sequence has are
+ * left as they are.  Two new rows must not share a slot; a page may be in several
+ * tables while it is only read. */
 typedef struct qa_paged_kv {
   uint32_t dtype; /* the call's 16-bit format, or QA_E4M3 */
   int32_t page;
@@ -395,7 +396,9 @@ int qa_kv_append(qa_ctx* ctx, const qa_kv_append_desc* desc);
  * head h to kv head h / (nqh / nkvh), softmax of q.k / sqrt(hd) in f32,
  * out[t][h hd + j] = round(sum_t p_t v_t[j]).  Keys on an entry that is no page do
  * not count; a row without keys gives zeros.  What the pages hold behind a
- * sequence's last key is not looked at.  Scales may be any positive numbers.
+ * sequence's last key is not looked at.  Scales may be any positive numbers.  V has
+ * to be finite for all of a sequence's keys: a row multiplies those behind its
+ * position by 0, which leaves NaN of an infinity or NaN (K may hold either there).
  *   q    [tokens][nqh hd], row stride ldq, as qa_kv_append writes it
  *   out  [tokens][nqh hd], row stride ldo, the o projection's input
  *   workspace  16-byte aligned device memory for partial results, of the bytes

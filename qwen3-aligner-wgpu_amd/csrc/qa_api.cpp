@@ -487,6 +487,7 @@ int check_paged_sizes(const char* fn, const qa_paged_kv* kv, uint32_t dtype, int
     return fail(QA_EINVAL, "%s: need nqh (<= 65536) a multiple of nkvh > 0", fn);
   if (tokens < 0 || tokens > kI32 || kv->seqs < 0 || kv->seqs > kI32 || kv->max_rows < 0 || kv->max_rows > kI32)
     return fail(QA_EINVAL, "%s: tokens, seqs and max_rows must be in [0, 2^31)", fn);
+  if (tokens * (nqh / kv->nkvh) > 1 << 30) return fail(QA_EINVAL, "%s: the batch is too large for one launch", fn);
   if (kv->max_len < 0 || kv->max_len > 1 << 30)
     return fail(QA_EINVAL, "%s: max_len must be in [0, 2^30]", fn);
   return ok();

@@ -87,6 +87,18 @@ class Batch:
         self.max_rows, self.max_len = max(self.n + [0]), max(self.len + [0])
         self.k = self.v = self.k_scale = self.v_scale = None
 
+    @classmethod
+    def shared(cls, n, lens, *args, **kw):
+        """Many sequences over one's pages: each table names the pages of the longest."""
+        b = cls([0], [max(lens)], *args, tail_rows=0, **kw)
+        b.fill()
+        b.n, b.len, b.seqs = list(n), list(lens), len(n)
+        b.row_start = np.concatenate([[0], np.cumsum(n)]).astype(np.int32)
+        b.tokens, b.kv_len = int(b.row_start[-1]) + 2, np.array(b.len, np.int32)
+        b.table = np.tile(b.table, (b.seqs, 1))
+        b.max_rows = max(n)
+        return b
+
     def shapes(self):
         return (self.num_pages, self.nkv, self.page, self.hd), (self.num_pages, self.nkv, self.hd, self.page)
 
@@ -201,15 +213,15 @@ def attention(ctx, pkg, b, q, pad=8, out0=0x3C01, **kv):
     return np.ascontiguousarray(out[:, : q.shape[1]])
 
 
-def assert_attention(b, q, got, out0=0x3C01, rows=None, **cache):
+def assert_attention(b, q, got, out0=0x3C01, rows=None, seqs=None, **cache):
     """Every row within the derived bound of the definition in 64 bits: the f32
     score and accumulation errors and the two-term probabilities of
     conftest._attention_bound_rows (bf16 terms over an e4m3 cache), and half a
     step of the output.  Rows without keys are zeros, rows of no sequence what
-    they were."""
+    they were.  rows, seqs: those to look at (all of them)."""
     assert (got[b.row_start[-1]:] == out0).all()
     worst = 0.0
-    for s in range(b.seqs):
+    for s in range(b.seqs) if seqs is None else seqs:
         K, V, on = b.keys(s, **cache)
         r0, n, m = b.row_start[s], b.n[s], b.len[s]
         pick = range(n) if rows is None else [r for r in rows if r < n]

@@ -24,7 +24,8 @@ import pytest
 import paged
 from conftest import rope_tables, ulp16
 from hipgraph import Capture, hip
-from paged import BF16, E4M3, F16, Batch, append, assert_attention, attention, e4m3_codes, e4m3_step, e4m3_values, narrow, scale_for, widen
+from paged import (BF16, E4M3, F16, STALE8, STALE16, Batch, append, assert_attention, attention, e4m3_codes, e4m3_step, e4m3_values, narrow,
+                   scale_for, widen)
 
 pytestmark = pytest.mark.gpu
 
@@ -399,6 +400,87 @@ def test_attention_shared_pages_and_repeats(ctx, pkg):
 
 
 @FORMATS
+def test_attention_of_many_sequences(ctx, pkg, dtype, cache):
+    """150 sequences of no row, one, a few and many, in any order."""
+    rng = np.random.default_rng(101)
+    n = [int(x) for x in rng.choice([0, 1, 1, 1, 2, 9, 17, 40, 90], 150)]
+    lens = [int(rng.integers(k, 300)) for k in n]
+    b = Batch.shared(n, lens, 16, 4, 2, 64, dtype, cache, seed=102)
+    b.upload(ctx)
+    q = b.random_rows(4 * 64)
+    assert_attention(b, q, attention(ctx, pkg, b, q))
+    b.free()
+
+
+@FORMATS
+@pytest.mark.parametrize("page,hd", [(16, 64), (64, 64), (32, 128)])
+def test_attention_of_single_tokens_behind_many_pages(ctx, pkg, dtype, cache, page, hd):
+    """64 sequences, whose keys are not split: a wave goes through its page ids 16 blocks at a time.  A page in
+    the middle is none."""
+    b = Batch.shared([1] * 64, [9000, 4097, 8192] + [60] * 60 + [8300], page, 16, 8, hd, dtype, cache, seed=103)
+    b.table[[0, 63], 5000 // page] = -1
+    b.upload(ctx)
+    q = b.random_rows(16 * hd)
+    assert_attention(b, q, attention(ctx, pkg, b, q), seqs=(0, 1, 2, 30, 63))
+    b.free()
+
+
+@FORMATS
+@pytest.mark.parametrize("page,hd", [(16, 64), (64, 64), (32, 128)])
+def test_attention_of_rows_behind_many_pages(ctx, pkg, dtype, cache, page, hd):
+    """The same for 17 and more rows: 128 sequences of 2 kv heads."""
+    b = Batch.shared([17] * 127 + [20], [9000, 4500] + [60] * 125 + [8300], page, 2, 2, hd, dtype, cache, seed=104)
+    b.table[[0, 127], 5000 // page] = -1
+    b.upload(ctx)
+    q = b.random_rows(2 * hd)
+    assert_attention(b, q, attention(ctx, pkg, b, q), seqs=(0, 1, 77, 127))
+    b.free()
+
+
+@FORMATS
+@pytest.mark.parametrize("page,hd", [(16, 64), (64, 128)])
+def test_attention_of_long_tiles(ctx, pkg, dtype, cache, page, hd):
+    """6000 rows of 8 kv heads: tiles of 128 rows, with few and many keys, whole and not, beside a single token."""
+    b = Batch.shared([100] * 58 + [1, 130, 257], [4500, 100, 2100] + [130] * 55 + [700, 140, 600], page, 8, 8, hd, dtype, cache, seed=105)
+    b.table[0, 4096 // page] = -1
+    b.upload(ctx)
+    q = b.random_rows(8 * hd)
+    assert_attention(b, q, attention(ctx, pkg, b, q), seqs=(0, 1, 2, 40, 58, 59, 60), rows=(0, 1, 63, 64, 99, 127, 128, 129, 255, 256))
+    b.free()
+
+
+@FORMATS
+def test_attention_of_short_sequences_in_a_batch_with_no_room_for_them(ctx, pkg, dtype, cache):
+    """max_rows * seqs rows: the sizes say that every sequence has 20 rows, row_start says otherwise."""
+    b = Batch([20, 5, 20], [90, 300, 20], 16, 4, 2, 64, dtype, cache, seed=106, tail_rows=15)
+    assert b.seqs * b.max_rows == b.tokens
+    b.fill()
+    b.upload(ctx)
+    q = b.random_rows(4 * 64)
+    assert_attention(b, q, attention(ctx, pkg, b, q))
+    b.free()
+
+
+@FORMATS
+@pytest.mark.parametrize("n", [16, 90])
+def test_attention_keys_of_nan_behind_a_row(ctx, pkg, dtype, cache, n):
+    """A key that a row does not see may be NaN: the rows before it have the same bits as without."""
+    b = Batch([n], [200], 16, 2, 2, 64, dtype, cache, seed=107)
+    b.fill()
+    b.upload(ctx)
+    q = b.random_rows(2 * 64)
+    want = attention(ctx, pkg, b, q)
+    p, at = b.table[0, 199 // 16], 199 % 16
+    k = b.k.copy()
+    k[p, :, at] = STALE8 if cache == E4M3 else STALE16[dtype]
+    ctx.upload(b.dev["k"], k)
+    got = attention(ctx, pkg, b, q)
+    assert np.array_equal(got[: n - 1], want[: n - 1])
+    assert np.isnan(widen(got[n - 1], dtype)).all()
+    b.free()
+
+
+@FORMATS
 def test_pages_past_four_gigabytes(ctx, pkg, dtype, cache):
     """A pool of over 2^32 bytes of K: append to and attend over its last pages."""
     each = 1 if cache == E4M3 else 2
@@ -518,6 +600,42 @@ def test_graph_replays_follow_the_lengths(ctx, pkg):
     finally:
         cap.close()
     for x in d_in + [d_q, d_o, ws]:
+        x.free()
+    b.free()
+
+
+def test_graph_replays_of_prompts(ctx, pkg):
+    """A captured attention over bounds of 120 rows and 3000 keys, replayed on other batches with eager
+    calls between: the eager results."""
+    b = Batch([120, 60, 1], [3000, 60, 900], 32, 4, 2, 128, BF16, BF16, seed=83, tail_rows=40)
+    b.fill()
+    b.upload(ctx)
+    q = b.random_rows(4 * 128)
+    dq, do = ctx.to_device(q), ctx.alloc(q.nbytes)
+    d = paged.attention_desc(pkg, b, dq, q.shape[1], do, q.shape[1])
+    size = pkg.attention_paged_workspace(d)
+    assert size  # split: the join is captured too
+    ws = ctx.to_device(np.full(size, 0xFF, np.uint8))
+    d.workspace, d.workspace_bytes = int(ws), size
+    with Capture(ctx.stream) as cap:
+        ctx.attention_paged(d)
+    try:
+        for n, lens in (([120, 60, 1], [3000, 60, 900]), ([1, 1, 1], [2999, 1, 33]), ([16, 17, 120], [16, 60, 900]), ([0, 0, 0], [3000, 0, 5]),
+                        ([90, 0, 120], [1025, 60, 120]), ([120, 60, 1], [3000, 60, 900])):
+            b.n, b.len = n, lens
+            b.row_start = np.concatenate([[0], np.cumsum(n)]).astype(np.int32)
+            ctx.upload(b.dev["row_start"], b.row_start)
+            ctx.upload(b.dev["kv_len"], np.array(lens, np.int32))
+            outs = []
+            for go in (cap.replay, lambda: (ctx.attention_paged(d), ctx.sync())):
+                ctx.upload(do, np.full(q.shape, 0x3C01, np.uint16))
+                go()
+                outs.append(ctx.download(do, q.shape))
+            assert np.array_equal(*outs)
+            assert_attention(b, q, outs[0], rows=(0, 1, 16, 59, 89, 119))
+    finally:
+        cap.close()
+    for x in (dq, do, ws):
         x.free()
     b.free()
 

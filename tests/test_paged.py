@@ -112,6 +112,7 @@ def test_batches_past_one_launch_are_refused(pkg):
     wide = _mrope(pkg, tokens=2 ** 28, ldpos=2 ** 28)  # a grid of 2^32 threads
     _refused(pkg, pkg.lib().qa_mrope_rows, wide, pkg.QA_EINVAL, "too large")
     many = _kv(pkg, seqs=1, max_rows=4, max_len=128)
+    _refused(pkg, pkg.lib().qa_attention_paged, _attention(pkg, many, tokens=2 ** 30), pkg.QA_EINVAL, "too large")
     _refused(pkg, pkg.lib().qa_kv_append, _append(pkg, many, tokens=2 ** 26), pkg.QA_EINVAL, "too large")
     big = _kv(pkg, seqs=2 ** 23, max_rows=1, max_len=128)
     _refused(pkg, pkg.lib().qa_attention_paged, _attention(pkg, big, workspace_bytes=2 ** 62), pkg.QA_EINVAL, "too large")
