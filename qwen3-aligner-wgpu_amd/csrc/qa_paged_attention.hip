@@ -69,17 +69,16 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
 }
 // (a, b) minus their 16-bit roundings h = pack2(a, b), as two 16-bit values.  The
-// differences are exact in f32.  f16: v_fma_mix_f32 reads its half of h as it
-// lies, -h * 1 + a; a and b come from ordinary VALU instructions or v_exp_f32, and h,
-// a compiler instruction's result that reads both, lies between them and the
-// statements, so that no wait state is missing.
+// differences are exact in f32.  f16: as products with a 1 that the compiler does
+// not see, which become one v_fma_mix each, h's half read and the result's
+// written as they lie.
 template <int DT>
 __device__ __forceinline__ uint32_t residue2(uint32_t h, float a, float b) {
   if constexpr (DT == QA_F16) {
-    float x, y;
-    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(x) : "v"(h), "v"(a));
-    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(y) : "v"(h), "v"(b));
-    return pack2<DT>(x, y);
+    const f16x2 v = __builtin_bit_cast(f16x2, h);
+    float one = 1.f;
+    asm("" : "+s"(one));
+    return __builtin_bit_cast(uint32_t, f16x2{(_Float16)__builtin_fmaf(-(float)v[0], one, a), (_Float16)__builtin_fmaf(-(float)v[1], one, b)});
   } else {
     return pack2<DT>(a - __uint_as_float(h << 16), b - __uint_as_float(h & 0xffff0000u));
   }
@@ -119,6 +118,13 @@ __device__ __forceinline__ void wait_lds() {
 
 // A value that all of a wave's lanes have, as a scalar.
 __device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// m = max(m, a, b, c, d) in two instructions: the maximum of a product's elements
+// alone would take each of them through an instruction of its own first.
+__device__ __forceinline__ void max4(float& m, float a, float b, float c, float d) {
+  m = fmaxf(fmaxf(m, a), b);
+  m = fmaxf(fmaxf(m, c), d);
+}
 
 // Maximum and sum over the four lanes that share a column (lane ^ 16, lane ^ 32).
 __device__ __forceinline__ float column_max(float v) {
@@ -378,10 +384,10 @@ __device__ __forceinline__ void softmax(f32x4 (&sc)[4], int pos, int kg, int hav
       for (int e = 0; e < 4; ++e)
         if (4 * t + e >= see) sc[t][e] = -INFINITY;
   }
-  float x[4];
+  float x[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-  for (int t = 0; t < 4; ++t) x[t] = fmaxf(fmaxf(sc[t][0], sc[t][1]), fmaxf(sc[t][2], sc[t][3]));
-  const float bm = column_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * f);
+  for (int t = 0; t < 4; ++t) max4(x[t & 1], sc[t][0], sc[t][1], sc[t][2], sc[t][3]);
+  const float bm = column_max(fmaxf(x[0], x[1]) * f);
   if (__builtin_amdgcn_ballot_w64(bm > m + kLazy)) {
     const float mn = fmaxf(m, bm);
     const float al = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
@@ -789,10 +795,10 @@ __device__ __forceinline__ void softmax32(f32x16 (&sc)[2], int pos, int kg, cons
       for (int e = 0; e < 16; ++e)
         if (e >= see) sc[u][e] = -INFINITY;
     }
-    float x[4];
+    float x[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-    for (int t = 0; t < 4; ++t) x[t] = fmaxf(fmaxf(sc[u][4 * t], sc[u][4 * t + 1]), fmaxf(sc[u][4 * t + 2], sc[u][4 * t + 3]));
-    top[u] = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+    for (int t = 0; t < 4; ++t) max4(x[t & 1], sc[u][4 * t], sc[u][4 * t + 1], sc[u][4 * t + 2], sc[u][4 * t + 3]);
+    top[u] = fmaxf(x[0], x[1]);
   }
   const float bm = pair_max(F8 ? fmaxf(top[0] * f[0], top[1] * f[1]) : fmaxf(top[0], top[1]) * f[0]);
   if (__builtin_amdgcn_ballot_w64(bm > m + kLazy)) {
