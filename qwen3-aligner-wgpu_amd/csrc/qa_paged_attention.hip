@@ -159,14 +159,20 @@ struct Cfg {
 // How a call's rows and keys are divided among blocks, from its sizes alone (lengths
 // are on the device), so that the workspace is known without one.
 //  * few: a sequence of at most kFewRows (row, head) pairs is one column group; a
-//    block's four waves take turns at a chunk of its keys, each with tiles of its
-//    own.  Bound by the cache's bytes: enough blocks for the LDS of every CU, cut into
-//    chunks of 256 keys (a block of keys for each wave) or more and at most 32, as
-//    the join reads them all.  Unsplit up to 512 keys: one step behind 322 keys 9.2
-//    us in one part, 10.7 in two; behind 1500 13.1 in three of 512, 11.1 in six of 256.
-//    Blocks wanted, us: 64 heads behind 8000 (f16) 256 43.4, 512 45.9, 1024 52.6;
-//    256 behind 4352 (f16) 70.1, 73.8, 81; 192 behind 8192 (e4m3, whose blocks fit
-//    two to a CU) 62.8, 52.5, 53.4; 8 behind 32770 (e4m3) 19.2, in 64 parts 21.3.
+//    block's four waves take turns at a part of its keys, each with tiles of its own.
+//    Bound by the cache's bytes, so a sequence is cut where its block alone would be
+//    at work after the others, or CUs have none: a join costs about 5 us.  Unsplit up to
+//    20 keys for each sequence and kv head of the batch (us, unsplit / the best split;
+//    f16, hd 128: 64 of them behind up to 700 keys 10.8 / 11.0, 1500 15.5 / 13.4; 128
+//    behind 1500 17.1 / 19.2, 4300 49.1 / 39.3; 256 behind 4300 70.5 / 73.3), and up to
+//    4096 keys past 256 of them (512 behind 3300 93.7 / 93.9, e4m3 4352 73.2 / 67.5).
+//    Else into parts that give every CU its blocks (one, or two of e4m3 or hd 64, by
+//    their LDS), and with more sequences into more, down to 1024 keys, as their joins
+//    are one launch (e4m3, 512 behind 8192, in 1, 3, 5, 9 parts: 133.6, 124.7, 122.8,
+//    121.1; f16, 64 behind 8192 in 5 and 9: 26.5, 28.8).  The number is odd: blocks go to
+//    CUs in turns, and with an even one the same CUs get all the first, full parts
+//    (512 behind 4352, f16, in 3, 4, 5: 118.6, 148.9, 122).  A part is a multiple of 256
+//    keys, a block of 64 for each wave.
 //  * many: tiles of 64 or 128 pairs.  Of 64 up to 700 tiles: 128-row blocks load each
 //    tile for twice the rows, but are half as many, each with twice the steps (8 kv
 //    heads, no past, 64 -> 128, us: 1500 rows 29.8 -> 41.9, 2500 67 -> 65, 3500 108 ->
@@ -201,8 +207,18 @@ Split split_of(const PagedAttnParams& p, bool e4m3, int hd) {
   s.few = !s.many || (int64_t)p.kv.seqs * p.kv.max_rows > p.kv.tokens;
   s.few_chunks = s.many_chunks = 1;
   if (s.few) {
-    const int64_t want = !e4m3 && hd == 128 ? kCus : 2 * kCus, parts = heads ? (want + heads - 1) / heads : 1;
-    divide(len <= 512 ? 1 : parts < 32 ? parts : 32, 256, &s.few_chunk, &s.few_chunks);
+    const int64_t slots = !e4m3 && hd == 128 ? kCus : 2 * kCus;  // blocks that are at work at once
+    const int64_t whole = heads <= kCus ? 20 * heads : 4096;
+    int64_t parts = 1;
+    if (heads > 0 && len > (whole > 512 ? whole : 512)) {
+      const int64_t fill = (slots + heads - 1) / heads;
+      const int64_t some = (heads < 4096 ? heads : 4096) * len * slots >> 26, most = len / 1024, even = some < most ? some : most;
+      parts = (fill > even ? fill : even) | 1;
+      parts = parts < 33 ? parts : 33;
+    }
+    // (rounding a part to 256 keys may leave an even number of them)
+    do divide(parts, 256, &s.few_chunk, &s.few_chunks);
+    while (s.few_chunks % 2 == 0 && s.few_chunk > 256 && heads * s.few_chunks > slots && (parts += 2));
   }
   if (s.many) {
     // full tiles of a batch of this many rows, and a sequence's short last one; a

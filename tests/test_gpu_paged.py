@@ -426,6 +426,19 @@ def test_attention_of_single_tokens_behind_many_pages(ctx, pkg, dtype, cache, pa
 
 
 @FORMATS
+@pytest.mark.parametrize("page,hd", [(16, 64), (64, 128)])
+def test_attention_of_single_tokens_behind_pages_in_one_part(ctx, pkg, dtype, cache, page, hd):
+    """32 sequences of 8 kv heads behind up to 5000 keys: no call needs a workspace, a wave has up to 20 blocks."""
+    b = Batch.shared([1] * 32, [5000, 4097, 4352, 4353] + [60] * 27 + [4800], page, 16, 8, hd, dtype, cache, seed=108)
+    b.table[[0, 31], 4500 // page] = -1
+    b.upload(ctx)
+    q = b.random_rows(16 * hd)
+    assert pkg.attention_paged_workspace(paged.attention_desc(pkg, b, 0, 16 * hd, 0, 16 * hd)) == 0
+    assert_attention(b, q, attention(ctx, pkg, b, q), seqs=(0, 1, 2, 3, 30, 31))
+    b.free()
+
+
+@FORMATS
 @pytest.mark.parametrize("page,hd", [(16, 64), (64, 64), (32, 128)])
 def test_attention_of_rows_behind_many_pages(ctx, pkg, dtype, cache, page, hd):
     """The same for 17 and more rows: 128 sequences of 2 kv heads."""
