@@ -176,9 +176,11 @@ struct Cfg {
 //  * many: tiles of 64 or 128 pairs.  Of 64 up to 700 tiles: 128-row blocks load each
 //    tile for twice the rows, but are half as many, each with twice the steps (8 kv
 //    heads, no past, 64 -> 128, us: 1500 rows 29.8 -> 41.9, 2500 67 -> 65, 3500 108 ->
-//    92, 4334 155 -> 144).  Their keys are split while the CUs take the parts at once:
-//    64 rows behind 16000 keys 178 us whole, 28.8 in 32 parts; but 771 behind 1536
-//    (200 blocks) 35 whole, 45 in two, as half the CUs' parts have to wait.
+//    92, 4334 155 -> 144).  Their keys are split while the CUs take the parts at once,
+//    down to 256: 64 rows behind 16000 keys 178 us whole, 28.8 in 32 parts; 200 behind
+//    700 19.1 whole, 16.6 in four; but 771 behind 1536 (200 blocks) 35 whole, 45 in
+//    two, as half the CUs' parts have to wait.  Up to 640 keys there is no gain (600
+//    and none before, 4 kv heads of 64: 12.4 whole, 13.5 in three).
 constexpr int kFewRows = 16, kFewWaves = 4;
 constexpr int kManyWaves = 8;
 constexpr int kCus = 256;
@@ -225,12 +227,18 @@ Split split_of(const PagedAttnParams& p, bool e4m3, int hd) {
     // sequence has to have rows for that, more than few where `few` takes the others
     const int64_t pairs = p.kv.tokens * p.rep, least = s.few ? kFewRows + 1 : p.rep;
     const int64_t ends = pairs / least < p.kv.seqs ? pairs / least : p.kv.seqs;
-    auto about = [&](int64_t r) { return p.kv.nkvh * ((pairs + r - 1) / r > ends ? (pairs + r - 1) / r : ends); };
+    // what there will be: at least a tile of each such sequence, or the short ones of
+    // as few sequences as have the rows
+    const int64_t full = (p.kv.tokens + p.kv.max_rows - 1) / p.kv.max_rows;
+    auto most = [&](int64_t r) { return p.kv.seqs * ((rows + r - 1) / r); };
+    auto about = [&](int64_t r) {
+      const int64_t n = pairs / r + full > ends ? pairs / r + full : ends;
+      return p.kv.nkvh * (n < most(r) ? n : most(r));
+    };
     s.many_rows = about(64) > 700 ? 128 : 64;
-    const int64_t most = (int64_t)p.kv.seqs * ((rows + s.many_rows - 1) / s.many_rows);
-    s.tiles = (int)(pairs / s.many_rows + ends < most ? pairs / s.many_rows + ends : most);
+    s.tiles = (int)(pairs / s.many_rows + ends < most(s.many_rows) ? pairs / s.many_rows + ends : most(s.many_rows));
     const int64_t blocks = about(s.many_rows);
-    divide(blocks > 0 && blocks < kCus ? kCus / blocks : 1, 512, &s.many_chunk, &s.many_chunks);
+    divide(len > 640 && blocks > 0 && blocks < kCus ? kCus / blocks : 1, 256, &s.many_chunk, &s.many_chunks);
   }
   s.parts = s.many_chunks > s.few_chunks ? s.many_chunks : s.few_chunks;
   return s;
