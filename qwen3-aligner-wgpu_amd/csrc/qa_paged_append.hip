@@ -12,6 +12,10 @@
 // must, rounds what the page held again, and stores the rows, with no other
 // block to wait for.  The V page is [hd][page], so V goes through an LDS tile.
 //
+// Bound by the bytes: 4334 rows of 16 q and 8 kv heads of 128 into empty e4m3 pages, 67
+// MB, 18.1 us (3.7 TB/s; the f64 of K is 1.1 of them); a step's few rows by the
+// launch and a chain of loads, row_start, the table, the row: 32 single rows 3.8 us.
+//
 // e4m3 scales are powers of two, the least 2^e with amax <= 448 * 2^e: dividing by
 // one is exact, so a value is rounded once however often its page's scale
 // grows, but for what falls below e4m3's normal range (2^-6 of the scale).
@@ -79,6 +83,26 @@ __device__ __forceinline__ Turn load_turn(const float* nw, const float* cs, cons
   load8(t.si, sn + 8 * c);
   return t;
 }
+// The sum over the 4 or 8 lanes that share a head, by moves within a row of lanes:
+// each lane's neighbour, the neighbouring pair, and (8) the mirrored lane.
+template <int CTRL>
+__device__ __forceinline__ float moved(float v) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), CTRL, 0xF, 0xF, true));
+}
+template <int CTRL>
+__device__ __forceinline__ double moved(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)u, CTRL, 0xF, 0xF, true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, true);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+template <int HD, class T>
+__device__ __forceinline__ T head_sum(T s) {
+  s += moved<0xB1>(s);                              // quad_perm [1, 0, 3, 2]
+  s += moved<0x4E>(s);                              // quad_perm [2, 3, 0, 1]
+  if constexpr (HD == 128) s += moved<0x141>(s);    // row_half_mirror
+  return s;
+}
 // The normed and rotated chunks of a q or k head from its raw ones, for the HD / 16
 // lanes that share it (all of them call).
 template <int DT, int HD>
@@ -97,14 +121,46 @@ __device__ __forceinline__ void norm_rope(u32x4 va, u32x4 vb, const Turn& t, flo
     s += xa[e] * xa[e];
     s += xb[e] * xb[e];
   }
-#pragma unroll
-  for (int o = 1; o < HD / 16; o <<= 1) s += __shfl_xor(s, o, 64);
-  const float inv = 1.0f / sqrtf(s / (float)HD + eps);
+  const float inv = 1.0f / sqrtf(head_sum<HD>(s) / (float)HD + eps);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const float a = xa[e] * inv * t.wa[e], b = xb[e] * inv * t.wb[e];
     xa[e] = a * t.co[e] - b * t.si[e];
     xb[e] = b * t.co[e] + a * t.si[e];
+  }
+}
+
+// x to f32 so that a further rounding, to fewer bits, gives what rounding x itself
+// to those would: towards zero, with the last bit set where anything was lost.
+__device__ __forceinline__ float to_odd(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = (uint32_t)u, lost = (lo & 0x1fffffffu) + 0x1fffffffu;  // bit 29: some of the 29 bits is set
+  return (float)__builtin_bit_cast(double, (u & ~0xffffffffull) | ((lo | lost) & 0xe0000000u));
+}
+// The same for a k head that goes to e4m3, whose steps are 2^20 times f32's: in f32 a
+// few values of a long prompt end up on the other side of a step's middle than
+// their definition.  In f64 none does (4334 rows 17.0 -> 18.1 us).
+template <int DT, int HD>
+__device__ __forceinline__ void norm_rope_exact(u32x4 va, u32x4 vb, const Turn& t, float eps, float* xa, float* xb) {
+  float fa[8], fb[8];
+  double q[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const f32x2 a = widen2<DT>(va[e]), b = widen2<DT>(vb[e]);
+    fa[2 * e] = a[0];
+    fa[2 * e + 1] = a[1];
+    fb[2 * e] = b[0];
+    fb[2 * e + 1] = b[1];
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) q[e & 3] = fma((double)fa[e], (double)fa[e], fma((double)fb[e], (double)fb[e], q[e & 3]));
+  const double v = head_sum<HD>((q[0] + q[1]) + (q[2] + q[3])) * (1.0 / HD) + (double)eps, y = __builtin_amdgcn_rsq(v);  // y to 2^-23: one step of Newton's
+  const double inv = v < (double)INFINITY ? y * fma(-0.5 * v * y, y, 1.5) : v == v ? 0.0 : v;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const double a = (double)fa[e] * (double)t.wa[e] * inv, b = (double)fb[e] * (double)t.wb[e] * inv;
+    xa[e] = to_odd(fma(a, (double)t.co[e], -b * (double)t.si[e]));
+    xb[e] = to_odd(fma(b, (double)t.co[e], a * (double)t.si[e]));
   }
 }
 
@@ -188,6 +244,7 @@ __device__ __forceinline__ void kv_part(const AppendParams& p, int64_t b, int sl
   float ka = 0.f, va = 0.f;
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
+    if (i * RP >= nr) break;
     const int r = i * RP + tid / L, c = tid % L;
     const bool on = r < nr;
     const int at = on ? r : nr - 1;  // lanes past the last row do it again, and store nothing
@@ -206,7 +263,8 @@ __device__ __forceinline__ void kv_part(const AppendParams& p, int64_t b, int sl
         }
       }
     }
-    norm_rope<DT, HD>(wk[0], wk[1], turn, p.eps, xa[i], xb[i]);
+    if constexpr (F8) norm_rope_exact<DT, HD>(wk[0], wk[1], turn, p.eps, xa[i], xb[i]);
+    else norm_rope<DT, HD>(wk[0], wk[1], turn, p.eps, xa[i], xb[i]);
     if constexpr (F8) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) ka = fmaxf(ka, fmaxf(finite_abs(xa[i][e]), finite_abs(xb[i][e])));

@@ -8,6 +8,10 @@
 // equal, made on the device because positions of images and video are not a
 // running number: once for a step, for every layer's q / k rotation.
 //
+// Bound by the rows it writes: 30720 tokens of hd 128, 31 MB, 9.6 us, of which the
+// launch is 4 and the f64 of angles and series 1.5; 32 tokens 4.4 us.  (With the
+// library's sincos, whose reduction takes any angle, 10.7.)
+//
 // The angle is formed in f64 (a position of 2^20 leaves an f32 angle no more
 // than 4 bits of a turn's fraction), as are its cosine and sine: |angle| < 2^31
 // since theta >= 1, which lets two products of a quarter turn's halves reduce it

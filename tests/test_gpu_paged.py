@@ -234,6 +234,27 @@ def test_append_scales_that_are_no_powers_of_two(ctx, pkg):
         b.free()
 
 
+@DTYPES
+@pytest.mark.parametrize("hd", [64, 128])
+def test_append_rounds_keys_to_e4m3_once(ctx, pkg, dtype, hd):
+    """1500 keys a head: every code and scale is that of the 64-bit value.  The kernel's f64 is 2^-44 off at the most and a
+    value is within that of a step's middle with a chance of 2^-40: none of 2^20 is."""
+    b = Batch([1500], [1500], 32, 4, 4, hd, dtype, E4M3, seed=15)
+    b.stale()
+    b.upload(ctx)
+    qkv, qn, kn, c, s = _inputs(b, 1.0)
+    append(ctx, pkg, b, qkv, qn, kn, c, s)
+    after = b.read(ctx)
+    x = widen(qkv, dtype).reshape(b.tokens, -1, hd)[:1500, 4:8]
+    k = _turned(b, x, kn, c[:1500], s[:1500])[0]
+    for i in range(-(-1500 // 32)):
+        p, part = b.table[0, i], k[32 * i:32 * i + 32].transpose(1, 0, 2)
+        scale = scale_for(np.abs(part).max((1, 2)))
+        assert np.array_equal(after["k_scale"][p], scale)
+        assert np.array_equal(after["k"][p][:, : part.shape[1]], e4m3_codes(part / scale[:, None, None]))
+    b.free()
+
+
 def test_append_infinities_and_nan(ctx, pkg):
     """V with infinities and NaN in e4m3: the largest value and NaN, no part in the scale; in 16 bits as they are."""
     for cache in (E4M3, F16):
