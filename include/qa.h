@@ -397,8 +397,9 @@ int qa_kv_append(qa_ctx* ctx, const qa_kv_append_desc* desc);
  * out[t][h hd + j] = round(sum_t p_t v_t[j]).  Keys on an entry that is no page do
  * not count; a row without keys gives zeros.  What the pages hold behind a
  * sequence's last key is not looked at.  Scales may be any positive numbers.  V has
- * to be finite for all of a sequence's keys: a row multiplies those behind its
- * position by 0, which leaves NaN of an infinity or NaN (K may hold either there).
+ * to be finite, and below 2^100, for all of a sequence's keys: a row multiplies
+ * those behind its position by 0, which leaves NaN of an infinity or NaN (K may
+ * hold either there), and probabilities are up to 2^8 before they are divided.
  *   q    [tokens][nqh hd], row stride ldq, as qa_kv_append writes it
  *   out  [tokens][nqh hd], row stride ldo, the o projection's input
  *   workspace  16-byte aligned device memory for partial results, of the bytes

@@ -28,7 +28,8 @@ struct PagedParams {
 
 // A sequence's part of the batch: rows row0 .. row0 + n - 1, the first of them at
 // position pos0 (negative where the sequence has fewer keys than rows), len
-// keys in all.
+// keys in all.  Rows that are left out, past max_rows or the batch's end, keep
+// their positions: the others' do not move.
 struct SeqSpan {
   int64_t row0;
   int n, pos0, len;
@@ -38,11 +39,11 @@ QA_HD int64_t clamp64(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : 
 
 QA_HD SeqSpan seq_span(const PagedParams& p, int s) {
   const int64_t a = clamp64(p.row_start[s], 0, p.tokens);
-  const int64_t e = clamp64(p.row_start[s + 1], a, p.tokens);
+  const int64_t last = p.row_start[s + 1] > a ? p.row_start[s + 1] : a, e = last < p.tokens ? last : p.tokens;
   SeqSpan q;
   q.row0 = a;
   q.len = (int)clamp64(p.kv_len[s], 0, p.max_len);
-  q.pos0 = (int)(q.len - (e - a));
+  q.pos0 = (int)clamp64(q.len - (last - a), -(1 << 30), q.len);  // (a batch has at most 2^30 rows)
   q.n = (int)clamp64(e - a, 0, p.max_rows);
   return q;
 }

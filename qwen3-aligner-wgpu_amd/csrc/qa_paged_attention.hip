@@ -195,7 +195,7 @@ struct Split {
 
 Split split_of(const PagedAttnParams& p, bool e4m3, int hd) {
   Split s{};
-  const int64_t rows = (int64_t)p.kv.max_rows * p.rep, len = p.kv.max_len > 1 ? p.kv.max_len : 1;
+  const int64_t rows = (p.kv.max_rows < p.kv.tokens ? p.kv.max_rows : p.kv.tokens) * p.rep, len = p.kv.max_len > 1 ? p.kv.max_len : 1;
   const int64_t heads = (int64_t)p.kv.seqs * p.kv.nkvh;
   auto divide = [&](int64_t parts, int64_t least, int* chunk, int* chunks) {
     int64_t c = (len + parts - 1) / parts;

@@ -325,6 +325,7 @@ ATTENTION = [
     ([3, 4], [0, 2], 32, 4, 2, 64),
     ([0, 0], [5, 0], 16, 2, 1, 128),
     ([31, 17, 1, 16, 15], [31, 80, 81, 16, 47], 16, 10, 2, 64),
+    ([1, 3], [70, 40], 16, 200, 1, 64),                                   # a row's heads in several tiles
 ]
 
 
@@ -403,6 +404,36 @@ def test_attention_of_lengths_past_the_bounds(ctx, pkg, dtype, cache):
     assert_attention(b, q, attention(ctx, pkg, b, q))
     got = attention(ctx, pkg, b, q, max_rows=2)
     assert (got[3:5] == 0x3C01).all() and (got[:3] != 0x3C01).any(1).all()
+    b.free()
+
+
+@FORMATS
+def test_rows_past_the_batch_are_left_out(ctx, pkg, dtype, cache):
+    """The last sequence's last five rows lie past `tokens`: the others have the same positions, keys and bits as with
+    them, and nothing stands in for those."""
+    b = Batch([1, 40], [20, 45], 16, 4, 2, 64, dtype, cache, seed=46, tail_rows=0)
+    b.fill(kstd=0.3, vstd=0.3)
+    b.upload(ctx)
+    q = b.random_rows(4 * 64)
+    want = attention(ctx, pkg, b, q)
+    before, (qkv, qn, kn, c, s) = b.read(ctx), _inputs(b)
+    b.tokens -= 5
+    assert np.array_equal(attention(ctx, pkg, b, q[:36]), want[:36])
+    append(ctx, pkg, b, qkv[:36], qn, kn, c[:36], s[:36])
+    after = b.read(ctx)
+    p = b.table[1, 2]  # positions 32 .. 44: 40 .. 44 keep what they held, at the page's scale
+    if cache == E4M3:
+        held = e4m3_values(before["v"][p, :, :, 8:13]) * before["v_scale"][p].astype(np.float64)[:, None, None]
+        now = e4m3_values(after["v"][p, :, :, 8:13]) * after["v_scale"][p].astype(np.float64)[:, None, None]
+        if (after["v_scale"][p] == before["v_scale"][p]).all():
+            assert np.array_equal(held, now)
+        new = widen(qkv, dtype).reshape(41, -1, 64)[28:36, 6:].transpose(1, 2, 0)
+        got = e4m3_values(after["v"][p, :, :, :8]) * after["v_scale"][p].astype(np.float64)[:, None, None]
+        step = e4m3_step(new / after["v_scale"][p].astype(np.float64)[:, None, None]) * after["v_scale"][p].astype(np.float64)[:, None, None]
+        assert (np.abs(got - new) <= step / 2).all()
+    else:
+        assert np.array_equal(after["v"][p, :, :, 8:], before["v"][p, :, :, 8:])
+        assert np.array_equal(after["v"][p, :, :, :8], qkv.reshape(41, -1, 64)[28:36, 6:].transpose(1, 2, 0))
     b.free()
 
 

@@ -169,6 +169,8 @@ int main() {
           const qa::SeqSpan q = qa::seq_span(p, 0);
           if (q.n < 0 || q.n > max_rows || q.row0 < 0 || q.row0 + q.n > tokens || q.len < 0 || q.len > p.max_len) ++bad;
           if (q.n > 0 && (int64_t)q.pos0 + q.n > q.len) ++bad;  // a row's position is a key's
+          // a row that is kept has the position that it has without the bounds
+          if (q.n > 0 && a >= 0 && a < b && b < 1 << 30 && q.pos0 != q.len - ((int64_t)b - a)) ++bad;
           const int64_t elems = 17 * 2 * (128LL << lp);
           for (int i = -3; i < q.n + 3; ++i) {
             const int pos = q.pos0 + i;
