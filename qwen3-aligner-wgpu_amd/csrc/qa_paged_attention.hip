@@ -35,7 +35,7 @@
 // 35 us, 346 TFLOP/s, 519 with the products of the residues; 4334 rows 144 us.
 // Keys of long sequences are split among blocks, which leave (O, max, sum) in the
 // workspace for paged_join_kernel.
-#include <type_traits>
+#include <utility>
 
 #include "qa_internal.h"
 
@@ -195,7 +195,7 @@ struct Split {
 
 Split split_of(const PagedAttnParams& p, bool e4m3, int hd) {
   Split s{};
-  const int64_t rows = (p.kv.max_rows < p.kv.tokens ? p.kv.max_rows : p.kv.tokens) * p.rep, len = p.kv.max_len > 1 ? p.kv.max_len : 1;
+  const int64_t rows = (int64_t)p.kv.max_rows * p.rep, len = p.kv.max_len > 1 ? p.kv.max_len : 1;
   const int64_t heads = (int64_t)p.kv.seqs * p.kv.nkvh;
   auto divide = [&](int64_t parts, int64_t least, int* chunk, int* chunks) {
     int64_t c = (len + parts - 1) / parts;
@@ -311,26 +311,13 @@ __device__ __forceinline__ int v_swizzle(int c, int lcp) {
 struct Pages {
   int lo, hi;
 };
-template <int OF, int PER, class Off>
-__device__ __forceinline__ void copy_page(const unsigned char* src, int bytes, unsigned char* to, int mine, Off off) {
-  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(src), (short)0, bytes, 0x00020000);
-#pragma unroll
-  for (int b = 0; b < (PER + 3) / 4; ++b) {  // 4 KB: the reach of the instruction's offset
-    QA_LDS void* dst = (QA_LDS void*)(to + b * 4096 + mine * 1024);
-    const int at = b * 4096 + mine * 1024;
-    auto one = [&](auto i) {
-      constexpr int I = decltype(i)::value;
-      if constexpr (I * OF < 4)
-        if (b * 4 + I * OF < PER) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, dst, 16, off(b * 4 + I * OF), at, I * OF * 1024, 0);
-    };
-    one(std::integral_constant<int, 0>{});
-    one(std::integral_constant<int, 1>{});
-    one(std::integral_constant<int, 2>{});
-    one(std::integral_constant<int, 3>{});
-  }
+template <class F, int... I>
+__device__ __forceinline__ void each(F f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
 }
-template <int DT, bool F8, int HD, bool W32, int OF, int LP, bool K>
-__device__ __forceinline__ void load_pages(const PagedParams& kv, const Pages& pages, int j, int mine, unsigned char* to) {
+// Instructions FROM .. TO - 1 of a wave's LI / OF.
+template <int DT, bool F8, int HD, bool W32, int OF, int LP, bool K, int FROM = 0, int TO = Cfg<DT, F8, HD>::LI / OF>
+__device__ __forceinline__ void load_tile(const PagedParams& kv, const Pages& pages, int j, int mine, unsigned char* to) {
   using C = Cfg<DT, F8, HD>;
   constexpr int PER = C::LI >> (6 - LP), PB = HD * C::ES << LP;  // instructions and bytes of a page
   constexpr int CW = K ? C::CR : (1 << LP) * C::ES / 16;          // chunks of a row
@@ -355,30 +342,26 @@ __device__ __forceinline__ void load_pages(const PagedParams& kv, const Pages& p
     *bytes = hi < 0 ? 0 : PB;
     return (const unsigned char*)(K ? kv.k : kv.v) + ((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
   };
-  if constexpr (PER >= OF) {
-#pragma unroll
-    for (int pg = 0; pg < 64 >> LP; ++pg) {
+  auto one = [&](auto number) {
+    constexpr int I = decltype(number)::value;
+    if constexpr (I >= FROM && I < TO && PER >= OF) {
+      constexpr int PW = PER / OF, pg = I / PW, N = I % PW * OF;  // N: of the page, the first wave's
+      constexpr int B = N / 4 * 4096;                              // 4 KB: the reach of the instruction's offset
       int bytes;
       const unsigned char* src = page_src(pg, &bytes);
-      copy_page<OF, PER>(src, bytes, to + pg * PER * 1024, mine, [&](int n) { return off(n + mine, pg); });
-    }
-  } else {  // fewer instructions to a page than waves: pages side by side
-    constexpr int PP = OF / PER;
-#pragma unroll
-    for (int p0 = 0; p0 < 64 >> LP; p0 += PP) {
-      const int pg = p0 + mine / PER, n = mine % PER;
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(src), (short)0, bytes, 0x00020000);
+      QA_LDS void* dst = (QA_LDS void*)(to + pg * PER * 1024 + B + mine * 1024);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, dst, 16, off(N + mine, pg), B + mine * 1024, N % 4 * 1024, 0);
+    } else if constexpr (I >= FROM && I < TO) {  // fewer instructions to a page than waves: pages side by side
+      const int pg = I * (OF / PER) + mine / PER, n = mine % PER;
       int bytes;
       const unsigned char* src = page_src(pg, &bytes);
-      copy_page<1, 1>(src + n * 1024, bytes - n * 1024 > 0 ? bytes - n * 1024 : 0, to + (pg * PER + n) * 1024, 0,
-                      [&](int) { return off(n, pg); });
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(src), (short)0, bytes, 0x00020000);
+      QA_LDS void* dst = (QA_LDS void*)(to + (pg * PER + n) * 1024);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, dst, 16, off(n, pg), n * 1024, 0, 0);
     }
-  }
-}
-template <int DT, bool F8, int HD, bool W32, int OF, bool K>
-__device__ __forceinline__ void load_tile(const PagedParams& kv, const Pages& pages, int j, int mine, unsigned char* to) {
-  if (kv.lp == 6) load_pages<DT, F8, HD, W32, OF, 6, K>(kv, pages, j, mine, to);
-  else if (kv.lp == 5) load_pages<DT, F8, HD, W32, OF, 5, K>(kv, pages, j, mine, to);
-  else load_pages<DT, F8, HD, W32, OF, 4, K>(kv, pages, j, mine, to);
+  };
+  each(one, std::make_integer_sequence<int, 16>{});
 }
 // Fragment addresses in the tiles.  K: product t reads row 16 (c / 4) + 4 t + c % 4,
 // slice e the chunk 4 e + g.  V: row d, the chunks of keys 16 g ..
@@ -626,7 +609,7 @@ constexpr int few_lds() {
   constexpr int tiles = kFewWaves * 2 * Cfg<DT, F8, HD>::TILE, join = kFewWaves * 64 * (HD + 8);
   return tiles > join ? tiles : join;
 }
-template <int DT, bool F8, int HD>
+template <int DT, bool F8, int HD, int LP>
 __device__ __forceinline__ void few_block(const PagedAttnParams& p, const Split& sp, int block, unsigned char* smem) {
   using C = Cfg<DT, F8, HD>;
   const PagedParams& kv = p.kv;
@@ -643,7 +626,7 @@ __device__ __forceinline__ void few_block(const PagedAttnParams& p, const Split&
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const int nb = k1 > k0 ? (k1 - k0 + 63) >> 6 : 0, steps = (nb - wave + kFewWaves - 1) / kFewWaves;
   unsigned char *kt = smem + wave * 2 * C::TILE, *vt = kt + C::TILE;
-  const int lcp = kv.lp - (F8 ? 4 : 3);
+  constexpr int lcp = LP - (F8 ? 4 : 3);
   Pages pages = {-1, -1};
   float ksc = 1.f, vsc = 0.f;
   bool holes = false;
@@ -656,8 +639,8 @@ __device__ __forceinline__ void few_block(const PagedAttnParams& p, const Split&
   load_q<F8, HD>(p, col, g, q);
   if (steps > 0) {
     fetch(0, found);
-    load_tile<DT, F8, HD, false, 1, true>(kv, pages, 0, 0, kt);
-    load_tile<DT, F8, HD, false, 1, false>(kv, pages, 0, 0, vt);
+    load_tile<DT, F8, HD, false, 1, LP, true>(kv, pages, 0, 0, kt);
+    load_tile<DT, F8, HD, false, 1, LP, false>(kv, pages, 0, 0, vt);
   }
   keep(q);
   f32x4 o[C::ND] = {};
@@ -683,7 +666,7 @@ __device__ __forceinline__ void few_block(const PagedAttnParams& p, const Split&
     wait_lds();
     if (more) {
       if ((it & 15) == 15) fetch(it + 1, page_ids(kv, s, [&](int j) { return key_of(it + 1 + j); }));
-      load_tile<DT, F8, HD, false, 1, true>(kv, pages, (it + 1) & 15, 0, kt);
+      load_tile<DT, F8, HD, false, 1, LP, true>(kv, pages, (it + 1) & 15, 0, kt);
     }
     softmax<DT, F8, HD>(sc, col.pos, kg, have, p.scale * kLog2e * ks, vs, m, l, o, ph, pl);
     if (more) wait_vmcnt<C::LI>();  // V is there; the next K's loads came after it
@@ -691,16 +674,16 @@ __device__ __forceinline__ void few_block(const PagedAttnParams& p, const Split&
     if (__builtin_amdgcn_ballot_w64(have < 16)) clear_tail<DT, F8, HD>(vt, va, lcp, have);
     multiply_v<DT, F8, HD>(vt, va, lcp, ph, pl, o);
     wait_lds();
-    if (more) load_tile<DT, F8, HD, false, 1, false>(kv, pages, (it + 1) & 15, 0, vt);
+    if (more) load_tile<DT, F8, HD, false, 1, LP, false>(kv, pages, (it + 1) & 15, 0, vt);
   }
   __syncthreads();  // the tiles' LDS is the join's
   finish<DT, HD>(p, sp, sq, h, part, end <= sp.few_chunk, m, l, o, smem);
 }
 
-template <int DT, bool F8, int HD>
+template <int DT, bool F8, int HD, int LP>
 __global__ void __launch_bounds__(64 * kFewWaves) paged_few_kernel(const PagedAttnParams p, const Split sp) {
   __shared__ __attribute__((aligned(1024))) unsigned char smem[few_lds<DT, F8, HD>()];
-  few_block<DT, F8, HD>(p, sp, (int)blockIdx.x, smem);
+  few_block<DT, F8, HD, LP>(p, sp, (int)blockIdx.x, smem);
 }
 
 // ---- tiles of 64 or 128 (row, head) pairs ----
@@ -909,7 +892,7 @@ __device__ __forceinline__ bool find_tile(const PagedAttnParams& p, const Split&
   }
   return false;
 }
-template <int DT, bool F8, int HD, int GW>
+template <int DT, bool F8, int HD, int LP, int GW>
 __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const PagedAttnParams p, const Split sp) {
   using C = Cfg<DT, F8, HD>;
   constexpr int NS = kManyWaves / GW, NB = many_buffers<DT, F8, HD, GW>(), WL = C::LI / GW;  // WL: a wave's loads of a tile
@@ -919,7 +902,7 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
   const int mine = (int)blockIdx.x - sp.tiles * sp.many_chunks * kv.nkvh;
   if (mine >= 0) {  // behind them, the blocks of the sequences of few rows, four waves each
     // (the other waves end here, and a barrier waits for no wave that has ended)
-    if (threadIdx.x < 64 * kFewWaves) few_block<DT, F8, HD>(p, sp, mine, smem);
+    if (threadIdx.x < 64 * kFewWaves) few_block<DT, F8, HD, LP>(p, sp, mine, smem);
     return;
   }
   const int kvh = (int)(blockIdx.x % kv.nkvh);
@@ -940,7 +923,7 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
   unsigned char* base = smem + ns * 2 * NB * C::TILE;
   auto kt = [&](int it) { return base + (it & (NB - 1)) * C::TILE; };
   auto vt = [&](int it) { return base + (NB + (it & (NB - 1))) * C::TILE; };
-  const int lcp = kv.lp - (F8 ? 4 : 3), cp = 1 << lcp;
+  constexpr int lcp = LP - (F8 ? 4 : 3), cp = 1 << lcp;
   // two windows of 16 blocks' pages: loads run up to two blocks ahead of the softmax
   bool holes = false;
   Pages pages0 = {-1, -1}, pages1 = {-1, -1};
@@ -961,10 +944,10 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
   };
   auto pages_of = [&](int it) { return it >> 4 & 1 ? pages1 : pages0; };
   auto issue_k = [&](int it) {
-    load_tile<DT, F8, HD, true, GW, true>(kv, pages_of(it), scalar(it & 15), scalar(wg), smem + scalar((int)(kt(it) - smem)));
+    load_tile<DT, F8, HD, true, GW, LP, true>(kv, pages_of(it), scalar(it & 15), scalar(wg), smem + scalar((int)(kt(it) - smem)));
   };
   auto issue_v = [&](int it) {
-    load_tile<DT, F8, HD, true, GW, false>(kv, pages_of(it), scalar(it & 15), scalar(wg), smem + scalar((int)(vt(it) - smem)));
+    load_tile<DT, F8, HD, true, GW, LP, false>(kv, pages_of(it), scalar(it & 15), scalar(wg), smem + scalar((int)(vt(it) - smem)));
   };
   // refill(j), in step j's VALU phase: K of block j + NB (S of j has read its slot),
   // V of block j + NB - 1 (P.V of j - 1 has).  Step i's MFMA phase needs K(i) and
@@ -1207,17 +1190,17 @@ int64_t join_groups(const PagedAttnParams& p, const Split& sp, int hd, int64_t* 
   return sp.many_chunks == 1 ? 0 : (int64_t)sp.tiles * (sp.many_rows * hd / 1024);
 }
 
-template <int DT, bool F8, int HD>
+template <int DT, bool F8, int HD, int LP>
 hipError_t launch_one(const PagedAttnParams& p, hipStream_t s) {
   const Split sp = split_of(p, F8, HD);
   const int64_t heads = (int64_t)p.kv.seqs * p.kv.nkvh;
   if (sp.many) {
     const dim3 grid((unsigned)((int64_t)p.kv.nkvh * sp.tiles * sp.many_chunks + (sp.few ? heads * sp.few_chunks : 0)));
     const dim3 block(64 * kManyWaves);
-    if (sp.many_rows == 64) hipLaunchKernelGGL((paged_many_kernel<DT, F8, HD, 2>), grid, block, 0, s, p, sp);
-    else hipLaunchKernelGGL((paged_many_kernel<DT, F8, HD, 4>), grid, block, 0, s, p, sp);
+    if (sp.many_rows == 64) hipLaunchKernelGGL((paged_many_kernel<DT, F8, HD, LP, 2>), grid, block, 0, s, p, sp);
+    else hipLaunchKernelGGL((paged_many_kernel<DT, F8, HD, LP, 4>), grid, block, 0, s, p, sp);
   } else {
-    hipLaunchKernelGGL((paged_few_kernel<DT, F8, HD>), dim3((unsigned)(heads * sp.few_chunks)), dim3(64 * kFewWaves), 0, s, p, sp);
+    hipLaunchKernelGGL((paged_few_kernel<DT, F8, HD, LP>), dim3((unsigned)(heads * sp.few_chunks)), dim3(64 * kFewWaves), 0, s, p, sp);
   }
   if (sp.parts > 1) {
     int64_t few_rows;
@@ -1228,10 +1211,15 @@ hipError_t launch_one(const PagedAttnParams& p, hipStream_t s) {
   return hipGetLastError();
 }
 
+template <int DT, bool F8, int HD>
+hipError_t launch_lp(const PagedAttnParams& p, hipStream_t s) {
+  return p.kv.lp == 4 ? launch_one<DT, F8, HD, 4>(p, s) : p.kv.lp == 5 ? launch_one<DT, F8, HD, 5>(p, s) : launch_one<DT, F8, HD, 6>(p, s);
+}
+
 template <int DT>
 hipError_t launch_dt(bool e4m3, int hd, const PagedAttnParams& p, hipStream_t s) {
-  if (hd == 64) return e4m3 ? launch_one<DT, true, 64>(p, s) : launch_one<DT, false, 64>(p, s);
-  return e4m3 ? launch_one<DT, true, 128>(p, s) : launch_one<DT, false, 128>(p, s);
+  if (hd == 64) return e4m3 ? launch_lp<DT, true, 64>(p, s) : launch_lp<DT, false, 64>(p, s);
+  return e4m3 ? launch_lp<DT, true, 128>(p, s) : launch_lp<DT, false, 128>(p, s);
 }
 
 }  // namespace
