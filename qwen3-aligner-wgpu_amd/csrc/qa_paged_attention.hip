@@ -27,12 +27,12 @@
 // are multiplied as bf16 there, whose range takes any scale.
 //
 // Sequences of up to 16 pairs (single tokens): paged_few_kernel.  Bound by the
-// cache's bytes: 32 sequences of up to 4353 keys, 8 kv heads of 128, 342 MB in f16: 70 us,
-// 4.9 TB/s (a large copy: 5.1); 64 of up to 8193 in e4m3, 598 MB: 133 us, 4.5 TB/s.  The
-// smallest calls by latency: one sequence of 323 keys 8.9 us, of which launching is 4.
+// cache's bytes: 32 sequences of up to 4353 keys, 8 kv heads of 128, 342 MB in f16: 69 us,
+// 4.9 TB/s (a large copy: 5.1); 64 of up to 8193 in e4m3, 598 MB: 127 us, 4.7 TB/s.  The
+// smallest calls by latency: one sequence of 323 keys 8.3 us, of which launching is 4.
 // Longer ones: paged_many_kernel, bound by the two phases of a step, of which the
 // softmax is as long as the products: 771 rows behind 1536 keys, 16 heads of 128:
-// 35 us, 346 TFLOP/s, 519 with the products of the residues; 4334 rows 144 us.
+// 33 us, 367 TFLOP/s, 550 with the products of the residues.
 // Keys of long sequences are split among blocks, which leave (O, max, sum) in the
 // workspace for paged_join_kernel.
 #include <utility>
@@ -315,8 +315,7 @@ template <class F, int... I>
 __device__ __forceinline__ void each(F f, std::integer_sequence<int, I...>) {
   (f(std::integral_constant<int, I>{}), ...);
 }
-// Instructions FROM .. TO - 1 of a wave's LI / OF.
-template <int DT, bool F8, int HD, bool W32, int OF, int LP, bool K, int FROM = 0, int TO = Cfg<DT, F8, HD>::LI / OF>
+template <int DT, bool F8, int HD, bool W32, int OF, int LP, bool K>
 __device__ __forceinline__ void load_tile(const PagedParams& kv, const Pages& pages, int j, int mine, unsigned char* to) {
   using C = Cfg<DT, F8, HD>;
   constexpr int PER = C::LI >> (6 - LP), PB = HD * C::ES << LP;  // instructions and bytes of a page
@@ -344,15 +343,15 @@ __device__ __forceinline__ void load_tile(const PagedParams& kv, const Pages& pa
   };
   auto one = [&](auto number) {
     constexpr int I = decltype(number)::value;
-    if constexpr (I >= FROM && I < TO && PER >= OF) {
-      constexpr int PW = PER / OF, pg = I / PW, N = I % PW * OF;  // N: of the page, the first wave's
+    if constexpr (PER >= OF) {
+      constexpr int PW = PER < OF ? 1 : PER / OF, pg = I / PW, N = I % PW * OF;  // N: of the page, the first wave's
       constexpr int B = N / 4 * 4096;                              // 4 KB: the reach of the instruction's offset
       int bytes;
       const unsigned char* src = page_src(pg, &bytes);
       const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(src), (short)0, bytes, 0x00020000);
       QA_LDS void* dst = (QA_LDS void*)(to + pg * PER * 1024 + B + mine * 1024);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, dst, 16, off(N + mine, pg), B + mine * 1024, N % 4 * 1024, 0);
-    } else if constexpr (I >= FROM && I < TO) {  // fewer instructions to a page than waves: pages side by side
+    } else {  // fewer instructions to a page than waves: pages side by side
       const int pg = I * (OF / PER) + mine / PER, n = mine % PER;
       int bytes;
       const unsigned char* src = page_src(pg, &bytes);
@@ -361,7 +360,7 @@ __device__ __forceinline__ void load_tile(const PagedParams& kv, const Pages& pa
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, dst, 16, off(n, pg), n * 1024, 0, 0);
     }
   };
-  each(one, std::make_integer_sequence<int, 16>{});
+  each(one, std::make_integer_sequence<int, C::LI / OF>{});
 }
 // Fragment addresses in the tiles.  K: product t reads row 16 (c / 4) + 4 t + c % 4,
 // slice e the chunk 4 e + g.  V: row d, the chunks of keys 16 g ..
