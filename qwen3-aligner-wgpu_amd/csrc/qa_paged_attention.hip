@@ -173,12 +173,12 @@ struct Cfg {
 //    CUs in turns, and with an even one the same CUs get all the first, full parts
 //    (512 behind 4352, f16, in 3, 4, 5: 118.6, 148.9, 122).  A part is a multiple of 256
 //    keys, a block of 64 for each wave.
-//  * many: tiles of 64 or 128 pairs.  Of 64 up to 700 tiles: 128-row blocks load each
+//  * many: tiles of 64 or 128 pairs.  Of 64 up to 600 tiles: 128-row blocks load each
 //    tile for twice the rows, but are half as many, each with twice the steps (8 kv
-//    heads, no past, 64 -> 128, us: 1500 rows 29.8 -> 41.9, 2500 67 -> 65, 3500 108 ->
-//    92, 4334 155 -> 144).  Their keys are split while the CUs take the parts at once,
-//    down to 256: 64 rows behind 16000 keys 178 us whole, 28.8 in 32 parts; 200 behind
-//    700 19.1 whole, 16.6 in four; but 771 behind 1536 (200 blocks) 35 whole, 45 in
+//    heads, no past, 64 / 128, us: 1500 rows 28.1 / 37.9, 2500 62.6 / 59.8, 3500 101.7 /
+//    86.2, 4334 147 / 134).  Their keys are split while the CUs take the parts at once,
+//    down to 256: 64 rows behind 16000 keys 166 us whole, 28.8 in 32 parts; 200 behind
+//    700 18.1 whole, 16.3 in four; but 771 behind 1536 (200 blocks) 32 whole, 43 in
 //    two, as half the CUs' parts have to wait.  Up to 640 keys there is no gain (600
 //    and none before, 4 kv heads of 64: 12.4 whole, 13.5 in three).
 constexpr int kFewRows = 16, kFewWaves = 4;
@@ -235,7 +235,7 @@ Split split_of(const PagedAttnParams& p, bool e4m3, int hd) {
       const int64_t n = pairs / r + full > ends ? pairs / r + full : ends;
       return p.kv.nkvh * (n < most(r) ? n : most(r));
     };
-    s.many_rows = about(64) > 700 ? 128 : 64;
+    s.many_rows = about(64) > 600 ? 128 : 64;
     s.tiles = (int)(pairs / s.many_rows + ends < most(s.many_rows) ? pairs / s.many_rows + ends : most(s.many_rows));
     const int64_t blocks = about(s.many_rows);
     divide(len > 640 && blocks > 0 && blocks < kCus ? kCus / blocks : 1, 256, &s.many_chunk, &s.many_chunks);
