@@ -503,7 +503,7 @@ def test_attention_of_rows_behind_many_pages(ctx, pkg, dtype, cache, page, hd):
 
 
 @FORMATS
-@pytest.mark.parametrize("page,hd", [(16, 64), (64, 128)])
+@pytest.mark.parametrize("page,hd", [(16, 64), (32, 64), (64, 64), (16, 128), (32, 128), (64, 128)])
 def test_attention_of_long_tiles(ctx, pkg, dtype, cache, page, hd):
     """6000 rows of 8 kv heads: tiles of 128 rows, with few and many keys, whole and not, beside a single token."""
     b = Batch.shared([100] * 58 + [1, 130, 257], [4500, 100, 2100] + [130] * 55 + [700, 140, 600], page, 8, 8, hd, dtype, cache, seed=105)
@@ -511,6 +511,21 @@ def test_attention_of_long_tiles(ctx, pkg, dtype, cache, page, hd):
     b.upload(ctx)
     q = b.random_rows(8 * hd)
     assert_attention(b, q, attention(ctx, pkg, b, q), seqs=(0, 1, 2, 40, 58, 59, 60), rows=(0, 1, 63, 64, 99, 127, 128, 129, 255, 256))
+    b.free()
+
+
+@FORMATS
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_of_many_split_sequences(ctx, pkg, dtype, cache, hd):
+    """100 sequences of one kv head, single tokens and 20 rows in turn, whose keys are split: the join finds them past
+    the first 64."""
+    rng = np.random.default_rng(109)
+    lens = [2500, 2400] + [int(rng.integers(20, 2500)) for _ in range(98)]
+    b = Batch.shared([1, 20] * 50, lens, 16, 2, 1, hd, dtype, cache, seed=110)
+    b.upload(ctx)
+    q = b.random_rows(2 * hd)
+    assert pkg.attention_paged_workspace(paged.attention_desc(pkg, b, 0, 2 * hd, 0, 2 * hd)) > 0
+    assert_attention(b, q, attention(ctx, pkg, b, q))
     b.free()
 
 
