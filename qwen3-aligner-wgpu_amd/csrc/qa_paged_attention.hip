@@ -11,7 +11,7 @@
 // K and V go to LDS in blocks of 64 keys by DMA (buffer_load ... lds), page by page, a
 // page's resource being its own bytes, so that a hole in the table comes as
 // zeros.  (Straight from the pages into fragments, a load instruction touches 16
-// rows, and the address unit bounds the kernel: 90 us where the tiles take 35.)  Chunks of
+// rows, and the address unit bounds the kernel: 90 us where the tiles take 33.)  Chunks of
 // 16 bytes lie within their row in an order that leaves fragment reads without
 // bank conflicts (0.3 % of LDS cycles; 28 % in plain order).  The rows of a product
 // are given those keys that leave a lane with 16 consecutive keys of its column, in the
@@ -302,12 +302,8 @@ __device__ __forceinline__ int v_swizzle(int c, int lcp) {
   if (F8) return lcp == 2 ? swap3(c >> 2) : 0;
   return lcp == 3 ? (c >> 1) & 5 : c >> 3;
 }
-// A DMA instruction copies 1 KB; those of a tile are dealt out to OF waves, of which
-// this is `mine`.  A page's are a run of PER, and what they add to the page's and the
-// tile's address is the same, so it goes into the instruction.  Pages that are
-// none come as zeros (a resource of no bytes).  Pages: lane 4 j + a holds where the
-// page of keys 16 a .. of block j begins, in bytes from either pool's start, or a
-// negative number.
+// Where pages begin: lane 4 j + a holds, for the page of keys 16 a .. of block j, the
+// bytes from either pool's start, or a negative number.
 struct Pages {
   int lo, hi;
 };
@@ -315,6 +311,9 @@ template <class F, int... I>
 __device__ __forceinline__ void each(F f, std::integer_sequence<int, I...>) {
   (f(std::integral_constant<int, I>{}), ...);
 }
+// Block j's tile by DMA, 1 KB to an instruction; a tile's are dealt out to OF waves, of
+// which this is `mine`.  A page's are a run of PER.  Pages that are none come as
+// zeros (a resource of no bytes).  W32: in the order for the 32-row products below.
 template <int DT, bool F8, int HD, bool W32, int OF, int LP, bool K>
 __device__ __forceinline__ void load_tile(const PagedParams& kv, const Pages& pages, int j, int mine, unsigned char* to) {
   using C = Cfg<DT, F8, HD>;
