@@ -2,19 +2,20 @@
 // RMSNorm and rotation as in qk_norm_rope_kernel, q to its rows, K and V to the
 // slots of their sequences' pages, in the 16-bit format or in e4m3.
 //
-// One grid.  The first blocks take the q heads, a wave to a row, HD / 16 lanes to a
-// head, each lane with the 8-element chunk c and its rotation partners, chunk c +
-// HD / 16; the row's cosines and sines and the norm's weights stay in registers
-// from head to head.
-// Each other block takes one (sequence, page, kv head): the rows of this call
-// that fall into that page, K and V.  A page is one block's because an e4m3 page
-// has one scale: its block finds the largest new value, raises the scale if it
-// must, rounds what the page held again, and stores the rows, with no other
+// One grid.  Its first blocks take one (sequence, page, kv head) each: the rows of
+// this call that fall into that page, K and V.  A page is one block's because an
+// e4m3 page has one scale: its block finds the largest new value, raises the scale
+// if it must, rounds what the page held again, and stores the rows, with no other
 // block to wait for.  The V page is [hd][page], so V goes through an LDS tile.
+// The other blocks take the q heads, a wave to a row, HD / 16 lanes to a head, each
+// lane with the 8-element chunk c and its rotation partners, chunk c + HD / 16; the
+// row's cosines and sines and the norm's weights stay in registers from head to
+// head.  (The pages' blocks are the longer ones, with two barriers and V's turn:
+// behind the rows' instead of before them, 18.4 us for 15.7 at 4334 rows.)
 //
 // Bound by the bytes: 4334 rows of 16 q and 8 kv heads of 128 into empty e4m3 pages, 67
-// MB, 18.1 us (3.7 TB/s; the f64 of K is 1.1 of them); a step's few rows by the
-// launch and a chain of loads, row_start, the table, the row: 32 single rows 3.8 us.
+// MB, 15.7 us (4.2 TB/s); a step's few rows by the launch and a chain of loads,
+// row_start, the table, the row: 32 single rows 3.8 us.
 //
 // e4m3 scales are powers of two, the least 2^e with amax <= 448 * 2^e: dividing by
 // one is exact, so a value is rounded once however often its page's scale
@@ -139,7 +140,7 @@ __device__ __forceinline__ float to_odd(double x) {
 }
 // The same for a k head that goes to e4m3, whose steps are 2^20 times f32's: in f32 a
 // few values of a long prompt end up on the other side of a step's middle than
-// their definition.  In f64 none does (4334 rows 17.0 -> 18.1 us).
+// their definition.  In f64 none does (4334 rows 15.5 -> 15.7 us).
 template <int DT, int HD>
 __device__ __forceinline__ void norm_rope_exact(u32x4 va, u32x4 vb, const Turn& t, float eps, float* xa, float* xb) {
   float fa[8], fb[8];
@@ -360,17 +361,17 @@ __device__ __forceinline__ void kv_part(const AppendParams& p, int64_t b, int sl
 }
 
 template <int DT, bool F8, int HD, int NP>
-__global__ void __launch_bounds__(256) kv_append_kernel(const AppendParams p, int64_t qblocks, int slots) {
-  if ((int64_t)blockIdx.x < qblocks) q_part<DT, HD>(p, blockIdx.x);
-  else kv_part<DT, F8, HD, NP>(p, blockIdx.x - qblocks, slots);
+__global__ void __launch_bounds__(256) kv_append_kernel(const AppendParams p, int64_t pages, int slots) {
+  if ((int64_t)blockIdx.x < pages) kv_part<DT, F8, HD, NP>(p, blockIdx.x, slots);
+  else q_part<DT, HD>(p, blockIdx.x - pages);
 }
 
 template <int DT, bool F8, int HD>
 hipError_t launch_one(const AppendParams& p, hipStream_t s) {
-  const int64_t qb = (p.kv.tokens + 3) / 4, slots = pages_touched(p.kv.max_rows, p.kv.lp);
-  const dim3 grid((unsigned)(qb + slots * p.kv.seqs * p.kv.nkvh));
-  if (HD == 128 && p.kv.lp == 6) hipLaunchKernelGGL((kv_append_kernel<DT, F8, HD, HD / 64>), grid, dim3(256), 0, s, p, qb, (int)slots);
-  else hipLaunchKernelGGL((kv_append_kernel<DT, F8, HD, 1>), grid, dim3(256), 0, s, p, qb, (int)slots);
+  const int64_t slots = pages_touched(p.kv.max_rows, p.kv.lp), pages = slots * p.kv.seqs * p.kv.nkvh;
+  const dim3 grid((unsigned)(pages + (p.kv.tokens + 3) / 4));
+  if (HD == 128 && p.kv.lp == 6) hipLaunchKernelGGL((kv_append_kernel<DT, F8, HD, HD / 64>), grid, dim3(256), 0, s, p, pages, (int)slots);
+  else hipLaunchKernelGGL((kv_append_kernel<DT, F8, HD, 1>), grid, dim3(256), 0, s, p, pages, (int)slots);
   return hipGetLastError();
 }
 
