@@ -8,9 +8,9 @@
 // equal, made on the device because positions of images and video are not a
 // running number: once for a step, for every layer's q / k rotation.
 //
-// Bound by the rows it writes: 30720 tokens of hd 128, 31 MB, 9.6 us, of which the
-// launch is 4 and the f64 of angles and series 1.5; 32 tokens 4.4 us.  (With the
-// library's sincos, whose reduction takes any angle, 10.7.)
+// Bound by the rows it writes: 30720 tokens of hd 128, 31 MB, 8.5 us, of which the
+// f64 of angles and series is 1; 32 tokens 4.4 us, the launch.  (With the library's
+// sincos, whose reduction takes any angle, 1 more.)
 //
 // The angle is formed in f64 (a position of 2^20 leaves an f32 angle no more
 // than 4 bits of a turn's fraction), as are its cosine and sine: |angle| < 2^31
@@ -75,12 +75,14 @@ __global__ void __launch_bounds__(256) mrope_rows_kernel(const MropeParams p) {
     c[e] = round16<DT>(cd);
     s[e] = round16<DT>(sd);
   }
+  // past the caches, which a long batch's rows would only go through (9.6 us before); an
+  // append behind this call takes as long either way, for few rows too
   float* co = p.cos + t * p.hd + j0;
   float* so = p.sin + t * p.hd + j0;
-  *reinterpret_cast<f32x4*>(co) = c;
-  *reinterpret_cast<f32x4*>(co + half) = c;
-  *reinterpret_cast<f32x4*>(so) = s;
-  *reinterpret_cast<f32x4*>(so + half) = s;
+  __builtin_nontemporal_store(c, reinterpret_cast<f32x4*>(co));
+  __builtin_nontemporal_store(c, reinterpret_cast<f32x4*>(co + half));
+  __builtin_nontemporal_store(s, reinterpret_cast<f32x4*>(so));
+  __builtin_nontemporal_store(s, reinterpret_cast<f32x4*>(so + half));
 }
 
 }  // namespace
