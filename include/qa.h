@@ -407,7 +407,10 @@ int qa_kv_append(qa_ctx* ctx, const qa_kv_append_desc* desc);
  *        that is 0); its contents need not be kept or cleared, and calls that may
  *        run at the same time (two graphs, two contexts) need one each
  * Strides multiples of 8; q and out 16-byte aligned.  The probabilities enter
- * the P.V product as two 16-bit terms, as in qa_attention_prefill's default. */
+ * the P.V product as sums of 16-bit terms: two of f16 over f16 pages (22 bits of a
+ * probability), two of bf16 over bf16 pages (16 bits; both as in
+ * qa_attention_prefill's default), three of bf16 over QA_E4M3 pages (24 bits), and over
+ * bf16 pages too for sequences whose rows times nqh / nkvh are at most 16. */
 typedef struct qa_paged_attention_desc {
   uint32_t dtype;
   uint32_t flags; /* reserved, must be 0 */

@@ -19,12 +19,17 @@
 // other in registers.
 //
 // Online softmax in the log2 domain; the maximum moves only when it grows by more
-// than 2^8, so nearly every step leaves O as it is.  Probabilities go into the
-// product as two 16-bit terms (value and rounding residue), which keeps P.V at
-// f32's accuracy for a second product of P's; in f16 they are scaled by 2^7, so that
-// small ones stay normal.  Over an e4m3 cache K is widened to the call's format
-// (exactly), its scale goes into the score's factor, and V's into p in f32; P and V
-// are multiplied as bf16 there, whose range takes any scale.
+// than 2^8, so nearly every step leaves O as it is.  Over an e4m3 cache K is widened
+// to the call's format (exactly), its scale goes into the score's factor, and V's into
+// p in f32; P and V are multiplied as bf16 there, whose range takes any scale.
+// Probabilities go into the product as a sum of 16-bit terms, a value and the rounding
+// of what it leaves: two of f16 (scaled by 2^7, so that small ones stay normal),
+// which hold 22 bits of p, or three of bf16, which hold all 24.  (Two of bf16 hold 16:
+// 2.3e-6 of the result, which moved 0.24 % of bf16 outputs to the neighbouring value
+// where three move 0.06 %, as many as a sum in another order; 64 sequences over e4m3
+// 127.4 us with two, 127.9 with three.)  Two of bf16 are left in the longer tiles over
+// bf16 pages, as in qa_attention_prefill's default, where a third product costs most: 771
+// rows behind 1536 keys 33.5 us with two, 38.7 with three (e4m3 pages 37.5 and 42.3).
 //
 // Sequences of up to 16 pairs (single tokens): paged_few_kernel.  Bound by the
 // cache's bytes: 32 sequences of up to 4353 keys, 8 kv heads of 128, 342 MB in f16: 69 us,
@@ -68,8 +73,8 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   else
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
 }
-// (a, b) minus their 16-bit roundings h = pack2(a, b), as two 16-bit values.  The
-// differences are exact in f32.  f16: as products with a 1 that the compiler does
+// (a, b) minus the 16-bit values h = pack2(a, b), exact in f32, rounded
+// to two 16-bit values again.  f16: as products with a 1 that the compiler does
 // not see, which become one v_fma_mix each, h's half read and the result's
 // written as they lie.
 template <int DT>
@@ -82,6 +87,12 @@ __device__ __forceinline__ uint32_t residue2(uint32_t h, float a, float b) {
   } else {
     return pack2<DT>(a - __uint_as_float(h << 16), b - __uint_as_float(h & 0xffff0000u));
   }
+}
+// What a second term leaves, of bf16.
+__device__ __forceinline__ uint32_t residue2(uint32_t h, uint32_t l, float a, float b) {
+  a -= __uint_as_float(h << 16);
+  b -= __uint_as_float(h & 0xffff0000u);
+  return residue2<QA_BF16>(l, a, b);
 }
 // Eight e4m3 values (two words) as a 16-bit fragment; exact in both formats.
 template <int DT>
@@ -144,6 +155,8 @@ __device__ __forceinline__ float column_sum(float v) {
 template <int DT, bool F8, int HD>
 struct Cfg {
   static constexpr int PV = F8 ? (int)QA_BF16 : DT;              // format of the P.V product
+  static constexpr int NT = PV == QA_F16 ? 2 : 3;                // 16-bit terms of a probability
+  static constexpr int NL = F8 ? 3 : 2;                          // in the longer tiles
   static constexpr float kBias = PV == QA_F16 ? 7.f : 0.f;       // f16 p scaled by 2^7: normal down to 2^-21
   static constexpr int ES = F8 ? 1 : 2;                          // bytes of a cache element
   static constexpr int CR = HD * ES / 16;                        // 16-byte chunks of a K row
@@ -374,12 +387,12 @@ __device__ __forceinline__ int v_frag(int c, int g, int e, int lcp) {
   return ((((x >> lcp) * HD + c) << lcp) + ((x & ((1 << lcp) - 1)) ^ v_swizzle<F8>(c, lcp))) * 16;
 }
 
-// Mask, online softmax and the two 16-bit terms of P.  `have`: how many of the
+// Mask, online softmax and the 16-bit terms of P.  `have`: how many of the
 // lane's 16 keys from kg on the sequence has (on a page); `f`: the scores'
 // factor, log2 e / sqrt(hd) and the K scale; `vs`: the V scale.
 template <int DT, bool F8, int HD>
 __device__ __forceinline__ void softmax(f32x4 (&sc)[4], int pos, int kg, int have, float f, float vs, float& m, float& l, f32x4 (&o)[HD / 16],
-                                        u32x4 (&ph)[2], u32x4 (&pl)[2]) {
+                                        u32x4 (&ph)[2], u32x4 (&pl)[2], u32x4 (&pm)[2]) {
   using C = Cfg<DT, F8, HD>;
   const int see = min(have, pos + 1 - kg);
   if (__builtin_amdgcn_ballot_w64(see < 16)) {
@@ -415,9 +428,10 @@ __device__ __forceinline__ void softmax(f32x4 (&sc)[4], int pos, int kg, int hav
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const uint32_t hi = pack2<C::PV>(w[2 * e], w[2 * e + 1]);
+      const uint32_t hi = pack2<C::PV>(w[2 * e], w[2 * e + 1]), lo = residue2<C::PV>(hi, w[2 * e], w[2 * e + 1]);
       ph[t >> 1][2 * (t & 1) + e] = hi;
-      pl[t >> 1][2 * (t & 1) + e] = residue2<C::PV>(hi, w[2 * e], w[2 * e + 1]);
+      pl[t >> 1][2 * (t & 1) + e] = lo;
+      if constexpr (C::NT == 3) pm[t >> 1][2 * (t & 1) + e] = residue2(hi, lo, w[2 * e], w[2 * e + 1]);
     }
   }
   l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
@@ -478,7 +492,7 @@ __device__ __forceinline__ void multiply_k(const unsigned char* kt, int ka, cons
 }
 template <int DT, bool F8, int HD>
 __device__ __forceinline__ void multiply_v(const unsigned char* vt, const int (&va)[Cfg<DT, F8, HD>::VS], int lcp, const u32x4 (&ph)[2],
-                                           const u32x4 (&pl)[2], f32x4 (&o)[HD / 16]) {
+                                           const u32x4 (&pl)[2], const u32x4 (&pm)[2], f32x4 (&o)[HD / 16]) {
   using C = Cfg<DT, F8, HD>;
   constexpr int B = kAhead + 1;
   int at[C::VS];
@@ -504,6 +518,7 @@ __device__ __forceinline__ void multiply_v(const unsigned char* vt, const int (&
       else a = x[d % B][j];
       o[d] = mfma<C::PV>(a, ph[j], o[d]);
       o[d] = mfma<C::PV>(a, pl[j], o[d]);
+      if constexpr (C::NT == 3) o[d] = mfma<C::PV>(a, pm[j], o[d]);
     }
   }
 }
@@ -659,18 +674,18 @@ __device__ __forceinline__ void few_block(const PagedAttnParams& p, const Split&
     }
     wait_vmcnt<C::LI>();  // K is there; V's loads came after it
     f32x4 sc[4];
-    u32x4 ph[2], pl[2];
+    u32x4 ph[2], pl[2], pm[2];
     multiply_k<DT, F8, HD>(kt, ka, q, sc);
     wait_lds();
     if (more) {
       if ((it & 15) == 15) fetch(it + 1, page_ids(kv, s, [&](int j) { return key_of(it + 1 + j); }));
       load_tile<DT, F8, HD, false, 1, LP, true>(kv, pages, (it + 1) & 15, 0, kt);
     }
-    softmax<DT, F8, HD>(sc, col.pos, kg, have, p.scale * kLog2e * ks, vs, m, l, o, ph, pl);
+    softmax<DT, F8, HD>(sc, col.pos, kg, have, p.scale * kLog2e * ks, vs, m, l, o, ph, pl, pm);
     if (more) wait_vmcnt<C::LI>();  // V is there; the next K's loads came after it
     else wait_vmcnt<0>();
     if (__builtin_amdgcn_ballot_w64(have < 16)) clear_tail<DT, F8, HD>(vt, va, lcp, have);
-    multiply_v<DT, F8, HD>(vt, va, lcp, ph, pl, o);
+    multiply_v<DT, F8, HD>(vt, va, lcp, ph, pl, pm, o);
     wait_lds();
     if (more) load_tile<DT, F8, HD, false, 1, LP, false>(kv, pages, (it + 1) & 15, 0, vt);
   }
@@ -720,7 +735,7 @@ __device__ __forceinline__ float pair_sum(float v) {
 // formed outside the loop and held there.)
 template <int DT, bool F8, int HD, bool PVT, bool SQT>
 __device__ __forceinline__ void multiply32(const unsigned char* vt, const int (&va)[F8 ? 2 : 4], int lcp, const u32x4 (&ph)[2][2],
-                                           const u32x4 (&pl)[2][2], f32x16 (&o)[HD / 32], const unsigned char* kt, int ka,
+                                           const u32x4 (&pl)[2][2], const u32x4 (&pm)[2][2], f32x16 (&o)[HD / 32], const unsigned char* kt, int ka,
                                            const u32x4 (&q)[HD / 16], f32x16 (&sc)[2]) {
   using C = Cfg<DT, F8, HD>;
   constexpr int N = HD / 16, DP = HD / 64;  // slices, pairs of d tiles
@@ -777,6 +792,10 @@ __device__ __forceinline__ void multiply32(const unsigned char* vt, const int (&
     if constexpr (PVT) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) o[d + u] = mfma32<C::PV>(v[u], pl[half][j], o[d + u]);
+      if constexpr (C::NL == 3) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) o[d + u] = mfma32<C::PV>(v[u], pm[half][j], o[d + u]);
+      }
     }
     constexpr int R = (PVT ? 2 : 0) + (SQT ? 2 : 0);
     if (reads) __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
@@ -788,8 +807,8 @@ __device__ __forceinline__ void multiply32(const unsigned char* vt, const int (&
 // runs of 16, a page each).
 template <int DT, bool F8, int HD>
 __device__ __forceinline__ void softmax32(f32x16 (&sc)[2], int pos, int kg, const int (&have)[2], const float (&f)[2],
-                                          const float (&vs)[2], float& m, float& l, f32x16 (&o)[HD / 32], u32x4 (&ph)[2][2],
-                                          u32x4 (&pl)[2][2]) {
+                                          const float (&vs)[2], float& m, float& l, f32x16 (&o)[HD / 32],
+                                          u32x4 (&ph)[2][2], u32x4 (&pl)[2][2], u32x4 (&pm)[2][2]) {
   using C = Cfg<DT, F8, HD>;
   float top[2];
 #pragma unroll
@@ -829,9 +848,10 @@ __device__ __forceinline__ void softmax32(f32x16 (&sc)[2], int pos, int kg, cons
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const uint32_t hi = pack2<C::PV>(w[2 * e], w[2 * e + 1]);
+        const uint32_t hi = pack2<C::PV>(w[2 * e], w[2 * e + 1]), lo = residue2<C::PV>(hi, w[2 * e], w[2 * e + 1]);
         ph[u][t >> 1][2 * (t & 1) + e] = hi;
-        pl[u][t >> 1][2 * (t & 1) + e] = residue2<C::PV>(hi, w[2 * e], w[2 * e + 1]);
+        pl[u][t >> 1][2 * (t & 1) + e] = lo;
+        if constexpr (C::NL == 3) pm[u][t >> 1][2 * (t & 1) + e] = residue2(hi, lo, w[2 * e], w[2 * e + 1]);
       }
     }
   l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
@@ -991,7 +1011,7 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
   f32x16 o[HD / 32] = {};
   float m = -INFINITY, l = 0.f;
   f32x16 sc[2];
-  u32x4 ph[2][2], pl[2][2];
+  u32x4 ph[2][2], pl[2][2], pm[2][2];
   // fragment addresses: K row of the lane's key in a 32-key product, slice e at ^ (e << 5);
   // V row c, the chunks of the lane's keys
   const int key = 16 * (c >> 2 & 1) + 4 * (c >> 3) + (c & 3);
@@ -1023,9 +1043,9 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
               *x &= u32x4{tail_mask<C::ES>(left, 0), tail_mask<C::ES>(left, 1), tail_mask<C::ES>(left, 2), tail_mask<C::ES>(left, 3)};
             }
         }
-        if (it > 0 && it < steps) multiply32<DT, F8, HD, true, true>(vt(it - 1), va, lcp, ph, pl, o, kt(it), ka, q, sc);
-        else if (it > 0) multiply32<DT, F8, HD, true, false>(vt(it - 1), va, lcp, ph, pl, o, kt(it), ka, q, sc);
-        else if (steps > 0) multiply32<DT, F8, HD, false, true>(vt(it), va, lcp, ph, pl, o, kt(it), ka, q, sc);
+        if (it > 0 && it < steps) multiply32<DT, F8, HD, true, true>(vt(it - 1), va, lcp, ph, pl, pm, o, kt(it), ka, q, sc);
+        else if (it > 0) multiply32<DT, F8, HD, true, false>(vt(it - 1), va, lcp, ph, pl, pm, o, kt(it), ka, q, sc);
+        else if (steps > 0) multiply32<DT, F8, HD, false, true>(vt(it), va, lcp, ph, pl, pm, o, kt(it), ka, q, sc);
       } else {
         const int kg = key_of(it) + 16 * h, j = scalar(it & 15);
         float f[2], vs[2] = {0.f, 0.f};
@@ -1042,7 +1062,7 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
         if (it > 0 && (it & 15) == 0 && 16 * (it >> 4) + 16 < steps) fetch((it >> 4) + 1);
         if (it + NB < steps) issue_k(it + NB);
         if (it + NB - 1 < steps) issue_v(it + NB - 1);
-        softmax32<DT, F8, HD>(sc, pos, kg, have, f, vs, m, l, o, ph, pl);
+        softmax32<DT, F8, HD>(sc, pos, kg, have, f, vs, m, l, o, ph, pl, pm);
       }
     }
     const int next = ph_no + 1 - off;

@@ -1,0 +1,77 @@
+"""qa_kv_append and qa_attention_paged on an MI355X where the batch's bounds, the
+pages' contents or the formats' last bits decide (definitions: tests/paged.py)."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from conftest import ulp16
+from paged import BF16, E4M3, F16, Batch, attention, e4m3_codes, narrow, widen
+
+pytestmark = pytest.mark.gpu
+
+FORMATS = pytest.mark.parametrize("dtype,cache", [(F16, F16), (BF16, BF16), (F16, E4M3), (BF16, E4M3)],
+                                  ids=["f16", "bf16", "f16-e4m3", "bf16-e4m3"])
+
+
+def _put(b, s, K, V, scale=2.0 ** -6):
+    """Sequence s's keys: K, V [nkv, len, hd], exact in the cache's format (e4m3: at this scale)."""
+    for i in range(-(-b.len[s] // b.page)):
+        p, at = b.table[s, i], slice(i * b.page, (i + 1) * b.page)
+        k, v = K[:, at], V[:, at].transpose(0, 2, 1)
+        m = k.shape[1]
+        if b.cache == E4M3:
+            b.k_scale[p], b.v_scale[p] = scale, scale
+            k, v = e4m3_codes(k / scale), e4m3_codes(v / scale)
+        else:
+            k, v = narrow(k, b.dtype), narrow(v, b.dtype)
+        b.k[p, :, :m], b.v[p, :, :, :m] = k, v
+
+
+@FORMATS
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n,lens", [([1] * 24, list(range(3, 27))), ([1], [1500]), ([40], [300]), ([70, 1], [1500, 20])])
+def test_probabilities_keep_their_last_bits(ctx, pkg, dtype, cache, hd, n, lens):
+    """Two keys of nearly the same score with V = 1 and -1, the others' V 0: out = (p1 - p2) / sum p is 2^-13 of p1, and shows
+    what was lost of either.  Scores are exact in f32 (one or two products of few bits).  What may be lost, over p1 / sum p:
+      * p1, p2: the exponent's factor and rounding, 2^-25 (|arg| < 0.2; in f16, whose p carry a factor of 2^7, the
+        exponent's last bit is 2^-22, times ln 2), exp2's 2^-23: 2.5 2^-23 for both (f16: 3 2^-23 more);
+      * the terms in the product: f16 2^-22 each; three of bf16 nothing; two (bf16 pages, more than 16 rows and heads) 2^-18 each;
+      * the sum of up to six products: 6 2^-24;
+    then (keys + 16) 2^-24 of the result, the sum of p, and half a step of the output."""
+    nq, nkv = 4, 2
+    b = Batch(n, lens, 16, nq, nkv, hd, dtype, cache, seed=hd + sum(lens))
+    b.stale()
+    for s, m in enumerate(lens):
+        K, V = np.zeros((nkv, m, hd)), np.zeros((nkv, m, hd))
+        K[:, :, 0] = b.rng.integers(-8, 4, (nkv, m)) / 8.0
+        K[:, 0, 0] = 1.0
+        if m > 2:
+            K[:, 1, 0] = K[:, 2, 0] = b.rng.integers(4, 8, nkv) / 8.0
+            K[:, 1, 1], V[:, 1], V[:, 2] = 1.0, 1.0, -1.0
+        _put(b, s, K, V)
+    b.upload(ctx)
+    x = np.zeros((b.tokens, nq, hd))
+    x[..., 0] = b.rng.integers(64, 128, x.shape[:2]) / 128.0 * np.sqrt(hd / 64)  # 6 or 7 bits (sqrt 2 at hd 128: rounded to the format)
+    x[..., 1] = 2.0 ** -10 * (1 + b.rng.integers(0, 128, x.shape[:2]) / 128.0)
+    q = narrow(x.reshape(b.tokens, -1), dtype)
+    got = widen(attention(ctx, pkg, b, q), dtype).reshape(b.tokens, nq, hd)
+    x = widen(q, dtype).reshape(b.tokens, nq, hd)
+    per_p = 2.5 * 2.0 ** -23 + 6 * 2.0 ** -24
+    two = cache == BF16
+    for s, m in enumerate(lens):
+        K, _, _ = b.keys(s)
+        for r in range(n[s]):
+            t, see = b.row_start[s] + r, m - n[s] + r + 1
+            if see < 3:
+                continue
+            lost = per_p + (5 * 2.0 ** -23 if cache == F16 else 2 * 2.0 ** -18 if two and n[s] * nq // nkv > 16 else 0.0)
+            for h in range(nq):
+                sc = K[h * nkv // nq, :see] @ x[t, h] / np.sqrt(hd)
+                p = np.exp(sc - sc.max())
+                want = (p[1] - p[2]) / p.sum()
+                bound = lost * p[1] / p.sum() + abs(want) * (see + 16) * 2.0 ** -24
+                bound += float(ulp16(np.array(abs(want) + bound), dtype)) / 2
+                err = np.abs(got[t, h] - want).max()
+                assert err <= bound, (s, r, h, err / bound)
+    b.free()
