@@ -395,10 +395,11 @@ int qa_kv_append(qa_ctx* ctx, const qa_kv_append_desc* desc);
  * qa_kv_append): the row at position p attends to its sequence's keys 0 .. p, q
  * head h to kv head h / (nqh / nkvh), softmax of q.k / sqrt(hd) in f32,
  * out[t][h hd + j] = round(sum_t p_t v_t[j]).  Keys on an entry that is no page do
- * not count; a row without keys gives zeros.  What the pages hold behind a
- * sequence's last key is not looked at.  Scales may be any positive numbers.  V has
- * to be finite, and below 2^100, for all of a sequence's keys: a row multiplies
- * those behind its position by 0, which leaves NaN of an infinity or NaN (K may
+ * not count; a row without keys gives zeros.  What the pages and their scales hold
+ * behind the last key that a row of the sequence sees (slots of rows that were left
+ * out among it) is not looked at.  Scales may be any positive numbers.  V has
+ * to be finite, and below 2^100, up to that key: a row multiplies
+ * what is behind its own position by 0, which leaves NaN of an infinity or NaN (K may
  * hold either there), and probabilities are up to 2^8 before they are divided.
  *   q    [tokens][nqh hd], row stride ldq, as qa_kv_append writes it
  *   out  [tokens][nqh hd], row stride ldo, the o projection's input

@@ -29,10 +29,12 @@ struct PagedParams {
 // A sequence's part of the batch: rows row0 .. row0 + n - 1, the first of them at
 // position pos0 (negative where the sequence has fewer keys than rows), len
 // keys in all.  Rows that are left out, past max_rows or the batch's end, keep
-// their positions: the others' do not move.
+// their positions: the others' do not move.  seen() keys are seen by any row; those
+// behind, of rows that are left out, may be slots that nothing was written to.
 struct SeqSpan {
   int64_t row0;
   int n, pos0, len;
+  QA_HD int seen() const { return pos0 + n; }
 };
 
 QA_HD int64_t clamp64(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }

@@ -388,7 +388,7 @@ __device__ __forceinline__ int v_frag(int c, int g, int e, int lcp) {
 }
 
 // Mask, online softmax and the 16-bit terms of P.  `have`: how many of the
-// lane's 16 keys from kg on the sequence has (on a page); `f`: the scores'
+// lane's 16 keys from kg on some row of the sequence sees (on a page); `f`: the scores'
 // factor, log2 e / sqrt(hd) and the K scale; `vs`: the V scale.
 template <int DT, bool F8, int HD>
 __device__ __forceinline__ void softmax(f32x4 (&sc)[4], int pos, int kg, int have, float f, float vs, float& m, float& l, f32x4 (&o)[HD / 16],
@@ -443,7 +443,7 @@ __device__ __forceinline__ uint32_t tail_mask(int left, int w) {
   const int n = left - w * (4 / ES);
   return n >= 4 / ES ? ~0u : n <= 0 ? 0u : (1u << (8 * ES * n)) - 1;
 }
-// What a V tile holds behind the sequence's keys, or for no page, may be anything, NaN
+// What a V tile holds behind the keys that rows see, or for no page, may be anything, NaN
 // too, and 0 * NaN is not 0: a lane clears those elements of the chunks that it
 // will read itself.
 template <int DT, bool F8, int HD>
@@ -585,7 +585,7 @@ template <bool F8, int HD, class Key>
 __device__ __forceinline__ void fetch_pages(const PagedParams& kv, const SeqSpan& sq, int found, int h, int left, Key key, Pages* pages,
                                             float* ks, float* vs, bool* holes) {
   const int lane = threadIdx.x & 63, pos = key(lane >> 2) + 16 * (lane & 3);
-  const bool in = (lane >> 2) < left && pos < sq.len;
+  const bool in = (lane >> 2) < left && pos < sq.seen();
   const int id = in ? found : -1;
   *holes |= __builtin_amdgcn_ballot_w64(in && id < 0) != 0;
   const int64_t at = id < 0 ? -1 : page_base(kv, id, h, HD) * (F8 ? 1 : 2);
@@ -633,7 +633,7 @@ __device__ __forceinline__ void few_block(const PagedAttnParams& p, const Split&
   const int found = page_ids(kv, s, key_of);
   const SeqSpan sq = seq_span(kv, s);
   if (sq.n == 0 || sq.n * p.rep > kFewRows) return;
-  const int end = sq.pos0 + sq.n;  // keys that the last row sees
+  const int end = sq.seen();
   const int k1 = min(k0 + sp.few_chunk, end);
   if (part > 0 && k0 >= end) return;
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
@@ -665,7 +665,7 @@ __device__ __forceinline__ void few_block(const PagedAttnParams& p, const Split&
   for (int it = 0; it < steps; ++it) {
     const bool more = it + 1 < steps;
     const int kg = key_of(it) + 16 * g;
-    int have = sq.len - kg;
+    int have = sq.seen() - kg;
     if (holes && of_keys(pages.hi, it & 15, g) < 0) have = 0;
     float ks = 1.f, vs = 0.f;
     if constexpr (F8) {
@@ -903,7 +903,6 @@ __device__ __forceinline__ bool find_tile(const PagedAttnParams& p, const Split&
       sq->row0 = __builtin_amdgcn_readlane((int)q.row0, at);
       sq->n = __builtin_amdgcn_readlane(q.n, at);
       sq->pos0 = __builtin_amdgcn_readlane(q.pos0, at);
-      sq->len = __builtin_amdgcn_readlane(q.len, at);
       return true;
     }
     u -= __builtin_amdgcn_readlane(upto, 63);
@@ -1032,7 +1031,7 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
     if (my >= 0 && my <= 2 * steps) {
       if ((my & 1) == 0) {
         if (it > 0 && __builtin_amdgcn_ballot_w64(min(have[0], have[1]) < 16)) {
-          // V behind the sequence's keys, or for no page, may be anything, NaN too: a
+          // V behind the keys that rows see, or for no page, may be anything, NaN too: a
           // lane clears those elements of the chunks that it will read itself
 #pragma unroll
           for (int e = 0; e < VX; ++e)
@@ -1051,7 +1050,7 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
         float f[2], vs[2] = {0.f, 0.f};
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          have[u] = sq.len - kg - 32 * u;
+          have[u] = sq.seen() - kg - 32 * u;
           if (holes && of_half(pages_of(it).hi, 4 * j + 2 * u, h) < 0) have[u] = 0;
           f[u] = p.scale * kLog2e;
           if constexpr (F8) {

@@ -5,8 +5,8 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from conftest import ulp16
-from paged import BF16, E4M3, F16, Batch, attention, e4m3_codes, narrow, widen
+from conftest import rope_tables, ulp16
+from paged import BF16, E4M3, F16, STALE8, STALE16, Batch, append, assert_attention, attention, e4m3_codes, narrow, widen
 
 pytestmark = pytest.mark.gpu
 
@@ -74,4 +74,51 @@ def test_probabilities_keep_their_last_bits(ctx, pkg, dtype, cache, hd, n, lens)
                 bound += float(ulp16(np.array(abs(want) + bound), dtype)) / 2
                 err = np.abs(got[t, h] - want).max()
                 assert err <= bound, (s, r, h, err / bound)
+    b.free()
+
+
+def _rows(b):
+    """qkv, norm weights, cosines and sines for b's rows."""
+    qkv = b.random_rows((b.nq + 2 * b.nkv) * b.hd)
+    w = [(1.0 + 0.2 * b.rng.standard_normal(b.hd)).astype(np.float32) for _ in range(2)]
+    return (qkv, *w, *rope_tables(b.tokens, b.hd, 0, dtype=b.dtype))
+
+
+def _nothing_as_zero(b, cache):
+    """The cache with zeros where nothing was ever written (0 * NaN would reach the definition's sums)."""
+    def nothing(a):  # (an e4m3 page that is rounded again keeps its NaN, but not their signs)
+        return a & 0x7F == STALE8 if b.cache == E4M3 else a == STALE16[b.dtype]
+
+    return {n: np.where(nothing(a), 0, a).astype(a.dtype) if n in ("k", "v") else np.nan_to_num(a, nan=1.0) for n, a in cache.items()}
+
+
+@FORMATS
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("n,lens,max_rows,cut", [([40], [45], 30, 0), ([5, 3, 1], [20, 70, 64], 2, 0), ([1, 40], [20, 45], 40, 5),
+                                                 ([90, 1], [1500, 3], 20, 0), ([200], [200], 64, 0), ([1, 6], [7, 260], 3, 0)])
+def test_slots_of_rows_left_out_are_not_looked_at(ctx, pkg, dtype, cache, page, n, lens, max_rows, cut):
+    """Rows past max_rows or past `tokens`: what their slots and pages' scales hold (NaN: nothing was written yet) reaches no
+    row that is kept, and they are left as they are."""
+    b = Batch(n, lens, page, 4, 2, 64, dtype, cache, seed=sum(lens) + page, tail_rows=0 if cut else 2)
+    b.fill([m - k for k, m in zip(n, lens)])
+    b.upload(ctx)
+    x, q, before = _rows(b), b.random_rows(4 * 64), b.read(ctx)
+    b.tokens -= cut
+    qkv, qn, kn, c, s = x
+    append(ctx, pkg, b, qkv[: b.tokens], qn, kn, c[: b.tokens], s[: b.tokens], max_rows=max_rows)
+    after = b.read(ctx)
+    got = attention(ctx, pkg, b, q[: b.tokens], max_rows=max_rows)
+    held = _nothing_as_zero(b, after)
+    kept = [min(k, max_rows) for k in n]
+    kept[-1] = min(kept[-1], n[-1] - cut)
+    for sq in range(b.seqs):
+        r0 = b.row_start[sq]
+        assert (got[r0 + kept[sq]: r0 + n[sq]] == 0x3C01).all()
+        for pos in range(lens[sq] - n[sq] + kept[sq], lens[sq]):
+            p, at = b.table[sq, pos // page], pos % page
+            for a, z in ((after["k"][p, :, at], before["k"][p, :, at]), (after["v"][p, :, :, at], before["v"][p, :, :, at])):
+                assert np.array_equal(a & 0x7F, z & 0x7F) if cache == E4M3 else np.array_equal(a, z)  # NaN, whose sign may change
+    out = np.concatenate([got, np.full((cut, got.shape[1]), 0x3C01, np.uint16)])  # the definition's batch is the whole one
+    for sq in range(b.seqs):
+        assert_attention(b, q, out, rows=range(kept[sq]), seqs=[sq], **held)
     b.free()
