@@ -340,8 +340,8 @@ int qa_mrope_rows(qa_ctx* ctx, const qa_mrope_desc* desc);
  * table, row_start and kv_len are device memory, read by the kernels, and whatever
  * they hold no call reads or writes outside its buffers: rows past the batch or
  * past max_rows, positions below zero and entries that are no page are left out,
- * and a kv_len past max_len counts as max_len.  Rows that no sequence has are
- * left as they are.  Two new rows must not share a slot; a page may be in several
+ * and a kv_len past max_len counts as max_len.  Rows of q_out and out that no
+ * sequence has, or past max_rows, are left as they are.  Two new rows must not share a slot; a page may be in several
  * tables while it is only read. */
 typedef struct qa_paged_kv {
   uint32_t dtype; /* the call's 16-bit format, or QA_E4M3 */

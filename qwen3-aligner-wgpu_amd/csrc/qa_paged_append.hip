@@ -170,14 +170,32 @@ __device__ __forceinline__ u32x4 pack8(const float* x) {
   return u32x4{narrow2<DT>(x[0], x[1]), narrow2<DT>(x[2], x[3]), narrow2<DT>(x[4], x[5]), narrow2<DT>(x[6], x[7])};
 }
 
+// Row t's place in its sequence, for the whole wave: row_start rises, and each step looks
+// at 64 of what is left of it, so that 64 sequences take one load, which does not wait
+// for the others of q_part.  row_start[0] <= t < row_start[seqs].
+__device__ __forceinline__ int64_t row_in_sequence(const PagedParams& kv, int64_t t) {
+  const int lane = threadIdx.x & 63;
+  for (int lo = 0, n = kv.seqs;;) {  // the last start <= t is one of lo .. lo + n - 1
+    const int step = (n - 1) / 64 + 1;
+    const int start = lane * (int64_t)step < n ? kv.row_start[lo + lane * step] : 0x7fffffff;
+    const uint64_t upto = __builtin_amdgcn_ballot_w64(start <= t);
+    const int at = upto ? 63 - __builtin_clzll(upto) : 0;
+    if (step == 1) return t - max(__builtin_amdgcn_readlane(start, at), 0);
+    lo += at * step;
+    n = min(step, n - at * step);
+  }
+}
+
 template <int DT, int HD>
 __device__ __forceinline__ void q_part(const AppendParams& p, int64_t bx) {
   constexpr int L = HD / 16, hpw = 64 / L;  // lanes to a head, heads at once
   const int lane = threadIdx.x & 63, c = lane % L, sub = lane / L;
   const int64_t t = bx * 4 + (threadIdx.x >> 6);
-  // rows of no sequence keep what they hold
+  // rows of no sequence keep what they hold, and those past max_rows, which only a batch
+  // of more rows can have
   const int64_t t0 = p.kv.row_start[0], t1 = p.kv.row_start[p.kv.seqs];
-  if (t >= p.kv.tokens || t < t0 || t >= t1) return;
+  const bool past = p.kv.max_rows < p.kv.tokens && t < p.kv.tokens && row_in_sequence(p.kv, t) >= p.kv.max_rows;
+  if (t >= p.kv.tokens || t < t0 || t >= t1 || past) return;
   const Turn turn = load_turn<HD>(p.qn, p.cos + t * HD, p.sin + t * HD, c);
   const uint16_t* src = p.qkv + t * p.ldqkv + 8 * c;
   uint16_t* dst = p.q_out + t * p.ldq + 8 * c;

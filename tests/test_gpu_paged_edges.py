@@ -122,3 +122,57 @@ def test_slots_of_rows_left_out_are_not_looked_at(ctx, pkg, dtype, cache, page, 
     for sq in range(b.seqs):
         assert_attention(b, q, out, rows=range(kept[sq]), seqs=[sq], **held)
     b.free()
+
+
+@FORMATS
+@pytest.mark.parametrize("n,lens,page,max_rows", [([40, 1, 5], [70, 9, 64], 16, 4), ([90], [200], 32, 33), ([3, 0, 2, 2], [3, 5, 40, 2], 64, 1)])
+def test_append_of_rows_past_max_rows(ctx, pkg, dtype, cache, n, lens, page, max_rows):
+    """q, pages and scales are those of a call for each sequence that has its first max_rows rows alone; the other rows of
+    q stay as they were."""
+    b = Batch(n, lens, page, 6, 2, 64, dtype, cache, seed=sum(lens))
+    b.fill([m - k for k, m in zip(n, lens)], kstd=0.3, vstd=0.3)
+    b.upload(ctx)
+    x, before = _rows(b), b.read(ctx)
+    got, after = append(ctx, pkg, b, *x, max_rows=max_rows), b.read(ctx)
+    for name, a in before.items():
+        ctx.upload(b.dev[name], a)
+    want = np.full_like(got, 0x1234)
+    for s, k in enumerate(n):
+        kept, r0 = min(k, max_rows), b.row_start[s]
+        one = {name: ctx.to_device(a) for name, a in (("row_start", np.array([r0, r0 + kept], np.int32)), ("table", b.table[s]),
+                                                      ("kv_len", np.array([lens[s] - k + kept], np.int32)))}
+        q = append(ctx, pkg, b, *x, seqs=1, **{name: int(d) for name, d in one.items()})
+        want[r0:r0 + kept] = q[r0:r0 + kept]
+        for d in one.values():
+            d.free()
+    assert (want != 0x1234).any(1).sum() == sum(min(k, max_rows) for k in n)
+    assert np.array_equal(got, want)
+    each = b.read(ctx)
+    assert all(np.array_equal(after[name], each[name], equal_nan=after[name].dtype == np.float32) for name in after)
+    b.free()
+
+
+@pytest.mark.parametrize("seqs", [63, 64, 65, 4000, 5000])
+def test_append_finds_a_row_among_many_sequences(ctx, pkg, seqs):
+    """Up to four rows a sequence, two of them kept: the kept ones' q and slots have the bits of a call with all of them."""
+    rng = np.random.default_rng(seqs)
+    n = [int(x) for x in rng.choice([0, 1, 2, 3, 4], seqs)]
+    n[0], n[-1] = 0, 3
+    b = Batch(n, [k + int(rng.integers(0, 9)) for k in n], 16, 2, 1, 64, F16, F16, seed=seqs + 1)
+    b.stale()
+    b.upload(ctx)
+    x, before = _rows(b), b.read(ctx)
+    all_q, whole = append(ctx, pkg, b, *x), b.read(ctx)
+    for name, a in before.items():
+        ctx.upload(b.dev[name], a)
+    q, after = append(ctx, pkg, b, *x, max_rows=2), b.read(ctx)
+    place = np.concatenate([np.arange(k) for k in n] + [np.full(b.tokens - sum(n), 9)])
+    assert np.array_equal(q, np.where((place < 2)[:, None], all_q, 0x1234))
+    k, v = before["k"].copy(), before["v"].copy()
+    for s in range(seqs):
+        for i in range(min(n[s], 2)):
+            pos = b.len[s] - n[s] + i
+            p, at = b.table[s, pos // 16], pos % 16
+            k[p, :, at], v[p, :, :, at] = whole["k"][p, :, at], whole["v"][p, :, :, at]
+    assert np.array_equal(after["k"], k) and np.array_equal(after["v"], v)
+    b.free()
