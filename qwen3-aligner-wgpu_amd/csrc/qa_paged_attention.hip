@@ -203,7 +203,9 @@ struct Split {
   int many_chunk, many_chunks;
   int many_rows;                // pairs of a tile
   int tiles;                    // tiles that all sequences of `many` can have together
-  int parts;                    // partial results per row; 1: no workspace
+  int few_pairs;                // pairs that a sequence of `few` can have
+  int by_seq;                   // where partial results of `few` lie, see part_index()
+  int64_t few_parts, many_parts;  // partial results of either kind in the workspace
 };
 
 Split split_of(const PagedAttnParams& p, bool e4m3, int hd) {
@@ -253,16 +255,25 @@ Split split_of(const PagedAttnParams& p, bool e4m3, int hd) {
     const int64_t blocks = about(s.many_rows);
     divide(len > 640 && blocks > 0 && blocks < kCus ? kCus / blocks : 1, 256, &s.many_chunk, &s.many_chunks);
   }
-  s.parts = s.many_chunks > s.few_chunks ? s.many_chunks : s.few_chunks;
+  s.few_pairs = (int)(rows < kFewRows ? rows : kFewRows);
+  const int64_t of_rows = p.kv.tokens * p.nqh, of_seqs = heads * s.few_pairs;
+  s.by_seq = of_seqs < of_rows;
+  s.few_parts = s.few_chunks > 1 ? (s.by_seq ? of_seqs : of_rows) * s.few_chunks : 0;
+  s.many_parts = s.many_chunks > 1 ? of_rows * s.many_chunks : 0;
   return s;
 }
 
-// Partial results in the workspace: O of (row, head, part), then its max and sum.
-__device__ __forceinline__ int64_t part_index(const PagedAttnParams& p, const Split& sp, int64_t t, int head, int part) {
-  return (t * p.nqh + head) * sp.parts + part;
+// Partial results in the workspace: all their O's, then all their maxima and sums.
+// First those of short sequences, by (sequence, kv head, pair) or by (row, head), of
+// which the sizes allow fewer: a prompt's rows in the batch take none of these many
+// parts, nor one step's sequences the pairs of longer ones.  Then those of the
+// longer tiles, by (row, head).  `pair`: of the sequence and kv head.
+__device__ __forceinline__ int64_t part_index(const PagedAttnParams& p, const Split& sp, bool few, int s, int h, int pair, int64_t t, int head, int part) {
+  if (!few) return sp.few_parts + (t * p.nqh + head) * sp.many_chunks + part;
+  return (sp.by_seq ? ((int64_t)s * p.kv.nkvh + h) * sp.few_pairs + pair : t * p.nqh + head) * sp.few_chunks + part;
 }
 __device__ __forceinline__ float* part_stats(const PagedAttnParams& p, const Split& sp, int hd) {
-  return p.ws + p.kv.tokens * p.nqh * sp.parts * hd;
+  return p.ws + (sp.few_parts + sp.many_parts) * hd;
 }
 
 // The (row, head) pair of a lane's column; columns past the last repeat it and store
@@ -526,7 +537,7 @@ __device__ __forceinline__ void multiply_v(const unsigned char* vt, const int (&
 // The waves' results joined through LDS (in order), each wave with its share of the d
 // tiles, and the result or its part written.
 template <int DT, int HD>
-__device__ __forceinline__ void finish(const PagedAttnParams& p, const Split& sp, const SeqSpan& sq, int h, int part, bool whole, float m, float l,
+__device__ __forceinline__ void finish(const PagedAttnParams& p, const Split& sp, const SeqSpan& sq, int s, int h, int part, bool whole, float m, float l,
                                        const f32x4 (&o)[HD / 16], unsigned char* smem) {
   constexpr int ND = HD / 16, NM = ND / kFewWaves;
   const int lane = threadIdx.x & 63, wave = scalar((int)(threadIdx.x >> 6)), g = lane >> 4;
@@ -564,7 +575,7 @@ __device__ __forceinline__ void finish(const PagedAttnParams& p, const Split& sp
       *reinterpret_cast<u32x2*>(dst + (wave * NM + d) * 16) = u32x2{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
     }
   } else {
-    const int64_t at = part_index(p, sp, col.tok, col.head, part);
+    const int64_t at = part_index(p, sp, true, s, h, lane & 15, col.tok, col.head, part);
     float* dst = p.ws + at * HD + 4 * g;
 #pragma unroll
     for (int d = 0; d < NM; ++d) *reinterpret_cast<f32x4*>(dst + (wave * NM + d) * 16) = w[d];
@@ -690,7 +701,7 @@ __device__ __forceinline__ void few_block(const PagedAttnParams& p, const Split&
     if (more) load_tile<DT, F8, HD, false, 1, LP, false>(kv, pages, (it + 1) & 15, 0, vt);
   }
   __syncthreads();  // the tiles' LDS is the join's
-  finish<DT, HD>(p, sp, sq, h, part, end <= sp.few_chunk, m, l, o, smem);
+  finish<DT, HD>(p, sp, sq, s, h, part, end <= sp.few_chunk, m, l, o, smem);
 }
 
 template <int DT, bool F8, int HD, int LP>
@@ -1112,7 +1123,7 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
       *reinterpret_cast<u32x2*>(dst + d_of(i)) = u32x2{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
     }
   } else {
-    const int64_t at = part_index(p, sp, tok, head, part);
+    const int64_t at = part_index(p, sp, false, s, kvh, 0, tok, head, part);
 #pragma unroll
     for (int i = 0; i < NM; ++i) *reinterpret_cast<f32x4*>(p.ws + at * HD + d_of(i)) = w[i];
     if (ns == 0 && h == 0) *reinterpret_cast<f32x2*>(part_stats(p, sp, HD) + at * 2) = (f32x2){mm, ll};
@@ -1128,7 +1139,7 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
 template <int HD>
 constexpr int kJoinPairs = 1024 / HD;
 template <int DT, int HD>
-__global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p, const Split sp, int groups, int few_rows) {
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p, const Split sp, int groups) {
   constexpr int TP = HD / 4, NP = kJoinPairs<HD>;
   __shared__ f32x4 xo[NP][TP];
   __shared__ float xs[NP];
@@ -1136,14 +1147,15 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p
   const int lane = threadIdx.x & 63, pt = threadIdx.x / TP, d = threadIdx.x % TP;
   const bool few = mine >= 0;
   SeqSpan sq;
-  int R;
+  int R, s;
   if (few) {
-    sq = seq_span(p.kv, mine / few_rows);
-    R = mine % few_rows;
+    s = mine / sp.few_pairs;
+    sq = seq_span(p.kv, s);
+    R = mine % sp.few_pairs;
     if (sq.n * p.rep > kFewRows) return;
   } else {
     const int per = sp.many_rows / NP;  // blocks of a tile
-    int s, tile;
+    int tile;
     if (!(sp.many_rows == 64 ? find_tile<64>(p, sp, b / per, &s, &sq, &tile) : find_tile<128>(p, sp, b / per, &s, &sq, &tile))) return;
     R = tile * sp.many_rows + b % per * NP + pt;
   }
@@ -1155,7 +1167,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p
   if (keys <= chunk) return;  // its tile has written the result
   const int parts = (keys + chunk - 1) / chunk;
   const int i = R / p.rep, head = h * p.rep + R % p.rep;
-  const int64_t t = sq.row0 + i, at = part_index(p, sp, t, head, 0);
+  const int64_t t = sq.row0 + i, at = part_index(p, sp, few, s, h, R, t, head, 0);
   const float* st = part_stats(p, sp, HD) + at * 2;
   const float* src = p.ws + at * HD + d * 4;
   float mm = -INFINITY;
@@ -1200,13 +1212,6 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p
   *reinterpret_cast<u32x2*>(p.out + t * p.ldo + (int64_t)head * HD + d * 4) = u32x2{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
 }
 
-// Blocks of the join, for a kv head: the tiles', and those of a short sequence.
-int64_t join_groups(const PagedAttnParams& p, const Split& sp, int hd, int64_t* few_rows) {
-  const int64_t rows = (int64_t)p.kv.max_rows * p.rep;
-  *few_rows = sp.few_chunks == 1 ? 0 : rows < kFewRows ? rows : kFewRows;
-  return sp.many_chunks == 1 ? 0 : (int64_t)sp.tiles * (sp.many_rows * hd / 1024);
-}
-
 template <int DT, bool F8, int HD, int LP>
 hipError_t launch_one(const PagedAttnParams& p, hipStream_t s) {
   const Split sp = split_of(p, F8, HD);
@@ -1219,11 +1224,10 @@ hipError_t launch_one(const PagedAttnParams& p, hipStream_t s) {
   } else {
     hipLaunchKernelGGL((paged_few_kernel<DT, F8, HD, LP>), dim3((unsigned)(heads * sp.few_chunks)), dim3(64 * kFewWaves), 0, s, p, sp);
   }
-  if (sp.parts > 1) {
-    int64_t few_rows;
-    const int64_t groups = join_groups(p, sp, HD, &few_rows);
-    hipLaunchKernelGGL((paged_join_kernel<DT, HD>), dim3((unsigned)(p.kv.nkvh * groups + heads * few_rows)), dim3(256), 0, s, p, sp, (int)groups,
-                       (int)few_rows);
+  if (sp.few_parts + sp.many_parts > 0) {
+    const int64_t groups = sp.many_chunks == 1 ? 0 : (int64_t)sp.tiles * (sp.many_rows * HD / 1024);  // the tiles' blocks, for a kv head
+    const int64_t pairs = sp.few_chunks == 1 ? 0 : heads * sp.few_pairs;
+    hipLaunchKernelGGL((paged_join_kernel<DT, HD>), dim3((unsigned)(p.kv.nkvh * groups + pairs)), dim3(256), 0, s, p, sp, (int)groups);
   }
   return hipGetLastError();
 }
@@ -1251,7 +1255,7 @@ int64_t paged_attention_blocks(bool e4m3, int hd, const PagedAttnParams& p) {
 
 size_t paged_attention_workspace(bool e4m3, int hd, const PagedAttnParams& p) {
   const Split sp = split_of(p, e4m3, hd);
-  return sp.parts > 1 ? (size_t)p.kv.tokens * p.nqh * sp.parts * (hd + 2) * sizeof(float) : 0;
+  return (size_t)(sp.few_parts + sp.many_parts) * (hd + 2) * sizeof(float);
 }
 
 hipError_t launch_attention_paged(int dtype, bool e4m3, int hd, const PagedAttnParams& p, hipStream_t s) {

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 from conftest import rope_tables, ulp16
-from paged import BF16, E4M3, F16, STALE8, STALE16, Batch, append, assert_attention, attention, e4m3_codes, narrow, widen
+from paged import BF16, E4M3, F16, STALE8, STALE16, Batch, append, assert_attention, attention, attention_desc, e4m3_codes, narrow, widen
 
 pytestmark = pytest.mark.gpu
 
@@ -175,4 +175,29 @@ def test_append_finds_a_row_among_many_sequences(ctx, pkg, seqs):
             p, at = b.table[s, pos // 16], pos % 16
             k[p, :, at], v[p, :, :, at] = whole["k"][p, :, at], whole["v"][p, :, :, at]
     assert np.array_equal(after["k"], k) and np.array_equal(after["v"], v)
+    b.free()
+
+
+@FORMATS
+@pytest.mark.parametrize("n,lens,max_rows", [([300, 1, 1], [300, 3000, 900], 300), ([1] * 20, [3000, 40] * 10, 16), ([1, 1, 1], [5000, 2, 1300], 1),
+                                             ([90], [3000], 90), ([90, 1, 2], [3000, 2000, 100], 90), ([3, 8, 8], [4000, 4001, 8], 8)])
+def test_workspace_is_all_that_is_written(ctx, pkg, dtype, cache, n, lens, max_rows):
+    """Partial results of short and of long sequences, in either order: the call is right with exactly the bytes that it asks
+    for, whatever they hold before, and nothing behind them changes."""
+    b = Batch(n, lens, 32, 4, 2, 64, dtype, cache, seed=sum(lens))
+    b.fill()
+    b.upload(ctx)
+    q = b.random_rows(4 * 64)
+    dq, do = ctx.to_device(q), ctx.to_device(np.full(q.shape, 0x3C01, np.uint16))
+    d = attention_desc(pkg, b, dq, q.shape[1], do, q.shape[1], max_rows=max_rows)
+    size = pkg.attention_paged_workspace(d)
+    assert size > 0
+    ws = ctx.to_device(np.concatenate([np.full(size, 0xFF, np.uint8), np.full(8192, 0xA5, np.uint8)]))
+    d.workspace, d.workspace_bytes = int(ws), size
+    ctx.attention_paged(d)
+    got = ctx.download(do, q.shape)
+    assert (ctx.download(ws, (8192,), np.uint8, size) == 0xA5).all()
+    assert_attention(b, q, got)
+    for x in (dq, do, ws):
+        x.free()
     b.free()
