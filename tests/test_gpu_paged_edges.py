@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 from conftest import rope_tables, ulp16
-from paged import BF16, E4M3, F16, STALE8, STALE16, Batch, append, assert_attention, attention, attention_desc, e4m3_codes, narrow, widen
+from paged import BF16, E4M3, F16, STALE8, STALE16, Batch, append, assert_attention, attention, attention_desc, e4m3_codes, e4m3_values, narrow, widen
 
 pytestmark = pytest.mark.gpu
 
@@ -200,4 +200,48 @@ def test_workspace_is_all_that_is_written(ctx, pkg, dtype, cache, n, lens, max_r
     assert_attention(b, q, got)
     for x in (dq, do, ws):
         x.free()
+    b.free()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("n,lens,cut", [([1, 40], [20, 45], 5), ([1, 6], [20, 30], 3)])
+def test_append_to_e4m3_leaves_the_slots_of_rows_past_the_batch(ctx, pkg, dtype, n, lens, cut):
+    """The last rows lie past `tokens`.  Their slots hold finite values: in a page whose first slot is new its codes stay as they
+    are, whatever its scale becomes; in a page that held rows before they are rounded again with it."""
+    b = Batch(n, lens, 16, 4, 2, 64, dtype, E4M3, seed=sum(lens), tail_rows=0)
+    b.fill(kstd=0.3, vstd=0.3)
+    b.upload(ctx)
+    (qkv, qn, kn, c, s), before = _rows(b), b.read(ctx)
+    b.tokens -= cut
+    append(ctx, pkg, b, qkv[: b.tokens], qn, kn, c[: b.tokens], s[: b.tokens])
+    after = b.read(ctx)
+    first, page = lens[1] - n[1], (lens[1] - cut) // 16
+    assert (lens[1] - 1) // 16 == page
+    p, at = b.table[1, page], np.arange(lens[1] - cut, lens[1]) % 16
+    fresh = first <= page * 16
+    assert fresh == (n[1] == 40)
+    for name, axis in (("k", 1), ("v", 2)):
+        old, now = (x[name + "_scale"][p].astype(np.float64) for x in (before, after))
+        assert (now > old).all()  # these rows' values are smaller than the new ones
+        held, got = (np.take(x[name][p], at, axis) for x in (before, after))
+        want = held if fresh else e4m3_codes(e4m3_values(held) * (old / now)[:, None, None])
+        assert np.array_equal(got, want), name
+    b.free()
+
+
+@FORMATS
+@pytest.mark.parametrize("page", [16, 32, 64])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_a_wave_goes_through_several_windows_of_pages(ctx, pkg, dtype, cache, page, hd):
+    """One token behind 20011 keys under a bound of 2^20, which leaves the keys in one part: each of four waves goes through 78
+    blocks of 64 keys, whose pages are looked up 16 blocks at a time.  Pages in the third and fourth windows are none."""
+    b = Batch([1], [20011], page, 4, 2, hd, dtype, cache, seed=hd + page, tail_rows=0, extra_slots=2 ** 20 // page)
+    b.fill()
+    b.table[0, [9001 // page, 15000 // page, 20000 // page]] = -1
+    b.upload(ctx)
+    q = b.random_rows(4 * hd)
+    size = pkg.attention_paged_workspace(attention_desc(pkg, b, 0, 4 * hd, 0, 4 * hd, max_len=2 ** 20))
+    parts = size // (4 * (hd + 2) * 4)
+    assert parts * 4 * (hd + 2) * 4 == size and 2 ** 20 // parts > 20011  # no part ends before the keys do
+    assert_attention(b, q, attention(ctx, pkg, b, q, max_len=2 ** 20))
     b.free()
