@@ -14,8 +14,8 @@
 // behind the rows' instead of before them, 18.4 us for 15.7 at 4334 rows.)
 //
 // Bound by the bytes: 4334 rows of 16 q and 8 kv heads of 128 into empty e4m3 pages, 67
-// MB, 15.7 us (4.2 TB/s); a step's few rows by the launch and a chain of loads,
-// row_start, the table, the row: 32 single rows 3.8 us.
+// MB, 15.7 us (4.2 TB/s), into 16-bit pages, 75 MB, 15.0; a step's few rows by the
+// launch and a chain of loads, row_start, the table, the row: 32 single rows 4.2 us.
 //
 // e4m3 scales are powers of two, the least 2^e with amax <= 448 * 2^e: dividing by
 // one is exact, so a value is rounded once however often its page's scale
@@ -191,11 +191,9 @@ __device__ __forceinline__ void q_part(const AppendParams& p, int64_t bx) {
   constexpr int L = HD / 16, hpw = 64 / L;  // lanes to a head, heads at once
   const int lane = threadIdx.x & 63, c = lane % L, sub = lane / L;
   const int64_t t = bx * 4 + (threadIdx.x >> 6);
-  // rows of no sequence keep what they hold, and those past max_rows, which only a batch
-  // of more rows can have
+  // rows of no sequence keep what they hold
   const int64_t t0 = p.kv.row_start[0], t1 = p.kv.row_start[p.kv.seqs];
-  const bool past = p.kv.max_rows < p.kv.tokens && t < p.kv.tokens && row_in_sequence(p.kv, t) >= p.kv.max_rows;
-  if (t >= p.kv.tokens || t < t0 || t >= t1 || past) return;
+  if (t >= p.kv.tokens || t < t0 || t >= t1) return;
   const Turn turn = load_turn<HD>(p.qn, p.cos + t * HD, p.sin + t * HD, c);
   const uint16_t* src = p.qkv + t * p.ldqkv + 8 * c;
   uint16_t* dst = p.q_out + t * p.ldq + 8 * c;
@@ -206,6 +204,9 @@ __device__ __forceinline__ void q_part(const AppendParams& p, int64_t bx) {
   };
   u32x4 va, vb, na, nb;
   load(sub, &va, &vb);
+  // ... and so do those past max_rows, which only a batch of more rows can have; the first
+  // loads are under way by now (8 prompts of 771 rows 16.2 us, 16.1 without this, 16.6 with it before them)
+  if (p.kv.max_rows < p.kv.tokens && row_in_sequence(p.kv, t) >= p.kv.max_rows) return;
   for (int h0 = 0; h0 < p.nqh; h0 += hpw) {
     load(h0 + hpw + sub, &na, &nb);  // the next heads, while these are at work
     float xa[8], xb[8];
