@@ -397,8 +397,9 @@ int qa_kv_append(qa_ctx* ctx, const qa_kv_append_desc* desc);
  * out[t][h hd + j] = round(sum_t p_t v_t[j]).  Keys on an entry that is no page do
  * not count; a row without keys gives zeros.  What the pages and their scales hold
  * behind the last key that a row of the sequence sees (slots of rows that were left
- * out among it) is not looked at.  Scales may be any positive numbers.  V has
- * to be finite, and below 2^100, up to that key: a row multiplies
+ * out among it) is not looked at.  Scales may be any positive normal
+ * numbers that keep the scores within f32 (below 2^-110 a V scale costs bits of the
+ * probabilities).  V has to be finite, and below 2^100, up to that key: a row multiplies
  * what is behind its own position by 0, which leaves NaN of an infinity or NaN (K may
  * hold either there), and probabilities are up to 2^8 before they are divided.
  *   q    [tokens][nqh hd], row stride ldq, as qa_kv_append writes it
@@ -411,7 +412,8 @@ int qa_kv_append(qa_ctx* ctx, const qa_kv_append_desc* desc);
  * the P.V product as sums of 16-bit terms: two of f16 over f16 pages (22 bits of a
  * probability), two of bf16 over bf16 pages (16 bits; both as in
  * qa_attention_prefill's default), three of bf16 over QA_E4M3 pages (24 bits), and over
- * bf16 pages too for sequences whose rows times nqh / nkvh are at most 16. */
+ * bf16 pages too for short sequences (rows times nqh / nkvh at most 16; not where
+ * max_rows is more and seqs * max_rows = tokens, which a batch without any has). */
 typedef struct qa_paged_attention_desc {
   uint32_t dtype;
   uint32_t flags; /* reserved, must be 0 */

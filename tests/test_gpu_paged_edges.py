@@ -245,3 +245,20 @@ def test_a_wave_goes_through_several_windows_of_pages(ctx, pkg, dtype, cache, pa
     assert parts * 4 * (hd + 2) * 4 == size and 2 ** 20 // parts > 20011  # no part ends before the keys do
     assert_attention(b, q, attention(ctx, pkg, b, q, max_len=2 ** 20))
     b.free()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("n,lens", [([1, 1], [37, 700]), ([40], [100])])
+def test_scales_at_the_ends_of_their_range(ctx, pkg, dtype, n, lens):
+    """K scales of the smallest normal number (all scores round to 0) and of 2^100 with K of zeros: every key that a row sees has
+    the same weight, the ones that it does not see none."""
+    for scale, k in ((2.0 ** -126, None), (2.0 ** 100, 0)):
+        b = Batch(n, lens, 16, 4, 2, 64, dtype, E4M3, seed=sum(lens))
+        b.fill()
+        b.k_scale[:] = scale
+        if k is not None:
+            b.k[:] = k
+        b.upload(ctx)
+        q = b.random_rows(4 * 64)
+        assert_attention(b, q, attention(ctx, pkg, b, q))
+        b.free()
