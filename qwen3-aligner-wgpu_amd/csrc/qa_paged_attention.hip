@@ -34,7 +34,7 @@
 // Sequences of up to 16 pairs (single tokens): paged_few_kernel.  Bound by the
 // cache's bytes: 32 sequences of up to 4353 keys, 8 kv heads of 128, 342 MB in f16: 69 us,
 // 4.9 TB/s (a large copy: 5.1); 64 of up to 8193 in e4m3, 598 MB: 127 us, 4.7 TB/s.  The
-// smallest calls by latency: one sequence of 323 keys 8.3 us, of which launching is 4.
+// smallest calls by latency: one sequence of 323 keys 8.4 us, of which launching is 4.
 // Longer ones: paged_many_kernel, bound by the two phases of a step, of which the
 // softmax is as long as the products: 771 rows behind 1536 keys, 16 heads of 128:
 // 33 us, 367 TFLOP/s, 550 with the products of the residues.
@@ -179,21 +179,33 @@ struct Cfg {
 //    f16, hd 128: 64 of them behind up to 700 keys 10.8 / 11.0, 1500 15.5 / 13.4; 128
 //    behind 1500 17.1 / 19.2, 4300 49.1 / 39.3; 256 behind 4300 70.5 / 73.3), and up to
 //    4096 keys past 256 of them (512 behind 3300 93.7 / 93.9, e4m3 4352 73.2 / 67.5).
+//    That line is good at full rounds of blocks; where the last round has few, the best
+//    split wins earlier (all as long, f16, hd 128: 264 behind 1000 32.3 / 34.7, 2000 58.4 /
+//    49.8, 4096 127.5 / 105.0; 320 behind 1000 32.8 / 36.6, 2000 66.5 / 62.4, 4096 133.1 /
+//    122.6; 384 behind 4096 140.6 / 142.6; 576 behind 4096 222.4 / 210.8; e4m3 264 behind
+//    4096 63.0 / 51.4, 320 71.6 / 63.2, 384 81.3 / 78.0).
 //    Else into parts that give every CU its blocks (one, or two of e4m3 or hd 64, by
-//    their LDS), and with more sequences into more, down to 1024 keys, as their joins
-//    are one launch (e4m3, 512 behind 8192, in 1, 3, 5, 9 parts: 133.6, 124.7, 122.8,
+//    their LDS), and with more sequences into more, down to about 1024 keys, as their
+//    joins are one launch (e4m3, 512 behind 8192, in 1, 3, 5, 9 parts: 133.6, 124.7, 122.8,
 //    121.1; f16, 64 behind 8192 in 5 and 9: 26.5, 28.8).  The number is odd: blocks go to
 //    CUs in turns, and with an even one the same CUs get all the first, full parts
 //    (512 behind 4352, f16, in 3, 4, 5: 118.6, 148.9, 122).  A part is a multiple of 256
 //    keys, a block of 64 for each wave.
 //  * many: tiles of 64 or 128 pairs.  Of 64 up to 600 tiles: 128-row blocks load each
 //    tile for twice the rows, but are half as many, each with twice the steps (8 kv
-//    heads, no past, 64 / 128, us: 1500 rows 28.1 / 37.9, 2500 62.6 / 59.8, 3500 101.7 /
-//    86.2, 4334 147 / 134).  Their keys are split while the CUs take the parts at once,
-//    down to 256: 64 rows behind 16000 keys 166 us whole, 28.8 in 32 parts; 200 behind
-//    700 18.1 whole, 16.3 in four; but 771 behind 1536 (200 blocks) 32 whole, 43 in
-//    two, as half the CUs' parts have to wait.  Up to 640 keys there is no gain (600
-//    and none before, 4 kv heads of 64: 12.4 whole, 13.5 in three).
+//    heads of 128, no past, 64 / 128, us: 1500 rows 28.1 / 37.9, 2500 62.6 / 59.8, 3500
+//    101.7 / 86.2, 4334 153 / 141; prompts of 323 rows, 4 of them 20.9 / 16.2, which the
+//    line misses, 8 32.2 / 29.3, 16 60.5 / 45.2; of 771, 2 24.0 / 24.5, 4 43.7 / 39.2; 2 of
+//    1500 55.2 / 44.2; one of 4334 and 4 of 771 188 / 167, in either order; e4m3: 4 of 323
+//    23.0 / 19.3, 8 35.5 / 34.9, 2 of 771 27.2 / 31.9, 4 51.6 / 49.3).
+//    Their keys are split while the CUs take the parts at once, down to 256: 64 rows
+//    behind 16000 keys 166 us whole, 28.8 in 32 parts; 200 behind 700 18.1 whole, 16.3 in
+//    four; 8 prompts of up to 100 rows behind 1500 (4 of 64) 24.2 whole, 20.4 in the two
+//    that this gives, 19.7 in three; but 771 behind 1536 (200 blocks) 32 whole, 43 in two,
+//    as half the CUs' parts have to wait.  Up to 640 keys there is no gain (600 and none
+//    before, 4 kv heads of 64: 12.4 whole, 13.5 in three).
+//  * kCus is a whole device's: the workspace has to be known without a device, so that
+//    on a partition of one the parts are more than its CUs need.
 constexpr int kFewRows = 16, kFewWaves = 4;
 constexpr int kManyWaves = 8;
 constexpr int kCus = 256;

@@ -9,7 +9,7 @@
 // running number: once for a step, for every layer's q / k rotation.
 //
 // Bound by the rows it writes: 30720 tokens of hd 128, 31 MB, 8.5 us, of which the
-// f64 of angles and series is 1; 32 tokens 4.4 us, the launch.  (With the library's
+// f64 of angles and series is 1; 32 tokens 4.8 us, the launch.  (With the library's
 // sincos, whose reduction takes any angle, 1 more.)
 //
 // The angle is formed in f64 (a position of 2^20 leaves an f32 angle no more
