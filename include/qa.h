@@ -412,8 +412,8 @@ int qa_kv_append(qa_ctx* ctx, const qa_kv_append_desc* desc);
  * the P.V product as sums of 16-bit terms: two of f16 over f16 pages (22 bits of a
  * probability), two of bf16 over bf16 pages (16 bits; both as in
  * qa_attention_prefill's default), three of bf16 over QA_E4M3 pages (24 bits), and over
- * bf16 pages too for short sequences (rows times nqh / nkvh at most 16; not where
- * max_rows is more and seqs * max_rows = tokens, which a batch without any has). */
+ * bf16 pages too for short sequences (rows times nqh / nkvh at most 16, where max_rows
+ * is no more either or seqs * max_rows > tokens says that there may be shorter ones). */
 typedef struct qa_paged_attention_desc {
   uint32_t dtype;
   uint32_t flags; /* reserved, must be 0 */
