@@ -273,7 +273,7 @@ _ctx = None
 
 def _list(pkg, s, prefix=""):
     """Every layer's pages: a pool's planes."""
-    each = [(x.data_ptr(), x.element_size() * x[0, 0].numel()) for n in _planes(s["case"]) for x in s[prefix + n]]
+    each = [(x.data_ptr(), x.element_size() * x[0].numel()) for n in _planes(s["case"]) for x in s[prefix + n]]
     return (pkg.PagePlane * len(each))(*each)
 
 
