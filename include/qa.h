@@ -433,6 +433,180 @@ int qa_attention_paged(qa_ctx* ctx, const qa_paged_attention_desc* desc);
  * at.  Host function, no device needed. */
 int qa_attention_paged_workspace(const qa_paged_attention_desc* desc, size_t* bytes);
 
+/* qa_attention_paged with a window and sinks: the row at position p attends to its
+ * sequence's keys j <= p with j > p - window or j < sinks, so that a cache need not
+ * keep what lies between (qa_pages_fork gives those pages back).  Everything else is
+ * as in qa_attention_paged, for the keys that rows see; what the pages hold that no row of
+ * its sequence sees is not looked at, in front of the window as behind the last key, and
+ * table entries there may be anything.  window in [1, 2^30], sinks in [0, 2^30]. */
+typedef struct qa_paged_window_desc {
+  uint32_t dtype;
+  uint32_t flags; /* reserved, must be 0 */
+  int64_t tokens;
+  int32_t nqh;
+  const void* q;
+  int64_t ldq;
+  const qa_paged_kv* kv;
+  void* out;
+  int64_t ldo;
+  int64_t window, sinks;
+  void* workspace;
+  size_t workspace_bytes;
+} qa_paged_window_desc;
+int qa_attention_paged_window(qa_ctx* ctx, const qa_paged_window_desc* desc);
+/* Its workspace in bytes, from the sizes, window and sinks. */
+int qa_attention_paged_window_workspace(const qa_paged_window_desc* desc, size_t* bytes);
+
+/* ---- a pool's pages: shared, forked, given back, moved ----
+ *
+ * A pool is what qa_paged_kv's page numbers name, over all the caches (layers) that
+ * use the same tables: a list of planes, each [num_pages][bytes], K and V of every layer
+ * and in a QA_E4M3 cache their scales.  The list is host memory, read during the call.
+ * refs, int32 [num_pages] on the device, holds how many table entries name each page;
+ * a page with none (or fewer) is free.  A page is written by one sequence alone
+ * (qa_kv_append), so that sequences share full pages and the last, partly filled one
+ * only until either goes on.  Whatever tables, lengths, parents and references
+ * hold, no call reads or writes outside its buffers.
+ * No counterpart in the reference. */
+typedef struct qa_page_plane {
+  void* base;    /* 16-byte aligned */
+  int64_t bytes; /* of a page: a multiple of 16, or of 4 up to 4096, less than 2^31 */
+} qa_page_plane;
+
+/* pairs of pages (src, dst) int32 [npairs][2], on the device: dst takes src's bytes in
+ * every plane.  The lists of planes have the same bytes, plane by plane, and may be
+ * the same.  A pair with a number outside either pool is left out.  No page may be written
+ * twice, nor read and written in one call. */
+typedef struct qa_pages_copy_desc {
+  uint32_t flags; /* reserved, must be 0 */
+  int64_t nplanes;
+  const qa_page_plane* src;
+  int64_t src_pages;
+  const qa_page_plane* dst;
+  int64_t dst_pages;
+  const int32_t* pairs;
+  int64_t npairs;
+} qa_pages_copy_desc;
+int qa_pages_copy(qa_ctx* ctx, const qa_pages_copy_desc* desc);
+
+/* The sequences of the next step out of those of the last: sequence i goes on from source
+ * parent[i] (several may have one parent; a number outside [0, src_seqs) gives a
+ * sequence without keys or pages).  Its table has its parent's pages, shared, up to the
+ * parent's length; with window > 0 without those that no row from there on sees through
+ * qa_attention_paged_window (all of the page at or behind `sinks` and at or before
+ * length - window), whose entries become -1.  grow[i] rows are to be appended: len[i] is
+ * the parent's length and grow[i], the kv_len of the next call, at most ldtable * page,
+ * with new pages for them.  A last, partly filled page that is to be written on becomes
+ * the sequence's own: it is copied to a new page unless all that hold it are to write
+ * on it and the sequence is the first of those.
+ * The sources end with the call, with all that their rows name, reserved pages too,
+ * unless QA_PAGES_KEEP: then they stay, and hold what they held.  References follow.  New
+ * pages are the lowest that are free behind that, in the order of sequences and
+ * positions; *missing (int32, device) is how many there were too few.  Where it is not 0
+ * refs and pages stay as they were, and the new sequences are empty.
+ *   src_table  int32 [src_seqs][ldtable], src_len int32 [src_seqs] (held to
+ *              [0, ldtable * page])
+ *   table      int32 [seqs][ldtable] and len int32 [seqs], written; no part of the
+ *              sources
+ *   parent     int32 [seqs]; grow int32 [seqs] (below 0: 0), or NULL for none
+ *   workspace  16-byte aligned, of the bytes that qa_pages_fork_workspace gives; its
+ *              contents need not be kept, and calls that may run at the same time
+ *              need one each
+ * page 16, 32 or 64 tokens; seqs and src_seqs at most 8192. */
+enum { QA_PAGES_KEEP = 1u << 0 };
+typedef struct qa_pages_fork_desc {
+  uint32_t flags; /* 0 or QA_PAGES_KEEP */
+  int32_t page;
+  int64_t num_pages;
+  const qa_page_plane* planes;
+  int64_t nplanes;
+  int32_t* refs;
+  int64_t src_seqs, seqs, ldtable;
+  const int32_t* src_table;
+  const int32_t* src_len;
+  const int32_t* parent;
+  int32_t* table;
+  int32_t* len;
+  const int32_t* grow;
+  int64_t window, sinks;
+  int32_t* missing;
+  void* workspace;
+  size_t workspace_bytes;
+} qa_pages_fork_desc;
+int qa_pages_fork(qa_ctx* ctx, const qa_pages_fork_desc* desc);
+int qa_pages_fork_workspace(const qa_pages_fork_desc* desc, size_t* bytes);
+
+/* The used pages (refs > 0) to the front of the pool: with n of them, the k-th used page
+ * behind the first n goes into the k-th gap among those, and every other stays.
+ *   refs_out   int32 [num_pages]: the references behind that, 0 from n on
+ *   table      int32 [seqs][ldtable], table_out the same with the pages' new numbers;
+ *              an entry that names no used page becomes -1.  refs_out and table_out may
+ *              be refs and table.
+ *   map        int32 [num_pages], each page's new number or -1, for tables elsewhere; or
+ *              NULL
+ *   used       int32: n
+ *   workspace  as in qa_pages_fork, of qa_pages_compact_workspace's bytes */
+typedef struct qa_pages_compact_desc {
+  uint32_t flags; /* reserved, must be 0 */
+  int64_t num_pages;
+  const qa_page_plane* planes;
+  int64_t nplanes;
+  const int32_t* refs;
+  int32_t* refs_out;
+  int64_t seqs, ldtable;
+  const int32_t* table;
+  int32_t* table_out;
+  int32_t* map;
+  int32_t* used;
+  void* workspace;
+  size_t workspace_bytes;
+} qa_pages_compact_desc;
+int qa_pages_compact(qa_ctx* ctx, const qa_pages_compact_desc* desc);
+int qa_pages_compact_workspace(const qa_pages_compact_desc* desc, size_t* bytes);
+
+/* The step of a beam search: for each group the `width` best continuations of its
+ * `beams` sequences by score[b] + log softmax(logits[b])[t] over all b and t, best first,
+ * ties to the lowest b and then t.  Sums of exponentials are f32 within 64 KB of a row
+ * and f64 beyond; continuations are ranked in f64.
+ *   logits  [groups * beams][vocab], row stride ldl, QA_F16, QA_BF16 or QA_F32; -inf
+ *           is a token of probability 0, and so is NaN or +inf here: it is not chosen and
+ *           not counted
+ *   score   f32 [groups * beams]; a sequence whose score is -inf, NaN or +inf is
+ *           none (the first step of a search: one score of 0 and -inf for the others)
+ *   done    int32 [groups * beams] or NULL: a sequence where it is not 0 has ended,
+ *           and goes on with the token `end` alone, at its score
+ *   end     the token that ends a sequence, in [0, vocab), or -1 (done must be NULL)
+ *   parent, token  int32 [groups * width]: b as a row of logits (qa_pages_fork's parent)
+ *           and t; -1, with the score -inf, where a group has no more continuations of a
+ *           probability above 0
+ *   score_out f32 [groups * width], rounded from f64
+ *   done_out  int32 [groups * width]: the parent had ended, or the token is `end`
+ *   workspace as in qa_attention_paged, of the bytes that qa_beam_select_workspace
+ *           gives
+ * The outputs are no part of the inputs.  beams and width in [1, 64]; ldl a multiple of 8 (QA_F32: of 4), logits 16-byte
+ * aligned. */
+enum { QA_F32 = 3 }; /* qa_beam_desc.dtype alone */
+typedef struct qa_beam_desc {
+  uint32_t dtype;
+  uint32_t flags; /* reserved, must be 0 */
+  int64_t groups;
+  int32_t beams, width;
+  int64_t vocab;
+  const void* logits;
+  int64_t ldl;
+  const float* score;
+  const int32_t* done;
+  int32_t end;
+  int32_t* parent;
+  int32_t* token;
+  float* score_out;
+  int32_t* done_out;
+  void* workspace;
+  size_t workspace_bytes;
+} qa_beam_desc;
+int qa_beam_select(qa_ctx* ctx, const qa_beam_desc* desc);
+int qa_beam_select_workspace(const qa_beam_desc* desc, size_t* bytes);
+
 /* ---- audio tower ops around the projections ---- */
 
 /* qa_conv_desc.flags */

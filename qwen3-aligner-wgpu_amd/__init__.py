@@ -36,6 +36,8 @@ ACCUMULATE, EPI_GELU, EPI_SILU_MUL, TRANSB, BIAS_ROWS = 1, 2, 4, 8, 16
 QA_ATTN_P16 = 1  # qa_attention_desc.flags
 QA_CONV_GELU, QA_CONV_TOKEN_MAJOR = 1, 2  # qa_conv_desc.flags
 MROPE_INTERLEAVED = 1  # qa_mrope_desc.flags
+F32 = 3  # qa_beam_desc.dtype alone
+PAGES_KEEP = 1  # qa_pages_fork_desc.flags
 
 _STATUS = {
     QA_EINVAL: "QA_EINVAL",
@@ -239,6 +241,122 @@ class PagedAttentionDesc(ctypes.Structure):
     ]
 
 
+class PagedWindowDesc(ctypes.Structure):
+    """qa_paged_window_desc (include/qa.h)."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_uint32),
+        ("flags", ctypes.c_uint32),
+        ("tokens", ctypes.c_int64),
+        ("nqh", ctypes.c_int32),
+        ("q", ctypes.c_void_p),
+        ("ldq", ctypes.c_int64),
+        ("kv", ctypes.POINTER(PagedKV)),
+        ("out", ctypes.c_void_p),
+        ("ldo", ctypes.c_int64),
+        ("window", ctypes.c_int64),
+        ("sinks", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class PagePlane(ctypes.Structure):
+    """qa_page_plane (include/qa.h)."""
+
+    _fields_ = [
+        ("base", ctypes.c_void_p),
+        ("bytes", ctypes.c_int64),
+    ]
+
+
+class PagesCopyDesc(ctypes.Structure):
+    """qa_pages_copy_desc (include/qa.h)."""
+
+    _fields_ = [
+        ("flags", ctypes.c_uint32),
+        ("nplanes", ctypes.c_int64),
+        ("src", ctypes.POINTER(PagePlane)),
+        ("src_pages", ctypes.c_int64),
+        ("dst", ctypes.POINTER(PagePlane)),
+        ("dst_pages", ctypes.c_int64),
+        ("pairs", ctypes.c_void_p),
+        ("npairs", ctypes.c_int64),
+    ]
+
+
+class PagesForkDesc(ctypes.Structure):
+    """qa_pages_fork_desc (include/qa.h)."""
+
+    _fields_ = [
+        ("flags", ctypes.c_uint32),
+        ("page", ctypes.c_int32),
+        ("num_pages", ctypes.c_int64),
+        ("planes", ctypes.POINTER(PagePlane)),
+        ("nplanes", ctypes.c_int64),
+        ("refs", ctypes.c_void_p),
+        ("src_seqs", ctypes.c_int64),
+        ("seqs", ctypes.c_int64),
+        ("ldtable", ctypes.c_int64),
+        ("src_table", ctypes.c_void_p),
+        ("src_len", ctypes.c_void_p),
+        ("parent", ctypes.c_void_p),
+        ("table", ctypes.c_void_p),
+        ("len", ctypes.c_void_p),
+        ("grow", ctypes.c_void_p),
+        ("window", ctypes.c_int64),
+        ("sinks", ctypes.c_int64),
+        ("missing", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class PagesCompactDesc(ctypes.Structure):
+    """qa_pages_compact_desc (include/qa.h)."""
+
+    _fields_ = [
+        ("flags", ctypes.c_uint32),
+        ("num_pages", ctypes.c_int64),
+        ("planes", ctypes.POINTER(PagePlane)),
+        ("nplanes", ctypes.c_int64),
+        ("refs", ctypes.c_void_p),
+        ("refs_out", ctypes.c_void_p),
+        ("seqs", ctypes.c_int64),
+        ("ldtable", ctypes.c_int64),
+        ("table", ctypes.c_void_p),
+        ("table_out", ctypes.c_void_p),
+        ("map", ctypes.c_void_p),
+        ("used", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class BeamDesc(ctypes.Structure):
+    """qa_beam_desc (include/qa.h)."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_uint32),
+        ("flags", ctypes.c_uint32),
+        ("groups", ctypes.c_int64),
+        ("beams", ctypes.c_int32),
+        ("width", ctypes.c_int32),
+        ("vocab", ctypes.c_int64),
+        ("logits", ctypes.c_void_p),
+        ("ldl", ctypes.c_int64),
+        ("score", ctypes.c_void_p),
+        ("done", ctypes.c_void_p),
+        ("end", ctypes.c_int32),
+        ("parent", ctypes.c_void_p),
+        ("token", ctypes.c_void_p),
+        ("score_out", ctypes.c_void_p),
+        ("done_out", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 class LayerNormDesc(ctypes.Structure):
     """qa_layer_norm_desc (include/qa.h)."""
 
@@ -368,6 +486,8 @@ EXPORTS = (
     "qa_time_next_launch",
     "qa_mlp_fused", "qa_rms_norm", "qa_qk_norm_rope", "qa_attention_prefill",
     "qa_mrope_rows", "qa_kv_append", "qa_attention_paged", "qa_attention_paged_workspace",
+    "qa_attention_paged_window", "qa_attention_paged_window_workspace", "qa_pages_copy", "qa_pages_fork",
+    "qa_pages_fork_workspace", "qa_pages_compact", "qa_pages_compact_workspace", "qa_beam_select", "qa_beam_select_workspace",
     "qa_layer_norm", "qa_window_attention", "qa_add_position_table", "qa_conv2d_3x3s2",
     "qa_mel_filterbank", "qa_log_mel", "qa_rope_tables", "qa_embed_scatter", "qa_timestamp_head",
     "qa_last_error", "qa_version",
@@ -409,6 +529,15 @@ def lib() -> ctypes.CDLL:
         L.qa_kv_append.argtypes = [vp, ctypes.POINTER(KvAppendDesc)]
         L.qa_attention_paged.argtypes = [vp, ctypes.POINTER(PagedAttentionDesc)]
         L.qa_attention_paged_workspace.argtypes = [ctypes.POINTER(PagedAttentionDesc), ctypes.POINTER(sz)]
+        L.qa_attention_paged_window.argtypes = [vp, ctypes.POINTER(PagedWindowDesc)]
+        L.qa_attention_paged_window_workspace.argtypes = [ctypes.POINTER(PagedWindowDesc), ctypes.POINTER(sz)]
+        L.qa_pages_copy.argtypes = [vp, ctypes.POINTER(PagesCopyDesc)]
+        L.qa_pages_fork.argtypes = [vp, ctypes.POINTER(PagesForkDesc)]
+        L.qa_pages_fork_workspace.argtypes = [ctypes.POINTER(PagesForkDesc), ctypes.POINTER(sz)]
+        L.qa_pages_compact.argtypes = [vp, ctypes.POINTER(PagesCompactDesc)]
+        L.qa_pages_compact_workspace.argtypes = [ctypes.POINTER(PagesCompactDesc), ctypes.POINTER(sz)]
+        L.qa_beam_select.argtypes = [vp, ctypes.POINTER(BeamDesc)]
+        L.qa_beam_select_workspace.argtypes = [ctypes.POINTER(BeamDesc), ctypes.POINTER(sz)]
         L.qa_layer_norm.argtypes = [vp, ctypes.POINTER(LayerNormDesc)]
         L.qa_window_attention.argtypes = [vp, ctypes.POINTER(WindowAttentionDesc)]
         L.qa_add_position_table.argtypes = [vp, ctypes.POINTER(PositionAddDesc)]
@@ -550,6 +679,21 @@ class Context:
     def attention_paged(self, desc: PagedAttentionDesc) -> None:
         check(lib().qa_attention_paged(self.handle, ctypes.byref(desc)))
 
+    def attention_paged_window(self, desc: PagedWindowDesc) -> None:
+        check(lib().qa_attention_paged_window(self.handle, ctypes.byref(desc)))
+
+    def pages_copy(self, desc: PagesCopyDesc) -> None:
+        check(lib().qa_pages_copy(self.handle, ctypes.byref(desc)))
+
+    def pages_fork(self, desc: PagesForkDesc) -> None:
+        check(lib().qa_pages_fork(self.handle, ctypes.byref(desc)))
+
+    def pages_compact(self, desc: PagesCompactDesc) -> None:
+        check(lib().qa_pages_compact(self.handle, ctypes.byref(desc)))
+
+    def beam_select(self, desc: BeamDesc) -> None:
+        check(lib().qa_beam_select(self.handle, ctypes.byref(desc)))
+
     def layer_norm(self, desc: LayerNormDesc) -> None:
         check(lib().qa_layer_norm(self.handle, ctypes.byref(desc)))
 
@@ -576,6 +720,34 @@ def attention_paged_workspace(desc: PagedAttentionDesc) -> int:
     """qa_attention_paged_workspace (host): bytes of workspace for a call of desc's sizes."""
     size = ctypes.c_size_t()
     check(lib().qa_attention_paged_workspace(ctypes.byref(desc), ctypes.byref(size)))
+    return size.value
+
+
+def attention_paged_window_workspace(desc: PagedWindowDesc) -> int:
+    """qa_attention_paged_window_workspace (host)."""
+    size = ctypes.c_size_t()
+    check(lib().qa_attention_paged_window_workspace(ctypes.byref(desc), ctypes.byref(size)))
+    return size.value
+
+
+def pages_fork_workspace(desc: PagesForkDesc) -> int:
+    """qa_pages_fork_workspace (host)."""
+    size = ctypes.c_size_t()
+    check(lib().qa_pages_fork_workspace(ctypes.byref(desc), ctypes.byref(size)))
+    return size.value
+
+
+def pages_compact_workspace(desc: PagesCompactDesc) -> int:
+    """qa_pages_compact_workspace (host)."""
+    size = ctypes.c_size_t()
+    check(lib().qa_pages_compact_workspace(ctypes.byref(desc), ctypes.byref(size)))
+    return size.value
+
+
+def beam_select_workspace(desc: BeamDesc) -> int:
+    """qa_beam_select_workspace (host)."""
+    size = ctypes.c_size_t()
+    check(lib().qa_beam_select_workspace(ctypes.byref(desc), ctypes.byref(size)))
     return size.value
 
 

@@ -528,6 +528,166 @@ qa::PagedParams paged_params(const qa_paged_kv& kv, int64_t tokens) {
   return p;
 }
 
+qa::PagedAttnParams paged_attn_params(const qa_paged_attention_desc& d, int64_t window, int64_t sinks) {
+  qa::PagedAttnParams p{};
+  p.kv = paged_params(*d.kv, d.tokens);
+  p.nqh = d.nqh;
+  p.rep = d.nqh / d.kv->nkvh;
+  p.window = (int)window;
+  p.sinks = (int)sinks;
+  return p;
+}
+// qa_attention_paged, and with window > 0 qa_attention_paged_window.
+int attention_paged(const char* fn, qa_ctx* ctx, const qa_paged_attention_desc& d, int64_t window, int64_t sinks) {
+  if (d.flags) return fail(QA_EINVAL, "%s: flags must be 0", fn);
+  if (int rc = check_paged(fn, d.kv, d.dtype, d.tokens, d.nqh)) return rc;
+  const qa_paged_kv& kv = *d.kv;
+  const int64_t width = (int64_t)d.nqh * kv.hd;
+  if (d.ldq < width || d.ldq % 8 || d.ldo < width || d.ldo % 8)
+    return fail(QA_EINVAL, "%s: ldq and ldo must be >= nqh*hd and multiples of 8", fn);
+  if (!d.q || !d.out) return fail(QA_EINVAL, "%s: null pointer", fn);
+  if (!aligned(d.q, 16) || !aligned(d.out, 16) || !aligned(d.workspace, 16))
+    return fail(QA_EINVAL, "%s: buffers must be 16-byte aligned", fn);
+  qa::PagedAttnParams p = paged_attn_params(d, window, sinks);
+  const size_t need = qa::paged_attention_workspace(kv.dtype == QA_E4M3, kv.hd, p);
+  if (need && (!d.workspace || d.workspace_bytes < need))
+    return fail(QA_EINVAL, "%s: a workspace of %zu bytes is needed, %zu given", fn, need, d.workspace ? d.workspace_bytes : (size_t)0);
+  if (qa::paged_attention_blocks(kv.dtype == QA_E4M3, kv.hd, p) > kBlocks)
+    return fail(QA_EINVAL, "%s: the batch is too large for one launch", fn);
+  if (!ctx) return fail(QA_EINVAL, "%s: null context", fn);
+  if (d.tokens == 0 || kv.seqs == 0 || kv.max_rows == 0) return ok();
+  if (int rc = set_device(ctx)) return rc;
+  p.q = (const uint16_t*)d.q;
+  p.out = (uint16_t*)d.out;
+  p.ws = (float*)d.workspace;
+  p.ldq = d.ldq;
+  p.ldo = d.ldo;
+  p.scale = 1.0f / sqrtf((float)kv.hd);
+  const hipError_t e = qa::launch_attention_paged((int)d.dtype, kv.dtype == QA_E4M3, kv.hd, p, ctx->stream);
+  return e == hipSuccess ? ok() : fail(QA_EDEVICE, "%s launch: %s (%d)", fn, hipGetErrorString(e), (int)e);
+}
+int check_window(const char* fn, const qa_paged_window_desc& d) {
+  if (d.window < 1 || d.window > 1 << 30 || d.sinks < 0 || d.sinks > 1 << 30)
+    return fail(QA_EINVAL, "%s: need window in [1, 2^30] and sinks in [0, 2^30]", fn);
+  return ok();
+}
+qa_paged_attention_desc without_window(const qa_paged_window_desc& d) {
+  return {d.dtype, d.flags, d.tokens, d.nqh, d.q, d.ldq, d.kv, d.out, d.ldo, d.workspace, d.workspace_bytes};
+}
+
+bool bytes_overlap(const void* a, size_t an, const void* b, size_t bn) {
+  return an && bn && (uintptr_t)a < (uintptr_t)b + bn && (uintptr_t)b < (uintptr_t)a + an;
+}
+int check_planes(const char* fn, const qa_page_plane* planes, int64_t n, int64_t pages) {
+  if (pages <= 0 || pages > kI32) return fail(QA_EINVAL, "%s: the number of pages must be in (0, 2^31)", fn);
+  if (n < 0 || n > 65536) return fail(QA_EINVAL, "%s: nplanes must be in [0, 65536]", fn);
+  if (n && !planes) return fail(QA_EINVAL, "%s: null planes", fn);
+  for (int64_t i = 0; i < n; ++i) {
+    const int64_t b = planes[i].bytes;
+    if (b <= 0 || b > kI32 || b % 4 || (b % 16 && b > 4096))
+      return fail(QA_EINVAL, "%s: plane %lld has pages of %lld bytes (a multiple of 16, or of 4 up to 4096)", fn, (long long)i, (long long)b);
+    if (!planes[i].base || !aligned(planes[i].base, 16))
+      return fail(QA_EINVAL, "%s: plane %lld is null or not 16-byte aligned", fn, (long long)i);
+  }
+  return ok();
+}
+// The pairs' pages, in as many launches as the planes need.
+int copy_planes(const char* fn, qa_ctx* ctx, const qa_page_plane* src, const qa_page_plane* dst, int64_t n, const qa::PagesCopyParams& p) {
+  for (int64_t i0 = 0; i0 < n; i0 += qa::kPagePlanes) {
+    qa::PagePlanes planes{};
+    planes.n = (int)std::min<int64_t>(n - i0, qa::kPagePlanes);
+    for (int i = 0; i < planes.n; ++i)
+      planes.at[i] = {(const unsigned char*)src[i0 + i].base, (unsigned char*)dst[i0 + i].base, (uint32_t)src[i0 + i].bytes};
+    const hipError_t e = qa::launch_pages_copy(planes, p, ctx->stream);
+    if (e != hipSuccess) return fail(QA_EDEVICE, "%s launch: %s (%d)", fn, hipGetErrorString(e), (int)e);
+  }
+  return ok();
+}
+int check_fork_sizes(const char* fn, const qa_pages_fork_desc& d) {
+  if (d.page != 16 && d.page != 32 && d.page != 64) return fail(QA_EUNSUPPORTED, "%s: page=%d (16, 32 or 64)", fn, d.page);
+  if (d.num_pages <= 0 || d.num_pages > kI32) return fail(QA_EINVAL, "%s: num_pages must be in (0, 2^31)", fn);
+  if (d.src_seqs < 0 || d.seqs < 0 || d.ldtable < 0 || d.ldtable > kI32)
+    return fail(QA_EINVAL, "%s: src_seqs, seqs and ldtable must not be negative", fn);
+  if (d.src_seqs > qa::kForkSeqs || d.seqs > qa::kForkSeqs)
+    return fail(QA_EUNSUPPORTED, "%s: at most %d sequences", fn, qa::kForkSeqs);
+  if (d.src_seqs * d.ldtable > kI32 || d.seqs * d.ldtable > kI32) return fail(QA_EINVAL, "%s: a table has less than 2^31 entries", fn);
+  if (d.window < 0 || d.window > 1 << 30 || d.sinks < 0 || d.sinks > 1 << 30)
+    return fail(QA_EINVAL, "%s: window and sinks must be in [0, 2^30]", fn);
+  return ok();
+}
+qa::PagesForkParams fork_params(const qa_pages_fork_desc& d) {
+  qa::PagesForkParams p{};
+  p.src_table = d.src_table;
+  p.src_len = d.src_len;
+  p.parent = d.parent;
+  p.grow = d.grow;
+  p.refs = d.refs;
+  p.table = d.table;
+  p.len = d.len;
+  p.missing = d.missing;
+  p.num_pages = d.num_pages;
+  p.ldtable = d.ldtable;
+  p.src_seqs = (int)d.src_seqs;
+  p.seqs = (int)d.seqs;
+  p.lp = d.page == 16 ? 4 : d.page == 32 ? 5 : 6;
+  p.keep = (d.flags & QA_PAGES_KEEP) != 0;
+  p.window = d.window;
+  p.sinks = d.sinks;
+  p.ws = (int32_t*)d.workspace;
+  return p;
+}
+int check_compact_sizes(const char* fn, const qa_pages_compact_desc& d) {
+  if (d.num_pages <= 0 || d.num_pages > kI32) return fail(QA_EINVAL, "%s: num_pages must be in (0, 2^31)", fn);
+  if (d.seqs < 0 || d.seqs > kI32 || d.ldtable < 0 || d.ldtable > kI32 || d.seqs * d.ldtable > kI32)
+    return fail(QA_EINVAL, "%s: a table has less than 2^31 entries", fn);
+  return ok();
+}
+qa::PagesCompactParams compact_params(const qa_pages_compact_desc& d) {
+  qa::PagesCompactParams p{};
+  p.refs = d.refs;
+  p.table = d.table;
+  p.refs_out = d.refs_out;
+  p.table_out = d.table_out;
+  p.map = d.map;
+  p.used = d.used;
+  p.num_pages = d.num_pages;
+  p.entries = d.seqs * d.ldtable;
+  p.ws = (int32_t*)d.workspace;
+  return p;
+}
+int check_beam_sizes(const char* fn, const qa_beam_desc& d) {
+  if (d.dtype != QA_F16 && d.dtype != QA_BF16 && d.dtype != QA_F32)
+    return fail(QA_EINVAL, "%s: dtype %u is none of QA_F16, QA_BF16 and QA_F32", fn, d.dtype);
+  if (d.beams < 1 || d.beams > 64 || d.width < 1 || d.width > 64)
+    return fail(QA_EUNSUPPORTED, "%s: beams=%d and width=%d (1 to 64)", fn, d.beams, d.width);
+  if (d.groups < 0 || d.groups > kI32 / 64 || d.vocab < 1 || d.vocab > kI32)
+    return fail(QA_EINVAL, "%s: groups or vocab out of range", fn);
+  qa::BeamParams p{};
+  p.groups = d.groups;
+  p.beams = d.beams;
+  p.vocab = d.vocab;
+  if (qa::beam_select_blocks((int)d.dtype, p) > kBlocks) return fail(QA_EINVAL, "%s: the batch is too large for one launch", fn);
+  return ok();
+}
+qa::BeamParams beam_params(const qa_beam_desc& d) {
+  qa::BeamParams p{};
+  p.logits = d.logits;
+  p.score = d.score;
+  p.done = d.done;
+  p.parent = d.parent;
+  p.token = d.token;
+  p.done_out = d.done_out;
+  p.score_out = d.score_out;
+  p.groups = d.groups;
+  p.vocab = d.vocab;
+  p.ldl = d.ldl;
+  p.beams = d.beams;
+  p.width = d.width;
+  p.end = d.end;
+  p.ws = d.workspace;
+  return p;
+}
+
 // Launch a validated, planned projection with split-K partials in `ws`.
 int launch_linear(qa_ctx* ctx, const qa_linear_desc* d, const qa::Plan& plan, float* ws,
                   const NextLaunch& nl) {
@@ -992,46 +1152,155 @@ int qa_attention_paged_workspace(const qa_paged_attention_desc* d, size_t* bytes
   if (!d || !bytes) return fail(QA_EINVAL, "qa_attention_paged_workspace: null argument");
   *bytes = 0;
   if (int rc = check_paged_sizes("qa_attention_paged_workspace", d->kv, d->dtype, d->tokens, d->nqh)) return rc;
-  qa::PagedAttnParams p{};
-  p.kv = paged_params(*d->kv, d->tokens);
-  p.nqh = d->nqh;
-  p.rep = d->nqh / d->kv->nkvh;
-  *bytes = qa::paged_attention_workspace(d->kv->dtype == QA_E4M3, d->kv->hd, p);
+  *bytes = qa::paged_attention_workspace(d->kv->dtype == QA_E4M3, d->kv->hd, paged_attn_params(*d, 0, 0));
   return ok();
 }
 
 int qa_attention_paged(qa_ctx* ctx, const qa_paged_attention_desc* d) {
   if (!d) return fail(QA_EINVAL, "qa_attention_paged: null argument");
-  if (d->flags) return fail(QA_EINVAL, "qa_attention_paged: flags must be 0");
-  if (int rc = check_paged("qa_attention_paged", d->kv, d->dtype, d->tokens, d->nqh)) return rc;
-  const qa_paged_kv& kv = *d->kv;
-  const int64_t width = (int64_t)d->nqh * kv.hd;
-  if (d->ldq < width || d->ldq % 8 || d->ldo < width || d->ldo % 8)
-    return fail(QA_EINVAL, "qa_attention_paged: ldq and ldo must be >= nqh*hd and multiples of 8");
-  if (!d->q || !d->out) return fail(QA_EINVAL, "qa_attention_paged: null pointer");
-  if (!aligned(d->q, 16) || !aligned(d->out, 16) || !aligned(d->workspace, 16))
-    return fail(QA_EINVAL, "qa_attention_paged: buffers must be 16-byte aligned");
-  qa::PagedAttnParams p{};
-  p.kv = paged_params(kv, d->tokens);
-  p.nqh = d->nqh;
-  p.rep = d->nqh / kv.nkvh;
-  const size_t need = qa::paged_attention_workspace(kv.dtype == QA_E4M3, kv.hd, p);
-  if (need && (!d->workspace || d->workspace_bytes < need))
-    return fail(QA_EINVAL, "qa_attention_paged: a workspace of %zu bytes is needed, %zu given", need,
-                d->workspace ? d->workspace_bytes : (size_t)0);
-  if (qa::paged_attention_blocks(kv.dtype == QA_E4M3, kv.hd, p) > kBlocks)
-    return fail(QA_EINVAL, "qa_attention_paged: the batch is too large for one launch");
-  if (!ctx) return fail(QA_EINVAL, "qa_attention_paged: null context");
-  if (d->tokens == 0 || kv.seqs == 0 || kv.max_rows == 0) return ok();
+  return attention_paged("qa_attention_paged", ctx, *d, 0, 0);
+}
+
+int qa_attention_paged_window_workspace(const qa_paged_window_desc* d, size_t* bytes) {
+  if (!d || !bytes) return fail(QA_EINVAL, "qa_attention_paged_window_workspace: null argument");
+  *bytes = 0;
+  if (int rc = check_paged_sizes("qa_attention_paged_window_workspace", d->kv, d->dtype, d->tokens, d->nqh)) return rc;
+  if (int rc = check_window("qa_attention_paged_window_workspace", *d)) return rc;
+  *bytes = qa::paged_attention_workspace(d->kv->dtype == QA_E4M3, d->kv->hd, paged_attn_params(without_window(*d), d->window, d->sinks));
+  return ok();
+}
+
+int qa_attention_paged_window(qa_ctx* ctx, const qa_paged_window_desc* d) {
+  if (!d) return fail(QA_EINVAL, "qa_attention_paged_window: null argument");
+  if (int rc = check_window("qa_attention_paged_window", *d)) return rc;
+  return attention_paged("qa_attention_paged_window", ctx, without_window(*d), d->window, d->sinks);
+}
+
+int qa_pages_copy(qa_ctx* ctx, const qa_pages_copy_desc* d) {
+  if (!d) return fail(QA_EINVAL, "qa_pages_copy: null argument");
+  if (d->flags) return fail(QA_EINVAL, "qa_pages_copy: flags must be 0");
+  if (int rc = check_planes("qa_pages_copy", d->src, d->nplanes, d->src_pages)) return rc;
+  if (int rc = check_planes("qa_pages_copy", d->dst, d->nplanes, d->dst_pages)) return rc;
+  for (int64_t i = 0; i < d->nplanes; ++i)
+    if (d->src[i].bytes != d->dst[i].bytes)
+      return fail(QA_EINVAL, "qa_pages_copy: plane %lld has pages of %lld and %lld bytes", (long long)i, (long long)d->src[i].bytes,
+                  (long long)d->dst[i].bytes);
+  if (d->npairs < 0 || d->npairs > kI32) return fail(QA_EINVAL, "qa_pages_copy: npairs must be in [0, 2^31)");
+  if (d->npairs && !d->pairs) return fail(QA_EINVAL, "qa_pages_copy: null pointer");
+  if (!aligned(d->pairs, 4)) return fail(QA_EINVAL, "qa_pages_copy: misaligned pointer");
+  if (!ctx) return fail(QA_EINVAL, "qa_pages_copy: null context");
+  if (d->npairs == 0 || d->nplanes == 0) return ok();
   if (int rc = set_device(ctx)) return rc;
-  p.q = (const uint16_t*)d->q;
-  p.out = (uint16_t*)d->out;
-  p.ws = (float*)d->workspace;
-  p.ldq = d->ldq;
-  p.ldo = d->ldo;
-  p.scale = 1.0f / sqrtf((float)kv.hd);
-  const hipError_t e = qa::launch_attention_paged((int)d->dtype, kv.dtype == QA_E4M3, kv.hd, p, ctx->stream);
-  return e == hipSuccess ? ok() : hip_fail(e, "qa_attention_paged launch");
+  return copy_planes("qa_pages_copy", ctx, d->src, d->dst, d->nplanes, {d->pairs, d->npairs, nullptr, d->src_pages, d->dst_pages});
+}
+
+int qa_pages_fork_workspace(const qa_pages_fork_desc* d, size_t* bytes) {
+  if (!d || !bytes) return fail(QA_EINVAL, "qa_pages_fork_workspace: null argument");
+  *bytes = 0;
+  if (int rc = check_fork_sizes("qa_pages_fork_workspace", *d)) return rc;
+  *bytes = qa::pages_fork_workspace(fork_params(*d));
+  return ok();
+}
+
+int qa_pages_fork(qa_ctx* ctx, const qa_pages_fork_desc* d) {
+  if (!d) return fail(QA_EINVAL, "qa_pages_fork: null argument");
+  if (d->flags & ~(uint32_t)QA_PAGES_KEEP)
+    return fail(QA_EINVAL, "qa_pages_fork: unknown flags 0x%x", d->flags & ~(uint32_t)QA_PAGES_KEEP);
+  if (int rc = check_fork_sizes("qa_pages_fork", *d)) return rc;
+  if (int rc = check_planes("qa_pages_fork", d->planes, d->nplanes, d->num_pages)) return rc;
+  const bool from = d->src_seqs > 0, to = d->seqs > 0, any = d->ldtable > 0;
+  if (!d->refs || !d->missing || (from && (!d->src_len || (any && !d->src_table))) || (to && (!d->parent || !d->len || (any && !d->table))))
+    return fail(QA_EINVAL, "qa_pages_fork: null pointer");
+  if (!aligned(d->refs, 4) || !aligned(d->missing, 4) || !aligned(d->src_table, 4) || !aligned(d->src_len, 4) || !aligned(d->parent, 4) ||
+      !aligned(d->table, 4) || !aligned(d->len, 4) || !aligned(d->grow, 4) || !aligned(d->workspace, 16))
+    return fail(QA_EINVAL, "qa_pages_fork: misaligned pointer (the workspace 16-byte aligned)");
+  const size_t rows = (size_t)d->ldtable * 4;
+  if (bytes_overlap(d->src_table, d->src_seqs * rows, d->table, d->seqs * rows) || bytes_overlap(d->src_len, (size_t)d->src_seqs * 4, d->len, (size_t)d->seqs * 4))
+    return fail(QA_EINVAL, "qa_pages_fork: table and len may be no part of the sources");
+  const qa::PagesForkParams p = fork_params(*d);
+  const size_t need = qa::pages_fork_workspace(p);
+  if (!d->workspace || d->workspace_bytes < need)
+    return fail(QA_EINVAL, "qa_pages_fork: a workspace of %zu bytes is needed, %zu given", need, d->workspace ? d->workspace_bytes : (size_t)0);
+  if (!ctx) return fail(QA_EINVAL, "qa_pages_fork: null context");
+  if (int rc = set_device(ctx)) return rc;
+  qa::PagesCopyParams moves{};
+  const hipError_t e = qa::launch_pages_fork(p, &moves, ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, "qa_pages_fork launch");
+  return copy_planes("qa_pages_fork", ctx, d->planes, d->planes, d->nplanes, moves);
+}
+
+int qa_pages_compact_workspace(const qa_pages_compact_desc* d, size_t* bytes) {
+  if (!d || !bytes) return fail(QA_EINVAL, "qa_pages_compact_workspace: null argument");
+  *bytes = 0;
+  if (int rc = check_compact_sizes("qa_pages_compact_workspace", *d)) return rc;
+  *bytes = qa::pages_compact_workspace(compact_params(*d));
+  return ok();
+}
+
+int qa_pages_compact(qa_ctx* ctx, const qa_pages_compact_desc* d) {
+  if (!d) return fail(QA_EINVAL, "qa_pages_compact: null argument");
+  if (d->flags) return fail(QA_EINVAL, "qa_pages_compact: flags must be 0");
+  if (int rc = check_compact_sizes("qa_pages_compact", *d)) return rc;
+  if (int rc = check_planes("qa_pages_compact", d->planes, d->nplanes, d->num_pages)) return rc;
+  const size_t entries = (size_t)(d->seqs * d->ldtable) * 4;
+  if (!d->refs || !d->refs_out || !d->used || (entries && (!d->table || !d->table_out)))
+    return fail(QA_EINVAL, "qa_pages_compact: null pointer");
+  if (!aligned(d->refs, 4) || !aligned(d->refs_out, 4) || !aligned(d->used, 4) || !aligned(d->table, 4) || !aligned(d->table_out, 4) ||
+      !aligned(d->map, 4) || !aligned(d->workspace, 16))
+    return fail(QA_EINVAL, "qa_pages_compact: misaligned pointer (the workspace 16-byte aligned)");
+  const size_t list = (size_t)d->num_pages * 4;
+  if ((d->refs != d->refs_out && bytes_overlap(d->refs, list, d->refs_out, list)) ||
+      (d->table != d->table_out && bytes_overlap(d->table, entries, d->table_out, entries)))
+    return fail(QA_EINVAL, "qa_pages_compact: refs_out and table_out are refs and table, or no part of them");
+  const qa::PagesCompactParams p = compact_params(*d);
+  const size_t need = qa::pages_compact_workspace(p);
+  if (!d->workspace || d->workspace_bytes < need)
+    return fail(QA_EINVAL, "qa_pages_compact: a workspace of %zu bytes is needed, %zu given", need, d->workspace ? d->workspace_bytes : (size_t)0);
+  if (!ctx) return fail(QA_EINVAL, "qa_pages_compact: null context");
+  if (int rc = set_device(ctx)) return rc;
+  qa::PagesCopyParams moves{};
+  const hipError_t e = qa::launch_pages_compact(p, &moves, ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, "qa_pages_compact launch");
+  return copy_planes("qa_pages_compact", ctx, d->planes, d->planes, d->nplanes, moves);
+}
+
+int qa_beam_select_workspace(const qa_beam_desc* d, size_t* bytes) {
+  if (!d || !bytes) return fail(QA_EINVAL, "qa_beam_select_workspace: null argument");
+  *bytes = 0;
+  if (int rc = check_beam_sizes("qa_beam_select_workspace", *d)) return rc;
+  *bytes = qa::beam_select_workspace((int)d->dtype, beam_params(*d));
+  return ok();
+}
+
+int qa_beam_select(qa_ctx* ctx, const qa_beam_desc* d) {
+  if (!d) return fail(QA_EINVAL, "qa_beam_select: null argument");
+  if (d->flags) return fail(QA_EINVAL, "qa_beam_select: flags must be 0");
+  if (int rc = check_beam_sizes("qa_beam_select", *d)) return rc;
+  const int64_t unit = d->dtype == QA_F32 ? 4 : 8;
+  if (d->ldl < d->vocab || d->ldl % unit || d->ldl > ((int64_t)1 << 40))
+    return fail(QA_EINVAL, "qa_beam_select: ldl must be >= vocab and a multiple of %d", (int)unit);
+  if (d->end < -1 || d->end >= d->vocab || (d->end < 0 && d->done))
+    return fail(QA_EINVAL, "qa_beam_select: end must be a token, or -1 without done");
+  if (!d->logits || !d->score || !d->parent || !d->token || !d->score_out || !d->done_out)
+    return fail(QA_EINVAL, "qa_beam_select: null pointer");
+  if (!aligned(d->logits, 16) || !aligned(d->workspace, 16) || !aligned(d->score, 4) || !aligned(d->done, 4) || !aligned(d->parent, 4) ||
+      !aligned(d->token, 4) || !aligned(d->score_out, 4) || !aligned(d->done_out, 4))
+    return fail(QA_EINVAL, "qa_beam_select: misaligned pointer (logits and the workspace 16-byte aligned)");
+  const qa::BeamParams p = beam_params(*d);
+  const size_t need = qa::beam_select_workspace((int)d->dtype, p);
+  if (need && (!d->workspace || d->workspace_bytes < need))
+    return fail(QA_EINVAL, "qa_beam_select: a workspace of %zu bytes is needed, %zu given", need, d->workspace ? d->workspace_bytes : (size_t)0);
+  const size_t in = (size_t)(d->groups * d->beams) * 4, out = (size_t)(d->groups * d->width) * 4;
+  const void* const ins[] = {d->score, d->done};
+  const void* const outs[] = {d->parent, d->token, d->score_out, d->done_out};
+  for (const void* a : ins)
+    for (const void* b : outs)
+      if (a && bytes_overlap(a, in, b, out)) return fail(QA_EINVAL, "qa_beam_select: the outputs may be no part of score or done");
+  if (!ctx) return fail(QA_EINVAL, "qa_beam_select: null context");
+  if (d->groups == 0) return ok();
+  if (int rc = set_device(ctx)) return rc;
+  const hipError_t e = qa::launch_beam_select((int)d->dtype, p, ctx->stream);
+  return e == hipSuccess ? ok() : hip_fail(e, "qa_beam_select launch");
 }
 
 int qa_conv2d_3x3s2(qa_ctx* ctx, const qa_conv_desc* d) {

@@ -380,6 +380,7 @@ struct PagedAttnParams {
   float* ws;
   int64_t ldq, ldo;
   int nqh, rep;  // rep = nqh / nkvh
+  int window, sinks;  // window 0: a row sees all keys up to its own
   float scale;
   PagedParams kv;
 };
@@ -387,6 +388,60 @@ struct PagedAttnParams {
 int64_t paged_attention_blocks(bool e4m3, int hd, const PagedAttnParams& p);
 size_t paged_attention_workspace(bool e4m3, int hd, const PagedAttnParams& p);
 hipError_t launch_attention_paged(int dtype, bool e4m3, int hd, const PagedAttnParams& p, hipStream_t s);
+
+// qa_pages_copy, qa_pages_fork and qa_pages_compact (qa_pages.hip).
+constexpr int kPagePlanes = 128;  // of one launch: kernel arguments have 4 KB
+struct PagePlanes {
+  int n;
+  struct {
+    const unsigned char* src;
+    unsigned char* dst;
+    uint32_t bytes;  // of a page
+  } at[kPagePlanes];
+};
+struct PagesCopyParams {
+  const int32_t* pairs;  // [count][2]
+  int64_t npairs;        // pairs at most
+  const int32_t* count;  // how many there are, or nullptr: npairs
+  int64_t src_pages, dst_pages;
+};
+constexpr int kForkSeqs = 8192;  // sequences, and sources, of a call at most
+struct PagesForkParams {
+  const int32_t *src_table, *src_len, *parent, *grow;
+  int32_t *refs, *table, *len, *missing;
+  int64_t num_pages, ldtable;
+  int src_seqs, seqs, lp, keep;
+  int64_t window, sinks;
+  int32_t* ws;
+};
+struct PagesCompactParams {
+  const int32_t *refs, *table;
+  int32_t *refs_out, *table_out, *map, *used;
+  int64_t num_pages, entries;  // entries of the table
+  int32_t* ws;
+};
+size_t pages_fork_workspace(const PagesForkParams& p);
+size_t pages_compact_workspace(const PagesCompactParams& p);
+// The planes' pages are moved by launch_pages_copy behind the other two, with the
+// pairs and their number in the workspace.
+hipError_t launch_pages_copy(const PagePlanes& planes, const PagesCopyParams& p, hipStream_t s);
+hipError_t launch_pages_fork(const PagesForkParams& p, PagesCopyParams* moves, hipStream_t s);
+hipError_t launch_pages_compact(const PagesCompactParams& p, PagesCopyParams* moves, hipStream_t s);
+
+// qa_beam_select (qa_beam.hip).
+struct BeamParams {
+  const void* logits;
+  const float* score;
+  const int32_t* done;
+  int32_t *parent, *token, *done_out;
+  float* score_out;
+  int64_t groups, vocab, ldl;
+  int beams, width, end;
+  void* ws;
+};
+size_t beam_select_workspace(int dtype, const BeamParams& p);
+int64_t beam_select_blocks(int dtype, const BeamParams& p);
+hipError_t launch_beam_select(int dtype, const BeamParams& p, hipStream_t s);
 
 // p16: probabilities rounded once to the 16-bit format (else two 16-bit terms).
 hipError_t launch_attention(int dtype, const AttnParams& p, bool p16, hipStream_t stream);

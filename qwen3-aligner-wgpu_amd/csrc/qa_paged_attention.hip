@@ -220,9 +220,20 @@ struct Split {
   int64_t few_parts, many_parts;  // partial results of either kind in the workspace
 };
 
+// Keys that a tile of `rows` rows goes through at most, blocks of the sinks and the window's
+// ends in full (Reach).
+int64_t keys_at_most(const PagedAttnParams& p, int64_t rows) {
+  const int64_t len = p.kv.max_len > 1 ? p.kv.max_len : 1;
+  if (p.window <= 0) return len;
+  rows = rows < p.kv.max_rows ? rows : p.kv.max_rows;
+  const int64_t most = (((int64_t)p.sinks + 63) & ~(int64_t)63) + p.window + rows + 62;
+  return most < len ? most : len;
+}
+
 Split split_of(const PagedAttnParams& p, bool e4m3, int hd) {
   Split s{};
-  const int64_t rows = (int64_t)p.kv.max_rows * p.rep, len = p.kv.max_len > 1 ? p.kv.max_len : 1;
+  const int64_t rows = (int64_t)p.kv.max_rows * p.rep;
+  int64_t len = keys_at_most(p, kFewRows / p.rep);
   const int64_t heads = (int64_t)p.kv.seqs * p.kv.nkvh;
   auto divide = [&](int64_t parts, int64_t least, int* chunk, int* chunks) {
     int64_t c = (len + parts - 1) / parts;
@@ -265,6 +276,7 @@ Split split_of(const PagedAttnParams& p, bool e4m3, int hd) {
     s.many_rows = about(64) > 600 ? 128 : 64;
     s.tiles = (int)(pairs / s.many_rows + ends < most(s.many_rows) ? pairs / s.many_rows + ends : most(s.many_rows));
     const int64_t blocks = about(s.many_rows);
+    len = keys_at_most(p, s.many_rows / p.rep + 2);
     divide(len > 640 && blocks > 0 && blocks < kCus ? kCus / blocks : 1, 256, &s.many_chunk, &s.many_chunks);
   }
   s.few_pairs = (int)(rows < kFewRows ? rows : kFewRows);
@@ -287,6 +299,27 @@ __device__ __forceinline__ int64_t part_index(const PagedAttnParams& p, const Sp
 __device__ __forceinline__ float* part_stats(const PagedAttnParams& p, const Split& sp, int hd) {
   return p.ws + (sp.few_parts + sp.many_parts) * hd;
 }
+
+// With a window, a tile goes through the blocks of 64 keys that its rows see, those of
+// the sinks and from the one that the first row's window begins in, as one run of keys:
+// key number v of it is the sequence's key(v).  Without, key(v) is v.
+template <bool WIN>
+struct Reach {
+  int near = 0, front = 0, skip = 0, sinks = 0;  // the window's first key; keys of the sinks' blocks; keys left out behind them
+  __device__ __forceinline__ Reach(const PagedAttnParams& p, int first_pos) {
+    if constexpr (WIN) {
+      sinks = p.sinks;
+      near = max(max(first_pos, 0) - p.window + 1, 0);
+      front = (p.sinks + 63) & ~63;
+      skip = max((near & ~63) - front, 0);
+    }
+  }
+  __device__ __forceinline__ int key(int v) const { return WIN && v >= front ? v + skip : v; }
+  // whether some row sees one of `n` keys, n a power of two, around key k: a block's, a page's
+  __device__ __forceinline__ bool sees(int k, int n) const { return !WIN || (k | (n - 1)) >= near || (k & -n) < sinks; }
+};
+// The first of the keys from kg on that a row at `pos` sees through its window; those below `sinks - kg` it sees all the same.
+__device__ __forceinline__ int window_from(const PagedAttnParams& p, int pos, int kg) { return max(pos, 0) - p.window + 1 - kg; }
 
 // The (row, head) pair of a lane's column; columns past the last repeat it and store
 // nothing.
@@ -352,6 +385,7 @@ __device__ __forceinline__ void each(F f, std::integer_sequence<int, I...>) {
 // zeros (a resource of no bytes).  W32: in the order for the 32-row products below.
 template <int DT, bool F8, int HD, bool W32, int OF, int LP, bool K>
 __device__ __forceinline__ void load_tile(const PagedParams& kv, const Pages& pages, int j, int mine, unsigned char* to) {
+#if defined(__HIP_DEVICE_COMPILE__)  // (the host's pass knows no buffer resources)
   using C = Cfg<DT, F8, HD>;
   constexpr int PER = C::LI >> (6 - LP), PB = HD * C::ES << LP;  // instructions and bytes of a page
   constexpr int CW = K ? C::CR : (1 << LP) * C::ES / 16;          // chunks of a row
@@ -396,6 +430,7 @@ __device__ __forceinline__ void load_tile(const PagedParams& kv, const Pages& pa
     }
   };
   each(one, std::make_integer_sequence<int, C::LI / OF>{});
+#endif
 }
 // Fragment addresses in the tiles.  K: product t reads row 16 (c / 4) + 4 t + c % 4,
 // slice e the chunk 4 e + g.  V: row d, the chunks of keys 16 g ..
@@ -413,9 +448,9 @@ __device__ __forceinline__ int v_frag(int c, int g, int e, int lcp) {
 // Mask, online softmax and the 16-bit terms of P.  `have`: how many of the
 // lane's 16 keys from kg on some row of the sequence sees (on a page); `f`: the scores'
 // factor, log2 e / sqrt(hd) and the K scale; `vs`: the V scale.
-template <int DT, bool F8, int HD>
-__device__ __forceinline__ void softmax(f32x4 (&sc)[4], int pos, int kg, int have, float f, float vs, float& m, float& l, f32x4 (&o)[HD / 16],
-                                        u32x4 (&ph)[2], u32x4 (&pl)[2], u32x4 (&pm)[2]) {
+template <int DT, bool F8, int HD, bool WIN>
+__device__ __forceinline__ void softmax(const PagedAttnParams& p, f32x4 (&sc)[4], int pos, int kg, int have, float f, float vs, float& m, float& l,
+                                        f32x4 (&o)[HD / 16], u32x4 (&ph)[2], u32x4 (&pl)[2], u32x4 (&pm)[2]) {
   using C = Cfg<DT, F8, HD>;
   const int see = min(have, pos + 1 - kg);
   if (__builtin_amdgcn_ballot_w64(see < 16)) {
@@ -424,6 +459,16 @@ __device__ __forceinline__ void softmax(f32x4 (&sc)[4], int pos, int kg, int hav
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (4 * t + e >= see) sc[t][e] = -INFINITY;
+  }
+  if constexpr (WIN) {
+    const int from = window_from(p, pos, kg), sink = p.sinks - kg;
+    if (__builtin_amdgcn_ballot_w64(from > max(sink, 0))) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (4 * t + e < from && 4 * t + e >= sink) sc[t][e] = -INFINITY;
+    }
   }
   float x[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -466,15 +511,32 @@ __device__ __forceinline__ uint32_t tail_mask(int left, int w) {
   const int n = left - w * (4 / ES);
   return n >= 4 / ES ? ~0u : n <= 0 ? 0u : (1u << (8 * ES * n)) - 1;
 }
-// What a V tile holds behind the keys that rows see, or for no page, may be anything, NaN
+// ... of which those in front of `from` are not seen either, but for the first `sink`.
+struct Seen {
+  int have, from, sink;
+};
+template <bool WIN>
+__device__ __forceinline__ Seen seen_of(const Reach<WIN>& r, int have, int kg) {
+  return {have, WIN ? r.near - kg : 0, WIN ? r.sinks - kg : 0};
+}
+template <bool WIN>
+__device__ __forceinline__ bool some_unseen(const Seen& s) {
+  return s.have < 16 || (WIN && s.from > max(s.sink, 0));
+}
+template <int ES, bool WIN>
+__device__ __forceinline__ uint32_t seen_mask(const Seen& s, int first, int w) {
+  const uint32_t m = tail_mask<ES>(s.have - first, w);
+  return WIN ? m & (~tail_mask<ES>(s.from - first, w) | tail_mask<ES>(s.sink - first, w)) : m;
+}
+// What a V tile holds where no row sees it, or for no page, may be anything, NaN
 // too, and 0 * NaN is not 0: a lane clears those elements of the chunks that it
 // will read itself.
-template <int DT, bool F8, int HD>
-__device__ __forceinline__ void clear_tail(unsigned char* vt, const int (&va)[Cfg<DT, F8, HD>::VS], int lcp, int have) {
+template <int DT, bool F8, int HD, bool WIN>
+__device__ __forceinline__ void clear_unseen(unsigned char* vt, const int (&va)[Cfg<DT, F8, HD>::VS], int lcp, const Seen& seen) {
   using C = Cfg<DT, F8, HD>;
   uint32_t keep[C::VS * 4];
 #pragma unroll
-  for (int w = 0; w < C::VS * 4; ++w) keep[w] = tail_mask<C::ES>(have, w);
+  for (int w = 0; w < C::VS * 4; ++w) keep[w] = seen_mask<C::ES, WIN>(seen, 0, w);
 #pragma unroll 1
   for (int d = 0; d < C::ND; ++d)
 #pragma unroll
@@ -604,11 +666,12 @@ __device__ __forceinline__ int page_ids(const PagedParams& kv, int s, Key key) {
   const int lane = threadIdx.x & 63;
   return page_at(kv, s, key(lane >> 2) + 16 * (lane & 3));
 }
-template <bool F8, int HD, class Key>
-__device__ __forceinline__ void fetch_pages(const PagedParams& kv, const SeqSpan& sq, int found, int h, int left, Key key, Pages* pages,
-                                            float* ks, float* vs, bool* holes) {
+// A page that no row sees any key of is none, and no hole either.
+template <bool F8, int HD, bool WIN, class Key>
+__device__ __forceinline__ void fetch_pages(const PagedParams& kv, const SeqSpan& sq, const Reach<WIN>& reach, int found, int h, int left, Key key,
+                                            Pages* pages, float* ks, float* vs, bool* holes) {
   const int lane = threadIdx.x & 63, pos = key(lane >> 2) + 16 * (lane & 3);
-  const bool in = (lane >> 2) < left && pos < sq.seen();
+  const bool in = (lane >> 2) < left && pos < sq.seen() && reach.sees(pos, 1 << kv.lp);
   const int id = in ? found : -1;
   *holes |= __builtin_amdgcn_ballot_w64(in && id < 0) != 0;
   const int64_t at = id < 0 ? -1 : page_base(kv, id, h, HD) * (F8 ? 1 : 2);
@@ -645,18 +708,21 @@ constexpr int few_lds() {
   constexpr int tiles = kFewWaves * 2 * Cfg<DT, F8, HD>::TILE, join = kFewWaves * 64 * (HD + 8);
   return tiles > join ? tiles : join;
 }
-template <int DT, bool F8, int HD, int LP>
+template <int DT, bool F8, int HD, int LP, bool WIN>
 __device__ __forceinline__ void few_block(const PagedAttnParams& p, const Split& sp, int block, unsigned char* smem) {
   using C = Cfg<DT, F8, HD>;
   const PagedParams& kv = p.kv;
   const int h = block % kv.nkvh;
   const int part = block / kv.nkvh % sp.few_chunks, s = block / kv.nkvh / sp.few_chunks;
   const int wave = scalar((int)(threadIdx.x >> 6)), k0 = part * sp.few_chunk;
-  auto key_of = [&](int it) { return k0 + (wave + it * kFewWaves) * 64; };
-  const int found = page_ids(kv, s, key_of);
+  int found;
+  if constexpr (!WIN) found = page_ids(kv, s, [&](int it) { return k0 + (wave + it * kFewWaves) * 64; });
   const SeqSpan sq = seq_span(kv, s);
   if (sq.n == 0 || sq.n * p.rep > kFewRows) return;
-  const int end = sq.seen();
+  const Reach<WIN> reach(p, sq.pos0);
+  auto key_of = [&](int it) { return reach.key(k0 + (wave + it * kFewWaves) * 64); };
+  if constexpr (WIN) found = page_ids(kv, s, key_of);
+  const int end = sq.seen() - reach.skip;
   const int k1 = min(k0 + sp.few_chunk, end);
   if (part > 0 && k0 >= end) return;
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
@@ -667,7 +733,7 @@ __device__ __forceinline__ void few_block(const PagedAttnParams& p, const Split&
   float ksc = 1.f, vsc = 0.f;
   bool holes = false;
   auto fetch = [&](int it, int ids) {
-    fetch_pages<F8, HD>(kv, sq, ids, h, steps - it, [&](int j) { return key_of(it + j); }, &pages, &ksc, &vsc, &holes);
+    fetch_pages<F8, HD>(kv, sq, reach, ids, h, steps - it, [&](int j) { return key_of(it + j); }, &pages, &ksc, &vsc, &holes);
   };
   Column col;
   col.set(p, sq, h, c);
@@ -704,10 +770,11 @@ __device__ __forceinline__ void few_block(const PagedAttnParams& p, const Split&
       if ((it & 15) == 15) fetch(it + 1, page_ids(kv, s, [&](int j) { return key_of(it + 1 + j); }));
       load_tile<DT, F8, HD, false, 1, LP, true>(kv, pages, (it + 1) & 15, 0, kt);
     }
-    softmax<DT, F8, HD>(sc, col.pos, kg, have, p.scale * kLog2e * ks, vs, m, l, o, ph, pl, pm);
+    softmax<DT, F8, HD, WIN>(p, sc, col.pos, kg, have, p.scale * kLog2e * ks, vs, m, l, o, ph, pl, pm);
     if (more) wait_vmcnt<C::LI>();  // V is there; the next K's loads came after it
     else wait_vmcnt<0>();
-    if (__builtin_amdgcn_ballot_w64(have < 16)) clear_tail<DT, F8, HD>(vt, va, lcp, have);
+    const Seen seen = seen_of(reach, have, kg);
+    if (__builtin_amdgcn_ballot_w64(some_unseen<WIN>(seen))) clear_unseen<DT, F8, HD, WIN>(vt, va, lcp, seen);
     multiply_v<DT, F8, HD>(vt, va, lcp, ph, pl, pm, o);
     wait_lds();
     if (more) load_tile<DT, F8, HD, false, 1, LP, false>(kv, pages, (it + 1) & 15, 0, vt);
@@ -716,10 +783,10 @@ __device__ __forceinline__ void few_block(const PagedAttnParams& p, const Split&
   finish<DT, HD>(p, sp, sq, s, h, part, end <= sp.few_chunk, m, l, o, smem);
 }
 
-template <int DT, bool F8, int HD, int LP>
+template <int DT, bool F8, int HD, int LP, bool WIN>
 __global__ void __launch_bounds__(64 * kFewWaves) paged_few_kernel(const PagedAttnParams p, const Split sp) {
   __shared__ __attribute__((aligned(1024))) unsigned char smem[few_lds<DT, F8, HD>()];
-  few_block<DT, F8, HD, LP>(p, sp, (int)blockIdx.x, smem);
+  few_block<DT, F8, HD, LP, WIN>(p, sp, (int)blockIdx.x, smem);
 }
 
 // ---- tiles of 64 or 128 (row, head) pairs ----
@@ -828,8 +895,8 @@ __device__ __forceinline__ void multiply32(const unsigned char* vt, const int (&
 
 // softmax() for a lane with one column and keys kg + 16 h .., kg + 32 + 16 h .. (two
 // runs of 16, a page each).
-template <int DT, bool F8, int HD>
-__device__ __forceinline__ void softmax32(f32x16 (&sc)[2], int pos, int kg, const int (&have)[2], const float (&f)[2],
+template <int DT, bool F8, int HD, bool WIN>
+__device__ __forceinline__ void softmax32(const PagedAttnParams& p, f32x16 (&sc)[2], int pos, int kg, const int (&have)[2], const float (&f)[2],
                                           const float (&vs)[2], float& m, float& l, f32x16 (&o)[HD / 32],
                                           u32x4 (&ph)[2][2], u32x4 (&pl)[2][2], u32x4 (&pm)[2][2]) {
   using C = Cfg<DT, F8, HD>;
@@ -841,6 +908,14 @@ __device__ __forceinline__ void softmax32(f32x16 (&sc)[2], int pos, int kg, cons
 #pragma unroll
       for (int e = 0; e < 16; ++e)
         if (e >= see) sc[u][e] = -INFINITY;
+    }
+    if constexpr (WIN) {
+      const int from = window_from(p, pos, kg + 32 * u), sink = p.sinks - kg - 32 * u;
+      if (__builtin_amdgcn_ballot_w64(from > max(sink, 0))) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (e < from && e >= sink) sc[u][e] = -INFINITY;
+      }
     }
     float x[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -932,7 +1007,7 @@ __device__ __forceinline__ bool find_tile(const PagedAttnParams& p, const Split&
   }
   return false;
 }
-template <int DT, bool F8, int HD, int LP, int GW>
+template <int DT, bool F8, int HD, int LP, int GW, bool WIN>
 __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const PagedAttnParams p, const Split sp) {
   using C = Cfg<DT, F8, HD>;
   constexpr int NS = kManyWaves / GW, NB = many_buffers<DT, F8, HD, GW>(), WL = C::LI / GW;  // WL: a wave's loads of a tile
@@ -942,7 +1017,7 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
   const int mine = (int)blockIdx.x - sp.tiles * sp.many_chunks * kv.nkvh;
   if (mine >= 0) {  // behind them, the blocks of the sequences of few rows, four waves each
     // (the other waves end here, and a barrier waits for no wave that has ended)
-    if (threadIdx.x < 64 * kFewWaves) few_block<DT, F8, HD, LP>(p, sp, mine, smem);
+    if (threadIdx.x < 64 * kFewWaves) few_block<DT, F8, HD, LP, WIN>(p, sp, mine, smem);
     return;
   }
   const int kvh = (int)(blockIdx.x % kv.nkvh);
@@ -951,7 +1026,8 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
   SeqSpan sq;
   if (!find_tile<TR>(p, sp, blockIdx.x / kv.nkvh % sp.tiles, &s, &sq, &tile)) return;
   const int NR = sq.n * p.rep;
-  const int end = sq.pos0 + (min((tile + 1) * TR, NR) - 1) / p.rep + 1;
+  const Reach<WIN> reach(p, sq.pos0 + tile * TR / p.rep);
+  const int end = sq.pos0 + (min((tile + 1) * TR, NR) - 1) / p.rep + 1 - reach.skip;
   const int k0 = part * sp.many_chunk, k1 = min(k0 + sp.many_chunk, end);
   if (part > 0 && k0 >= end) return;
   // (the wave's number is left to the compiler as a lane's value: with scalar
@@ -959,7 +1035,7 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 31, h = lane >> 5;
   const int ns = wave / GW, wg = wave % GW, off = ns / (NS / 2);
   const int nb = k1 > k0 ? (k1 - k0 + 63) >> 6 : 0, steps = (nb - ns + NS - 1) / NS;
-  auto key_of = [&](int it) { return k0 + (ns + it * NS) * 64; };
+  auto key_of = [&](int it) { return reach.key(k0 + (ns + it * NS) * 64); };
   unsigned char* base = smem + ns * 2 * NB * C::TILE;
   auto kt = [&](int it) { return base + (it & (NB - 1)) * C::TILE; };
   auto vt = [&](int it) { return base + (NB + (it & (NB - 1))) * C::TILE; };
@@ -972,7 +1048,7 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
     Pages pg = {-1, -1};
     float x = 1.f, y = 0.f;
     auto key = [&](int j) { return key_of(16 * w + j); };
-    fetch_pages<F8, HD>(kv, sq, page_ids(kv, s, key), kvh, steps - 16 * w, key, &pg, &x, &y, &holes);
+    fetch_pages<F8, HD>(kv, sq, reach, page_ids(kv, s, key), kvh, steps - 16 * w, key, &pg, &x, &y, &holes);
     pages0.lo = w & 1 ? pages0.lo : pg.lo;
     pages0.hi = w & 1 ? pages0.hi : pg.hi;
     ks0 = w & 1 ? ks0 : x;
@@ -1045,6 +1121,7 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
     va[e] = ((((x >> lcp) * HD + c) << lcp) + ((x & (cp - 1)) ^ (c >> (4 - lcp) & (cp - 1)))) * 16;
   }
   int have[2] = {16, 16};  // the lane's keys in the block of the last softmax
+  int last_kg = 0;         // and the first of them
   const int n0 = (nb + NS - 1) / NS, n1 = (nb + NS / 2 - 1) / NS;  // most steps of either half
   const int phases = max(2 * n0 + 1, 2 * n1 + 2);
   if (off == 0) wait_vmcnt<0>();
@@ -1053,16 +1130,19 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
     const int my = ph_no - off, it = my >> 1;
     if (my >= 0 && my <= 2 * steps) {
       if ((my & 1) == 0) {
-        if (it > 0 && __builtin_amdgcn_ballot_w64(min(have[0], have[1]) < 16)) {
-          // V behind the keys that rows see, or for no page, may be anything, NaN too: a
+        const Seen seen[2] = {seen_of(reach, have[0], last_kg), seen_of(reach, have[1], last_kg + 32)};
+        if (it > 0 && __builtin_amdgcn_ballot_w64(some_unseen<WIN>(seen[0]) || some_unseen<WIN>(seen[1]))) {
+          // V where no row sees it, or for no page, may be anything, NaN too: a
           // lane clears those elements of the chunks that it will read itself
 #pragma unroll
           for (int e = 0; e < VX; ++e)
 #pragma unroll 1
             for (int d = 0; d < HD / 32; ++d) {
               u32x4* x = reinterpret_cast<u32x4*>(vt(it - 1) + va[e] + (d * 512 << lcp));
-              const int left = F8 ? have[e] : have[e >> 1] - 8 * (e & 1);
-              *x &= u32x4{tail_mask<C::ES>(left, 0), tail_mask<C::ES>(left, 1), tail_mask<C::ES>(left, 2), tail_mask<C::ES>(left, 3)};
+              const Seen& y = seen[F8 ? e : e >> 1];
+              const int first = F8 ? 0 : 8 * (e & 1);
+              *x &= u32x4{seen_mask<C::ES, WIN>(y, first, 0), seen_mask<C::ES, WIN>(y, first, 1), seen_mask<C::ES, WIN>(y, first, 2),
+                          seen_mask<C::ES, WIN>(y, first, 3)};
             }
         }
         if (it > 0 && it < steps) multiply32<DT, F8, HD, true, true>(vt(it - 1), va, lcp, ph, pl, pm, o, kt(it), ka, q, sc);
@@ -1071,6 +1151,7 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
       } else {
         const int kg = key_of(it) + 16 * h, j = scalar(it & 15);
         float f[2], vs[2] = {0.f, 0.f};
+        if constexpr (WIN) last_kg = kg;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           have[u] = sq.seen() - kg - 32 * u;
@@ -1084,7 +1165,7 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
         if (it > 0 && (it & 15) == 0 && 16 * (it >> 4) + 16 < steps) fetch((it >> 4) + 1);
         if (it + NB < steps) issue_k(it + NB);
         if (it + NB - 1 < steps) issue_v(it + NB - 1);
-        softmax32<DT, F8, HD>(sc, pos, kg, have, f, vs, m, l, o, ph, pl, pm);
+        softmax32<DT, F8, HD, WIN>(p, sc, pos, kg, have, f, vs, m, l, o, ph, pl, pm);
       }
     }
     const int next = ph_no + 1 - off;
@@ -1150,7 +1231,7 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
 // sequences' pairs; of either as many as had to be split.
 template <int HD>
 constexpr int kJoinPairs = 1024 / HD;
-template <int DT, int HD>
+template <int DT, int HD, bool WIN>
 __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p, const Split sp, int groups) {
   constexpr int TP = HD / 4, NP = kJoinPairs<HD>;
   __shared__ f32x4 xo[NP][TP];
@@ -1175,7 +1256,8 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p
   if (R >= NR) return;  // (few: the block as one)
   const int chunk = few ? sp.few_chunk : sp.many_chunk;
   const int last = few ? NR - 1 : min((R / sp.many_rows + 1) * sp.many_rows, NR) - 1;
-  const int keys = sq.pos0 + last / p.rep + 1;
+  const Reach<WIN> reach(p, sq.pos0 + (few ? 0 : R / sp.many_rows * sp.many_rows / p.rep));
+  const int keys = sq.pos0 + last / p.rep + 1 - reach.skip;
   if (keys <= chunk) return;  // its tile has written the result
   const int parts = (keys + chunk - 1) / chunk;
   const int i = R / p.rep, head = h * p.rep + R % p.rep;
@@ -1224,29 +1306,34 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p
   *reinterpret_cast<u32x2*>(p.out + t * p.ldo + (int64_t)head * HD + d * 4) = u32x2{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
 }
 
-template <int DT, bool F8, int HD, int LP>
+template <int DT, bool F8, int HD, int LP, bool WIN>
 hipError_t launch_one(const PagedAttnParams& p, hipStream_t s) {
   const Split sp = split_of(p, F8, HD);
   const int64_t heads = (int64_t)p.kv.seqs * p.kv.nkvh;
   if (sp.many) {
     const dim3 grid((unsigned)((int64_t)p.kv.nkvh * sp.tiles * sp.many_chunks + (sp.few ? heads * sp.few_chunks : 0)));
     const dim3 block(64 * kManyWaves);
-    if (sp.many_rows == 64) hipLaunchKernelGGL((paged_many_kernel<DT, F8, HD, LP, 2>), grid, block, 0, s, p, sp);
-    else hipLaunchKernelGGL((paged_many_kernel<DT, F8, HD, LP, 4>), grid, block, 0, s, p, sp);
+    if (sp.many_rows == 64) hipLaunchKernelGGL((paged_many_kernel<DT, F8, HD, LP, 2, WIN>), grid, block, 0, s, p, sp);
+    else hipLaunchKernelGGL((paged_many_kernel<DT, F8, HD, LP, 4, WIN>), grid, block, 0, s, p, sp);
   } else {
-    hipLaunchKernelGGL((paged_few_kernel<DT, F8, HD, LP>), dim3((unsigned)(heads * sp.few_chunks)), dim3(64 * kFewWaves), 0, s, p, sp);
+    hipLaunchKernelGGL((paged_few_kernel<DT, F8, HD, LP, WIN>), dim3((unsigned)(heads * sp.few_chunks)), dim3(64 * kFewWaves), 0, s, p, sp);
   }
   if (sp.few_parts + sp.many_parts > 0) {
     const int64_t groups = sp.many_chunks == 1 ? 0 : (int64_t)sp.tiles * (sp.many_rows * HD / 1024);  // the tiles' blocks, for a kv head
     const int64_t pairs = sp.few_chunks == 1 ? 0 : heads * sp.few_pairs;
-    hipLaunchKernelGGL((paged_join_kernel<DT, HD>), dim3((unsigned)(p.kv.nkvh * groups + pairs)), dim3(256), 0, s, p, sp, (int)groups);
+    hipLaunchKernelGGL((paged_join_kernel<DT, HD, WIN>), dim3((unsigned)(p.kv.nkvh * groups + pairs)), dim3(256), 0, s, p, sp, (int)groups);
   }
   return hipGetLastError();
 }
 
+template <int DT, bool F8, int HD, int LP>
+hipError_t launch_win(const PagedAttnParams& p, hipStream_t s) {
+  return p.window > 0 ? launch_one<DT, F8, HD, LP, true>(p, s) : launch_one<DT, F8, HD, LP, false>(p, s);
+}
+
 template <int DT, bool F8, int HD>
 hipError_t launch_lp(const PagedAttnParams& p, hipStream_t s) {
-  return p.kv.lp == 4 ? launch_one<DT, F8, HD, 4>(p, s) : p.kv.lp == 5 ? launch_one<DT, F8, HD, 5>(p, s) : launch_one<DT, F8, HD, 6>(p, s);
+  return p.kv.lp == 4 ? launch_win<DT, F8, HD, 4>(p, s) : p.kv.lp == 5 ? launch_win<DT, F8, HD, 5>(p, s) : launch_win<DT, F8, HD, 6>(p, s);
 }
 
 template <int DT>
