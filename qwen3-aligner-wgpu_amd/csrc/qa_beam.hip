@@ -16,20 +16,51 @@ namespace {
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.44269504088896341f;
-constexpr int kThreads = 256, kChunk = 8192, kEach = kChunk / kThreads;
+constexpr int kThreads = 256;
 
-// The workspace: each chunk's maximum and sum, then each chunk's candidates (logit,
-// token), best first, token -1 behind the last.
+// A candidate as one number: the larger logit first, then the lower token; 0 is behind all.
+__device__ __forceinline__ uint64_t key_of(float x, int token) {
+  const uint32_t u = __float_as_uint(x + 0.f);  // -0 is 0
+  return (uint64_t)(u & 0x80000000u ? ~u : u | 0x80000000u) << 32 | (uint32_t)~token;
+}
+__device__ __forceinline__ float logit_of(uint64_t key) {
+  const uint32_t u = (uint32_t)(key >> 32);
+  return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
+__device__ __forceinline__ int token_of(uint64_t key) { return (int)~(uint32_t)key; }
+
+// The workspace: each chunk's maximum and sum of exponentials (0 where it has none), then
+// the keys of each chunk's candidates, best first, 0 behind the last.
 struct Stat {
   float top, sum;
 };
-struct Cand {
-  float x;
-  int token;
-};
-__host__ __device__ __forceinline__ int64_t chunks_of(const BeamParams& p) { return (p.vocab + kChunk - 1) / kChunk; }
+// A barrier for what waves exchange through LDS: loads and stores of memory go on across
+// it, where __syncthreads() waits for them.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(0xF | (0x3 << 14) | (0x7 << 4) | (0x0 << 8));
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// The places of a list for the lanes of a wave that have something for it.
+__device__ __forceinline__ int list_place(int* length, bool mine) {
+  const uint64_t who = __builtin_amdgcn_ballot_w64(mine);
+  const int lane = threadIdx.x & 63, first = __builtin_ctzll(who);
+  int at = 0;
+  if (lane == first) at = atomicAdd(length, __popcll(who));
+  return __builtin_amdgcn_readlane(at, first) + __popcll(who & ((1ull << lane) - 1));
+}
+
+// Chunks of a row: as few as hold kThreads * each_of() logits at most, all as long but for the
+// last.
+int each_of(const BeamParams& p) { return p.groups * p.beams * ((p.vocab + 8191) / 8192) < 512 ? 8 : 32; }
+int64_t chunks_of(const BeamParams& p) { return (p.vocab + kThreads * each_of(p) - 1) / (kThreads * each_of(p)); }
+int chunk_of(const BeamParams& p) { return (int)(((p.vocab + chunks_of(p) - 1) / chunks_of(p) + 7) & ~7LL); }
 __device__ __forceinline__ Stat* stats(const BeamParams& p) { return (Stat*)p.ws; }
-__device__ __forceinline__ Cand* cands(const BeamParams& p) { return (Cand*)(stats(p) + p.groups * p.beams * chunks_of(p)); }
+__device__ __forceinline__ uint64_t* cands(const BeamParams& p, int64_t chunks) { return (uint64_t*)(stats(p) + p.groups * p.beams * chunks); }
 
 // A beam that has no continuations of its own: none, or ended.
 __device__ __forceinline__ bool is_none(float score) { return !(score > -INFINITY && score < INFINITY); }
@@ -38,34 +69,32 @@ template <class V, class I>
 __device__ __forceinline__ bool before(V v, I i, V w, I j) {
   return v > w || (v == w && i < j);
 }
-template <class V, class I>
-__device__ __forceinline__ void wave_best(V& v, I& i) {
-#pragma unroll
-  for (int e = 32; e > 0; e >>= 1) {
-    const V w = __shfl_xor(v, e, 64);
-    const I j = __shfl_xor(i, e, 64);
-    if (before(w, j, v, i)) {
-      v = w;
-      i = j;
-    }
-  }
+
+// f over the lanes whose numbers have the lowest bits of `apart`, a power of two from 1
+// (all of them) to 64, in common; by lane moves.
+template <int CTRL>
+__device__ __forceinline__ float moved(float x) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xF, 0xF, true));
 }
-template <class V, class I>
-__device__ __forceinline__ void block_best(V& v, I& i, V* vs, I* is) {
-  wave_best(v, i);
-  if ((threadIdx.x & 63) == 0) {
-    vs[threadIdx.x >> 6] = v;
-    is[threadIdx.x >> 6] = i;
+template <class F>
+__device__ __forceinline__ float over_lanes(float x, int apart, F f) {
+  if (apart <= 1) x = f(x, moved<0x121>(x));  // a row of 16 turned by 1, by 2 ..
+  if (apart <= 2) x = f(x, moved<0x122>(x));
+  if (apart <= 4) x = f(x, moved<0x124>(x));
+  if (apart <= 8) x = f(x, moved<0x128>(x));
+  if (apart <= 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
   }
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w)
-    if (before(vs[w], is[w], v, i)) {
-      v = vs[w];
-      i = is[w];
-    }
-  __syncthreads();
+  if (apart <= 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  }
+  return x;
 }
+__device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ float smaller(float a, float b) { return fminf(a, b); }
+__device__ __forceinline__ float sum_of(float a, float b) { return a + b; }
 
 // A thread's logits of a chunk: kEach / N runs of N, a run of 16 bytes.
 template <int DT>
@@ -95,142 +124,292 @@ __device__ __forceinline__ void unpack(u32x4 w, float* x) {
   }
 }
 
-template <int DT>
-__global__ void __launch_bounds__(kThreads) beam_chunk_kernel(const BeamParams p) {
-  constexpr int N = kRun<DT>, RUNS = kEach / N;
-  __shared__ float vs[kThreads / 64];
-  __shared__ int is[kThreads / 64];
-  const int64_t chunks = chunks_of(p), row = blockIdx.x / chunks, chunk = blockIdx.x - row * chunks;
+// The best `width` of a block's logits: the threads are taken as 4 to 64 groups, at least
+// `width` of them (every 4th to every 64th thread, so that a short chunk's have logits in
+// all), and what is below the least of the groups' best cannot be among them.  The others, about width * log width, are listed in LDS, and each one's rank is the
+// number of those before it.  More than the list holds, which many equal numbers can be,
+// go by rounds of the block.
+constexpr int kList = 1024;
+__device__ __forceinline__ int groups_of(int width) { return width <= 4 ? 4 : width <= 8 ? 8 : width <= 16 ? 16 : width <= 32 ? 32 : 64; }
+
+template <int DT, int EACH>
+__global__ void __launch_bounds__(kThreads) beam_chunk_kernel(const BeamParams p, int chunks, int chunk_len) {
+  constexpr int N = kRun<DT>, RUNS = EACH / N, ES = DT == QA_F32 ? 4 : 2;
+  constexpr float kLowest = -3.402823466e38f;
+  __shared__ float best[kThreads / 64][64], vs[kThreads / 64];
+  __shared__ int is[kThreads / 64], ranks[kThreads / 64][64], length;
+  __shared__ __attribute__((aligned(16))) uint64_t list[kList];
+  const int t = threadIdx.x, lane = t & 63, groups = groups_of(p.width);
+  const int row = blockIdx.x / (uint32_t)chunks;
+  const int64_t t0 = (int64_t)(blockIdx.x - row * chunks) * chunk_len, t1 = t0 + chunk_len < p.vocab ? t0 + chunk_len : p.vocab;
+  const char* src = (const char*)p.logits + row * p.ldl * ES;
+  // all loads first, of the chunk's first run where a thread has none
+  u32x4 raw[RUNS] = {};
+  if (t1 - t0 >= N)
+#pragma unroll
+    for (int r = 0; r < RUNS; ++r) {
+      const int64_t at = t0 + (r * kThreads + t) * N;
+      raw[r] = *reinterpret_cast<const u32x4*>(src + (at + N <= t1 ? at : t0) * ES);
+    }
   if (is_none(p.score[row]) || (p.done && p.done[row])) return;
-  const int t = threadIdx.x;
-  const int64_t t0 = chunk * kChunk;
-  const char* src = (const char*)p.logits + row * p.ldl * (DT == QA_F32 ? 4 : 2);
-  float x[kEach];
+  float x[EACH];
 #pragma unroll
   for (int r = 0; r < RUNS; ++r) {
+    unpack<DT>(raw[r], x + r * N);
     const int64_t at = t0 + (r * kThreads + t) * N;
-    if (at + N <= p.vocab) {
-      unpack<DT>(*reinterpret_cast<const u32x4*>(src + at * (DT == QA_F32 ? 4 : 2)), x + r * N);
-    } else {
+    if (at + N > t1)
 #pragma unroll
-      for (int e = 0; e < N; ++e) x[r * N + e] = at + e < p.vocab ? logit<DT>(src, at + e) : -INFINITY;
-    }
+      for (int e = 0; e < N; ++e) x[r * N + e] = at + e < t1 ? logit<DT>(src, at + e) : -INFINITY;
   }
   auto token = [&](int j) { return (int)(t0 + (j / N * kThreads + t) * N + j % N); };
+  if (t == 0) length = 0;
+  float own, top, least, sum;
+  for (;;) {
+    own = -INFINITY;
 #pragma unroll
-  for (int j = 0; j < kEach; ++j) x[j] = x[j] < INFINITY ? x[j] : -INFINITY;  // NaN too
-  // its best that comes behind (v, i)
-  auto next = [&](float v, int i, float* bv, int* bi) {
-    *bv = -INFINITY;
-    *bi = INT32_MAX;
+    for (int j = 0; j < EACH; ++j) own = fmaxf(own, x[j]);  // NaN is not the larger
+    best[t >> 6][lane] = over_lanes(own, groups, larger);
+    lds_barrier();
+    const float m = fmaxf(fmaxf(best[0][lane], best[1][lane]), fmaxf(best[2][lane], best[3][lane]));
+    top = over_lanes(m, 1, larger);
+    least = fmaxf(over_lanes(m, 1, smaller), kLowest);
+    const float off = top == -INFINITY ? 0.f : top;
+    float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < kEach; ++j)
-      if (before(v, i, x[j], token(j)) && x[j] > *bv) {
-        *bv = x[j];
-        *bi = token(j);
+    for (int j = 0; j < EACH; ++j) part[j & 3] += __builtin_amdgcn_exp2f((x[j] - off) * kLog2e);
+    sum = over_lanes((part[0] + part[1]) + (part[2] + part[3]), 1, sum_of);
+    if (lane == 0) vs[t >> 6] = sum;
+    lds_barrier();
+    sum = (vs[0] + vs[1]) + (vs[2] + vs[3]);
+    if (sum < INFINITY) break;
+    // a NaN, or an infinity, from which it is NaN: again without
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) x[j] = x[j] < INFINITY ? x[j] : -INFINITY;
+  }
+  if (t == 0) stats(p)[blockIdx.x] = {top, sum};
+  if (own >= least) {  // a few lanes
+#pragma unroll
+    for (int j0 = 0; j0 < EACH; j0 += 4)
+      if (fmaxf(fmaxf(x[j0], x[j0 + 1]), fmaxf(x[j0 + 2], x[j0 + 3])) >= least)
+#pragma unroll
+        for (int j = j0; j < j0 + 4; ++j)
+          if (x[j] >= least) {
+            const int at = list_place(&length, true);
+            if (at < kList) list[at] = key_of(x[j], token(j));
+          }
+  }
+  lds_barrier();
+  uint64_t* out = cands(p, chunks) + (int64_t)blockIdx.x * p.width;
+  const int n = __builtin_amdgcn_readfirstlane(length);
+  if (n <= 64) {  // a lane for each, compared with a quarter of the others by each wave
+    const uint64_t mine = lane < n ? list[lane] : 0;
+    int rank = 0;
+    for (int k = __builtin_amdgcn_readfirstlane(t >> 6); k < n; k += kThreads / 64) {
+      const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), k) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)mine, k);
+      rank += other > mine;
+    }
+    ranks[t >> 6][lane] = rank;
+    lds_barrier();
+    if (t < 64) {
+      rank = lane < n ? (ranks[0][lane] + ranks[1][lane]) + (ranks[2][lane] + ranks[3][lane]) : lane;
+      if (rank < p.width) out[rank] = mine;
+    }
+  } else if (n <= kList) {
+    for (int c = t; c < n; c += kThreads) {
+      const uint64_t mine = list[c];
+      int rank = 0;
+#pragma unroll 8
+      for (int k = 0; k < n; ++k) rank += list[k] > mine;
+      if (rank < p.width) out[rank] = mine;
+    }
+  } else {
+    // the thread's best that comes behind (v, i); read again: held until here, the logits
+    // would take registers of which the CU's other blocks live
+    auto next = [&](float v, int i, float* bv, int* bi) {
+      *bv = -INFINITY;
+      *bi = INT32_MAX;
+      for (int64_t k = t0 + t; k < t1; k += kThreads) {
+        const float y = logit<DT>(src, k);
+        if (y < INFINITY && before(v, i, y, (int)k) && y > *bv) {
+          *bv = y;
+          *bi = (int)k;
+        }
       }
-  };
-  float mine;
-  int at;
-  next(INFINITY, -1, &mine, &at);
-  float v = mine;
-  int i = at;
-  block_best(v, i, vs, is);
-  const float top = v;
-  float sum = 0.f;
+    };
+    int at;
+    next(INFINITY, -1, &own, &at);
+    for (int k = 0; k < p.width; ++k) {
+      float v = own;
+      int i = at;
 #pragma unroll
-  for (int j = 0; j < kEach; ++j) sum += top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((x[j] - top) * kLog2e);
+      for (int e = 32; e > 0; e >>= 1) {
+        const float w = __shfl_xor(v, e, 64);
+        const int j = __shfl_xor(i, e, 64);
+        if (before(w, j, v, i)) {
+          v = w;
+          i = j;
+        }
+      }
+      lds_barrier();
+      if (lane == 0) {
+        vs[t >> 6] = v;
+        is[t >> 6] = i;
+      }
+      lds_barrier();
 #pragma unroll
-  for (int e = 32; e > 0; e >>= 1) sum += __shfl_xor(sum, e, 64);
-  if ((t & 63) == 0) vs[t >> 6] = sum;
-  __syncthreads();
-  if (t == 0) stats(p)[blockIdx.x] = {top, (vs[0] + vs[1]) + (vs[2] + vs[3])};
-  __syncthreads();
-  Cand* out = cands(p) + (int64_t)blockIdx.x * p.width;
-  for (int k = 0;; ) {
-    if (t == 0) out[k] = {v, v == -INFINITY ? -1 : i};
-    if (++k == p.width) break;
-    if (at == i) next(v, i, &mine, &at);
-    v = mine;
-    i = at;
-    block_best(v, i, vs, is);
+      for (int w = 0; w < kThreads / 64; ++w)
+        if (before(vs[w], is[w], v, i)) {
+          v = vs[w];
+          i = is[w];
+        }
+      if (t == 0) out[k] = key_of(v, i);
+      if (at == i) next(v, i, &own, &at);
+    }
   }
 }
 
-template <int DT>
-__global__ void __launch_bounds__(kThreads) beam_rank_kernel(const BeamParams p) {
-  __shared__ double vs[kThreads / 64], add[64];  // score - log sum of each beam
-  __shared__ int64_t is[kThreads / 64];
-  const int64_t chunks = chunks_of(p), g = blockIdx.x, row0 = g * p.beams;
-  const int t = threadIdx.x, lane = t & 63;
-  for (int b = t >> 6; b < p.beams; b += kThreads / 64) {
-    const float score = p.score[row0 + b];
-    if (is_none(score) || (p.done && p.done[row0 + b])) continue;
-    const Stat* st = stats(p) + (row0 + b) * chunks;
-    float top = -INFINITY;
-    for (int64_t c = lane; c < chunks; c += 64) top = fmaxf(top, st[c].top);
+// What lane ^ D holds, by lane moves: rows of 16 turned or mirrored, fours permuted, rows and
+// halves swapped.
+template <int D>
+__device__ __forceinline__ uint32_t from_lane(uint32_t x) {
+  constexpr int HI = D >> 2 & 3, LO = (D ^ (HI & 1 ? 3 : 0)) & 3;  // mirrors of 8 and of 16 turn fours round
+  constexpr int ROW = HI == 1 ? 0x141 : HI == 2 ? 0x128 : 0x140;
+  constexpr int FOUR = (LO ^ 0) | (LO ^ 1) << 2 | (LO ^ 2) << 4 | (LO ^ 3) << 6;
+  if constexpr (HI != 0) x = (uint32_t)__builtin_amdgcn_mov_dpp((int)x, ROW, 0xF, 0xF, true);
+  if constexpr (LO != 0) x = (uint32_t)__builtin_amdgcn_mov_dpp((int)x, FOUR, 0xF, 0xF, true);
+  if constexpr ((D & 16) != 0) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = threadIdx.x & 16 ? r[0] : r[1];
+  }
+  if constexpr ((D & 32) != 0) {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    x = threadIdx.x & 32 ? r[0] : r[1];
+  }
+  return x;
+}
+template <int D>
+__device__ __forceinline__ uint64_t from_lane(uint64_t x) {
+  return (uint64_t)from_lane<D>((uint32_t)(x >> 32)) << 32 | from_lane<D>((uint32_t)x);
+}
+template <int D>
+__device__ __forceinline__ double from_lane(double x) {
+  return __builtin_bit_cast(double, from_lane<D>(__builtin_bit_cast(uint64_t, x)));
+}
+// A continuation of a group: its value, and its beam and rank there as one number, the lower first.
+struct Total {
+  double v;
+  uint32_t at;
+};
+template <int D>
+__device__ __forceinline__ Total from_lane(Total x) {
+  return {from_lane<D>(x.v), from_lane<D>(x.at)};
+}
+__device__ __forceinline__ bool better(uint64_t a, uint64_t b) { return a > b; }
+__device__ __forceinline__ bool better(Total a, Total b) { return a.v > b.v || (a.v == b.v && a.at < b.at); }
+
+// Sorted runs of 2^LW numbers, one in each run's lanes, the best first, merged: the better
+// of one and the other turned round, lane by lane, are the better half of both, rising
+// and falling, which LW steps sort (Batcher's bitonic merge).  `turned`: that.
+template <int D, class T>
+__device__ __forceinline__ T sorted_steps(T x) {
+  if constexpr (D > 0) {
+    const T y = from_lane<D>(x);
+    if (better(y, x) != ((threadIdx.x & D) != 0)) x = y;
+    x = sorted_steps<D / 2>(x);
+  }
+  return x;
+}
+template <int LW, class T>
+__device__ __forceinline__ T merged(T run, T turned) {
+  return sorted_steps<(1 << LW) / 2>(better(turned, run) ? turned : run);
+}
+// All of a wave's runs as one, in every run's lanes.
+template <int LW, int D, class T>
+__device__ __forceinline__ T wave_run(T run) {
+  if constexpr (D < 64) run = wave_run<LW, 2 * D>(merged<LW>(run, from_lane<(D | ((1 << LW) - 1))>(run)));
+  return run;
+}
+template <int D>
+__device__ __forceinline__ double wave_sum(double x) {
+  if constexpr (D > 0) x = wave_sum<D / 2>(x + from_lane<D>(x));
+  return x;
+}
+
+// A block for each group, a wave for each of its beams in turn: the beam's chunks' sums
+// joined, and their candidates merged by logit; then, by one wave, the beams'.
+template <int LW>
+__global__ void __launch_bounds__(1024) beam_rank_kernel(const BeamParams p, int chunks) {
+  constexpr int W = 1 << LW, RUNS = 64 >> LW;
+  __shared__ double add[64];  // score - log sum of each beam
+  __shared__ uint64_t best[64 * W];
+  const int64_t row0 = (int64_t)blockIdx.x * p.beams;
+  const int t = threadIdx.x, lane = t & 63, k = lane & (W - 1), run = lane >> LW;
+  for (int b = t >> 6; b < p.beams; b += blockDim.x >> 6) {
+    const int64_t row = row0 + b;
+    const float score = p.score[row];
+    const bool over = p.done && p.done[row];
+    const Stat* st = stats(p) + row * chunks;
+    const uint64_t* cd = cands(p, chunks) + row * chunks * p.width;
+    auto load = [&](int c) { return c < chunks && k < p.width ? cd[(int64_t)c * p.width + k] : 0; };
+    const Stat first = lane < chunks ? st[lane] : Stat{-INFINITY, 0.f};
+    uint64_t x[4];
 #pragma unroll
-    for (int e = 32; e > 0; e >>= 1) top = fmaxf(top, __shfl_xor(top, e, 64));
-    double sum = 0.0;
-    for (int64_t c = lane; c < chunks; c += 64)
-      if (st[c].top > -INFINITY) sum += (double)st[c].sum * exp((double)st[c].top - (double)top);
+    for (int e = 0; e < 4; ++e) x[e] = load(e * RUNS + run);
+    if (is_none(score) || over) {
+      if (lane < W) best[b * W + lane] = lane == 0 && !is_none(score) ? key_of(0.f, p.end) : 0;
+      if (lane == 0) add[b] = score;
+      continue;
+    }
+    uint64_t acc = x[0];
+    for (int c0 = 0;;) {
 #pragma unroll
-    for (int e = 32; e > 0; e >>= 1) sum += __shfl_xor(sum, e, 64);
+      for (int e = 0; e < 4; ++e)
+        if (c0 + e * RUNS < chunks && c0 + e > 0) acc = merged<LW>(acc, from_lane<W - 1>(x[e]));
+      c0 += 4 * RUNS;
+      if (c0 >= chunks) break;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = load(c0 + e * RUNS + run);
+    }
+    acc = wave_run<LW, W>(acc);
+    float top = first.top;
+    for (int c = lane + 64; c < chunks; c += 64) top = fmaxf(top, st[c].top);
+    top = over_lanes(top, 1, larger);
+    double sum = first.sum == 0.f ? 0.0 : first.sum * exp((double)first.top - (double)top);
+    for (int c = lane + 64; c < chunks; c += 64)
+      if (st[c].sum != 0.f) sum += st[c].sum * exp((double)st[c].top - (double)top);
+    sum = wave_sum<32>(sum);
     if (lane == 0) add[b] = (double)score - ((double)top + log(sum));
+    if (lane < W) best[b * W + lane] = acc;
   }
-  __syncthreads();
-  const int64_t each = chunks * p.width, n = p.beams * each;
-  // candidate number c: its value and its (beam, token) as one index; false if it is none
-  auto candidate = [&](int64_t c, double* v, int64_t* i) {
-    const int64_t b = c / each;
-    const float score = p.score[row0 + b];
-    if (is_none(score)) return false;
-    if (p.done && p.done[row0 + b]) {
-      *v = score;
-      *i = b * p.vocab + p.end;
-      return c == b * each;
-    }
-    const Cand k = cands(p)[row0 * each + c];
-    *v = add[b] + (double)k.x;
-    *i = b * p.vocab + k.token;
-    return k.token >= 0;
+  lds_barrier();
+  if (t >= 64) return;
+  auto load = [&](int b) {
+    const uint64_t x = b < p.beams ? best[b * W + k] : 0;
+    return x ? Total{add[b] + (double)logit_of(x), (uint32_t)(b * W + k)} : Total{-INFINITY, ~0u};
   };
-  auto next = [&](double v, int64_t i, double* bv, int64_t* bi) {
-    *bv = -INFINITY;
-    *bi = INT64_MAX;
-    for (int64_t c = t; c < n; c += kThreads) {
-      double w;
-      int64_t j;
-      if (candidate(c, &w, &j) && before(v, i, w, j) && before(w, j, *bv, *bi)) {
-        *bv = w;
-        *bi = j;
-      }
-    }
-  };
-  double mine;
-  int64_t at;
-  next(INFINITY, -1, &mine, &at);
-  for (int k = 0; k < p.width; ++k) {
-    double v = mine;
-    int64_t i = at;
-    block_best(v, i, vs, is);
-    if (t == 0) {
-      const bool on = i != INT64_MAX;
-      const int64_t b = on ? i / p.vocab : 0, o = g * p.width + k;
-      p.parent[o] = on ? (int)(row0 + b) : -1;
-      p.token[o] = on ? (int)(i - b * p.vocab) : -1;
-      p.score_out[o] = on ? (float)v : -INFINITY;
-      p.done_out[o] = on && ((p.done && p.done[row0 + b]) || i - b * p.vocab == p.end);
-    }
-    if (at == i) next(v, i, &mine, &at);
-  }
+  Total acc = load(run);
+  for (int b0 = RUNS; b0 < p.beams; b0 += RUNS) acc = merged<LW>(acc, from_lane<W - 1>(load(b0 + run)));
+  acc = wave_run<LW, W>(acc);
+  if (lane >= p.width) return;
+  const bool on = acc.at != ~0u;
+  const int64_t row = row0 + (on ? acc.at >> LW : 0), o = (int64_t)blockIdx.x * p.width + lane;
+  const int token = on ? token_of(best[acc.at]) : -1;
+  p.parent[o] = on ? (int)row : -1;
+  p.token[o] = token;
+  p.score_out[o] = on ? (float)acc.v : -INFINITY;
+  p.done_out[o] = on && (token == p.end || (p.done && p.done[row]));
 }
 
 template <int DT>
-hipError_t launch(const BeamParams& p, hipStream_t s) {
-  hipLaunchKernelGGL((beam_chunk_kernel<DT>), dim3((unsigned)(p.groups * p.beams * chunks_of(p))), dim3(kThreads), 0, s, p);
-  hipLaunchKernelGGL((beam_rank_kernel<DT>), dim3((unsigned)p.groups), dim3(kThreads), 0, s, p);
-  return hipGetLastError();
+void launch_chunks(const BeamParams& p, hipStream_t s) {
+  const int chunks = (int)chunks_of(p);
+  const dim3 grid((unsigned)(p.groups * p.beams * chunks));
+  if (each_of(p) == 8) hipLaunchKernelGGL((beam_chunk_kernel<DT, 8>), grid, dim3(kThreads), 0, s, p, chunks, chunk_of(p));
+  else hipLaunchKernelGGL((beam_chunk_kernel<DT, 32>), grid, dim3(kThreads), 0, s, p, chunks, chunk_of(p));
+}
+template <int LW>
+void launch_rank(const BeamParams& p, hipStream_t s) {
+  hipLaunchKernelGGL((beam_rank_kernel<LW>), dim3((unsigned)p.groups), dim3(64 * (p.beams < 16 ? p.beams : 16)), 0, s, p, (int)chunks_of(p));
 }
 
 }  // namespace
@@ -240,10 +419,18 @@ int64_t beam_select_blocks(int, const BeamParams& p) {
   return n > 9e18 ? INT64_MAX : (int64_t)n;
 }
 size_t beam_select_workspace(int, const BeamParams& p) {
-  return (size_t)(p.groups * p.beams * chunks_of(p)) * (sizeof(Stat) + p.width * sizeof(Cand));
+  return (size_t)(p.groups * p.beams * chunks_of(p)) * (sizeof(Stat) + p.width * sizeof(uint64_t));
 }
 hipError_t launch_beam_select(int dtype, const BeamParams& p, hipStream_t s) {
-  return dtype == QA_F32 ? launch<QA_F32>(p, s) : dtype == QA_BF16 ? launch<QA_BF16>(p, s) : launch<QA_F16>(p, s);
+  if (dtype == QA_F32) launch_chunks<QA_F32>(p, s);
+  else if (dtype == QA_BF16) launch_chunks<QA_BF16>(p, s);
+  else launch_chunks<QA_F16>(p, s);
+  if (p.width <= 4) launch_rank<2>(p, s);
+  else if (p.width <= 8) launch_rank<3>(p, s);
+  else if (p.width <= 16) launch_rank<4>(p, s);
+  else if (p.width <= 32) launch_rank<5>(p, s);
+  else launch_rank<6>(p, s);
+  return hipGetLastError();
 }
 
 }  // namespace qa

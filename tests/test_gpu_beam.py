@@ -156,6 +156,17 @@ def test_equal_logits_go_by_their_place(ctx, pkg, dtype, width):
 
 
 @DT
+def test_zeros_of_either_sign_are_alike(ctx, pkg, dtype):
+    x = np.full((2, 9000), -1.0)
+    x[:, [7, 100, 2500, 8999]] = [-0.0, 0.0, -0.0, 0.0]
+    x[1] = -x[1] - 1.0
+    x[1, x[1] == 0] = -0.0
+    got = _check(ctx, pkg, x, dtype, [-1.0, -300.0], beams=2, width=6)
+    assert list(got[1][:4]) == [7, 100, 2500, 8999]
+    _check(ctx, pkg, np.where(np.arange(9000) % 3 == 1, 0.0, -0.0)[None], dtype, [0.0], width=40)
+
+
+@DT
 def test_rising_and_falling_logits(ctx, pkg, dtype):
     """The best are a thread's, a wave's or a chunk's own."""
     for n in (40, 2000, 9000):
@@ -184,6 +195,29 @@ def test_banned_and_broken_logits(ctx, pkg, dtype):
         _check(ctx, pkg, x, dtype, [-1.0] * 6, groups=6, width=8)
         _check(ctx, pkg, x, dtype, [-1.0, -1.1, -1.2, -1.3, -1.4, -1.5], beams=6, width=16)
         _check(ctx, pkg, np.full((1, 300), low), dtype, [0.0], width=3)
+
+
+@DT
+@pytest.mark.parametrize("width", [1, 4, 30, 64])
+def test_nan_of_every_kind(ctx, pkg, dtype, width):
+    """Quiet and signalling NaN of either sign in places that a thread, a group of lanes or a chunk has for itself."""
+    r = np.random.default_rng(width)
+    x = r.standard_normal((2, 12000))
+    bits = _stored(x, dtype) if dtype != F32 else x.astype(np.float32).view(np.uint32)
+    kinds = {F16: [0x7C01, 0xFC01, 0x7E00, 0xFFFF], BF16: [0x7F81, 0xFF81, 0x7FC0, 0xFFFF], F32: [0x7F800001, 0xFF800001, 0x7FC00000, 0xFFFFFFFF]}[dtype]
+    for k, kind in enumerate(kinds):
+        bits[0, 300 * k: 300 * k + 256] = kind      # groups of lanes in a run
+        bits[0, 2048 + k:: 4096] = kind
+        bits[1, k:8192:4] = kind                    # a whole chunk
+    if dtype == F32:
+        bits = bits.view(np.float32)
+    with np.errstate(invalid="ignore"):
+        score = np.array([-1.0, -1.5], np.float32)
+        call = Call(ctx, pkg, bits, dtype, 12000, score, None, -1, 2, 1, width).run()
+        got, want = call.read(), _want(_values(bits, dtype), score, None, -1, 2, 1, width)
+    assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+    assert (np.abs(got[2] - want[2]) <= SUM + 2.0 ** -21).all()
+    call.free()
 
 
 @DT
