@@ -412,6 +412,7 @@ struct PagesForkParams {
   int64_t num_pages, ldtable;
   int src_seqs, seqs, lp, keep;
   int64_t window, sinks;
+  FastDiv by_width;  // of a division by ldtable
   int32_t* ws;
 };
 struct PagesCompactParams {

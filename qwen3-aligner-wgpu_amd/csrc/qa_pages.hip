@@ -55,29 +55,34 @@ __device__ __forceinline__ int64_t capacity(const PagesForkParams& p) {
 __device__ __forceinline__ int src_length(const PagesForkParams& p, int s) { return (int)clamp64(p.src_len[s], 0, capacity(p)); }
 __device__ __forceinline__ int pages_of(const PagesForkParams& p, int keys) { return (int)(((int64_t)keys + (1 << p.lp) - 1) >> p.lp); }
 __device__ __forceinline__ bool is_source(const PagesForkParams& p, int q) { return q >= 0 && q < p.src_seqs; }
-// Whether a sequence of `keys` keys goes on with page number k of its source.
-__device__ __forceinline__ bool goes_on(const PagesForkParams& p, int keys, int64_t k) {
-  if (k << p.lp >= keys) return false;
-  return p.window <= 0 || k << p.lp < p.sinks || ((k + 1) << p.lp) > keys - p.window + 1;
+// The pages with which a sequence of `keys` keys goes on: those below `pages` that are
+// below sink_pages() or from `near` on.
+__device__ __forceinline__ int sink_pages(const PagesForkParams& p) { return p.window > 0 ? (int)((p.sinks + (1 << p.lp) - 1) >> p.lp) : 0; }
+struct Reach {
+  int pages, near;
+  __device__ __forceinline__ bool goes_on(int sinks, int64_t k) const { return k < pages && (k < sinks || k >= near); }
+};
+__device__ __forceinline__ Reach reach_of(const PagesForkParams& p, int keys) {
+  const int64_t seen = keys - p.window + 1;  // the first key of the next row's window
+  return {pages_of(p, keys), p.window > 0 && seen > 0 ? (int)(seen >> p.lp) : 0};
 }
 __device__ __forceinline__ int page_id(const PagesForkParams& p, int32_t id) { return id >= 0 && id < p.num_pages ? id : -1; }
 
-// What source s's entry k adds to its page's references: its children hold it, and the
+// What a source's entry k adds to its page's references: its children hold it, and the
 // source does no longer.
-__device__ __forceinline__ int change_of(const PagesForkParams& p, int keys, int children, int64_t k) {
-  return (goes_on(p, keys, k) ? children : 0) - (p.keep ? 0 : 1);
+__device__ __forceinline__ int change_of(const PagesForkParams& p, Reach r, int sinks, int children, int64_t k) {
+  return (r.goes_on(sinks, k) ? children : 0) - (p.keep ? 0 : 1);
 }
 
 // Blocks of sources: references; blocks of sequences: their rows of the table, up to
 // the last page that they share.
 __global__ void __launch_bounds__(256) fork_share_kernel(const PagesForkParams p) {
-  const int b = blockIdx.x;
+  const int b = blockIdx.x, sinks = sink_pages(p);
   if (b >= p.src_seqs) {
     const int i = b - p.src_seqs, q = p.parent[i];
-    const bool on = is_source(p, q);
-    const int keys = on ? src_length(p, q) : 0;
+    const Reach r = is_source(p, q) ? reach_of(p, src_length(p, q)) : Reach{0, 0};
     for (int64_t k = threadIdx.x; k < p.ldtable; k += 256)
-      p.table[i * p.ldtable + k] = on && goes_on(p, keys, k) ? page_id(p, p.src_table[q * p.ldtable + k]) : -1;
+      p.table[i * p.ldtable + k] = r.goes_on(sinks, k) ? page_id(p, p.src_table[q * p.ldtable + k]) : -1;
     return;
   }
   __shared__ int children;
@@ -87,11 +92,12 @@ __global__ void __launch_bounds__(256) fork_share_kernel(const PagesForkParams p
   for (int i = threadIdx.x; i < p.seqs; i += 256) mine += p.parent[i] == b;
   if (mine) atomicAdd(&children, mine);
   __syncthreads();
-  const int keys = src_length(p, b), all = children;
+  const Reach r = reach_of(p, src_length(p, b));
+  const int all = children;
   for (int64_t k = threadIdx.x; k < p.ldtable; k += 256) {
-    const int by = change_of(p, keys, all, k);
-    const int id = page_id(p, p.src_table[b * p.ldtable + k]);
-    if (by && id >= 0) atomicAdd(p.refs + id, by);
+    const int by = change_of(p, r, sinks, all, k);
+    const int id = by ? page_id(p, p.src_table[b * p.ldtable + k]) : -1;
+    if (id >= 0) atomicAdd(p.refs + id, by);
   }
 }
 
@@ -104,121 +110,233 @@ __device__ __forceinline__ int32_t* ws_first(const PagesForkParams& p) { return 
 // What one block writes and reads again, past its L1.
 __device__ __forceinline__ int32_t peek(const int32_t* x) { return __hip_atomic_load(x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ void poke(int32_t* x, int32_t v) { __hip_atomic_store(x, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+// ... behind everything that it wrote so far.
+__device__ __forceinline__ void settle() {
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+}
 
-struct Growth {
-  int have, now, last;  // keys before and behind; the page that is written on, or -1
+// Inclusive sum over a wave by lane moves: within rows of 16, then from row to row.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int plus_moved(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int wave_upto(int v) {
+  v = plus_moved<0x111, 0xF>(v);  // from 1, 2, 4, 8 lanes below
+  v = plus_moved<0x112, 0xF>(v);
+  v = plus_moved<0x114, 0xF>(v);
+  v = plus_moved<0x118, 0xF>(v);
+  v = plus_moved<0x142, 0xA>(v);  // the sum of the row below, to rows 1 and 3
+  return plus_moved<0x143, 0xC>(v);  // of the lower half, to the upper
+}
+// ... and over a block of 1024: the first wave sums up to N * 16 waves' sums, in LDS.
+template <int N>
+struct WaveSums {
+  int sum[N * 16], total;
+  __device__ __forceinline__ void put(int n, int v) { sum[n * 16 + (threadIdx.x >> 6)] = v; }  // by one lane
+  // Then, for all: before(n), the sum of what was put before the wave's n-th.
+  __device__ __forceinline__ void add_up() {
+    __syncthreads();
+    if (threadIdx.x < 64) {
+      const int lane = threadIdx.x, v = lane < N * 16 ? sum[lane] : 0, upto = wave_upto(v);
+      if (lane < N * 16) sum[lane] = upto - v;
+      if (lane == 63) total = upto;
+    }
+    __syncthreads();
+  }
+  __device__ __forceinline__ int before(int n) const { return sum[n * 16 + (threadIdx.x >> 6)]; }
 };
-__device__ __forceinline__ Growth growth(const PagesForkParams& p, int i) {
-  const int q = p.parent[i];
-  Growth g = {0, 0, -1};
-  if (!is_source(p, q)) return g;
-  g.have = src_length(p, q);
-  const int more = p.grow ? p.grow[i] : 0;
-  g.now = (int)clamp64((int64_t)g.have + (more > 0 ? more : 0), 0, capacity(p));
-  if ((g.have & ((1 << p.lp) - 1)) && g.now > g.have) g.last = p.table[i * p.ldtable + (g.have >> p.lp)];
-  return g;
-}
-
-// Inclusive sum over a block of 1024 (wave sums in LDS).
-__device__ __forceinline__ int block_sum(int v, int* waves, int* total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int e = 1; e < 64; e <<= 1) {
-    const int x = __shfl_up(v, e, 64);
-    v += lane >= e ? x : 0;
-  }
-  if (lane == 63) waves[wave] = v;
-  __syncthreads();
-  int before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < 16; ++w) {
-    const int x = waves[w];
-    before += w < wave ? x : 0;
-    all += x;
-  }
-  __syncthreads();
-  *total = all;
-  return before + v;
-}
 
 // One block: who copies its last page, how many pages each sequence takes, the lowest
-// free pages, dealt out in order.
-constexpr int kTake = 1024, kRound = 4;
+// free pages, dealt out in order.  SHARE: what fork_share_kernel does, too, which saves a
+// launch where there is little of it.
+// Sequences with the same last page are counted in an LDS table of pages, for up to kTake
+// of them, and in the workspace beyond (three trips to memory: 2 us).
+constexpr int kTake = 1024, kRound = 4, kSlots = 2048;
+template <bool SHARE>
 __global__ void __launch_bounds__(kTake) fork_take_kernel(const PagesForkParams p) {
-  __shared__ int start[kForkSeqs + 1];  // pages taken before sequence i; bit 31: its first is a copy
-  __shared__ int waves[kRound * 16];
+  __shared__ int start[kForkSeqs];  // pages taken before sequence i; bit 31: its first is a copy
+  __shared__ int held[kForkSeqs];   // its parent's keys
+  __shared__ int lasts[kForkSeqs];  // the page that it goes on writing, or -1
+  __shared__ int source[SHARE ? 2 * kTake : 1];  // SHARE: a source's keys, its children
+  __shared__ int slots[3 * kSlots];              // a page, how many write on it, the first of them
+  __shared__ WaveSums<kRound> sums;
+  __shared__ int copies;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, part = (1 << p.lp) - 1;
+  const bool few = p.seqs <= kTake;
+  if (t == 0) copies = 0;
+  if (few)
+    for (int i = t; i < kSlots; i += kTake) {
+      slots[i] = -1;
+      slots[kSlots + i] = 0;
+      slots[2 * kSlots + i] = p.seqs;
+    }
+  int own_parent = -1, own_grow = 0;
+  if constexpr (SHARE) {  // (a source and a sequence at most to a thread)
+    if (t < p.seqs) {
+      own_parent = p.parent[t];
+      own_grow = p.grow ? p.grow[t] : 0;
+    }
+    const bool on = is_source(p, own_parent);
+    source[t] = t < p.src_seqs ? src_length(p, t) : 0;
+    source[kTake + t] = 0;
+    __syncthreads();
+    if (on) atomicAdd(&source[kTake + own_parent], 1);
+    if (t < p.seqs) {
+      held[t] = on ? source[own_parent] : 0;
+      start[t] = own_parent;  // for now
+      lasts[t] = -1;
+    }
+    __syncthreads();
+    const int width = (int)p.ldtable, entries = p.seqs * width, sources = p.src_seqs * width, sinks = sink_pages(p);
+    const int most = entries > sources ? entries : sources;
+    constexpr int B = 4;  // entries of either table under way
+    for (int w0 = wave * 64; w0 < most; w0 += B * kTake) {
+      int id[B], gone[B], by[B];
+#pragma unroll
+      for (int e = 0; e < B; ++e) {
+        id[e] = gone[e] = -1;
+        if (w0 + e * kTake >= most) break;  // (the wave as one)
+        const int at = w0 + e * kTake + lane, row = fastdiv(at, p.by_width), k = at - row * width;
+        if (at < entries && reach_of(p, held[row]).goes_on(sinks, k)) id[e] = p.src_table[start[row] * width + k];
+        by[e] = at < sources ? change_of(p, reach_of(p, source[row]), sinks, source[kTake + row], k) : 0;
+        if (by[e]) gone[e] = p.src_table[at];
+      }
+#pragma unroll
+      for (int e = 0; e < B; ++e) {
+        if (w0 + e * kTake >= most) break;
+        const int at = w0 + e * kTake + lane;
+        if (at < entries) {
+          const int row = fastdiv(at, p.by_width), page = page_id(p, id[e]);
+          p.table[at] = page;
+          if (at - row * width == held[row] >> p.lp && (held[row] & part)) lasts[row] = page;
+        }
+        gone[e] = page_id(p, gone[e]);
+        if (gone[e] >= 0) atomicAdd(p.refs + gone[e], by[e]);
+      }
+    }
+    settle();
+  }
+  // every sequence's growth; start[i]: the pages behind its last
+  for (int i = t; i < p.seqs; i += kTake) {
+    const int q = SHARE ? own_parent : p.parent[i], more = !is_source(p, q) ? 0 : SHARE ? own_grow : p.grow ? p.grow[i] : 0;
+    int have;
+    if constexpr (SHARE) have = held[i];
+    else held[i] = have = is_source(p, q) ? src_length(p, q) : 0;
+    const int now = (int)clamp64((int64_t)have + (more > 0 ? more : 0), 0, capacity(p));
+    if (now == have) lasts[i] = -1;
+    else if constexpr (!SHARE) lasts[i] = have & part ? p.table[i * p.ldtable + (have >> p.lp)] : -1;
+    start[i] = pages_of(p, now) - pages_of(p, have);
+    p.len[i] = now;
+  }
   int32_t *pairs = ws_pairs(p), *writers = ws_writers(p), *first = ws_first(p);
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  for (int i = t; i < p.seqs; i += kTake) {
-    const Growth g = growth(p, i);
-    if (g.last < 0) continue;
-    poke(writers + g.last, 0);
-    poke(first + g.last, p.seqs);
+  uint32_t slot = 0;
+  if (few) {
+    if constexpr (!SHARE) __syncthreads();  // the slots are clear
+    const int last = t < p.seqs ? lasts[t] : -1;
+    if (last >= 0) {
+      slot = (uint32_t)last * 2654435761u >> 21;
+      for (;; slot = (slot + 1) & (kSlots - 1)) {  // (twice as many as sequences)
+        const int who = atomicCAS(&slots[slot], -1, last);
+        if (who == -1 || who == last) break;
+      }
+      atomicAdd(&slots[kSlots + slot], 1);
+      atomicMin(&slots[2 * kSlots + slot], t);
+    }
+  } else {
+    for (int i = t; i < p.seqs; i += kTake)
+      if (lasts[i] >= 0) {
+        poke(writers + lasts[i], 0);
+        poke(first + lasts[i], p.seqs);
+      }
+    settle();
+    for (int i = t; i < p.seqs; i += kTake)
+      if (lasts[i] >= 0) {
+        atomicAdd(writers + lasts[i], 1);
+        atomicMin(first + lasts[i], i);
+      }
+    settle();
   }
+  const int mine0 = t < p.seqs && lasts[t] >= 0 ? peek(p.refs + lasts[t]) : 1;  // of the thread's first sequence
+  // A round of the search for free pages; the first one's loads go out here.
+  uint64_t free[kRound];
+  auto look = [&](int64_t p0) {
+    bool is[kRound];
+#pragma unroll
+    for (int e = 0; e < kRound; ++e) {
+      const int64_t at = p0 + e * kTake + t;
+      is[e] = at < p.num_pages && peek(p.refs + at) <= 0;
+    }
+#pragma unroll
+    for (int e = 0; e < kRound; ++e) free[e] = __builtin_amdgcn_ballot_w64(is[e]);
+  };
+  look(0);
   __syncthreads();
-  for (int i = t; i < p.seqs; i += kTake) {
-    const Growth g = growth(p, i);
-    if (g.last < 0) continue;
-    atomicAdd(writers + g.last, 1);
-    atomicMin(first + g.last, i);
-  }
-  __syncthreads();
-  int need = 0, copies = 0;  // so far, of all
+  int need = 0;
   for (int i0 = 0; i0 < p.seqs; i0 += kTake) {
     const int i = i0 + t;
     int mine = 0;
     bool copy = false;
     if (i < p.seqs) {
-      const Growth g = growth(p, i);
-      copy = g.last >= 0 && !(p.refs[g.last] == peek(writers + g.last) && peek(first + g.last) == i);
-      mine = pages_of(p, g.now) - pages_of(p, g.have) + copy;
-      p.len[i] = g.now;
+      const int last = lasts[i];
+      if (last >= 0) {
+        const int refs = i0 == 0 ? mine0 : peek(p.refs + last);
+        const int n = few ? slots[kSlots + slot] : peek(writers + last), least = few ? slots[2 * kSlots + slot] : peek(first + last);
+        copy = !(refs == n && least == i);
+      }
+      mine = start[i] + copy;
     }
-    int all, each;
-    const int upto = block_sum(mine, waves, &all), number = block_sum(copy, waves, &each);
-    if (i < p.seqs) start[i] = (need + upto - mine) | (copy ? 1 << 31 : 0);
-    if (copy) {  // the page and, for now, the sequence
-      const int c = copies + number - 1;
-      pairs[2 * c] = p.table[i * p.ldtable + (src_length(p, p.parent[i]) >> p.lp)];
-      pairs[2 * c + 1] = i;
-    }
-    need += all;
-    copies += each;
+    const int upto = wave_upto(mine);
+    if (lane == 63) sums.put(0, upto);
+    if (lane < kRound - 1) sums.put(lane + 1, 0);
+    sums.add_up();
+    if (i < p.seqs) start[i] = (need + sums.before(0) + upto - mine) | (copy ? 1 << 31 : 0);
+    need += sums.total;
+    __syncthreads();
   }
-  __syncthreads();
-  auto place = [&](int k) {  // the entry of the k-th page taken: its sequence is the last that starts at or before k
+  // the k-th page taken: its sequence is the last that starts at or before k
+  auto take = [&](int k, int page) {
     int lo = 0, hi = p.seqs;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if ((start[mid] & 0x7fffffff) <= k) lo = mid;
       else hi = mid;
     }
-    const int have = src_length(p, p.parent[lo]), j = k - (start[lo] & 0x7fffffff);
-    return lo * p.ldtable + (start[lo] < 0 ? have >> p.lp : pages_of(p, have)) + j;
+    const int j = k - (start[lo] & 0x7fffffff);
+    const bool partial = start[lo] < 0;
+    p.table[lo * p.ldtable + (partial ? held[lo] >> p.lp : pages_of(p, held[lo])) + j] = page;
+    p.refs[page] = 1;
+    if (partial && j == 0) {
+      const int c = atomicAdd(&copies, 1);
+      pairs[2 * c] = lasts[lo];
+      pairs[2 * c + 1] = page;
+      atomicAdd(p.refs + lasts[lo], -1);
+    }
   };
+  // what a round finds: before which page of the wave's n-th 64 how many lie, and how many there are
+  auto add_up = [&] {
+    if (lane == 0)
+#pragma unroll
+      for (int e = 0; e < kRound; ++e) sums.put(e, __popcll(free[e]));
+    sums.add_up();
+  };
+  auto give = [&](int64_t p0, int found) {
+#pragma unroll
+    for (int e = 0; e < kRound; ++e) {
+      const int k = found + sums.before(e) + __popcll(free[e] & ((1ull << lane) - 1));
+      if ((free[e] >> lane & 1) && k < need) take(k, (int)(p0 + e * kTake + t));
+    }
+  };
+  // Nothing is given out before there is enough, so that a call without changes nothing:
+  // what is needed lies in the first round, mostly, or is looked for twice.
   int found = 0;
-  for (int64_t p0 = 0; p0 < p.num_pages && found < need; p0 += kRound * kTake) {
-    uint64_t free[kRound];
-#pragma unroll
-    for (int e = 0; e < kRound; ++e) {
-      const int64_t at = p0 + e * kTake + t;
-      free[e] = __builtin_amdgcn_ballot_w64(at < p.num_pages && p.refs[at] <= 0);
-      if (lane == 0) waves[e * 16 + wave] = __popcll(free[e]);
-    }
-    __syncthreads();
-    int all = found;
-#pragma unroll
-    for (int e = 0; e < kRound; ++e) {
-      int k = all + __popcll(free[e] & ((1ull << lane) - 1));
-#pragma unroll
-      for (int w = 0; w < 16; ++w) {
-        const int x = waves[e * 16 + w];
-        k += w < wave ? x : 0;
-        all += x;
-      }
-      if ((free[e] >> lane & 1) && k < need) p.table[place(k)] = (int32_t)(p0 + e * kTake + t);
-    }
-    found = all;
+  int64_t p0 = 0;
+  while (need > 0) {
+    add_up();
+    found += sums.total;
+    if (found >= need || p0 + kRound * kTake >= p.num_pages) break;
+    p0 += kRound * kTake;
+    look(p0);
     __syncthreads();
   }
   if (found < need) {  // nothing is taken, and what the sources held is theirs again
@@ -227,24 +345,30 @@ __global__ void __launch_bounds__(kTake) fork_take_kernel(const PagesForkParams 
     for (int q = wave; q < p.src_seqs; q += kTake / 64) {
       int children = 0;
       for (int i0 = 0; i0 < p.seqs; i0 += 64) children += __popcll(__builtin_amdgcn_ballot_w64(i0 + lane < p.seqs && p.parent[i0 + lane] == q));
-      const int keys = src_length(p, q);
+      const Reach r = reach_of(p, src_length(p, q));
       for (int64_t k = lane; k < p.ldtable; k += 64) {
-        const int by = change_of(p, keys, children, k);
-        const int id = page_id(p, p.src_table[q * p.ldtable + k]);
-        if (by && id >= 0) atomicAdd(p.refs + id, -by);
+        const int by = change_of(p, r, sink_pages(p), children, k);
+        const int id = by ? page_id(p, p.src_table[q * p.ldtable + k]) : -1;
+        if (id >= 0) atomicAdd(p.refs + id, -by);
       }
     }
-  } else {
-    for (int k = t; k < need; k += kTake) p.refs[p.table[place(k)]] = 1;
-    for (int c = t; c < copies; c += kTake) {
-      const int old = pairs[2 * c], i = pairs[2 * c + 1];
-      atomicAdd(p.refs + old, -1);
-      pairs[2 * c + 1] = p.table[i * p.ldtable + (src_length(p, p.parent[i]) >> p.lp)];
+  } else if (need > 0 && p0 == 0) {
+    give(0, 0);
+  } else if (need > 0) {
+    const int64_t last = p0;
+    int upto = 0;
+    for (p0 = 0; p0 <= last; p0 += kRound * kTake) {
+      __syncthreads();
+      look(p0);
+      add_up();
+      give(p0, upto);
+      upto += sums.total;
     }
   }
+  __syncthreads();
   if (t == 0) {
     *p.missing = found < need ? need - found : 0;
-    p.ws[0] = found < need ? 0 : copies;
+    p.ws[0] = copies;
   }
 }
 
@@ -259,6 +383,82 @@ __device__ __forceinline__ int32_t* ws_counts(const PagesCompactParams& p) { ret
 __device__ __forceinline__ int32_t* ws_moves(const PagesCompactParams& p) { return p.ws + 4 + ((chunks_of(p) + 1) & ~1LL); }
 __device__ __forceinline__ int32_t* ws_held(const PagesCompactParams& p) { return ws_moves(p) + (p.num_pages & ~1LL); }
 __device__ __forceinline__ int32_t* ws_new(const PagesCompactParams& p) { return ws_held(p) + p.num_pages / 2; }
+
+// All of it in one block, the pages' new numbers in LDS, for a small pool and tables: a
+// launch in the place of three.
+constexpr int kSmallPool = 4 * 1024, kSmallTable = 16 * 1024;
+__global__ void __launch_bounds__(1024) compact_small_kernel(const PagesCompactParams p) {
+  constexpr int N = kSmallPool / 1024;
+  __shared__ int name[kSmallPool], gaps[kSmallPool / 2];
+  __shared__ WaveSums<N> sums;
+  const int t = threadIdx.x, lane = t & 63, pages = (int)p.num_pages;
+  int32_t* moves = ws_moves(p);
+  int refs[N], rank[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) refs[e] = e * 1024 + t < pages ? p.refs[e * 1024 + t] : 0;
+  uint64_t on[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    on[e] = __builtin_amdgcn_ballot_w64(refs[e] > 0);
+    if (lane == 0) sums.put(e, __popcll(on[e]));
+  }
+  sums.add_up();
+  const int used = sums.total;
+#pragma unroll
+  for (int e = 0; e < N; ++e) rank[e] = sums.before(e) + __popcll(on[e] & ((1ull << lane) - 1));  // used pages in front
+  __syncthreads();
+  // of those that stay: the used pages among the first `used`
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const uint64_t stay = __builtin_amdgcn_ballot_w64(e * 1024 + t < used && refs[e] > 0);
+    if (lane == 0) sums.put(e, __popcll(stay));
+    if (e * 1024 + t < used && refs[e] <= 0) gaps[e * 1024 + t - rank[e]] = e * 1024 + t;
+  }
+  sums.add_up();
+  const int front = sums.total;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const int at = e * 1024 + t;
+    if (at >= pages) continue;
+    const bool moved = at >= used && refs[e] > 0;
+    const int to = moved ? gaps[rank[e] - front] : refs[e] > 0 ? at : -1;
+    name[at] = to;
+    if (p.map) p.map[at] = to;
+    if (refs[e] > 0) p.refs_out[to] = refs[e];
+    if (at >= used) p.refs_out[at] = 0;  // (no page goes there)
+    if (moved) {
+      moves[2 * (rank[e] - front)] = at;
+      moves[2 * (rank[e] - front) + 1] = to;
+    }
+  }
+  __syncthreads();
+  for (int i = t; i < (int)p.entries; i += 1024) {
+    const int id = p.table[i];
+    p.table_out[i] = id >= 0 && id < pages ? name[id] : -1;
+  }
+  if (t == 0) {
+    p.ws[0] = used - front;
+    *p.used = used;
+  }
+}
+
+// Inclusive sum over a block of 1024 (wave sums in LDS).
+__device__ __forceinline__ int block_sum(int v, int* waves, int* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  v = wave_upto(v);
+  if (lane == 63) waves[wave] = v;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) {
+    const int x = waves[w];
+    before += w < wave ? x : 0;
+    all += x;
+  }
+  __syncthreads();
+  *total = all;
+  return before + v;
+}
 
 // Used pages among [from, to), by a block of 1024.
 __device__ __forceinline__ int count_used(const PagesCompactParams& p, int64_t from, int64_t to, int* waves) {
@@ -348,20 +548,31 @@ hipError_t launch_pages_copy(const PagePlanes& planes, const PagesCopyParams& p,
   return hipGetLastError();
 }
 
-hipError_t launch_pages_fork(const PagesForkParams& p, PagesCopyParams* moves, hipStream_t s) {
-  if (p.src_seqs + p.seqs > 0) hipLaunchKernelGGL(fork_share_kernel, dim3(p.src_seqs + p.seqs), dim3(256), 0, s, p);
-  hipLaunchKernelGGL(fork_take_kernel, dim3(1), dim3(kTake), 0, s, p);
+hipError_t launch_pages_fork(const PagesForkParams& call, PagesCopyParams* moves, hipStream_t s) {
+  PagesForkParams p = call;
+  const bool little = p.seqs <= kTake && p.src_seqs <= kTake && (p.seqs + p.src_seqs) * p.ldtable <= 4 * kTake;
+  if (little) {
+    p.by_width = fastdiv_make((uint32_t)(p.ldtable > 0 ? p.ldtable : 1));
+    hipLaunchKernelGGL((fork_take_kernel<true>), dim3(1), dim3(kTake), 0, s, p);
+  } else {
+    hipLaunchKernelGGL(fork_share_kernel, dim3(p.src_seqs + p.seqs), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((fork_take_kernel<false>), dim3(1), dim3(kTake), 0, s, p);
+  }
   *moves = {p.ws + 4, p.seqs, p.ws, p.num_pages, p.num_pages};
   return hipGetLastError();
 }
 
 hipError_t launch_pages_compact(const PagesCompactParams& p, PagesCopyParams* moves, hipStream_t s) {
+  *moves = {p.ws + 4 + ((chunks_of(p) + 1) & ~1LL), p.num_pages / 2, p.ws, p.num_pages, p.num_pages};
+  if (p.num_pages <= kSmallPool && p.entries <= kSmallTable) {
+    hipLaunchKernelGGL(compact_small_kernel, dim3(1), dim3(1024), 0, s, p);
+    return hipGetLastError();
+  }
   const unsigned chunks = (unsigned)chunks_of(p);
   hipLaunchKernelGGL(compact_count_kernel, dim3(chunks), dim3(1024), 0, s, p);
   hipLaunchKernelGGL(compact_plan_kernel, dim3(chunks), dim3(1024), 0, s, p);
   const int64_t most = p.num_pages > p.entries ? p.num_pages : p.entries;
   hipLaunchKernelGGL(compact_rename_kernel, dim3((unsigned)(most / 256 < 1024 ? most / 256 + 1 : 1024)), dim3(256), 0, s, p);
-  *moves = {p.ws + 4 + ((chunks_of(p) + 1) & ~1LL), p.num_pages / 2, p.ws, p.num_pages, p.num_pages};
   return hipGetLastError();
 }
 

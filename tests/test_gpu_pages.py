@@ -127,6 +127,26 @@ def test_fork_of_many(ctx, pkg):
     pool.free()
 
 
+@pytest.mark.parametrize("seqs,src,width", [(1024, 1024, 2), (1025, 3, 2), (3, 1025, 2), (1, 1, 2048), (1, 1, 2049), (512, 512, 4), (512, 513, 4), (1030, 1030, 9)])
+def test_fork_around_the_small_calls(ctx, pkg, seqs, src, width):
+    """Both sides of the sizes that one block takes, and of those whose shared pages are counted in LDS."""
+    r = np.random.default_rng(seqs + width)
+    total = src * width + seqs * 3 + 50
+    pool = Pool(ctx, pkg, total, (16, 4), seed=1)
+    table = np.full((src, width), -1, np.int32)
+    length = r.integers(0, 16 * width - 3, src).astype(np.int32)
+    order = iter(r.permutation(total).tolist())
+    for q in range(src):
+        for j in range(-(-int(length[q]) // 16)):
+            table[q, j] = table[q - 1, j] if q % 3 == 2 and length[q] == length[q - 1] else next(order)
+    refs = np.zeros(total, np.int32)
+    np.add.at(refs, table[table >= 0], 1)
+    parent = r.integers(0, src, seqs).astype(np.int32)
+    _fork(ctx, pkg, pool, 16, refs, table, length, parent, r.integers(0, 3, seqs).astype(np.int32))
+    _fork(ctx, pkg, pool, 16, refs, table, length, np.full(seqs, src - 1, np.int32), np.ones(seqs, np.int32), window=20, sinks=3, keep=True)
+    pool.free()
+
+
 def test_fork_of_a_wide_table(ctx, pkg):
     """One sequence that takes thousands of pages at once."""
     pool = Pool(ctx, pkg, 9000, (16,), seed=8)
@@ -200,6 +220,21 @@ def test_compact(ctx, pkg, num_pages, used, in_place):
     got = compact(ctx, pkg, pool, refs, table, in_place)
     for name, a, b in zip(("refs", "table", "map", "used"), got, want):
         assert np.array_equal(a, b), name
+    pool.move(want[4])
+    pool.check()
+    pool.free()
+
+
+@pytest.mark.parametrize("num_pages,entries", [(300, 16384), (300, 16385), (4096, 1), (4097, 1), (4096, 40000)])
+def test_compact_around_the_small_pools(ctx, pkg, num_pages, entries):
+    """Both sides of the sizes that one block takes."""
+    r = np.random.default_rng(entries)
+    pool = Pool(ctx, pkg, num_pages, (48,), seed=3)
+    refs = (r.random(num_pages) < 0.6).astype(np.int32)
+    table = r.integers(-1, num_pages, (1, entries)).astype(np.int32)
+    want = compact_model(refs, table)
+    for a, b in zip(compact(ctx, pkg, pool, refs, table, True), want):
+        assert np.array_equal(a, b)
     pool.move(want[4])
     pool.check()
     pool.free()
