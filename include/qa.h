@@ -469,8 +469,8 @@ int qa_attention_paged_window_workspace(const qa_paged_window_desc* desc, size_t
  * hold, no call reads or writes outside its buffers.
  * No counterpart in the reference. */
 typedef struct qa_page_plane {
-  void* base;    /* 16-byte aligned */
-  int64_t bytes; /* of a page: a multiple of 16, or of 4 up to 4096, less than 2^31 */
+  void* base;    /* 16-byte aligned, or 4-byte aligned where pages have at most 4096 bytes */
+  int64_t bytes; /* of a page: a multiple of 16 less than 2^31, or of 4 up to 4096 */
 } qa_page_plane;
 
 /* pairs of pages (src, dst) int32 [npairs][2], on the device: dst takes src's bytes in

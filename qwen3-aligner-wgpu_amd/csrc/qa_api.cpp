@@ -586,8 +586,8 @@ int check_planes(const char* fn, const qa_page_plane* planes, int64_t n, int64_t
     const int64_t b = planes[i].bytes;
     if (b <= 0 || b > kI32 || b % 4 || (b % 16 && b > 4096))
       return fail(QA_EINVAL, "%s: plane %lld has pages of %lld bytes (a multiple of 16, or of 4 up to 4096)", fn, (long long)i, (long long)b);
-    if (!planes[i].base || !aligned(planes[i].base, 16))
-      return fail(QA_EINVAL, "%s: plane %lld is null or not 16-byte aligned", fn, (long long)i);
+    if (!planes[i].base || !aligned(planes[i].base, b > 4096 ? 16 : 4))
+      return fail(QA_EINVAL, "%s: plane %lld is null or not %d-byte aligned", fn, (long long)i, b > 4096 ? 16 : 4);
   }
   return ok();
 }

@@ -204,6 +204,18 @@ struct Cfg {
 //    that this gives, 19.7 in three; but 771 behind 1536 (200 blocks) 32 whole, 43 in two,
 //    as half the CUs' parts have to wait.  Up to 640 keys there is no gain (600 and none
 //    before, 4 kv heads of 64: 12.4 whole, 13.5 in three).
+//  * A window that is shorter than the longest sequence makes all of them about as long. Few:
+//    parts for one block a CU, in even numbers too, and none where the rounds of unsplit
+//    blocks are at least 0.7 full (us, unsplit / these parts / the rule above; windows of 4096:
+//    128 of them f16 56.2 / 55.8 / 59.6, e4m3 40.1 / 31.8 / 35.8; 384 f16 147.8 / - / 150.3,
+//    e4m3 of 4 heads 83.1 / - / 89.6). Many: a round of 128-pair blocks takes 1.7 of one of
+//    64-pair ones, so the fewer rounds by that (windows of 2048, 8 kv heads of 128, 64 / 128:
+//    600 rows 36.1 / 58.2, 1201 73.9 / 62.4, 2400 108.6 / 122.8, e4m3 1201 89.5 / 77.5; of 512,
+//    1201 rows 36.9 / 29.1; 12 prompts of up to 100 rows 74.7 / 64.7).  Its keys are split as
+//    far as there are CUs beside the short sequences' blocks (20 of those, 4 kv heads of 64,
+//    and 501 rows, window 700: 19.3 whole, 26.1 in two parts, which are more than the CUs),
+//    and into two from 900 keys on (400 rows, 8 of 128, whole / two: window 500 20.6 / 22.6,
+//    800 23.3 / 23.0, 1200 27.4 / 26.1).
 //  * kCus is a whole device's: the workspace has to be known without a device, so that
 //    on a partition of one the parts are more than its CUs need.
 constexpr int kFewRows = 16, kFewWaves = 4;
@@ -249,16 +261,20 @@ Split split_of(const PagedAttnParams& p, bool e4m3, int hd) {
   if (s.few) {
     const int64_t slots = !e4m3 && hd == 128 ? kCus : 2 * kCus;  // blocks that are at work at once
     const int64_t whole = heads <= kCus ? 20 * heads : 4096;
+    const bool alike = len < p.kv.max_len;  // a window cuts the sequences to one length
     int64_t parts = 1;
     if (heads > 0 && len > (whole > 512 ? whole : 512)) {
       const int64_t fill = (slots + heads - 1) / heads;
       const int64_t some = (heads < 4096 ? heads : 4096) * len * slots >> 26, most = len / 1024, even = some < most ? some : most;
       parts = (fill > even ? fill : even) | 1;
+      // rounds of blocks in tenths of what they could hold
+      const int64_t full = 10 * heads / ((heads + slots - 1) / slots * slots);
+      if (alike) parts = heads <= kCus ? kCus / heads : full >= 7 ? 1 : parts;
       parts = parts < 33 ? parts : 33;
     }
     // (rounding a part to 256 keys may leave an even number of them)
     do divide(parts, 256, &s.few_chunk, &s.few_chunks);
-    while (s.few_chunks % 2 == 0 && s.few_chunk > 256 && heads * s.few_chunks > slots && (parts += 2));
+    while (!alike && s.few_chunks % 2 == 0 && s.few_chunk > 256 && heads * s.few_chunks > slots && (parts += 2));
   }
   if (s.many) {
     // full tiles of a batch of this many rows, and a sequence's short last one; a
@@ -274,10 +290,19 @@ Split split_of(const PagedAttnParams& p, bool e4m3, int hd) {
       return p.kv.nkvh * (n < most(r) ? n : most(r));
     };
     s.many_rows = about(64) > 600 ? 128 : 64;
+    if (keys_at_most(p, 128 / p.rep + 2) < p.kv.max_len) {  // tiles of one length: by rounds of blocks
+      const int64_t small = (about(64) + kCus - 1) / kCus, large = (about(128) + kCus - 1) / kCus;
+      s.many_rows = 10 * small > 17 * large ? 128 : 64;
+    }
     s.tiles = (int)(pairs / s.many_rows + ends < most(s.many_rows) ? pairs / s.many_rows + ends : most(s.many_rows));
     const int64_t blocks = about(s.many_rows);
     len = keys_at_most(p, s.many_rows / p.rep + 2);
-    divide(len > 640 && blocks > 0 && blocks < kCus ? kCus / blocks : 1, 256, &s.many_chunk, &s.many_chunks);
+    int64_t parts = len > 640 && blocks > 0 && blocks < kCus ? kCus / blocks : 1;
+    if (len < p.kv.max_len && parts > 1) {  // the short sequences' blocks want their CUs too
+      const int64_t room = kCus - (s.few ? heads * s.few_chunks : 0);
+      parts = room < 2 * blocks || (room < 3 * blocks && len <= 900) ? 1 : room / blocks;
+    }
+    divide(parts, 256, &s.many_chunk, &s.many_chunks);
   }
   s.few_pairs = (int)(rows < kFewRows ? rows : kFewRows);
   const int64_t of_rows = p.kv.tokens * p.nqh, of_seqs = heads * s.few_pairs;

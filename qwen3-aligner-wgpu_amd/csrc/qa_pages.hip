@@ -10,14 +10,14 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 // ---- pages from one place to another ----
 //
 // blockIdx.y is the plane.  A wave takes 4 KB of a page at a time, four 16-byte loads
-// in flight for each lane; pages that are no multiple of 16 bytes, and short ones (scales), go
+// in flight for each lane; short pages (scales), and those that are not in 16 bytes, go
 // by words, a lane each.
 constexpr int kPiece = 4096;
 __global__ void __launch_bounds__(256) page_copy_kernel(const PagePlanes planes, const PagesCopyParams p) {
   const auto& pl = planes.at[blockIdx.y];
   const int64_t count = p.count ? clamp64(*p.count, 0, p.npairs) : p.npairs;
   const int64_t bytes = pl.bytes;
-  if (bytes % 16 || bytes < 1024) {
+  if (((uint64_t)pl.src | (uint64_t)pl.dst | (uint64_t)bytes) % 16 || bytes < 1024) {
     const int64_t words = bytes / 4;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count * words; i += (int64_t)gridDim.x * 256) {
       const int64_t pair = i / words, w = i - pair * words;

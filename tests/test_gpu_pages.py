@@ -273,6 +273,27 @@ def test_copy(ctx, pkg, sizes, n):
         x.free()
 
 
+def test_copy_of_planes_in_one_buffer(ctx, pkg):
+    """Every layer's scales in one tensor: planes that begin at any 4 bytes, also from and to different ones."""
+    n, layers, size = 7, 5, 12  # 84 bytes a layer
+    r = np.random.default_rng(6)
+    for words, sizes in ((3, (12,)), (1, (2048,)), (0, (4096,))):
+        size, extra = sizes[0], 4 * words
+        host = [r.integers(0, 256, 64 + layers * (n * size + extra), np.uint8) for _ in range(2)]
+        dev = [ctx.to_device(x) for x in host]
+        at = [[8 * k + i * (n * size + extra) for i in range(layers)] for k in range(2)]
+        src, dst = ((pkg.PagePlane * layers)(*[(int(d) + o, size) for o in at[k]]) for k, d in enumerate(dev))
+        pairs = np.array([[0, 6], [5, 1], [3, 3]], np.int32)
+        p = ctx.to_device(pairs)
+        ctx.pages_copy(pkg.PagesCopyDesc(flags=0, nplanes=layers, src=src, src_pages=n, dst=dst, dst_pages=n, pairs=int(p), npairs=3))
+        for i in range(layers):
+            for a, b in pairs:
+                host[1][at[1][i] + b * size: at[1][i] + (b + 1) * size] = host[0][at[0][i] + a * size: at[0][i] + (a + 1) * size]
+        assert np.array_equal(ctx.download(dev[1], host[1].shape, np.uint8), host[1])
+        for x in dev + [p]:
+            x.free()
+
+
 def test_copy_leaves_out_what_is_no_page(ctx, pkg):
     a, b = Pool(ctx, pkg, 9, SIZES, seed=1), Pool(ctx, pkg, 5, SIZES, seed=2)
     pairs = np.array([[0, 5], [9, 0], [-1, 1], [3, -1], [8, 4], [2 ** 31 - 1, 2], [2, 2 ** 31 - 1], [-2 ** 31, 3]], np.int32)

@@ -73,7 +73,8 @@ def test_copy_refusals(pkg):
         _refused(pkg, fn, _copy(pkg, sizes), needle)
     for kw, needle in ((dict(flags=1), "flags"), (dict(src_pages=0), "pages"), (dict(dst_pages=2 ** 31), "pages"), (dict(nplanes=-1), "nplanes"), (dict(nplanes=65537), "nplanes"),
                        (dict(npairs=-1), "npairs"), (dict(npairs=2 ** 31), "npairs"), (dict(pairs=None), "null"), (dict(pairs=0x300002), "misaligned"),
-                       (dict(src=None), "null planes"), (dict(dst=_planes(pkg, 4096, 48)), "48 bytes"), (dict(dst=_planes(pkg, 4096, 32, base=0x1000008)), "aligned"),
+                       (dict(src=None), "null planes"), (dict(dst=_planes(pkg, 4096, 48)), "48 bytes"), (dict(dst=_planes(pkg, 4096, 32, base=0x1000002)), "aligned"),
+                       (dict(dst=_planes(pkg, 8192, 32, base=0x1000008), src=_planes(pkg, 8192, 32)), "aligned"), (dict(dst=_planes(pkg, 4096, 32, base=0x1000004)), "null context"),
                        (dict(dst=_planes(pkg, 4096, 32, base=0)), "null"), (dict(), "null context")):
         _refused(pkg, fn, _copy(pkg, **kw), needle)
     assert fn(None, None) == pkg.QA_EINVAL
