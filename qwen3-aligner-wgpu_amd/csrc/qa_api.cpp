@@ -1286,7 +1286,7 @@ int qa_beam_select(qa_ctx* ctx, const qa_beam_desc* d) {
   if (!aligned(d->logits, 16) || !aligned(d->workspace, 16) || !aligned(d->score, 4) || !aligned(d->done, 4) || !aligned(d->parent, 4) ||
       !aligned(d->token, 4) || !aligned(d->score_out, 4) || !aligned(d->done_out, 4))
     return fail(QA_EINVAL, "qa_beam_select: misaligned pointer (logits and the workspace 16-byte aligned)");
-  qa::BeamParams p = beam_params(*d);
+  const qa::BeamParams p = beam_params(*d);
   const size_t need = qa::beam_select_workspace((int)d->dtype, p);
   if (need && (!d->workspace || d->workspace_bytes < need))
     return fail(QA_EINVAL, "qa_beam_select: a workspace of %zu bytes is needed, %zu given", need, d->workspace ? d->workspace_bytes : (size_t)0);
@@ -1299,7 +1299,6 @@ int qa_beam_select(qa_ctx* ctx, const qa_beam_desc* d) {
   if (!ctx) return fail(QA_EINVAL, "qa_beam_select: null context");
   if (d->groups == 0) return ok();
   if (int rc = set_device(ctx)) return rc;
-  p.cus = ctx->num_cus;
   const hipError_t e = qa::launch_beam_select((int)d->dtype, p, ctx->stream);
   return e == hipSuccess ? ok() : hip_fail(e, "qa_beam_select launch");
 }

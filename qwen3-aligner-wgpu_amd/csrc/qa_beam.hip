@@ -14,6 +14,7 @@ namespace qa {
 namespace {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr int kThreads = 256;
@@ -45,18 +46,14 @@ __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// The places of a list for the lanes of a wave that have something for it.
-__device__ __forceinline__ int list_place(int* length, bool mine) {
-  const uint64_t who = __builtin_amdgcn_ballot_w64(mine);
-  const int lane = threadIdx.x & 63, first = __builtin_ctzll(who);
-  int at = 0;
-  if (lane == first) at = atomicAdd(length, __popcll(who));
-  return __builtin_amdgcn_readlane(at, first) + __popcll(who & ((1ull << lane) - 1));
+// Logits of a thread, by how many there are in all: 8 below 0.5 M, 16 below 3 M, 32 beyond.  Small
+// chunks are more blocks and longer lists to merge (us with 8 / 16 / 32: 8 rows of 60000 9.8 / 9.8 /
+// 10.3, 64 of 12000 9.7 / 10.2 / 11.3, 4 of 151936 11.0 / 10.2 / 10.2, 12 of them 13.4 / 11.6 / 11.7,
+// 24 14.4 / 11.9 / 11.3, 192 39.7 / 27.9 / 22.8; 192 of 12000 10.8 / 10.8 / 11.6, of 32000 15.0 / 13.2 / 12.5).
+int each_of(const BeamParams& p) {
+  const int64_t all = p.groups * p.beams * p.vocab;
+  return all < 500000 ? 8 : all < 3000000 ? 16 : 32;
 }
-
-// Chunks of a row: as few as hold kThreads * each_of() logits at most, all as long but for the
-// last.
-int each_of(const BeamParams& p) { return p.groups * p.beams * ((p.vocab + 8191) / 8192) < 512 ? 8 : 32; }
 int64_t chunks_of(const BeamParams& p) { return (p.vocab + kThreads * each_of(p) - 1) / (kThreads * each_of(p)); }
 int chunk_of(const BeamParams& p) { return (int)(((p.vocab + chunks_of(p) - 1) / chunks_of(p) + 7) & ~7LL); }
 __device__ __forceinline__ Stat* stats(const BeamParams& p) { return (Stat*)p.ws; }
@@ -126,10 +123,12 @@ __device__ __forceinline__ void unpack(u32x4 w, float* x) {
 
 // The best `width` of a block's logits: the threads are taken as 4 to 64 groups, at least
 // `width` of them (every 4th to every 64th thread, so that a short chunk's have logits in
-// all), and what is below the least of the groups' best cannot be among them.  The others, about width * log width, are listed in LDS, and each one's rank is the
-// number of those before it.  More than the list holds, which many equal numbers can be,
-// go by rounds of the block.
-constexpr int kList = 1024;
+// all), and what is below the least of the groups' best cannot be among them.  The
+// others, about width * log width, are listed in LDS, each wave's apart (a shared counter
+// is a trip to the LDS for each of them), and each one's rank is the number of those
+// before it.  More than a wave's list holds, which many equal numbers can be, go by rounds
+// of the block.
+constexpr int kList = 256;
 __device__ __forceinline__ int groups_of(int width) { return width <= 4 ? 4 : width <= 8 ? 8 : width <= 16 ? 16 : width <= 32 ? 32 : 64; }
 
 template <int DT, int EACH>
@@ -137,8 +136,8 @@ __global__ void __launch_bounds__(kThreads) beam_chunk_kernel(const BeamParams p
   constexpr int N = kRun<DT>, RUNS = EACH / N, ES = DT == QA_F32 ? 4 : 2;
   constexpr float kLowest = -3.402823466e38f;
   __shared__ float best[kThreads / 64][64], vs[kThreads / 64];
-  __shared__ int is[kThreads / 64], ranks[kThreads / 64][64], length;
-  __shared__ __attribute__((aligned(16))) uint64_t list[kList];
+  __shared__ int is[kThreads / 64], ranks[kThreads / 64][64], lengths[kThreads / 64];
+  __shared__ __attribute__((aligned(16))) uint64_t lists[kThreads / 64][kList + 8];
   const int t = threadIdx.x, lane = t & 63, groups = groups_of(p.width);
   const int row = blockIdx.x / (uint32_t)chunks;
   const int64_t t0 = (int64_t)(blockIdx.x - row * chunks) * chunk_len, t1 = t0 + chunk_len < p.vocab ? t0 + chunk_len : p.vocab;
@@ -162,7 +161,6 @@ __global__ void __launch_bounds__(kThreads) beam_chunk_kernel(const BeamParams p
       for (int e = 0; e < N; ++e) x[r * N + e] = at + e < t1 ? logit<DT>(src, at + e) : -INFINITY;
   }
   auto token = [&](int j) { return (int)(t0 + (j / N * kThreads + t) * N + j % N); };
-  if (t == 0) length = 0;
   float own, top, least, sum;
   for (;;) {
     own = -INFINITY;
@@ -187,39 +185,67 @@ __global__ void __launch_bounds__(kThreads) beam_chunk_kernel(const BeamParams p
     for (int j = 0; j < EACH; ++j) x[j] = x[j] < INFINITY ? x[j] : -INFINITY;
   }
   if (t == 0) stats(p)[blockIdx.x] = {top, sum};
-  if (own >= least) {  // a few lanes
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  int mine_n = 0;  // the wave as one
 #pragma unroll
-    for (int j0 = 0; j0 < EACH; j0 += 4)
-      if (fmaxf(fmaxf(x[j0], x[j0 + 1]), fmaxf(x[j0 + 2], x[j0 + 3])) >= least)
+  for (int j0 = 0; j0 < EACH; j0 += 4)
+    if (__builtin_amdgcn_ballot_w64(fmaxf(fmaxf(x[j0], x[j0 + 1]), fmaxf(x[j0 + 2], x[j0 + 3])) >= least))
 #pragma unroll
-        for (int j = j0; j < j0 + 4; ++j)
-          if (x[j] >= least) {
-            const int at = list_place(&length, true);
-            if (at < kList) list[at] = key_of(x[j], token(j));
-          }
-  }
+      for (int j = j0; j < j0 + 4; ++j)
+        if (const uint64_t who = __builtin_amdgcn_ballot_w64(x[j] >= least)) {
+          const int at = mine_n + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+          if (x[j] >= least && at < kList) lists[wave][at] = key_of(x[j], token(j));
+          mine_n += __popcll(who);
+        }
+  if (lane < 8 && mine_n <= kList) lists[wave][mine_n + lane] = 0;  // behind the last
+  if (lane == 0) lengths[wave] = mine_n;
   lds_barrier();
   uint64_t* out = cands(p, chunks) + (int64_t)blockIdx.x * p.width;
-  const int n = __builtin_amdgcn_readfirstlane(length);
+  int ends[kThreads / 64], longest = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) {
+    const int n = __builtin_amdgcn_readfirstlane(lengths[w]);
+    longest = n > longest ? n : longest;
+    ends[w] = n + (w ? ends[w - 1] : 0);
+  }
+  const int n = ends[kThreads / 64 - 1];
+  // candidate number c of all
+  auto listed = [&](int c) {
+    int w = 0, first = 0;
+#pragma unroll
+    for (int v = 1; v < kThreads / 64; ++v)
+      if (c >= ends[v - 1]) {
+        w = v;
+        first = ends[v - 1];
+      }
+    return lists[w][c - first];
+  };
   if (n <= 64) {  // a lane for each, compared with a quarter of the others by each wave
-    const uint64_t mine = lane < n ? list[lane] : 0;
+    const uint64_t mine = lane < n ? listed(lane) : 0;
     int rank = 0;
-    for (int k = __builtin_amdgcn_readfirstlane(t >> 6); k < n; k += kThreads / 64) {
+    for (int k = wave; k < n; k += kThreads / 64) {
       const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), k) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)mine, k);
       rank += other > mine;
     }
-    ranks[t >> 6][lane] = rank;
+    ranks[wave][lane] = rank;
     lds_barrier();
     if (t < 64) {
       rank = lane < n ? (ranks[0][lane] + ranks[1][lane]) + (ranks[2][lane] + ranks[3][lane]) : lane;
       if (rank < p.width) out[rank] = mine;
     }
-  } else if (n <= kList) {
+  } else if (longest <= kList) {  // a thread for each, eight of the others at once
     for (int c = t; c < n; c += kThreads) {
-      const uint64_t mine = list[c];
+      const uint64_t mine = listed(c);
       int rank = 0;
-#pragma unroll 8
-      for (int k = 0; k < n; ++k) rank += list[k] > mine;
+#pragma unroll
+      for (int w = 0; w < kThreads / 64; ++w)
+        for (int k = 0; k < ends[w] - (w ? ends[w - 1] : 0); k += 8) {
+          u64x2 other[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) other[e] = *reinterpret_cast<const u64x2*>(lists[w] + k + 2 * e);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) rank += (other[e][0] > mine) + (other[e][1] > mine);
+        }
       if (rank < p.width) out[rank] = mine;
     }
   } else {
@@ -335,68 +361,82 @@ __device__ __forceinline__ double wave_sum(double x) {
   return x;
 }
 
-// A block for each group, a wave for each of its beams in turn: the beam's chunks' sums
-// joined, and their candidates merged by logit; then, by one wave, the beams'.
+// A block for each group, whose waves take the beams by turns, or, where one's lists are many
+// runs (kLong), several a part of them each: lists are merged by logit, the chunks' sums
+// joined by the first.  Then one wave merges the beams' by value.
+constexpr int kRankWaves = 16, kLong = 16;
 template <int LW>
-__global__ void __launch_bounds__(1024) beam_rank_kernel(const BeamParams p, int chunks) {
+__global__ void __launch_bounds__(64 * kRankWaves) beam_rank_kernel(const BeamParams p, int chunks, int of_beam) {
   constexpr int W = 1 << LW, RUNS = 64 >> LW;
   __shared__ double add[64];  // score - log sum of each beam
-  __shared__ uint64_t best[64 * W];
+  __shared__ uint64_t best[64 * W], parts[kRankWaves][W];
   const int64_t row0 = (int64_t)blockIdx.x * p.beams;
-  const int t = threadIdx.x, lane = t & 63, k = lane & (W - 1), run = lane >> LW;
-  for (int b = t >> 6; b < p.beams; b += blockDim.x >> 6) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int k = lane & (W - 1), run = lane >> LW;
+  const int part = wave % of_beam, teams = (int)(blockDim.x >> 6) / of_beam;
+  for (int b0 = 0; b0 < p.beams; b0 += teams) {  // (the same number of rounds for all waves)
+    const int b = b0 + wave / of_beam;
     const int64_t row = row0 + b;
-    const float score = p.score[row];
-    const bool over = p.done && p.done[row];
+    const float score = b < p.beams ? p.score[row] : -INFINITY;
+    const bool over = b < p.beams && p.done && p.done[row], live = !is_none(score) && !over;
     const Stat* st = stats(p) + row * chunks;
-    const uint64_t* cd = cands(p, chunks) + row * chunks * p.width;
-    auto load = [&](int c) { return c < chunks && k < p.width ? cd[(int64_t)c * p.width + k] : 0; };
-    const Stat first = lane < chunks ? st[lane] : Stat{-INFINITY, 0.f};
-    uint64_t x[4];
+    Stat first = {-INFINITY, 0.f};
+    uint64_t acc = 0;
+    if (live) {
+      const uint64_t* cd = cands(p, chunks) + row * chunks * p.width;
+      const int step = RUNS * of_beam;
+      auto load = [&](int c) { return c < chunks && k < p.width ? cd[(int64_t)c * p.width + k] : 0; };
+      if (part == 0 && lane < chunks) first = st[lane];
+      for (int c0 = part * RUNS; c0 < chunks; c0 += 4 * step) {
+        uint64_t x[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = load(e * RUNS + run);
-    if (is_none(score) || over) {
-      if (lane < W) best[b * W + lane] = lane == 0 && !is_none(score) ? key_of(0.f, p.end) : 0;
+        for (int e = 0; e < 4; ++e) x[e] = load(c0 + e * step + run);
+        if (c0 == part * RUNS) acc = x[0];
+        else acc = merged<LW>(acc, from_lane<W - 1>(x[0]));
+#pragma unroll
+        for (int e = 1; e < 4; ++e)
+          if (c0 + e * step < chunks) acc = merged<LW>(acc, from_lane<W - 1>(x[e]));
+      }
+      acc = wave_run<LW, W>(acc);
+    }
+    for (int n = of_beam / 2; n > 0; n /= 2) {  // the parts in pairs
+      if (lane < W) parts[wave][lane] = acc;
+      lds_barrier();
+      if (part < n) acc = merged<LW>(acc, parts[wave + n][W - 1 - k]);
+      lds_barrier();
+    }
+    if (part > 0 || b >= p.beams) continue;
+    if (live) {
+      float top = first.top;
+      for (int c = lane + 64; c < chunks; c += 64) top = fmaxf(top, st[c].top);
+      top = over_lanes(top, 1, larger);
+      double sum = first.sum == 0.f ? 0.0 : first.sum * exp((double)first.top - (double)top);
+      for (int c = lane + 64; c < chunks; c += 64)
+        if (st[c].sum != 0.f) sum += st[c].sum * exp((double)st[c].top - (double)top);
+      sum = wave_sum<32>(sum);
+      if (lane == 0) add[b] = (double)score - ((double)top + log(sum));
+    } else {
+      acc = k == 0 && !is_none(score) ? key_of(0.f, p.end) : 0;
       if (lane == 0) add[b] = score;
-      continue;
     }
-    uint64_t acc = x[0];
-    for (int c0 = 0;;) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (c0 + e * RUNS < chunks && c0 + e > 0) acc = merged<LW>(acc, from_lane<W - 1>(x[e]));
-      c0 += 4 * RUNS;
-      if (c0 >= chunks) break;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = load(c0 + e * RUNS + run);
-    }
-    acc = wave_run<LW, W>(acc);
-    float top = first.top;
-    for (int c = lane + 64; c < chunks; c += 64) top = fmaxf(top, st[c].top);
-    top = over_lanes(top, 1, larger);
-    double sum = first.sum == 0.f ? 0.0 : first.sum * exp((double)first.top - (double)top);
-    for (int c = lane + 64; c < chunks; c += 64)
-      if (st[c].sum != 0.f) sum += st[c].sum * exp((double)st[c].top - (double)top);
-    sum = wave_sum<32>(sum);
-    if (lane == 0) add[b] = (double)score - ((double)top + log(sum));
     if (lane < W) best[b * W + lane] = acc;
   }
   lds_barrier();
-  if (t >= 64) return;
+  if (wave > 0) return;
   auto load = [&](int b) {
     const uint64_t x = b < p.beams ? best[b * W + k] : 0;
     return x ? Total{add[b] + (double)logit_of(x), (uint32_t)(b * W + k)} : Total{-INFINITY, ~0u};
   };
-  Total acc = load(run);
-  for (int b0 = RUNS; b0 < p.beams; b0 += RUNS) acc = merged<LW>(acc, from_lane<W - 1>(load(b0 + run)));
-  acc = wave_run<LW, W>(acc);
+  Total all = load(run);
+  for (int b0 = RUNS; b0 < p.beams; b0 += RUNS) all = merged<LW>(all, from_lane<W - 1>(load(b0 + run)));
+  all = wave_run<LW, W>(all);
   if (lane >= p.width) return;
-  const bool on = acc.at != ~0u;
-  const int64_t row = row0 + (on ? acc.at >> LW : 0), o = (int64_t)blockIdx.x * p.width + lane;
-  const int token = on ? token_of(best[acc.at]) : -1;
+  const bool on = all.at != ~0u;
+  const int64_t row = row0 + (on ? all.at >> LW : 0), o = (int64_t)blockIdx.x * p.width + lane;
+  const int token = on ? token_of(best[all.at]) : -1;
   p.parent[o] = on ? (int)row : -1;
   p.token[o] = token;
-  p.score_out[o] = on ? (float)acc.v : -INFINITY;
+  p.score_out[o] = on ? (float)all.v : -INFINITY;
   p.done_out[o] = on && (token == p.end || (p.done && p.done[row]));
 }
 
@@ -404,12 +444,19 @@ template <int DT>
 void launch_chunks(const BeamParams& p, hipStream_t s) {
   const int chunks = (int)chunks_of(p);
   const dim3 grid((unsigned)(p.groups * p.beams * chunks));
-  if (each_of(p) == 8) hipLaunchKernelGGL((beam_chunk_kernel<DT, 8>), grid, dim3(kThreads), 0, s, p, chunks, chunk_of(p));
+  const int each = each_of(p);
+  if (each == 8) hipLaunchKernelGGL((beam_chunk_kernel<DT, 8>), grid, dim3(kThreads), 0, s, p, chunks, chunk_of(p));
+  else if (each == 16) hipLaunchKernelGGL((beam_chunk_kernel<DT, 16>), grid, dim3(kThreads), 0, s, p, chunks, chunk_of(p));
   else hipLaunchKernelGGL((beam_chunk_kernel<DT, 32>), grid, dim3(kThreads), 0, s, p, chunks, chunk_of(p));
 }
 template <int LW>
 void launch_rank(const BeamParams& p, hipStream_t s) {
-  hipLaunchKernelGGL((beam_rank_kernel<LW>), dim3((unsigned)p.groups), dim3(64 * (p.beams < 16 ? p.beams : 16)), 0, s, p, (int)chunks_of(p));
+  const int chunks = (int)chunks_of(p);
+  int of_beam = 1;
+  if (chunks > kLong * (64 >> LW))
+    while (2 * of_beam * p.beams <= kRankWaves) of_beam *= 2;
+  const int teams = p.beams < kRankWaves / of_beam ? p.beams : kRankWaves / of_beam;
+  hipLaunchKernelGGL((beam_rank_kernel<LW>), dim3((unsigned)p.groups), dim3(64 * of_beam * teams), 0, s, p, chunks, of_beam);
 }
 
 }  // namespace

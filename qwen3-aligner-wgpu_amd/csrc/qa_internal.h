@@ -438,7 +438,6 @@ struct BeamParams {
   float* score_out;
   int64_t groups, vocab, ldl;
   int beams, width, end;
-  int cus;
   void* ws;
 };
 size_t beam_select_workspace(int dtype, const BeamParams& p);
