@@ -495,8 +495,8 @@ int qa_pages_copy(qa_ctx* ctx, const qa_pages_copy_desc* desc);
  * parent's length; with window > 0 without those that no row from there on sees through
  * qa_attention_paged_window (all of the page at or behind `sinks` and at or before
  * length - window), whose entries become -1.  grow[i] rows are to be appended: len[i] is
- * the parent's length and grow[i], the kv_len of the next call, at most ldtable * page,
- * with new pages for them.  A last, partly filled page that is to be written on becomes
+ * the parent's length and grow[i], the kv_len of the next call, at most ldtable * page
+ * (and 2^30), with new pages for them.  A last, partly filled page that is to be written on becomes
  * the sequence's own: it is copied to a new page unless all that hold it are to write
  * on it and the sequence is the first of those.
  * The sources end with the call, with all that their rows name, reserved pages too,
@@ -506,9 +506,9 @@ int qa_pages_copy(qa_ctx* ctx, const qa_pages_copy_desc* desc);
  * refs and pages stay as they were, and the new sequences are empty.
  *   src_table  int32 [src_seqs][ldtable], src_len int32 [src_seqs] (held to
  *              [0, ldtable * page])
- *   table      int32 [seqs][ldtable] and len int32 [seqs], written; no part of the
- *              sources
+ *   table      int32 [seqs][ldtable] and len int32 [seqs], written
  *   parent     int32 [seqs]; grow int32 [seqs] (below 0: 0), or NULL for none
+ * What is written is no part of what is read.
  *   workspace  16-byte aligned, of the bytes that qa_pages_fork_workspace gives; its
  *              contents need not be kept, and calls that may run at the same time
  *              need one each

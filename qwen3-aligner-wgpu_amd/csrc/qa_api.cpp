@@ -1214,9 +1214,15 @@ int qa_pages_fork(qa_ctx* ctx, const qa_pages_fork_desc* d) {
   if (!aligned(d->refs, 4) || !aligned(d->missing, 4) || !aligned(d->src_table, 4) || !aligned(d->src_len, 4) || !aligned(d->parent, 4) ||
       !aligned(d->table, 4) || !aligned(d->len, 4) || !aligned(d->grow, 4) || !aligned(d->workspace, 16))
     return fail(QA_EINVAL, "qa_pages_fork: misaligned pointer (the workspace 16-byte aligned)");
-  const size_t rows = (size_t)d->ldtable * 4;
-  if (bytes_overlap(d->src_table, d->src_seqs * rows, d->table, d->seqs * rows) || bytes_overlap(d->src_len, (size_t)d->src_seqs * 4, d->len, (size_t)d->seqs * 4))
-    return fail(QA_EINVAL, "qa_pages_fork: table and len may be no part of the sources");
+  const size_t rows = (size_t)d->ldtable * 4, list = (size_t)d->seqs * 4;
+  const struct {
+    const void* at;
+    size_t bytes;
+  } in[] = {{d->src_table, d->src_seqs * rows}, {d->src_len, (size_t)d->src_seqs * 4}, {d->parent, list}, {d->grow, d->grow ? list : 0}},
+    out[] = {{d->table, d->seqs * rows}, {d->len, list}, {d->refs, (size_t)d->num_pages * 4}, {d->missing, 4}};
+  for (const auto& a : in)
+    for (const auto& b : out)
+      if (bytes_overlap(a.at, a.bytes, b.at, b.bytes)) return fail(QA_EINVAL, "qa_pages_fork: what is written may be no part of the sources, parent or grow");
   const qa::PagesForkParams p = fork_params(*d);
   const size_t need = qa::pages_fork_workspace(p);
   if (!d->workspace || d->workspace_bytes < need)

@@ -532,7 +532,9 @@ __global__ void __launch_bounds__(256) compact_rename_kernel(const PagesCompactP
 
 }  // namespace
 
-size_t pages_fork_workspace(const PagesForkParams& p) { return (4 + 2 * (size_t)p.seqs + 2 * (size_t)p.num_pages) * 4; }
+size_t pages_fork_workspace(const PagesForkParams& p) {
+  return (4 + 2 * (size_t)p.seqs + (p.seqs > kTake ? 2 * (size_t)p.num_pages : 0)) * 4;
+}
 size_t pages_compact_workspace(const PagesCompactParams& p) {
   return (size_t)(4 + ((chunks_of(p) + 1) & ~1LL) + (p.num_pages & ~1LL) + p.num_pages / 2 + p.num_pages) * 4;
 }
@@ -550,6 +552,8 @@ hipError_t launch_pages_copy(const PagePlanes& planes, const PagesCopyParams& p,
 
 hipError_t launch_pages_fork(const PagesForkParams& call, PagesCopyParams* moves, hipStream_t s) {
   PagesForkParams p = call;
+  // one launch up to 4096 entries, which are under way at once (8.4 us for 200, 13.2 in two
+  // launches); 11136 take 57.5 with the copies, 55.5 in two
   const bool little = p.seqs <= kTake && p.src_seqs <= kTake && (p.seqs + p.src_seqs) * p.ldtable <= 4 * kTake;
   if (little) {
     p.by_width = fastdiv_make((uint32_t)(p.ldtable > 0 ? p.ldtable : 1));

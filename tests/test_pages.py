@@ -92,8 +92,9 @@ def _fork(pkg, **kw):
     (dict(seqs=-1), "negative"), (dict(ldtable=-1), "negative"), (dict(seqs=8193), "8192"), (dict(src_seqs=8193), "8192"), (dict(ldtable=2 ** 30), "entries"),
     (dict(window=-1), "window"), (dict(sinks=2 ** 31), "sinks"), (dict(refs=None), "null"), (dict(missing=None), "null"), (dict(src_table=None), "null"), (dict(src_len=None), "null"),
     (dict(parent=None), "null"), (dict(table=None), "null"), (dict(len=None), "null"), (dict(grow=0x250001), "misaligned"), (dict(refs=0x100002), "misaligned"),
-    (dict(workspace=0x300008), "misaligned"), (dict(workspace=None), "workspace"), (dict(workspace_bytes=800), "workspace"), (dict(table=0x200000), "sources"),
-    (dict(table=0x200000 + 4 * 31), "sources"), (dict(len=0x210000 - 20), "sources"), (dict(nplanes=1, planes=None), "null planes"), (dict(), "null context")])
+    (dict(workspace=0x300008), "misaligned"), (dict(workspace=None), "workspace"), (dict(workspace_bytes=60), "workspace"), (dict(table=0x200000), "sources"),
+    (dict(table=0x200000 + 4 * 31), "sources"), (dict(len=0x210000 - 20), "sources"), (dict(len=0x220000), "sources"),
+    (dict(missing=0x250008), "sources"), (dict(refs=0x250000 - 396), "sources"), (dict(table=0x220000 - 4 * 47), "sources"), (dict(nplanes=1, planes=None), "null planes"), (dict(), "null context")])
 def test_fork_refusals(pkg, kw, needle):
     code = pkg.QA_EUNSUPPORTED if needle in ("page=8", "8192") else None
     _refused(pkg, pkg.lib().qa_pages_fork, _fork(pkg, **kw), needle, code)
@@ -116,7 +117,8 @@ def test_compact_refusals(pkg, kw, needle):
 
 def test_page_workspaces(pkg):
     """A few numbers for each page and sequence."""
-    assert 0 < pkg.pages_fork_workspace(_fork(pkg)) <= 64 + 8 * 6 + 8 * 100
+    assert 0 < pkg.pages_fork_workspace(_fork(pkg)) <= 64 + 8 * 6
+    assert pkg.pages_fork_workspace(_fork(pkg, seqs=1024)) <= 64 + 8 * 1024 < pkg.pages_fork_workspace(_fork(pkg, seqs=1025)) <= 64 + 8 * 1025 + 8 * 100
     assert 0 < pkg.pages_compact_workspace(_compact(pkg)) <= 64 + 12 * 100
     n = ctypes.c_size_t()
     assert pkg.lib().qa_pages_fork_workspace(ctypes.byref(_fork(pkg, page=5)), ctypes.byref(n)) == pkg.QA_EUNSUPPORTED
