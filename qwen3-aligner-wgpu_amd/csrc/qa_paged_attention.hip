@@ -40,6 +40,14 @@
 // 33 us, 367 TFLOP/s, 550 with the products of the residues.
 // Keys of long sequences are split among blocks, which leave (O, max, sum) in the
 // workspace for paged_join_kernel.
+//
+// With a window W and S sinks a row at p sees the keys j <= p with j > p - W or j < S.  The
+// kernels (WIN) go through the blocks of 64 keys that a tile's rows see as one run of keys
+// (Reach), so that what lies between costs nothing, and mask in the blocks where
+// some row's window begins, two comparisons a score.  One token in a window of 1024: 11.5 us,
+// 5 parts and their join (8.0 + 3.0); 48 tokens in windows of 4096 over e4m3, 32 q heads: 82.9 us,
+// 410 MB at 4.9 TB/s; 1201 rows in a window of 2048: 60.6 us, 152 blocks of 128 pairs, a
+// round on as many CUs of 256 (two rounds of 64-pair ones 70.9).
 #include <utility>
 
 #include "qa_internal.h"
