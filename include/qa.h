@@ -438,7 +438,9 @@ int qa_attention_paged_workspace(const qa_paged_attention_desc* desc, size_t* by
  * keep what lies between (qa_pages_fork gives those pages back).  Everything else is
  * as in qa_attention_paged, for the keys that rows see; what the pages hold that no row of
  * its sequence sees is not looked at, in front of the window as behind the last key, and
- * table entries there may be anything.  window in [1, 2^30], sinks in [0, 2^30]. */
+ * table entries there may be anything.  V has to be finite on all that some row of the
+ * sequence sees, and K may hold NaN where another row does not see it, as behind a
+ * row there.  window in [1, 2^30], sinks in [0, 2^30]. */
 typedef struct qa_paged_window_desc {
   uint32_t dtype;
   uint32_t flags; /* reserved, must be 0 */
@@ -511,7 +513,7 @@ int qa_pages_copy(qa_ctx* ctx, const qa_pages_copy_desc* desc);
  * What is written is no part of what is read.
  *   workspace  16-byte aligned, of the bytes that qa_pages_fork_workspace gives; its
  *              contents need not be kept, and calls that may run at the same time
- *              need one each
+ *              (over different pools) need one each
  * page 16, 32 or 64 tokens; seqs and src_seqs at most 8192. */
 enum { QA_PAGES_KEEP = 1u << 0 };
 typedef struct qa_pages_fork_desc {
@@ -540,8 +542,8 @@ int qa_pages_fork_workspace(const qa_pages_fork_desc* desc, size_t* bytes);
  * behind the first n goes into the k-th gap among those, and every other stays.
  *   refs_out   int32 [num_pages]: the references behind that, 0 from n on
  *   table      int32 [seqs][ldtable], table_out the same with the pages' new numbers;
- *              an entry that names no used page becomes -1.  refs_out and table_out may
- *              be refs and table.
+ *              an entry that names no used page becomes -1.  refs_out may be refs and
+ *              table_out table; what is written is else no part of the two.
  *   map        int32 [num_pages], each page's new number or -1, for tables elsewhere; or
  *              NULL
  *   used       int32: n

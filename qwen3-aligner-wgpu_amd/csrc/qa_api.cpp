@@ -1258,6 +1258,10 @@ int qa_pages_compact(qa_ctx* ctx, const qa_pages_compact_desc* d) {
   if ((d->refs != d->refs_out && bytes_overlap(d->refs, list, d->refs_out, list)) ||
       (d->table != d->table_out && bytes_overlap(d->table, entries, d->table_out, entries)))
     return fail(QA_EINVAL, "qa_pages_compact: refs_out and table_out are refs and table, or no part of them");
+  if (bytes_overlap(d->refs, list, d->table_out, entries) || bytes_overlap(d->table, entries, d->refs_out, list) ||
+      bytes_overlap(d->refs, list, d->map, d->map ? list : 0) || bytes_overlap(d->table, entries, d->map, d->map ? list : 0) ||
+      bytes_overlap(d->refs, list, d->used, 4) || bytes_overlap(d->table, entries, d->used, 4))
+    return fail(QA_EINVAL, "qa_pages_compact: what is written is no part of refs or table, but for refs_out and table_out in their place");
   const qa::PagesCompactParams p = compact_params(*d);
   const size_t need = qa::pages_compact_workspace(p);
   if (!d->workspace || d->workspace_bytes < need)
@@ -1297,11 +1301,12 @@ int qa_beam_select(qa_ctx* ctx, const qa_beam_desc* d) {
   if (need && (!d->workspace || d->workspace_bytes < need))
     return fail(QA_EINVAL, "qa_beam_select: a workspace of %zu bytes is needed, %zu given", need, d->workspace ? d->workspace_bytes : (size_t)0);
   const size_t in = (size_t)(d->groups * d->beams) * 4, out = (size_t)(d->groups * d->width) * 4;
-  const void* const ins[] = {d->score, d->done};
   const void* const outs[] = {d->parent, d->token, d->score_out, d->done_out};
-  for (const void* a : ins)
-    for (const void* b : outs)
-      if (a && bytes_overlap(a, in, b, out)) return fail(QA_EINVAL, "qa_beam_select: the outputs may be no part of score or done");
+  const size_t rows = (size_t)(d->groups * d->beams), esz = d->dtype == QA_F32 ? 4 : 2;
+  const size_t span = rows ? ((rows - 1) * (size_t)d->ldl + (size_t)d->vocab) * esz : 0;
+  for (const void* b : outs)
+    if (bytes_overlap(d->score, in, b, out) || bytes_overlap(d->done, d->done ? in : 0, b, out) || bytes_overlap(d->logits, span, b, out))
+      return fail(QA_EINVAL, "qa_beam_select: the outputs may be no part of logits, score or done");
   if (!ctx) return fail(QA_EINVAL, "qa_beam_select: null context");
   if (d->groups == 0) return ok();
   if (int rc = set_device(ctx)) return rc;

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 from hipgraph import Capture
-from paged import BF16, E4M3, F16, Batch, attention
+from paged import BF16, E4M3, F16, STALE8, STALE16, Batch, attention, widen
 from paged_window import assert_window, spoil_unseen, window_attention, window_desc
 
 pytestmark = pytest.mark.gpu
@@ -68,6 +68,22 @@ def test_all_keys_are_attention_paged(ctx, pkg, dtype, cache, n, lens, window, s
     b.upload(ctx)
     q = b.random_rows(4 * 128)
     assert np.array_equal(window_attention(ctx, pkg, b, q, window, sinks), attention(ctx, pkg, b, q))
+    b.free()
+
+
+@FORMATS
+@pytest.mark.parametrize("n", [8, 90])
+def test_keys_of_nan_in_front_of_a_window(ctx, pkg, dtype, cache, n):
+    """A key that the first row alone sees may be NaN: that row is, and no other."""
+    b = Batch([n], [200], 16, 2, 1, 64, dtype, cache, seed=42)
+    b.fill()
+    key = 200 - n - 59
+    b.k[b.table[0, key // 16], :, key % 16] = STALE8 if cache == E4M3 else STALE16[dtype]
+    b.upload(ctx)
+    q = b.random_rows(2 * 64)
+    got = window_attention(ctx, pkg, b, q, 60, 3)
+    assert_window(b, q, got, 60, 3, rows=range(1, n))
+    assert np.isnan(widen(got[0], dtype)).all()
     b.free()
 
 

@@ -110,6 +110,8 @@ def _compact(pkg, **kw):
     (dict(flags=1), "flags"), (dict(num_pages=0), "num_pages"), (dict(seqs=-1), "entries"), (dict(ldtable=2 ** 30), "entries"), (dict(refs=None), "null"),
     (dict(refs_out=None), "null"), (dict(used=None), "null"), (dict(table=None), "null"), (dict(table_out=None), "null"), (dict(map=0x220002), "misaligned"),
     (dict(workspace=0x300004), "misaligned"), (dict(workspace_bytes=100), "workspace"), (dict(refs_out=0x100004), "no part"), (dict(table_out=0x200000 + 4 * 47), "no part"),
+    (dict(map=0x100000), "no part"), (dict(map=0x200000 - 396), "no part"), (dict(used=0x200000 + 4 * 47), "no part"), (dict(used=0x100000), "no part"),
+    (dict(refs_out=0x200000), "no part"), (dict(table_out=0x100000), "no part"),
     (dict(refs_out=0x100000, table_out=0x200000), "null context"), (dict(), "null context")])
 def test_compact_refusals(pkg, kw, needle):
     _refused(pkg, pkg.lib().qa_pages_compact, _compact(pkg, **kw), needle)
@@ -158,7 +160,8 @@ def _beam(pkg, **kw):
     (dict(dtype=F32, ldl=1002), "ldl"), (dict(end=1000), "end"), (dict(end=-2), "end"), (dict(end=-1), "end"), (dict(logits=None), "null"), (dict(score=None), "null"),
     (dict(parent=None), "null"), (dict(done_out=None), "null"), (dict(logits=0x100008), "misaligned"), (dict(score=0x200002), "misaligned"), (dict(workspace=0x300004), "misaligned"),
     (dict(workspace=None), "workspace"), (dict(workspace_bytes=8), "workspace"), (dict(score_out=0x200000), "outputs"), (dict(done_out=0x210000), "outputs"),
-    (dict(parent=0x200000 - 60), "outputs"), (dict(groups=2 ** 24, vocab=10 ** 6, ldl=10 ** 6, workspace_bytes=2 ** 62), "too large"), (dict(dtype=F32, ldl=1004), "null context"),
+    (dict(parent=0x200000 - 60), "outputs"), (dict(token=0x100000 + 15996), "outputs"),
+    (dict(score_out=0x100000 + 31996, dtype=F32, ldl=1004), "outputs"), (dict(groups=2 ** 24, vocab=10 ** 6, ldl=10 ** 6, workspace_bytes=2 ** 62), "too large"), (dict(dtype=F32, ldl=1004), "null context"),
     (dict(done=None, end=-1), "null context"), (dict(), "null context")])
 def test_beam_refusals(pkg, kw, needle):
     code = pkg.QA_EUNSUPPORTED if needle.startswith(("beams", "width")) else None
