@@ -380,9 +380,9 @@ struct PagedAttnParams {
   float* ws;
   int64_t ldq, ldo;
   int nqh, rep;  // rep = nqh / nkvh
-  int window, sinks;  // window 0: a row sees all keys up to its own
   float scale;
   PagedParams kv;
+  int window, sinks;  // window 0: a row sees all keys up to its own
 };
 // Blocks of the larger of a call's launches, and the bytes of its workspace.
 int64_t paged_attention_blocks(bool e4m3, int hd, const PagedAttnParams& p);

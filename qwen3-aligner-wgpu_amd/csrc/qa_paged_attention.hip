@@ -34,7 +34,7 @@
 // Sequences of up to 16 pairs (single tokens): paged_few_kernel.  Bound by the
 // cache's bytes: 32 sequences of up to 4353 keys, 8 kv heads of 128, 342 MB in f16: 69 us,
 // 4.9 TB/s (a large copy: 5.1); 64 of up to 8193 in e4m3, 598 MB: 127 us, 4.7 TB/s.  The
-// smallest calls by latency: one sequence of 323 keys 8.4 us, of which launching is 4.
+// smallest calls by latency: one sequence of 323 keys 8.2 us, of which launching is 4.
 // Longer ones: paged_many_kernel, bound by the two phases of a step, of which the
 // softmax is as long as the products: 771 rows behind 1536 keys, 16 heads of 128:
 // 33 us, 367 TFLOP/s, 550 with the products of the residues.
@@ -44,9 +44,9 @@
 // With a window W and S sinks a row at p sees the keys j <= p with j > p - W or j < S.  The
 // kernels (WIN) go through the blocks of 64 keys that a tile's rows see as one run of keys
 // (Reach), so that what lies between costs nothing, and mask in the blocks where
-// some row's window begins, two comparisons a score.  One token in a window of 1024: 11.5 us,
-// 5 parts and their join (8.0 + 3.0); 48 tokens in windows of 4096 over e4m3, 32 q heads: 82.9 us,
-// 410 MB at 4.9 TB/s; 1201 rows in a window of 2048: 60.6 us, 152 blocks of 128 pairs, a
+// some row's window begins, two comparisons a score.  One token in a window of 1024: 10.8 us,
+// 5 parts and their join (7.6 + 2.8); 48 tokens in windows of 4096 over e4m3, 32 q heads: 81.8 us,
+// 410 MB at 5.0 TB/s; 1201 rows in a window of 2048: 60.0 us, 152 blocks of 128 pairs, a
 // round on as many CUs of 256 (two rounds of 64-pair ones 70.9).
 #include <utility>
 
@@ -333,6 +333,15 @@ __device__ __forceinline__ float* part_stats(const PagedAttnParams& p, const Spl
   return p.ws + (sp.few_parts + sp.many_parts) * hd;
 }
 
+// A kernel's arguments, 64 bytes to a line of the scalar cache, all asked for at once: as the
+// code comes to them each line is a trip to memory of its own.  One token behind 322 keys 8.4 ->
+// 8.2 us, in a window of 1024 11.5 -> 10.8, of which 0.2 in the join; 1201 rows 60.6 -> 60.0.
+// Without a window, e4m3 and the join go without (64 tokens behind up to 8192 keys 128.0,
+// asked in either 128.7; 20 tokens and a prompt 20.0 and 20.2).
+__device__ __forceinline__ void ask_for(const PagedAttnParams& p, const Split& sp) {
+  asm volatile("" ::"s"(p.q), "s"(p.kv.k), "s"(p.kv.nkvh), "s"(sp.many_parts));
+  __builtin_amdgcn_sched_barrier(0);
+}
 // With a window, a tile goes through the blocks of 64 keys that its rows see, those of
 // the sinks and from the one that the first row's window begins in, as one run of keys:
 // key number v of it is the sequence's key(v).  Without, key(v) is v.
@@ -818,6 +827,7 @@ __device__ __forceinline__ void few_block(const PagedAttnParams& p, const Split&
 
 template <int DT, bool F8, int HD, int LP, bool WIN>
 __global__ void __launch_bounds__(64 * kFewWaves) paged_few_kernel(const PagedAttnParams p, const Split sp) {
+  if constexpr (!F8 || WIN) ask_for(p, sp);
   __shared__ __attribute__((aligned(1024))) unsigned char smem[few_lds<DT, F8, HD>()];
   few_block<DT, F8, HD, LP, WIN>(p, sp, (int)blockIdx.x, smem);
 }
@@ -1042,6 +1052,7 @@ __device__ __forceinline__ bool find_tile(const PagedAttnParams& p, const Split&
 }
 template <int DT, bool F8, int HD, int LP, int GW, bool WIN>
 __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const PagedAttnParams p, const Split sp) {
+  if constexpr (!F8 || WIN) ask_for(p, sp);
   using C = Cfg<DT, F8, HD>;
   constexpr int NS = kManyWaves / GW, NB = many_buffers<DT, F8, HD, GW>(), WL = C::LI / GW;  // WL: a wave's loads of a tile
   constexpr int TR = GW * 32, VX = F8 ? 2 : 4;
@@ -1154,7 +1165,6 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
     va[e] = ((((x >> lcp) * HD + c) << lcp) + ((x & (cp - 1)) ^ (c >> (4 - lcp) & (cp - 1)))) * 16;
   }
   int have[2] = {16, 16};  // the lane's keys in the block of the last softmax
-  int last_kg = 0;         // and the first of them
   const int n0 = (nb + NS - 1) / NS, n1 = (nb + NS / 2 - 1) / NS;  // most steps of either half
   const int phases = max(2 * n0 + 1, 2 * n1 + 2);
   if (off == 0) wait_vmcnt<0>();
@@ -1163,7 +1173,8 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
     const int my = ph_no - off, it = my >> 1;
     if (my >= 0 && my <= 2 * steps) {
       if ((my & 1) == 0) {
-        const Seen seen[2] = {seen_of(reach, have[0], last_kg), seen_of(reach, have[1], last_kg + 32)};
+        const int last = WIN ? key_of(it - 1) + 16 * h : 0;  // the first of them
+        const Seen seen[2] = {seen_of(reach, have[0], last), seen_of(reach, have[1], last + 32)};
         if (it > 0 && __builtin_amdgcn_ballot_w64(some_unseen<WIN>(seen[0]) || some_unseen<WIN>(seen[1]))) {
           // V where no row sees it, or for no page, may be anything, NaN too: a
           // lane clears those elements of the chunks that it will read itself
@@ -1184,7 +1195,6 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2) paged_many_kernel(const Pa
       } else {
         const int kg = key_of(it) + 16 * h, j = scalar(it & 15);
         float f[2], vs[2] = {0.f, 0.f};
-        if constexpr (WIN) last_kg = kg;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           have[u] = sq.seen() - kg - 32 * u;
@@ -1266,6 +1276,7 @@ template <int HD>
 constexpr int kJoinPairs = 1024 / HD;
 template <int DT, int HD, bool WIN>
 __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p, const Split sp, int groups) {
+  if constexpr (WIN) ask_for(p, sp);
   constexpr int TP = HD / 4, NP = kJoinPairs<HD>;
   __shared__ f32x4 xo[NP][TP];
   __shared__ float xs[NP];
