@@ -9,9 +9,9 @@
 // by less would change places.  Equal ones go by (beam, token), so every comparison is
 // of (value, index) pairs of which no two are alike: results do not depend on timing.
 //
-// 192 rows of 151936 f16 logits, the best 8 of 8 beams: 21.4 us, the chunks 16 (58 MB at 3.7
-// TB/s: loads and maxima alone take 11.4, the exponentials 2.5 more, the lists and their
-// ranks 4), the join 4.8.  4 rows: 10.1 us, two launches and 5 trips to memory.
+// 192 rows of 151936 f16 logits, the best 8 of 8 beams: 20.7 us, the chunks 15.6 (58 MB at 3.7
+// TB/s: loads and maxima alone take 11.4, the exponentials 2 more, the lists and their
+// ranks the rest), the join 4.7.  4 rows: 9.9 us, two launches and 5 trips to memory.
 #include "qa_internal.h"
 
 namespace qa {
@@ -142,29 +142,34 @@ __global__ void __launch_bounds__(kThreads) beam_chunk_kernel(const BeamParams p
   __shared__ float best[kThreads / 64][64], vs[kThreads / 64];
   __shared__ int is[kThreads / 64], ranks[kThreads / 64][64], lengths[kThreads / 64];
   __shared__ __attribute__((aligned(16))) uint64_t lists[kThreads / 64][kList + 8];
+  asm volatile("" ::"s"(p.logits), "s"(p.width), "s"(chunks));  // the arguments in one trip to memory
+  __builtin_amdgcn_sched_barrier(0);
   const int t = threadIdx.x, lane = t & 63, groups = groups_of(p.width);
   const int row = blockIdx.x / (uint32_t)chunks;
-  const int64_t t0 = (int64_t)(blockIdx.x - row * chunks) * chunk_len, t1 = t0 + chunk_len < p.vocab ? t0 + chunk_len : p.vocab;
-  const char* src = (const char*)p.logits + row * p.ldl * ES;
+  const int64_t first = (int64_t)(blockIdx.x - row * chunks) * chunk_len;
+  const int t0 = (int)(first < p.vocab ? first : p.vocab), len = (int)(p.vocab - t0 < chunk_len ? p.vocab - t0 : chunk_len);
+  const char* src = (const char*)p.logits + (row * p.ldl + t0) * ES;
+  const float score = p.score[row];
+  const int over = (p.done ? p.done : (const int32_t*)p.score)[row];  // (no branch in front of the loads)
   // all loads first, of the chunk's first run where a thread has none
   u32x4 raw[RUNS] = {};
-  if (t1 - t0 >= N)
+  if (len >= N)
 #pragma unroll
     for (int r = 0; r < RUNS; ++r) {
-      const int64_t at = t0 + (r * kThreads + t) * N;
-      raw[r] = *reinterpret_cast<const u32x4*>(src + (at + N <= t1 ? at : t0) * ES);
+      const int at = (r * kThreads + t) * N;
+      raw[r] = *reinterpret_cast<const u32x4*>(src + (uint32_t)(at + N <= len ? at * ES : 0));
     }
-  if (is_none(p.score[row]) || (p.done && p.done[row])) return;
+  if (is_none(score) || (p.done && over)) return;
   float x[EACH];
 #pragma unroll
   for (int r = 0; r < RUNS; ++r) {
     unpack<DT>(raw[r], x + r * N);
-    const int64_t at = t0 + (r * kThreads + t) * N;
-    if (at + N > t1)
+    const int at = (r * kThreads + t) * N;
+    if (at + N > len)
 #pragma unroll
-      for (int e = 0; e < N; ++e) x[r * N + e] = at + e < t1 ? logit<DT>(src, at + e) : -INFINITY;
+      for (int e = 0; e < N; ++e) x[r * N + e] = at + e < len ? logit<DT>(src, at + e) : -INFINITY;
   }
-  auto token = [&](int j) { return (int)(t0 + (j / N * kThreads + t) * N + j % N); };
+  auto token = [&](int j) { return t0 + (j / N * kThreads + t) * N + j % N; };
   float own, top, least, sum;
   for (;;) {
     own = -INFINITY;
@@ -258,11 +263,11 @@ __global__ void __launch_bounds__(kThreads) beam_chunk_kernel(const BeamParams p
     auto next = [&](float v, int i, float* bv, int* bi) {
       *bv = -INFINITY;
       *bi = INT32_MAX;
-      for (int64_t k = t0 + t; k < t1; k += kThreads) {
+      for (int k = t; k < len; k += kThreads) {
         const float y = logit<DT>(src, k);
-        if (y < INFINITY && before(v, i, y, (int)k) && y > *bv) {
+        if (y < INFINITY && before(v, i, y, t0 + k) && y > *bv) {
           *bv = y;
-          *bi = (int)k;
+          *bi = t0 + k;
         }
       }
     };
