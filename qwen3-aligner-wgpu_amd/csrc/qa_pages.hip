@@ -19,31 +19,55 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 //
 // blockIdx.y is the plane.  A wave takes 4 KB of a page at a time, four 16-byte loads
 // in flight for each lane; short pages (scales), and those that are not in 16 bytes, go
-// by words, a lane each.
+// by words, a lane each.  The next pair is read in front of a piece's loads, the first along
+// with the number of pairs, which may turn out to be without it (84 pages' copies 3.1 us for
+// 3.4, 21 pages of 28 layers 15.0 for 15.4).
 constexpr int kPiece = 4096;
+// Number u, u + step .. of the units of the pairs' pages, `each` to a page.
+struct Unit {
+  uint32_t pair, part, pairs, parts, each;
+  __device__ __forceinline__ Unit(uint32_t u, uint32_t step, uint32_t n)
+      : pair(u / n), part(u - u / n * n), pairs(step / n), parts(step - step / n * n), each(n) {}
+  __device__ __forceinline__ void next() {
+    part += parts;
+    const uint32_t over = part >= each;
+    part -= over * each;
+    pair += pairs + over;
+  }
+};
 __global__ void __launch_bounds__(256) page_copy_kernel(const PagePlanes planes, const PagesCopyParams p) {
-  const auto& pl = planes.at[blockIdx.y];
-  const int64_t count = p.count ? clamp64(*p.count, 0, p.npairs) : p.npairs;
+  const auto pl = planes.at[blockIdx.y];
+  asm volatile("" ::"s"(pl.src), "s"(pl.dst), "s"(pl.bytes), "s"(p.count), "s"(p.dst_pages));  // in one trip to memory
+  __builtin_amdgcn_sched_barrier(0);
   const int64_t bytes = pl.bytes;
+  const uint32_t held = (uint32_t)p.npairs;
+  auto at = [&](uint32_t pair) { return p.pairs + 2 * (int64_t)(pair < held ? pair : 0); };
+  auto count = [&] { return p.count ? (uint32_t)clamp64(*p.count, 0, p.npairs) : held; };
+  auto is_pair = [&](int32_t a, int32_t b) { return a >= 0 && a < p.src_pages && b >= 0 && b < p.dst_pages; };
   if (((uint64_t)pl.src | (uint64_t)pl.dst | (uint64_t)bytes) % 16 || bytes < 1024) {
-    const int64_t words = bytes / 4;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count * words; i += (int64_t)gridDim.x * 256) {
-      const int64_t pair = i / words, w = i - pair * words;
-      const int32_t a = p.pairs[2 * pair], b = p.pairs[2 * pair + 1];
-      if (a < 0 || a >= p.src_pages || b < 0 || b >= p.dst_pages) continue;
-      *reinterpret_cast<uint32_t*>(pl.dst + b * bytes + 4 * w) = *reinterpret_cast<const uint32_t*>(pl.src + a * bytes + 4 * w);
+    Unit u(blockIdx.x * 256 + threadIdx.x, gridDim.x * 256, (uint32_t)bytes / 4);
+    int32_t a = at(u.pair)[0], b = at(u.pair)[1];
+    for (const uint32_t n = count(); u.pair < n;) {
+      if (is_pair(a, b))
+        *reinterpret_cast<uint32_t*>(pl.dst + b * bytes + 4 * u.part) = *reinterpret_cast<const uint32_t*>(pl.src + a * bytes + 4 * u.part);
+      u.next();
+      a = at(u.pair)[0];
+      b = at(u.pair)[1];
     }
     return;
   }
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t pieces = (bytes + kPiece - 1) / kPiece;
-  for (int64_t u = (int64_t)blockIdx.x * 4 + wave; u < count * pieces; u += (int64_t)gridDim.x * 4) {
-    const int64_t pair = u / pieces;
-    const int64_t off = (u - pair * pieces) * kPiece + lane * 16;
-    const int32_t a = p.pairs[2 * pair], b = p.pairs[2 * pair + 1];
-    if (a < 0 || a >= p.src_pages || b < 0 || b >= p.dst_pages) continue;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  Unit u(blockIdx.x * 4 + wave, gridDim.x * 4, ((uint32_t)bytes + kPiece - 1) / kPiece);
+  int32_t a = at(u.pair)[0], b = at(u.pair)[1];
+  for (const uint32_t n = count(); u.pair < n;) {
+    const int64_t off = (int64_t)u.part * kPiece + lane * 16;
     const unsigned char* from = pl.src + a * bytes + off;
     unsigned char* to = pl.dst + b * bytes + off;
+    const bool on = is_pair(a, b);
+    u.next();
+    a = at(u.pair)[0];
+    b = at(u.pair)[1];
+    if (!on) continue;
     u32x4 x[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e)
