@@ -74,8 +74,8 @@ int fail(int code, const char* fmt, ...) {
 
 int ok() { return QA_OK; }
 
-int hip_fail(hipError_t e, const char* what) {
-  return fail(e == hipErrorOutOfMemory ? QA_ENOMEM : QA_EDEVICE, "%s: %s (%d)", what,
+int hip_fail(hipError_t e, const char* what, const char* more = "") {
+  return fail(e == hipErrorOutOfMemory ? QA_ENOMEM : QA_EDEVICE, "%s%s: %s (%d)", what, more,
               hipGetErrorString(e), (int)e);
 }
 
@@ -564,7 +564,7 @@ int attention_paged(const char* fn, qa_ctx* ctx, const qa_paged_attention_desc& 
   p.ldo = d.ldo;
   p.scale = 1.0f / sqrtf((float)kv.hd);
   const hipError_t e = qa::launch_attention_paged((int)d.dtype, kv.dtype == QA_E4M3, kv.hd, p, ctx->stream);
-  return e == hipSuccess ? ok() : fail(QA_EDEVICE, "%s launch: %s (%d)", fn, hipGetErrorString(e), (int)e);
+  return e == hipSuccess ? ok() : hip_fail(e, fn, " launch");
 }
 int check_window(const char* fn, const qa_paged_window_desc& d) {
   if (d.window < 1 || d.window > 1 << 30 || d.sinks < 0 || d.sinks > 1 << 30)
@@ -599,7 +599,7 @@ int copy_planes(const char* fn, qa_ctx* ctx, const qa_page_plane* src, const qa_
     for (int i = 0; i < planes.n; ++i)
       planes.at[i] = {(const unsigned char*)src[i0 + i].base, (unsigned char*)dst[i0 + i].base, (uint32_t)src[i0 + i].bytes};
     const hipError_t e = qa::launch_pages_copy(planes, p, ctx->stream);
-    if (e != hipSuccess) return fail(QA_EDEVICE, "%s launch: %s (%d)", fn, hipGetErrorString(e), (int)e);
+    if (e != hipSuccess) return hip_fail(e, fn, " launch");
   }
   return ok();
 }
