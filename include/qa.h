@@ -506,6 +506,10 @@ int qa_pages_copy(qa_ctx* ctx, const qa_pages_copy_desc* desc);
  * pages are the lowest that are free behind that, in the order of sequences and
  * positions; *missing (int32, device) is how many there were too few.  Where it is not 0
  * refs and pages stay as they were, and the new sequences are empty.
+ * Growth behind the end of a row is cut off, and no shortage: len[i] is then less than the
+ * parent's length and grow[i], and the sequence, whose last page others may hold, must not be
+ * appended to.  Where the host does not know the lengths QA_PAGES_STRICT makes it one: the pages
+ * that such rows would need behind their ends count as missing (at most 2^31 - 1 in all).
  *   src_table  int32 [src_seqs][ldtable], src_len int32 [src_seqs] (held to
  *              [0, ldtable * page])
  *   table      int32 [seqs][ldtable] and len int32 [seqs], written
@@ -515,9 +519,9 @@ int qa_pages_copy(qa_ctx* ctx, const qa_pages_copy_desc* desc);
  *              contents need not be kept, and calls that may run at the same time
  *              (over different pools) need one each
  * page 16, 32 or 64 tokens; seqs and src_seqs at most 8192. */
-enum { QA_PAGES_KEEP = 1u << 0 };
+enum { QA_PAGES_KEEP = 1u << 0, QA_PAGES_STRICT = 1u << 2 };
 typedef struct qa_pages_fork_desc {
-  uint32_t flags; /* 0 or QA_PAGES_KEEP */
+  uint32_t flags; /* QA_PAGES_KEEP, QA_PAGES_STRICT */
   int32_t page;
   int64_t num_pages;
   const qa_page_plane* planes;

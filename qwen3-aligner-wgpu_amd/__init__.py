@@ -37,7 +37,7 @@ QA_ATTN_P16 = 1  # qa_attention_desc.flags
 QA_CONV_GELU, QA_CONV_TOKEN_MAJOR = 1, 2  # qa_conv_desc.flags
 MROPE_INTERLEAVED = 1  # qa_mrope_desc.flags
 F32 = 3  # qa_beam_desc.dtype alone
-PAGES_KEEP = 1  # qa_pages_fork_desc.flags
+PAGES_KEEP, PAGES_STRICT = 1, 4  # qa_pages_fork_desc.flags
 
 _STATUS = {
     QA_EINVAL: "QA_EINVAL",

@@ -631,6 +631,7 @@ qa::PagesForkParams fork_params(const qa_pages_fork_desc& d) {
   p.seqs = (int)d.seqs;
   p.lp = d.page == 16 ? 4 : d.page == 32 ? 5 : 6;
   p.keep = (d.flags & QA_PAGES_KEEP) != 0;
+  p.strict = (d.flags & QA_PAGES_STRICT) != 0;
   p.window = d.window;
   p.sinks = d.sinks;
   p.ws = (int32_t*)d.workspace;
@@ -1204,8 +1205,8 @@ int qa_pages_fork_workspace(const qa_pages_fork_desc* d, size_t* bytes) {
 
 int qa_pages_fork(qa_ctx* ctx, const qa_pages_fork_desc* d) {
   if (!d) return fail(QA_EINVAL, "qa_pages_fork: null argument");
-  if (d->flags & ~(uint32_t)QA_PAGES_KEEP)
-    return fail(QA_EINVAL, "qa_pages_fork: unknown flags 0x%x", d->flags & ~(uint32_t)QA_PAGES_KEEP);
+  constexpr uint32_t known = QA_PAGES_KEEP | QA_PAGES_STRICT;
+  if (d->flags & ~known) return fail(QA_EINVAL, "qa_pages_fork: unknown flags 0x%x", d->flags & ~known);
   if (int rc = check_fork_sizes("qa_pages_fork", *d)) return rc;
   if (int rc = check_planes("qa_pages_fork", d->planes, d->nplanes, d->num_pages)) return rc;
   const bool from = d->src_seqs > 0, to = d->seqs > 0, any = d->ldtable > 0;

@@ -410,7 +410,7 @@ struct PagesForkParams {
   const int32_t *src_table, *src_len, *parent, *grow;
   int32_t *refs, *table, *len, *missing;
   int64_t num_pages, ldtable;
-  int src_seqs, seqs, lp, keep;
+  int src_seqs, seqs, lp, keep, strict;
   int64_t window, sinks;
   FastDiv by_width;  // of a division by ldtable
   int32_t* ws;

@@ -194,9 +194,13 @@ __global__ void __launch_bounds__(kTake) fork_take_kernel(const PagesForkParams 
   __shared__ int slots[3 * kSlots];              // a page, how many write on it, the first of them
   __shared__ WaveSums<kRound> sums;
   __shared__ int copies;
+  __shared__ unsigned long long past;  // strict: pages behind the ends of rows
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, part = (1 << p.lp) - 1;
   const bool few = p.seqs <= kTake;
-  if (t == 0) copies = 0;
+  if (t == 0) {
+    copies = 0;
+    past = 0;
+  }
   if (few)
     for (int i = t; i < kSlots; i += kTake) {
       slots[i] = -1;
@@ -249,13 +253,16 @@ __global__ void __launch_bounds__(kTake) fork_take_kernel(const PagesForkParams 
     }
     settle();
   }
+  if constexpr (!SHARE) __syncthreads();  // the slots and `past` are clear
   // every sequence's growth; start[i]: the pages behind its last
   for (int i = t; i < p.seqs; i += kTake) {
     const int q = SHARE ? own_parent : p.parent[i], more = !is_source(p, q) ? 0 : SHARE ? own_grow : p.grow ? p.grow[i] : 0;
     int have;
     if constexpr (SHARE) have = held[i];
     else held[i] = have = is_source(p, q) ? src_length(p, q) : 0;
-    const int now = (int)clamp64((int64_t)have + (more > 0 ? more : 0), 0, capacity(p));
+    const int64_t want = (int64_t)have + (more > 0 ? more : 0);
+    const int now = (int)clamp64(want, 0, capacity(p));
+    if (p.strict && want > now) atomicAdd(&past, (unsigned long long)(((want + part) >> p.lp) - pages_of(p, now)));
     if (now == have) lasts[i] = -1;
     else if constexpr (!SHARE) lasts[i] = have & part ? p.table[i * p.ldtable + (have >> p.lp)] : -1;
     start[i] = pages_of(p, now) - pages_of(p, have);
@@ -264,7 +271,6 @@ __global__ void __launch_bounds__(kTake) fork_take_kernel(const PagesForkParams 
   int32_t *pairs = ws_pairs(p), *writers = ws_writers(p), *first = ws_first(p);
   uint32_t slot = 0;
   if (few) {
-    if constexpr (!SHARE) __syncthreads();  // the slots are clear
     const int last = t < p.seqs ? lasts[t] : -1;
     if (last >= 0) {
       slot = (uint32_t)last * 2654435761u >> 21;
@@ -371,7 +377,7 @@ __global__ void __launch_bounds__(kTake) fork_take_kernel(const PagesForkParams 
     look(p0);
     __syncthreads();
   }
-  if (found < need) {  // nothing is taken, and what the sources held is theirs again
+  if (found < need || past) {  // nothing is taken, and what the sources held is theirs again
     for (int64_t k = t; k < p.seqs * p.ldtable; k += kTake) p.table[k] = -1;
     for (int i = t; i < p.seqs; i += kTake) p.len[i] = 0;
     for (int q = wave; q < p.src_seqs; q += kTake / 64) {
@@ -399,7 +405,7 @@ __global__ void __launch_bounds__(kTake) fork_take_kernel(const PagesForkParams 
   }
   __syncthreads();
   if (t == 0) {
-    *p.missing = found < need ? need - found : 0;
+    *p.missing = (int)clamp64((found < need ? need - found : 0) + (int64_t)past, 0, INT32_MAX);
     p.ws[0] = copies;
   }
 }
