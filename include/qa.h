@@ -508,11 +508,20 @@ int qa_pages_copy(qa_ctx* ctx, const qa_pages_copy_desc* desc);
  * refs and pages stay as they were, and the new sequences are empty.
  * Growth behind the end of a row is cut off, and no shortage: len[i] is then less than the
  * parent's length and grow[i], and the sequence, whose last page others may hold, must not be
- * appended to.  Where the host does not know the lengths QA_PAGES_STRICT makes it one: the pages
- * that such rows would need behind their ends count as missing (at most 2^31 - 1 in all).
+ * appended to.  And *missing is each call's own, and a fork of the empty sequences behind a
+ * shortage writes over the table that alone names the pages in use: read it before that.
+ * Where the host neither knows the lengths nor looks at *missing behind every call, which is
+ * then 0 before the first, QA_PAGES_STRICT
+ *   - has the pages that rows would need behind their ends count as missing (at most
+ *     2^31 - 1 in all), and
+ *   - lets a call that finds *missing other than 0 write nothing but lengths, all 0.
+ * So calls that take turns stop at the first shortage, and rows appended behind it go nowhere.  The
+ * table that the failed call went from still names what is held: a call from it, to no
+ * sequences and with *missing 0, gives it back.
  *   src_table  int32 [src_seqs][ldtable], src_len int32 [src_seqs] (held to
  *              [0, ldtable * page])
  *   table      int32 [seqs][ldtable] and len int32 [seqs], written
+ *   missing    int32, written; with QA_PAGES_STRICT read too
  *   parent     int32 [seqs]; grow int32 [seqs] (below 0: 0), or NULL for none
  * What is written is no part of what is read.
  *   workspace  16-byte aligned, of the bytes that qa_pages_fork_workspace gives; its

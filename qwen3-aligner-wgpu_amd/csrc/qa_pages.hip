@@ -106,13 +106,18 @@ __device__ __forceinline__ int change_of(const PagesForkParams& p, Reach r, int 
   return (r.goes_on(sinks, k) ? children : 0) - (p.keep ? 0 : 1);
 }
 
+// Not 0 in a strict call behind a shortage, which leaves all but the lengths as it is.  Read first
+// and looked at in front of the first write, so that it is no trip to memory of its own.
+__device__ __forceinline__ int32_t shortage(const PagesForkParams& p) { return p.strict ? *p.missing : 0; }
+
 // Blocks of sources: references; blocks of sequences: their rows of the table, up to
 // the last page that they share.
 __global__ void __launch_bounds__(256) fork_share_kernel(const PagesForkParams p) {
-  const int b = blockIdx.x, sinks = sink_pages(p);
+  const int b = blockIdx.x, sinks = sink_pages(p), held = shortage(p);
   if (b >= p.src_seqs) {
     const int i = b - p.src_seqs, q = p.parent[i];
     const Reach r = is_source(p, q) ? reach_of(p, src_length(p, q)) : Reach{0, 0};
+    if (held) return;
     for (int64_t k = threadIdx.x; k < p.ldtable; k += 256)
       p.table[i * p.ldtable + k] = r.goes_on(sinks, k) ? page_id(p, p.src_table[q * p.ldtable + k]) : -1;
     return;
@@ -126,6 +131,7 @@ __global__ void __launch_bounds__(256) fork_share_kernel(const PagesForkParams p
   __syncthreads();
   const Reach r = reach_of(p, src_length(p, b));
   const int all = children;
+  if (held) return;
   for (int64_t k = threadIdx.x; k < p.ldtable; k += 256) {
     const int by = change_of(p, r, sinks, all, k);
     const int id = by ? page_id(p, p.src_table[b * p.ldtable + k]) : -1;
@@ -197,6 +203,11 @@ __global__ void __launch_bounds__(kTake) fork_take_kernel(const PagesForkParams 
   __shared__ unsigned long long past;  // strict: pages behind the ends of rows
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, part = (1 << p.lp) - 1;
   const bool few = p.seqs <= kTake;
+  const int before = shortage(p);
+  auto hold = [&] {
+    for (int i = t; i < p.seqs; i += kTake) p.len[i] = 0;
+    if (t == 0) p.ws[0] = 0;
+  };
   if (t == 0) {
     copies = 0;
     past = 0;
@@ -224,6 +235,7 @@ __global__ void __launch_bounds__(kTake) fork_take_kernel(const PagesForkParams 
       lasts[t] = -1;
     }
     __syncthreads();
+    if (before) return hold();
     const int width = (int)p.ldtable, entries = p.seqs * width, sources = p.src_seqs * width, sinks = sink_pages(p);
     const int most = entries > sources ? entries : sources;
     constexpr int B = 4;  // entries of either table under way
@@ -253,7 +265,10 @@ __global__ void __launch_bounds__(kTake) fork_take_kernel(const PagesForkParams 
     }
     settle();
   }
-  if constexpr (!SHARE) __syncthreads();  // the slots and `past` are clear
+  if constexpr (!SHARE) {
+    if (before) return hold();
+    __syncthreads();  // the slots and `past` are clear
+  }
   // every sequence's growth; start[i]: the pages behind its last
   for (int i = t; i < p.seqs; i += kTake) {
     const int q = SHARE ? own_parent : p.parent[i], more = !is_source(p, q) ? 0 : SHARE ? own_grow : p.grow ? p.grow[i] : 0;

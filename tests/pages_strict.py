@@ -8,8 +8,11 @@ import pages
 STRICT = 4
 
 
-def strict_model(refs, src_table, src_len, parent, grow, page, num_pages, **kw):
-    """fork_model where growth behind the end of a row is a shortage."""
+def strict_model(refs, src_table, src_len, parent, grow, page, num_pages, before=0, table=None, **kw):
+    """fork_model where growth behind the end of a row is a shortage; `before`: what *missing holds, which if not 0 leaves
+    `table` and all but the lengths as they are."""
+    if before:
+        return table, np.zeros(len(parent), np.int32), refs.astype(np.int32), before, []
     width = src_table.shape[1]
     cap = min(width * page, 2 ** 30)
     past = 0
@@ -23,12 +26,13 @@ def strict_model(refs, src_table, src_len, parent, grow, page, num_pages, **kw):
     return table, length, after, min(missing + past, 2 ** 31 - 1), pairs
 
 
-def strict_fork(ctx, pkg, pool, page, refs, table, length, parent, grow, **kw):
+def strict_fork(ctx, pkg, pool, page, refs, table, length, parent, grow, before=0, **kw):
     """The call, checked against the model: every number, every byte of the pool."""
-    want = strict_model(refs, table, length, parent, grow, page, pool.num_pages, **kw)
+    was = np.full((len(parent), table.shape[1]), 77, np.int32)  # (Fork's)
+    want = strict_model(refs, table, length, parent, grow, page, pool.num_pages, before=before, table=was, **kw)
     call = pages.Fork(ctx, pkg, pool, page, refs, table, length, parent, grow, **kw)
     call.desc.flags |= STRICT
-    ctx.upload(call.missing, np.zeros(1, np.int32))
+    ctx.upload(call.missing, np.array([before], np.int32))
     got = call.run().read()
     for name, a, b in zip(("table", "len", "refs", "missing"), got, want):
         assert np.array_equal(a, b), (name, a, b)

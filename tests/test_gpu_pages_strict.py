@@ -1,5 +1,5 @@
-"""qa_pages_fork with QA_PAGES_STRICT on an MI355X: growth that a row of the table cannot hold is a shortage, and no
-sequence goes on in a page that others hold."""
+"""qa_pages_fork with QA_PAGES_STRICT on an MI355X: growth that a row of the table cannot hold is a shortage, no
+sequence goes on in a page that others hold, and the calls behind a shortage leave what it left."""
 from __future__ import annotations
 
 import ctypes
@@ -10,25 +10,25 @@ import pytest
 import pages
 from hipgraph import Capture
 from pages import Fork, Pool, random_sequences
-from pages_strict import STRICT, strict_fork
+from pages_strict import STRICT, strict_fork, strict_model
 
 pytestmark = pytest.mark.gpu
 
 HD = 64
 
 
-def _append(ctx, pkg, pool, call, rows, seed):
-    """A qa_kv_append of `rows` rows for each sequence of `call`, over the pool's two planes (K and V of one head of 64)."""
-    tokens, width = rows * call.seqs, 3 * HD
+def _append(ctx, pkg, pool, seqs, width, table, length, rows, seed):
+    """A qa_kv_append of `rows` rows for each sequence, over the pool's two planes (K and V of one head of 64)."""
+    tokens, ld = rows * seqs, 3 * HD
     r = np.random.default_rng(seed)
     put = ctx.to_device
-    qkv, q = put(r.standard_normal((tokens, width)).astype(np.float16).view(np.uint16)), put(np.zeros((tokens, HD), np.uint16))
+    qkv, q = put(r.standard_normal((tokens, ld)).astype(np.float16).view(np.uint16)), put(np.zeros((tokens, HD), np.uint16))
     ones = put(np.ones(HD, np.float32))
     cos, sin = put(np.ones((tokens, HD), np.float32)), put(np.zeros((tokens, HD), np.float32))
-    start = put((rows * np.arange(call.seqs + 1)).astype(np.int32))
-    kv = pkg.PagedKV(dtype=pkg.F16, page=16, nkvh=1, hd=HD, num_pages=pool.num_pages, k=int(pool.dev[0]), v=int(pool.dev[1]), table=int(call.table),
-                     ldtable=call.width, seqs=call.seqs, row_start=int(start), kv_len=int(call.len), max_rows=rows, max_len=16 * call.width)
-    ctx.kv_append(pkg.KvAppendDesc(dtype=pkg.F16, flags=0, tokens=tokens, nqh=1, eps=1e-6, qkv=int(qkv), ldqkv=width, qn_w=int(ones), kn_w=int(ones),
+    start = put((rows * np.arange(seqs + 1)).astype(np.int32))
+    kv = pkg.PagedKV(dtype=pkg.F16, page=16, nkvh=1, hd=HD, num_pages=pool.num_pages, k=int(pool.dev[0]), v=int(pool.dev[1]), table=int(table),
+                     ldtable=width, seqs=seqs, row_start=int(start), kv_len=int(length), max_rows=rows, max_len=16 * width)
+    ctx.kv_append(pkg.KvAppendDesc(dtype=pkg.F16, flags=0, tokens=tokens, nqh=1, eps=1e-6, qkv=int(qkv), ldqkv=ld, qn_w=int(ones), kn_w=int(ones),
                                    cos=int(cos), sin=int(sin), q_out=int(q), ldq=HD, kv=ctypes.pointer(kv)))
     ctx.sync()
     for x in (qkv, q, ones, cos, sin, start):
@@ -51,7 +51,7 @@ def test_children_of_a_full_row(ctx, pkg, length, grow):
     assert got[3] == short, got
     if short:
         assert (got[0] == -1).all() and (got[1] == 0).all() and np.array_equal(got[2], refs)
-        _append(ctx, pkg, pool, call, grow, seed=2)
+        _append(ctx, pkg, pool, 2, 3, call.table, call.len, rows=grow, seed=2)
         pool.check()
     call.free()
     pool.free()
@@ -120,4 +120,80 @@ def test_captured(ctx, pkg):
         assert (got[2] == refs).all() == (length == 64)
     cap.close()
     call.free()
+    pool.free()
+
+
+@pytest.mark.parametrize("before", [1, -1, 2 ** 31 - 1])
+@pytest.mark.parametrize("keep", [False, True])
+@pytest.mark.parametrize("seqs,src,width,num_pages", [(6, 5, 6, 64), (300, 200, 12, 3000), (1300, 700, 6, 9000), (3, 0, 0, 5), (0, 5, 6, 64)])
+def test_behind_a_shortage(ctx, pkg, keep, before, seqs, src, width, num_pages):
+    """*missing other than 0: lengths of 0, and nothing else is written."""
+    r = np.random.default_rng(seqs + src)
+    pool = Pool(ctx, pkg, num_pages, (64, 4), seed=4)
+    table, length, refs = random_sequences(r, src, 16, width, num_pages, max(width - 2, 0) * 16)
+    length = np.asarray(length, np.int32)
+    strict_fork(ctx, pkg, pool, 16, refs, table.reshape(src, width), length, r.integers(-1, max(src, 1), seqs).astype(np.int32), np.ones(seqs, np.int32),
+                keep=keep, before=before)
+    pool.free()
+
+
+@pytest.mark.parametrize("first", [0, 1, 2])
+@pytest.mark.parametrize("cause", ["pages", "rows"])
+@pytest.mark.parametrize("seqs", [6, 300, 1200])
+def test_captured_steps_that_take_turns(ctx, pkg, cause, first, seqs):
+    """Two forks whose tables take turns, replayed past a shortage in the first step, the second or the third: tables, references and
+    pages stay what the last step that went well left, rows appended behind it go nowhere, and a call to no sequences
+    gives every page back."""
+    width, n = 16, 6 * seqs
+    r = np.random.default_rng(seqs + first)
+    pool = Pool(ctx, pkg, n, (2048, 2048), seed=5)
+    table, length, refs = random_sequences(r, seqs, 16, width, n, 60)
+    parent, ones = r.integers(0, seqs, seqs).astype(np.int32), np.ones(seqs, np.int32)
+    a = Fork(ctx, pkg, pool, 16, refs, table, length, parent, ones)
+    b = Fork(ctx, pkg, pool, 16, refs, table, length, parent, ones)
+    b.desc.refs, b.desc.src_table, b.desc.src_len, b.desc.table, b.desc.len = a.desc.refs, a.desc.table, a.desc.len, a.desc.src_table, a.desc.src_len
+    b.desc.missing = a.desc.missing
+    ctx.upload(a.missing, np.zeros(1, np.int32))
+    calls, at = (a, b), ((a.table, a.len), (a.src, a.len0))  # and where each writes
+    state, grow = [(np.full((seqs, width), 77, np.int32), None), (table, length)], [ones, ones]
+    for x in calls:
+        x.desc.flags |= STRICT
+    with Capture(ctx.stream) as cap:
+        for x in calls:
+            ctx.pages_fork(x.desc)
+    missing = [0]
+    for replay in range(3):
+        if first // 2 == replay:  # 7 pages for each, which the pool has not; or more than a row holds for one
+            k = first % 2
+            grow[k] = 112 * ones if cause == "pages" else np.where(np.arange(seqs) == 1, 16 * width + 1, 1).astype(np.int32)
+            ctx.upload(calls[k].grow, grow[k])
+        for k in range(2):
+            t, le, refs, m, pairs = strict_model(refs, *state[1 - k], parent, grow[k], 16, n, before=missing[-1], table=state[k][0])
+            pool.move(pairs)
+            state[k] = (t, le)
+            missing.append(m)
+        cap.replay()
+        assert int(pages._back(ctx, a.missing, (1,))[0]) == missing[-1]
+        assert np.array_equal(pages._back(ctx, a.refs, refs.shape), refs)
+        for k in range(2):
+            for buf, want in zip(at[k], state[k]):
+                assert np.array_equal(pages._back(ctx, buf, want.shape), want), (replay, k)
+        pool.check()
+        for k in range(2):
+            if (state[k][1] == 0).all():
+                _append(ctx, pkg, pool, seqs, width, *at[k], rows=1, seed=replay)
+        pool.check()
+    assert [m != 0 for m in missing[1:]] == [step >= first for step in range(6)] and len(set(missing[first + 1:])) == 1
+    cap.close()
+    k = 1 - first % 2  # where the last step that went well left its sequences
+    count = np.zeros(n, np.int32)
+    np.add.at(count, state[k][0][state[k][0] >= 0], 1)
+    assert np.array_equal(count, refs) and refs.sum() > 0
+    call = calls[1 - k]  # goes from there
+    call.desc.seqs = 0
+    ctx.upload(a.missing, np.zeros(1, np.int32))
+    ctx.pages_fork(call.desc)
+    assert (pages._back(ctx, a.refs, refs.shape) == 0).all() and int(pages._back(ctx, a.missing, (1,))[0]) == 0
+    for x in (a, b):
+        x.free()
     pool.free()
