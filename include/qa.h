@@ -523,7 +523,8 @@ int qa_pages_copy(qa_ctx* ctx, const qa_pages_copy_desc* desc);
  *   table      int32 [seqs][ldtable] and len int32 [seqs], written
  *   missing    int32, written; with QA_PAGES_STRICT read too
  *   parent     int32 [seqs]; grow int32 [seqs] (below 0: 0), or NULL for none
- * What is written is no part of what is read.
+ * What is written is no part of what is read, and no two of table, len, refs, missing and the
+ * workspace overlap.
  *   workspace  16-byte aligned, of the bytes that qa_pages_fork_workspace gives; its
  *              contents need not be kept, and calls that may run at the same time
  *              (over different pools) need one each
@@ -556,7 +557,8 @@ int qa_pages_fork_workspace(const qa_pages_fork_desc* desc, size_t* bytes);
  *   refs_out   int32 [num_pages]: the references behind that, 0 from n on
  *   table      int32 [seqs][ldtable], table_out the same with the pages' new numbers;
  *              an entry that names no used page becomes -1.  refs_out may be refs and
- *              table_out table; what is written is else no part of the two.
+ *              table_out table; what is written is else no part of the two, and no
+ *              two of the outputs and the workspace overlap.
  *   map        int32 [num_pages], each page's new number or -1, for tables elsewhere; or
  *              NULL
  *   used       int32: n

@@ -578,6 +578,20 @@ qa_paged_attention_desc without_window(const qa_paged_window_desc& d) {
 bool bytes_overlap(const void* a, size_t an, const void* b, size_t bn) {
   return an && bn && (uintptr_t)a < (uintptr_t)b + bn && (uintptr_t)b < (uintptr_t)a + an;
 }
+struct Bytes {
+  const void* at;
+  size_t n;
+};
+// Whether `ws` overlaps one of the spans, or one of the last n of them another of those.
+template <size_t N>
+bool some_overlap(const Bytes (&spans)[N], size_t n, Bytes ws) {
+  for (size_t i = 0; i < N; ++i) {
+    if (bytes_overlap(spans[i].at, spans[i].n, ws.at, ws.n)) return true;
+    for (size_t j = i + 1; i >= N - n && j < N; ++j)
+      if (bytes_overlap(spans[i].at, spans[i].n, spans[j].at, spans[j].n)) return true;
+  }
+  return false;
+}
 int check_planes(const char* fn, const qa_page_plane* planes, int64_t n, int64_t pages) {
   if (pages <= 0 || pages > kI32) return fail(QA_EINVAL, "%s: the number of pages must be in (0, 2^31)", fn);
   if (n < 0 || n > 65536) return fail(QA_EINVAL, "%s: nplanes must be in [0, 65536]", fn);
@@ -1216,18 +1230,17 @@ int qa_pages_fork(qa_ctx* ctx, const qa_pages_fork_desc* d) {
       !aligned(d->table, 4) || !aligned(d->len, 4) || !aligned(d->grow, 4) || !aligned(d->workspace, 16))
     return fail(QA_EINVAL, "qa_pages_fork: misaligned pointer (the workspace 16-byte aligned)");
   const size_t rows = (size_t)d->ldtable * 4, list = (size_t)d->seqs * 4;
-  const struct {
-    const void* at;
-    size_t bytes;
-  } in[] = {{d->src_table, d->src_seqs * rows}, {d->src_len, (size_t)d->src_seqs * 4}, {d->parent, list}, {d->grow, d->grow ? list : 0}},
-    out[] = {{d->table, d->seqs * rows}, {d->len, list}, {d->refs, (size_t)d->num_pages * 4}, {d->missing, 4}};
+  const Bytes in[] = {{d->src_table, d->src_seqs * rows}, {d->src_len, (size_t)d->src_seqs * 4}, {d->parent, list}, {d->grow, d->grow ? list : 0}},
+              out[] = {{d->table, d->seqs * rows}, {d->len, list}, {d->refs, (size_t)d->num_pages * 4}, {d->missing, 4}};
   for (const auto& a : in)
     for (const auto& b : out)
-      if (bytes_overlap(a.at, a.bytes, b.at, b.bytes)) return fail(QA_EINVAL, "qa_pages_fork: what is written may be no part of the sources, parent or grow");
+      if (bytes_overlap(a.at, a.n, b.at, b.n)) return fail(QA_EINVAL, "qa_pages_fork: what is written may be no part of the sources, parent or grow");
   const qa::PagesForkParams p = fork_params(*d);
   const size_t need = qa::pages_fork_workspace(p);
   if (!d->workspace || d->workspace_bytes < need)
     return fail(QA_EINVAL, "qa_pages_fork: a workspace of %zu bytes is needed, %zu given", need, d->workspace ? d->workspace_bytes : (size_t)0);
+  if (some_overlap(in, 0, {d->workspace, need}) || some_overlap(out, 4, {d->workspace, need}))
+    return fail(QA_EINVAL, "qa_pages_fork: what is written and the workspace may not overlap");
   if (!ctx) return fail(QA_EINVAL, "qa_pages_fork: null context");
   if (int rc = set_device(ctx)) return rc;
   qa::PagesCopyParams moves{};
@@ -1267,6 +1280,9 @@ int qa_pages_compact(qa_ctx* ctx, const qa_pages_compact_desc* d) {
   const size_t need = qa::pages_compact_workspace(p);
   if (!d->workspace || d->workspace_bytes < need)
     return fail(QA_EINVAL, "qa_pages_compact: a workspace of %zu bytes is needed, %zu given", need, d->workspace ? d->workspace_bytes : (size_t)0);
+  const Bytes spans[] = {{d->refs, list}, {d->table, entries}, {d->refs_out, list}, {d->table_out, entries}, {d->map, d->map ? list : 0}, {d->used, 4}};
+  if (some_overlap(spans, 4, {d->workspace, need}))
+    return fail(QA_EINVAL, "qa_pages_compact: what is written and the workspace may not overlap");
   if (!ctx) return fail(QA_EINVAL, "qa_pages_compact: null context");
   if (int rc = set_device(ctx)) return rc;
   qa::PagesCopyParams moves{};
