@@ -410,10 +410,11 @@ struct PagesForkParams {
   const int32_t *src_table, *src_len, *parent, *grow;
   int32_t *refs, *table, *len, *missing;
   int64_t num_pages, ldtable;
-  int src_seqs, seqs, lp, keep, strict;
+  int src_seqs, seqs, lp, keep;
   int64_t window, sinks;
   FastDiv by_width;  // of a division by ldtable
   int32_t* ws;
+  int strict;  // for the launch, which has kernels of its own for it
 };
 struct PagesCompactParams {
   const int32_t *refs, *table;

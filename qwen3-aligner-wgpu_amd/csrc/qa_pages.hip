@@ -106,14 +106,21 @@ __device__ __forceinline__ int change_of(const PagesForkParams& p, Reach r, int 
   return (r.goes_on(sinks, k) ? children : 0) - (p.keep ? 0 : 1);
 }
 
-// Not 0 in a strict call behind a shortage, which leaves all but the lengths as it is.  Read first
-// and looked at in front of the first write, so that it is no trip to memory of its own.
-__device__ __forceinline__ int32_t shortage(const PagesForkParams& p) { return p.strict ? *p.missing : 0; }
+// STRICT: growth behind the end of a row is a shortage, and a call behind one leaves all but the
+// lengths as it is.  Not 0 then; read first and looked at in front of the first write, so that it is no
+// trip to memory of its own.  Kernels of their own, as a flag among the arguments is one in calls
+// without it (192 sequences 55.2 us, with such a flag 55.8; strict 55.6).
+template <bool STRICT>
+__device__ __forceinline__ int32_t shortage(const PagesForkParams& p) {
+  if constexpr (STRICT) return *p.missing;
+  else return 0;
+}
 
 // Blocks of sources: references; blocks of sequences: their rows of the table, up to
 // the last page that they share.
+template <bool STRICT>
 __global__ void __launch_bounds__(256) fork_share_kernel(const PagesForkParams p) {
-  const int b = blockIdx.x, sinks = sink_pages(p), held = shortage(p);
+  const int b = blockIdx.x, sinks = sink_pages(p), held = shortage<STRICT>(p);
   if (b >= p.src_seqs) {
     const int i = b - p.src_seqs, q = p.parent[i];
     const Reach r = is_source(p, q) ? reach_of(p, src_length(p, q)) : Reach{0, 0};
@@ -191,7 +198,7 @@ struct WaveSums {
 // Sequences with the same last page are counted in an LDS table of pages, for up to kTake
 // of them, and in the workspace beyond (three trips to memory: 2 us).
 constexpr int kTake = 1024, kRound = 4, kSlots = 2048;
-template <bool SHARE>
+template <bool SHARE, bool STRICT>
 __global__ void __launch_bounds__(kTake) fork_take_kernel(const PagesForkParams p) {
   __shared__ int start[kForkSeqs];  // pages taken before sequence i; bit 31: its first is a copy
   __shared__ int held[kForkSeqs];   // its parent's keys
@@ -200,17 +207,17 @@ __global__ void __launch_bounds__(kTake) fork_take_kernel(const PagesForkParams 
   __shared__ int slots[3 * kSlots];              // a page, how many write on it, the first of them
   __shared__ WaveSums<kRound> sums;
   __shared__ int copies;
-  __shared__ unsigned long long past;  // strict: pages behind the ends of rows
+  __shared__ unsigned long long past;  // STRICT: pages behind the ends of rows
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, part = (1 << p.lp) - 1;
   const bool few = p.seqs <= kTake;
-  const int before = shortage(p);
+  const int before = shortage<STRICT>(p);
   auto hold = [&] {
     for (int i = t; i < p.seqs; i += kTake) p.len[i] = 0;
     if (t == 0) p.ws[0] = 0;
   };
   if (t == 0) {
     copies = 0;
-    past = 0;
+    if constexpr (STRICT) past = 0;
   }
   if (few)
     for (int i = t; i < kSlots; i += kTake) {
@@ -265,10 +272,8 @@ __global__ void __launch_bounds__(kTake) fork_take_kernel(const PagesForkParams 
     }
     settle();
   }
-  if constexpr (!SHARE) {
-    if (before) return hold();
-    __syncthreads();  // the slots and `past` are clear
-  }
+  if (!SHARE && before) return hold();
+  int64_t behind = 0;  // STRICT: pages behind the ends of the thread's rows
   // every sequence's growth; start[i]: the pages behind its last
   for (int i = t; i < p.seqs; i += kTake) {
     const int q = SHARE ? own_parent : p.parent[i], more = !is_source(p, q) ? 0 : SHARE ? own_grow : p.grow ? p.grow[i] : 0;
@@ -277,7 +282,7 @@ __global__ void __launch_bounds__(kTake) fork_take_kernel(const PagesForkParams 
     else held[i] = have = is_source(p, q) ? src_length(p, q) : 0;
     const int64_t want = (int64_t)have + (more > 0 ? more : 0);
     const int now = (int)clamp64(want, 0, capacity(p));
-    if (p.strict && want > now) atomicAdd(&past, (unsigned long long)(((want + part) >> p.lp) - pages_of(p, now)));
+    if (STRICT && want > now) behind += ((want + part) >> p.lp) - pages_of(p, now);
     if (now == have) lasts[i] = -1;
     else if constexpr (!SHARE) lasts[i] = have & part ? p.table[i * p.ldtable + (have >> p.lp)] : -1;
     start[i] = pages_of(p, now) - pages_of(p, have);
@@ -286,6 +291,7 @@ __global__ void __launch_bounds__(kTake) fork_take_kernel(const PagesForkParams 
   int32_t *pairs = ws_pairs(p), *writers = ws_writers(p), *first = ws_first(p);
   uint32_t slot = 0;
   if (few) {
+    if constexpr (!SHARE) __syncthreads();  // the slots are clear
     const int last = t < p.seqs ? lasts[t] : -1;
     if (last >= 0) {
       slot = (uint32_t)last * 2654435761u >> 21;
@@ -310,6 +316,7 @@ __global__ void __launch_bounds__(kTake) fork_take_kernel(const PagesForkParams 
       }
     settle();
   }
+  if (STRICT && behind > 0) atomicAdd(&past, (unsigned long long)behind);
   const int mine0 = t < p.seqs && lasts[t] >= 0 ? peek(p.refs + lasts[t]) : 1;  // of the thread's first sequence
   // A round of the search for free pages; the first one's loads go out here.
   uint64_t free[kRound];
@@ -392,7 +399,7 @@ __global__ void __launch_bounds__(kTake) fork_take_kernel(const PagesForkParams 
     look(p0);
     __syncthreads();
   }
-  if (found < need || past) {  // nothing is taken, and what the sources held is theirs again
+  if (found < need || (STRICT && past)) {  // nothing is taken, and what the sources held is theirs again
     for (int64_t k = t; k < p.seqs * p.ldtable; k += kTake) p.table[k] = -1;
     for (int i = t; i < p.seqs; i += kTake) p.len[i] = 0;
     for (int q = wave; q < p.src_seqs; q += kTake / 64) {
@@ -420,7 +427,9 @@ __global__ void __launch_bounds__(kTake) fork_take_kernel(const PagesForkParams 
   }
   __syncthreads();
   if (t == 0) {
-    *p.missing = (int)clamp64((found < need ? need - found : 0) + (int64_t)past, 0, INT32_MAX);
+    const int lacking = found < need ? need - found : 0;
+    if constexpr (STRICT) *p.missing = (int)clamp64(lacking + (int64_t)past, 0, INT32_MAX);
+    else *p.missing = lacking;
     p.ws[0] = copies;
   }
 }
@@ -583,6 +592,20 @@ __global__ void __launch_bounds__(256) compact_rename_kernel(const PagesCompactP
   for (int64_t i = first; i < p.entries; i += step) p.table_out[i] = name(p.table[i]);
 }
 
+template <bool STRICT>
+void launch_fork(PagesForkParams p, hipStream_t s) {
+  // one launch up to 4096 entries, which are under way at once (8.4 us for 200, 13.2 in two
+  // launches); 11136 take 57.5 with the copies, 55.5 in two
+  const bool little = p.seqs <= kTake && p.src_seqs <= kTake && (p.seqs + p.src_seqs) * p.ldtable <= 4 * kTake;
+  if (little) {
+    p.by_width = fastdiv_make((uint32_t)(p.ldtable > 0 ? p.ldtable : 1));
+    hipLaunchKernelGGL((fork_take_kernel<true, STRICT>), dim3(1), dim3(kTake), 0, s, p);
+  } else {
+    hipLaunchKernelGGL((fork_share_kernel<STRICT>), dim3(p.src_seqs + p.seqs), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((fork_take_kernel<false, STRICT>), dim3(1), dim3(kTake), 0, s, p);
+  }
+}
+
 }  // namespace
 
 size_t pages_fork_workspace(const PagesForkParams& p) {
@@ -603,18 +626,9 @@ hipError_t launch_pages_copy(const PagePlanes& planes, const PagesCopyParams& p,
   return hipGetLastError();
 }
 
-hipError_t launch_pages_fork(const PagesForkParams& call, PagesCopyParams* moves, hipStream_t s) {
-  PagesForkParams p = call;
-  // one launch up to 4096 entries, which are under way at once (8.4 us for 200, 13.2 in two
-  // launches); 11136 take 57.5 with the copies, 55.5 in two
-  const bool little = p.seqs <= kTake && p.src_seqs <= kTake && (p.seqs + p.src_seqs) * p.ldtable <= 4 * kTake;
-  if (little) {
-    p.by_width = fastdiv_make((uint32_t)(p.ldtable > 0 ? p.ldtable : 1));
-    hipLaunchKernelGGL((fork_take_kernel<true>), dim3(1), dim3(kTake), 0, s, p);
-  } else {
-    hipLaunchKernelGGL(fork_share_kernel, dim3(p.src_seqs + p.seqs), dim3(256), 0, s, p);
-    hipLaunchKernelGGL((fork_take_kernel<false>), dim3(1), dim3(kTake), 0, s, p);
-  }
+hipError_t launch_pages_fork(const PagesForkParams& p, PagesCopyParams* moves, hipStream_t s) {
+  if (p.strict) launch_fork<true>(p, s);
+  else launch_fork<false>(p, s);
   *moves = {p.ws + 4, p.seqs, p.ws, p.num_pages, p.num_pages};
   return hipGetLastError();
 }
