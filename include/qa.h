@@ -585,7 +585,7 @@ int qa_pages_compact_workspace(const qa_pages_compact_desc* desc, size_t* bytes)
  * `beams` sequences by score[b] + log softmax(logits[b])[t] over all b and t, best first,
  * ties to the lowest b and then t.  Sums of exponentials are f32 within 8192 of a row's
  * logits and f64 beyond; continuations of one b are ranked by their logits, those of
- * several in f64.
+ * several in f64, with these sums.
  *   logits  [groups * beams][vocab], row stride ldl, QA_F16, QA_BF16 or QA_F32; -inf
  *           is a token of probability 0, and so is NaN or +inf here: it is not chosen and
  *           not counted

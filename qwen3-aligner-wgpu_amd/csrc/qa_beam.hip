@@ -6,12 +6,16 @@
 // its `width` largest logits in the workspace.  A second one, a block for each group,
 // joins the sums in f64 and ranks the chunks' candidates, in f64 too: an f32 sum of
 // a score near -50 and a log-probability has steps of 4e-6, and candidates that differ
-// by less would change places.  Equal ones go by (beam, token), so every comparison is
-// of (value, index) pairs of which no two are alike: results do not depend on timing.
+// by less would change places.  What is left of that is the chunks' f32 sums, at most 6e-6 of a
+// row's logarithm: it moves a beam's candidates together, so that those of one beam keep
+// their order, and only those of two that are as close can change places.  Equal ones go by
+// (beam, token), so every comparison is of (value, index) pairs of which no two are alike:
+// results do not depend on timing.
 //
 // 192 rows of 151936 f16 logits, the best 8 of 8 beams: 20.7 us, the chunks 15.6 (58 MB at 3.7
 // TB/s: loads and maxima alone take 11.4, the exponentials 2 more, the lists and their
-// ranks the rest), the join 4.7.  4 rows: 9.9 us, two launches and 5 trips to memory.
+// ranks the rest), the join 4.7; in f32 29.4, 117 MB.  4 rows: 9.9 us, two launches and 5 trips to
+// memory.
 #include "qa_internal.h"
 
 namespace qa {
@@ -53,7 +57,8 @@ __device__ __forceinline__ void lds_barrier() {
 // Logits of a thread, by how many there are in all: 8 below 0.5 M, 16 below 3 M, 32 beyond.  Small
 // chunks are more blocks and longer lists to merge (us with 8 / 16 / 32: 8 rows of 60000 9.8 / 9.8 /
 // 10.3, 64 of 12000 9.7 / 10.2 / 11.3, 4 of 151936 11.0 / 10.2 / 10.2, 12 of them 13.4 / 11.6 / 11.7,
-// 24 14.4 / 11.9 / 11.3, 192 39.7 / 27.9 / 22.8; 192 of 12000 10.8 / 10.8 / 11.6, of 32000 15.0 / 13.2 / 12.5).
+// 24 14.4 / 11.9 / 11.3, 192 39.7 / 27.9 / 22.8; 192 of 12000 10.8 / 10.8 / 11.6, of 32000 15.0 / 13.2 / 12.5;
+// with the ranks and the join as they were, what was 22.8 is 20.7 now).
 int each_of(const BeamParams& p) {
   const int64_t all = p.groups * p.beams * p.vocab;
   return all < 500000 ? 8 : all < 3000000 ? 16 : 32;

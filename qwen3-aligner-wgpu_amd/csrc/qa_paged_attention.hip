@@ -216,7 +216,8 @@ struct Cfg {
 //    parts for one block a CU, in even numbers too, and none where the rounds of unsplit
 //    blocks are at least 0.7 full (us, unsplit / these parts / the rule above; windows of 4096:
 //    128 of them f16 56.2 / 55.8 / 59.6, e4m3 40.1 / 31.8 / 35.8; 384 f16 147.8 / - / 150.3,
-//    e4m3 of 4 heads 83.1 / - / 89.6). Many: a round of 128-pair blocks takes 1.7 of one of
+//    e4m3 of 4 heads 83.1 / - / 89.6).  Nothing between 128 and 384 is measured: from 129 to
+//    255 this gives one part also where two blocks fit on a CU (e4m3, heads of 64).  Many: a round of 128-pair blocks takes 1.7 of one of
 //    64-pair ones, so the fewer rounds by that (windows of 2048, 8 kv heads of 128, 64 / 128:
 //    600 rows 36.1 / 58.2, 1201 73.9 / 62.4, 2400 108.6 / 122.8, e4m3 1201 89.5 / 77.5; of 512,
 //    1201 rows 36.9 / 29.1; 12 prompts of up to 100 rows 74.7 / 64.7).  Its keys are split as
@@ -336,8 +337,9 @@ __device__ __forceinline__ float* part_stats(const PagedAttnParams& p, const Spl
 // A kernel's arguments, 64 bytes to a line of the scalar cache, all asked for at once: as the
 // code comes to them each line is a trip to memory of its own.  One token behind 322 keys 8.4 ->
 // 8.2 us, in a window of 1024 11.5 -> 10.8, of which 0.2 in the join; 1201 rows 60.6 -> 60.0.
-// Without a window, e4m3 and the join go without (64 tokens behind up to 8192 keys 128.0,
-// asked in either 128.7; 20 tokens and a prompt 20.0 and 20.2).
+// Without a window, e4m3 and the join go without, as it gives them nothing: 64 tokens behind up
+// to 8192 keys 128.0, asked in either 128.7; 20 tokens and a prompt 20.0 and 20.2 (0.5 to 1%, no
+// more than two runs differ by).
 __device__ __forceinline__ void ask_for(const PagedAttnParams& p, const Split& sp) {
   asm volatile("" ::"s"(p.q), "s"(p.kv.k), "s"(p.kv.nkvh), "s"(sp.many_parts));
   __builtin_amdgcn_sched_barrier(0);
