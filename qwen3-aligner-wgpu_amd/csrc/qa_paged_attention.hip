@@ -217,8 +217,8 @@ struct Cfg {
 //    blocks are at least 0.7 full (us, unsplit / these parts / the rule above; windows of 4096:
 //    128 of them f16 56.2 / 55.8 / 59.6, e4m3 40.1 / 31.8 / 35.8; 384 f16 147.8 / - / 150.3,
 //    e4m3 of 4 heads 83.1 / - / 89.6).  Nothing between 128 and 384 is measured: from 129 to
-//    255 this gives one part also where two blocks fit on a CU (e4m3, heads of 64).  Many: a round of 128-pair blocks takes 1.7 of one of
-//    64-pair ones, so the fewer rounds by that (windows of 2048, 8 kv heads of 128, 64 / 128:
+//    255 this gives one part also where two blocks fit on a CU (e4m3, heads of 64).  Many: a
+//    round of 128-pair blocks takes 1.7 of one of 64-pair ones, so the fewer rounds by that (windows of 2048, 8 kv heads of 128, 64 / 128:
 //    600 rows 36.1 / 58.2, 1201 73.9 / 62.4, 2400 108.6 / 122.8, e4m3 1201 89.5 / 77.5; of 512,
 //    1201 rows 36.9 / 29.1; 12 prompts of up to 100 rows 74.7 / 64.7).  Its keys are split as
 //    far as there are CUs beside the short sequences' blocks (20 of those, 4 kv heads of 64,
